@@ -355,6 +355,119 @@ int vgx_attn_create_seqs(vgx_ctx* ctx, const vgx_attn_desc* desc, int nseq, vgx_
 int vgx_attn_seq_view(vgx_attn* a, int s, vgx_attn** out);
 int vgx_attn_block_seqs(vgx_attn* a, int layer, int pos, int nseq, const int16_t* qkv, int16_t* out);
 
+/* ---- a ragged batch over a paged KV cache.  No counterpart in the reference,
+ * which decodes one sequence into a contiguous cache; for servers whose
+ * sequences have different lengths.  Numbers here are floating point (sums,
+ * norms and softmax statistics in 32 bits or more), except where a type says
+ * q16 or q8.  Element types: */
+enum vgx_elem {
+    VGX_E_F32 = 1,
+    VGX_E_BF16 = 2,
+    VGX_E_F16 = 3,
+    VGX_E_Q16 = 4, /* int16, round(value * 256): the activations' grid */
+    VGX_E_Q8 = 5   /* int8, floor(value / step + 1/2): a cache's grid */
+};
+
+/* One layer's cache: num_pages pages of page_size positions, in the caller's
+ * device memory.  Value (page, head, slot, i) of K lies at element
+ * page * k_page + head * k_head + slot * k_row + i, and V likewise, so pages
+ * may be head-major, position-major or hold several layers.  kind BF16, F16
+ * or Q8; the compute type (queries, outputs) is BF16 for BF16 and F16 for the
+ * others.  k_step / v_step: the grid of Q8 (0: 1/16, the 8-bit KV grid).
+ * head_dim a multiple of 16, at most 256; pointers and strides multiples of
+ * 16 bytes; strides must keep the positions apart. */
+typedef struct vgx_paged {
+    int heads, kv_heads, head_dim;
+    int page_size, num_pages;
+    int kind;
+    float k_step, v_step;
+    void* k;
+    void* v;
+    int64_t k_page, k_head, k_row;
+    int64_t v_page, v_head, v_row;
+} vgx_paged;
+
+/* The batch: nseq sequences whose new tokens are ntok consecutive rows.
+ * Device arrays, read by the kernels (a captured call is replayed with new
+ * contents): sequence s has rows qstart[s] .. qstart[s+1]-1 (qstart[0] = 0,
+ * none is allowed), kvlen[s] positions counting those rows, and position p in
+ * page table[s * table_stride + p / page_size], slot p % page_size.  Its row
+ * r is position kvlen[s] - rows + r.  Rows at or behind qstart[nseq] are left
+ * as they are.  table_cols: entries a row of the table holds (entries past a
+ * sequence's length are not read).
+ * max_q, max_kv: the caller's bounds of the rows and positions of one
+ * sequence, by which launches are sized (0: ntok, and what the table holds).
+ * Bounds that the kernels check themselves, since the host cannot: a length
+ * outside the table's, the bounds above or the rotation's, and a page outside
+ * the pool, set bits (VGX_FAULT_*) in *fault (device int, may be NULL, never
+ * cleared here).  The rows concerned are not written by vgx_paged_append, and
+ * vgx_paged_attn leaves them with values that mean nothing; no access leaves
+ * the buffers. */
+enum vgx_fault { VGX_FAULT_LENGTH = 1, VGX_FAULT_PAGE = 2 };
+typedef struct vgx_ragged {
+    int nseq, ntok, max_q, max_kv;
+    const int* qstart;
+    const int* kvlen;
+    const int* table;
+    int table_cols;
+    int64_t table_stride;
+    int* fault;
+} vgx_ragged;
+
+/* vgx_paged_append: every row's q and K heads through an optional RMSNorm
+ * (x * rsqrt(mean(x^2) + eps) * w; q_norm / k_norm: head_dim f32, device, both
+ * or neither) and the rotation of their first rot values by the angles of the
+ * row's position (cos / sin: npos rows of rot/2 f32, device; rot a multiple of
+ * 16, 0: none; rope_half as in vgx_attn_desc), then q rounded into q (ntok rows
+ * of heads * head_dim, q_stride elements apart, compute type; may be NULL) and
+ * K and V rounded into the pages.  qkv: ntok rows of (heads + 2 * kv_heads) *
+ * head_dim values of kind F32, BF16, F16 or Q16 (vgx_gemm's output), stride
+ * elements apart.  A row whose position is negative (more rows than kvlen) is
+ * skipped. */
+typedef struct vgx_paged_rows {
+    int kind;
+    const void* qkv;
+    int64_t stride;
+    const float* cos;
+    const float* sin;
+    int npos, rot, rope_half;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+    void* q;
+    int64_t q_stride;
+} vgx_paged_rows;
+int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_rows* rows);
+
+/* vgx_paged_attn: out = softmax(scale * q.K) V for every row and head over its
+ * sequence's positions 0 .. its own (with window > 0 the last `window` of
+ * them).  q: ntok rows of heads * head_dim, compute type, q_stride elements
+ * apart; scale 0: 1/sqrt(head_dim).  out: rows of heads * head_dim, out_kind
+ * the compute type or Q16 (vgx_gemm's input), out_stride elements apart.  lse
+ * (may be NULL): f32, ntok x heads, the log of the softmax's denominator.  A
+ * row without a visible position gives zeros and an lse of -infinity.
+ * Positions a row does not see, and what a page holds behind its sequence's
+ * end, do not reach it, whatever values are there.
+ * ws: device memory of vgx_paged_attn_ws bytes, for the caller's use again
+ * after the call's work is done (calls in flight at once, and captured graphs
+ * replayed at once, need one each); with less, or NULL, long sequences are
+ * not split and the results are rounded differently.
+ * vgx_paged_attn_ws returns 0 for arguments that vgx_paged_attn refuses. */
+typedef struct vgx_paged_query {
+    const void* q;
+    int64_t q_stride;
+    float scale;
+    int window;
+    int out_kind;
+    void* out;
+    int64_t out_stride;
+    float* lse;
+    void* ws;
+    size_t ws_bytes;
+} vgx_paged_query;
+size_t vgx_paged_attn_ws(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, int window);
+int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_query* query);
+
 /* ---- LFM2 gated short convolution: replaces GPU::init_conv, set_conv_kernel,
  * conv_block's gate/conv3/gate passes and clear_conv_state
  * (engine/src/gpu_conv.cpp:10-225), between the in_proj GEMV (3*dim rows:

@@ -1,0 +1,474 @@
+"""The paged cache's append and attention against their definitions in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+from paged_ref import STEP, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def make(gpu, b, heads, k=None, v=None, **kw):
+    c = gpu.paged_cache(heads, b.kvh, b.hd, b.kind, (b.k if k is None else k).cuda() if k is None else k,
+                        (b.v if v is None else v).cuda() if v is None else v)
+    return c, c.batch(*b.device(), b.ntok, **kw)
+
+
+def tables(npos, rot, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    ang = torch.rand(npos, rot // 2, generator=g, dtype=torch.float64) * 6.28
+    return torch.cos(ang).float(), torch.sin(ang).float()
+
+
+def check_append(gpu, b, heads, act, rot, half, norm, x=None, cache=None, batch=None):
+    width = (heads + 2 * b.kvh) * b.hd
+    if x is None:
+        x = b.randn(b.ntok, width) * 1.5
+        x = torch.clamp(torch.round(x * 256), -32768, 32767).to(torch.int16) if act == torch.int16 else x.to(act)
+    qn = 1 + 0.3 * b.randn(b.hd) if norm else None
+    kn = 1 + 0.3 * b.randn(b.hd) if norm else None
+    cos, sin = tables(max(b.kv + [1]), rot) if rot else (None, None)
+    if cache is None:
+        cache, batch = make(gpu, b, heads)
+    dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    out = torch.full((b.ntok + 2, heads, b.hd), 7.0, dtype=ref.CTYPE[b.kind], device="cuda")
+    cache.append(batch, x.cuda(), dev(cos), dev(sin), half, dev(qn), dev(kn), out=out)
+    batch.check()
+    q, k, v, mag = ref.append(b, x, heads, cos, sin, half, qn, kn)
+    # 32-bit: head_dim additions, the root, three products and the rotation's two
+    err = mag * (b.hd + 24) * 2.0 ** -24
+    got_q, got_k, got_v = out.cpu(), cache.k.cpu(), cache.v.cpu()
+    want_k, want_v = b.k.clone(), b.v.clone()
+    for s, (n, m) in enumerate(zip(b.nq, b.kv)):
+        for r in range(n):
+            pos, t = m - n + r, int(b.qs[s]) + r
+            if pos < 0:
+                assert (got_q[t] == 7.0).all()
+                continue
+            pg, sl = int(b.table[s, pos // b.page]), pos % b.page
+            tiny = 2.0 ** -25 if b.kind != "bf16" else 0.0  # float16's subnormal step
+            half_q = ref.HALF_STEP[ref.CTYPE[b.kind]]
+            assert ((got_q[t].double() - q[t]).abs() <= q[t].abs() * half_q + 2 * err[t, :heads] + tiny).all()
+            for got, val, e, want in ((got_k, k, err[t, heads:], want_k), (got_v, v, v[t].abs() * 2.0 ** -23, want_v)):
+                g = got[pg, :, sl]
+                if b.kind == "q8":
+                    c = val[t].clamp(-128 * STEP, 127 * STEP)
+                    assert ((ref.value(g) - c).abs() <= STEP / 2 + e).all()
+                else:
+                    assert ((g.double() - val[t]).abs() <= val[t].abs() * half_q + 2 * e + tiny).all()
+                want[pg, :, sl] = g
+    # nothing else of the pool, nor the rows behind the last sequence, was written
+    assert torch.equal(got_k.view(torch.uint8), want_k.view(torch.uint8))
+    assert torch.equal(got_v.view(torch.uint8), want_v.view(torch.uint8))
+    assert (got_q[int(b.qs[-1]):] == 7.0).all()
+    return x, cache, batch
+
+
+ACTS = [torch.int16, torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("act", ACTS)
+def test_append_types(gpu, kind, act):
+    b = Batch(1, [1, 5, 0, 33], [17, 5, 9, 70], 2, 64, 16, kind)
+    check_append(gpu, b, 4, act, 64, True, True)
+
+
+@pytest.mark.parametrize("heads, kvh, hd", [(8, 4, 96), (3, 1, 16), (6, 2, 80), (5, 5, 128), (4, 2, 144), (2, 1, 256)])
+@pytest.mark.parametrize("half", [True, False])
+def test_append_heads(gpu, heads, kvh, hd, half):
+    b = Batch(2, [1, 3, 20], [300, 3, 41], kvh, hd, 32, "bf16")
+    check_append(gpu, b, heads, torch.float32, hd, half, True)
+    check_append(gpu, Batch(3, [2, 1], [2, 65], kvh, hd, 7, "q8"), heads, torch.int16, hd // 32 * 16, half, False)
+
+
+@pytest.mark.parametrize("page", [1, 3, 16, 24, 100, 4096])
+def test_append_pages(gpu, page):
+    b = Batch(4, [4, 130, 1], [4, 333, 1000], 2, 32, page, "f16")
+    check_append(gpu, b, 2, torch.float16, 0, True, False)
+
+
+def test_append_more_rows_than_positions(gpu):
+    """Rows before position 0 have no place: nothing of theirs is written."""
+    b = Batch(5, [6, 2, 3], [2, 0, 3], 1, 48, 16, "bf16")
+    check_append(gpu, b, 2, torch.bfloat16, 48, True, True)
+
+
+def test_append_many_sequences(gpu):
+    rng = np.random.default_rng(0)
+    nq = rng.integers(0, 4, 200).tolist()
+    kv = [n + int(m) for n, m in zip(nq, rng.integers(0, 40, 200))]
+    check_append(gpu, Batch(6, nq, kv, 1, 64, 16, "bf16"), 2, torch.int16, 64, True, True)
+
+
+def strided_pools(b):
+    """Position-major pages with room between the rows, both in one allocation."""
+    base = torch.zeros(b.pages, 2, b.page, b.kvh, b.hd + 16, dtype=b.k.dtype, device="cuda")
+    k, v = (base[:, i].transpose(1, 2)[..., :b.hd] for i in (0, 1))
+    k.copy_(b.k)
+    v.copy_(b.v)
+    return k, v
+
+
+def test_strides(gpu):
+    b = Batch(7, [3, 40, 1], [100, 40, 64], 2, 64, 16, "bf16")
+    k, v = strided_pools(b)
+    cache, batch = make(gpu, b, 4, k=k, v=v)
+    wide = torch.zeros(b.ntok, 640, dtype=torch.bfloat16)
+    wide[:, 64:576] = (b.randn(b.ntok, 512)).to(torch.bfloat16)
+    x, cos_sin = wide[:, 64:576], tables(100, 64)
+    q = torch.empty(b.ntok, 4, 96, dtype=torch.bfloat16, device="cuda").flatten(1)[:, :256]
+    xd = wide.cuda()[:, 64:576]
+    got = cache.append(batch, xd, cos_sin[0].cuda(), cos_sin[1].cuda(), out=q)
+    dense, dbatch = make(gpu, b, 4)
+    want = dense.append(dbatch, x.contiguous().cuda(), cos_sin[0].cuda(), cos_sin[1].cuda())
+    assert torch.equal(got, want.flatten(1))
+    assert torch.equal(k, dense.k) and torch.equal(v, dense.v)
+    o = torch.empty(b.ntok, 300, dtype=torch.bfloat16, device="cuda")[:, 8:264]
+    with pytest.raises(Exception):  # rows 600 bytes apart: not whole 16-byte steps
+        cache.attend(batch, q, out=o)
+    o = torch.empty(b.ntok, 512, dtype=torch.bfloat16, device="cuda")[:, 8:264]
+    cache.attend(batch, q, out=o)
+    assert torch.equal(o, dense.attend(dbatch, want)[0])
+
+
+def check_attn(gpu, b, heads, window=0, scale=None, q=None, out=None, cache=None, batch=None, spread=2.0):
+    ct = ref.CTYPE[b.kind]
+    if q is None:
+        q = (spread * b.randn(b.ntok, heads, b.hd)).to(ct)
+    if cache is None:
+        cache, batch = make(gpu, b, heads)
+    o, lse = cache.attend(batch, q.cuda(), scale=scale or 0.0, window=window, lse=True, out=out)
+    batch.check()
+    want, wl, mag, dots = ref.attend(b, q, heads, scale, window)
+    kind = "q16" if o.dtype == torch.int16 else None
+    bound = ref.attn_bound(b, ct, want, mag, dots, kind)
+    got = ref.value(o.cpu())[:b.ntok].view_as(want)
+    worst = (got - want).abs() - bound
+    assert torch.isfinite(got).all() and (worst <= 0).all(), float(worst.max())
+    lse = lse.cpu().double()
+    empty = wl == -math.inf
+    assert (lse[empty] == -math.inf).all() and (got[empty] == 0).all()
+    tol = dots * (b.hd + 8) * 2.0 ** -22 + (max(b.kv + [1]) + 32) * 2.0 ** -24 + wl.abs() * 2.0 ** -22
+    assert ((lse - wl).abs()[~empty] <= tol[~empty]).all()
+    return o
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("heads, kvh, hd", [(8, 4, 96), (16, 2, 64), (4, 1, 128), (3, 3, 16), (6, 2, 80), (5, 1, 144),
+                                            (2, 1, 256), (32, 1, 32)])
+def test_attn_tokens(gpu, kind, heads, kvh, hd):
+    b = Batch(11, [1, 1, 1, 1, 1], [1, 31, 33, 130, 700], kvh, hd, 16, kind)
+    check_attn(gpu, b, heads)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("heads, kvh, hd", [(8, 4, 96), (16, 2, 64), (4, 1, 128), (3, 3, 16), (6, 2, 80), (5, 1, 144),
+                                            (2, 1, 256)])
+def test_attn_chunks(gpu, kind, heads, kvh, hd):
+    b = Batch(12, [130, 1, 0, 64, 7], [130, 500, 20, 100, 263], kvh, hd, 32, kind)
+    check_attn(gpu, b, heads)
+
+
+@pytest.mark.parametrize("page", [1, 5, 16, 48, 64, 1000])
+@pytest.mark.parametrize("nq", [[2, 1], [90, 45]])
+def test_attn_pages(gpu, page, nq):
+    check_attn(gpu, Batch(13, nq, [301, 97], 2, 64, page, "f16"), 4)
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 65, 200, 5000])
+@pytest.mark.parametrize("nq", [[1, 3, 1, 2], [150, 40, 1, 70]])
+def test_attn_window(gpu, window, nq):
+    check_attn(gpu, Batch(14, nq, [150, 333, 900, 70], 2, 64, 16, "bf16"), 4, window=window)
+
+
+@pytest.mark.parametrize("nq", [[5, 2, 1], [70, 40, 1]])
+def test_attn_empty_rows(gpu, nq):
+    """More rows than positions: the first see nothing and give zeros."""
+    check_attn(gpu, Batch(15, nq, [3, 0, 1], 2, 64, 16, "bf16"), 4)
+
+
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_attn_long_splits(gpu, n):
+    """Few sequences, many keys: the keys are split over workgroups."""
+    b = Batch(16, [n, 1], [9000, 2500], 2, 64, 64, "bf16")
+    cache, batch = make(gpu, b, 4)
+    o = check_attn(gpu, b, 4, cache=cache, batch=batch)
+    assert batch.ws and min(batch.ws.values()) > 0  # the split path ran
+    # and without the workspace
+    import ctypes
+    from vgx import lib as vl
+    q = (2.0 * b.randn(b.ntok, 4, b.hd)).to(torch.bfloat16).cuda()
+    got = torch.empty_like(o)
+    r = vl.PagedQuery(q.data_ptr(), 256, 0.0, 0, vl.E_BF16, got.data_ptr(), 256, 0, 0, 0)
+    vl.check(vl.load().vgx_paged_attn(gpu.ctx, cache.ref, batch.ref, ctypes.byref(r)))
+    want = cache.attend(batch, q)[0]
+    # both within the same bound of the definition, so within twice of one another
+    w, _, mag, dots = ref.attend(b, q.cpu(), 4)
+    bound = 2 * ref.attn_bound(b, torch.bfloat16, w, mag, dots)
+    assert ((got.double() - want.double()).abs().cpu().view_as(w) <= bound).all()
+
+
+@pytest.mark.parametrize("nq", [[1, 2], [80, 3]])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+def test_attn_behind_the_end(gpu, nq, bad):
+    """What the last page holds behind a sequence's end, and the pages that
+    are not its own, do not reach its rows."""
+    b = Batch(17, nq, [85, 37], 2, 64, 32, "bf16")
+    clean = b.k.clone(), b.v.clone()
+    used = torch.zeros(b.pages, b.page, dtype=torch.bool)
+    for s, m in enumerate(b.kv):
+        for p in range(m):
+            used[int(b.table[s, p // b.page]), p % b.page] = True
+    q = (2 * b.randn(b.ntok, 4, 64)).to(torch.bfloat16)
+    want = make(gpu, b, 4)
+    want = want[0].attend(want[1], q.cuda())[0]
+    for t in (b.k, b.v):
+        t.masked_fill_(~used[:, None, :, None], bad)
+    got = make(gpu, b, 4)
+    assert torch.equal(got[0].attend(got[1], q.cuda())[0], want)
+    b.k, b.v = clean
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("nq, window", [([4, 2], 0), ([100, 30], 0), ([100, 30], 20), ([3, 1], 7)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attn_masked_values(gpu, kind, nq, window, bad):
+    """A NaN or infinity at a position reaches only the rows that see it."""
+    b = Batch(18, nq, [140, 61], 2, 64, 16, kind)
+    q = (2 * b.randn(b.ntok, 4, 64)).to(ref.CTYPE[kind])
+    want, _, mag, dots = ref.attend(b, q, 4, None, window)
+    bound = ref.attn_bound(b, ref.CTYPE[kind], want, mag, dots)
+    at = [(0, 138), (0, 110), (1, 59), (1, 45)]
+    for s, p in at:
+        pg, sl = int(b.table[s, p // 16]), p % 16
+        b.k[pg, :, sl, 5] = bad
+        b.v[pg, :, sl, 9] = bad
+    c, bt = make(gpu, b, 4)
+    got = c.attend(bt, q.cuda(), window=window)[0].cpu().double().view_as(want)
+    for s, (n, m) in enumerate(zip(b.nq, b.kv)):
+        for r in range(n):
+            pos, t = m - n + r, int(b.qs[s]) + r
+            sees = any(ss == s and p <= pos and (not window or p > pos - window) for ss, p in at)
+            if sees:
+                assert not torch.isfinite(got[t, :, 9]).any()
+            else:
+                assert ((got[t] - want[t]).abs() <= bound[t]).all(), (s, r)
+
+
+def test_attn_scores_past_every_exponent(gpu):
+    """Scores of +-30000: weights of one key, no overflow."""
+    b = Batch(19, [1, 90], [200, 90], 1, 64, 16, "bf16")
+    q = (100 * b.randn(b.ntok, 2, 64)).to(torch.bfloat16)
+    b.k = (30 * b.k.float()).to(torch.bfloat16)
+    o, _ = (lambda c: c[0].attend(c[1], q.cuda()))(make(gpu, b, 2))
+    want, _, mag, dots = ref.attend(b, q, 2)
+    assert torch.isfinite(o).all()
+    bound = ref.attn_bound(b, torch.bfloat16, want, mag, dots)
+    assert ((o.cpu().double().view_as(want) - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q8"])
+@pytest.mark.parametrize("nq", [[1, 1], [70, 3]])
+def test_attn_q16_out(gpu, kind, nq):
+    """The output as vgx_gemm's input; rows behind the last sequence stay."""
+    b = Batch(20, nq, [300, 50], 2, 96, 16, kind)
+    out = torch.full((b.ntok + 3, 4 * 96), 77, dtype=torch.int16, device="cuda")
+    check_attn(gpu, b, 4, out=out)
+    assert (out[b.ntok:] == 77).all()
+
+
+def test_rows_behind_the_last_sequence(gpu):
+    b = Batch(21, [2, 60, 0], [20, 90, 5], 2, 64, 16, "bf16")
+    cache, _ = make(gpu, b, 4)
+    batch = cache.batch(*b.device(), b.ntok + 9)  # nine rows of nobody's
+    q = torch.randn(b.ntok + 9, 4, 64, device="cuda").to(torch.bfloat16)
+    out = torch.full((b.ntok + 9, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+    before = cache.k.clone()
+    cache.attend(batch, q, out=out)
+    assert (out[b.ntok:] == 5).all() and not (out[:b.ntok] == 5).all(1).any()
+    x = torch.randn(b.ntok + 9, 512, device="cuda")
+    qo = torch.full((b.ntok + 9, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    cache.append(batch, x, out=qo)
+    assert (qo[b.ntok:] == 5).all()
+    same = (cache.k == before).all(-1).all(1)
+    assert int((~same).sum()) == sum(b.nq)
+    batch.check()
+
+
+def test_nothing_to_do(gpu):
+    b = Batch(22, [0, 0], [5, 0], 2, 64, 16, "bf16")
+    cache, batch = make(gpu, b, 4)
+    assert cache.append(batch, torch.empty(0, 512, device="cuda")).shape == (0, 4, 64)
+    o, z = cache.attend(batch, torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda"), lse=True)
+    assert o.shape == (0, 256) and z.shape == (0, 4)
+
+
+def test_far_pages(gpu):
+    """Offsets past 32 bits: pages 6 GiB apart in the pool."""
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 14 GiB")
+    b = Batch(23, [1, 40], [70, 64], 1, 64, 16, "bf16")
+    far = 3 << 30  # elements
+    base = torch.empty(far + (b.pages + 1) * 1024, dtype=torch.bfloat16, device="cuda")
+    step = far // (b.pages - 1) // 8 * 8
+    assert step * (b.pages - 1) * 2 > 1 << 32
+    k = base.as_strided((b.pages, 1, 16, 64), (step, 1024, 64, 1))
+    v = base.as_strided((b.pages, 1, 16, 64), (step, 1024, 64, 1), 1024)
+    k.copy_(b.k)
+    v.copy_(b.v)
+    cache, batch = make(gpu, b, 4, k=k, v=v)
+    check_append(gpu, b, 4, torch.float32, 64, True, True, cache=cache, batch=batch)
+    b.k, b.v = k.cpu(), v.cpu()
+    check_attn(gpu, b, 4, cache=cache, batch=batch)
+
+
+def test_faults_are_reported(gpu):
+    """A length past the table and a page outside the pool raise at check();
+    neither's rows are written, every other sequence's are."""
+    from vgx import lib as vl
+    b = Batch(24, [1, 1, 1], [20, 40, 33], 2, 64, 16, "bf16")
+    cache, batch = make(gpu, b, 4)
+    qs, kv, table = b.device()
+    x = torch.randn(3, 512, device="cuda")
+    q = torch.randn(3, 4, 64, device="cuda").to(torch.bfloat16)
+    good = cache.attend(batch, q)[0]
+    kv2 = kv.clone()
+    kv2[1] = 10 ** 6
+    bad = cache.batch(qs, kv2, table, 3)
+    before, before_v = cache.k.clone(), cache.v.clone()
+    cache.append(bad, x)
+    with pytest.raises(vl.VgxError, match="length"):
+        bad.check()
+    bad.check()  # cleared
+    changed = (cache.k != before).any(-1).any(1).nonzero()
+    assert {int(p) for p in changed[:, 0]} == {int(b.table[0, 1]), int(b.table[2, 2])}
+    cache.k.copy_(before)
+    cache.v.copy_(before_v)
+    t2 = table.clone()
+    t2[1, 2] = b.pages
+    t2[2, 2] = -1
+    bad = cache.batch(qs, kv, t2, 3)
+    o = cache.attend(bad, q)[0]
+    with pytest.raises(vl.VgxError, match="page"):
+        bad.check()
+    assert torch.equal(o[0], good[0])
+    before = cache.k.clone()
+    cache.append(bad, x)
+    with pytest.raises(vl.VgxError, match="page"):
+        bad.check()
+    changed = (cache.k != before).any(-1).any(1).nonzero()
+    assert {int(p) for p in changed[:, 0]} == {int(b.table[0, 1])}
+
+
+def test_bounds_are_held(gpu):
+    """A sequence longer than max_q or max_kv promised: reported, in bounds."""
+    from vgx import lib as vl
+    b = Batch(25, [3, 40], [20, 90], 2, 64, 16, "bf16")
+    cache, _ = make(gpu, b, 4)
+    q = torch.randn(b.ntok, 4, 64, device="cuda").to(torch.bfloat16)
+    for kw in (dict(max_q=4), dict(max_kv=64)):
+        batch = cache.batch(*b.device(), b.ntok, **kw)
+        cache.attend(batch, q)
+        with pytest.raises(vl.VgxError, match="length"):
+            batch.check()
+
+
+def test_other_stream(gpu):
+    """On a side stream, with the default stream busy; the context's own
+    stream is what it was."""
+    from vgx import lib as vl
+    b = Batch(26, [1, 50], [3000, 80], 2, 64, 16, "bf16")
+    cache, batch = make(gpu, b, 4)
+    q = torch.randn(b.ntok, 4, 64, device="cuda").to(torch.bfloat16)
+    want = cache.attend(batch, q)[0]
+    was = vl.load().vgx_ctx_stream(gpu.ctx)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [cache.attend(batch, q)[0] for _ in range(4)]
+    assert vl.load().vgx_ctx_stream(gpu.ctx) == was
+    side.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_graph_replays_with_new_lengths(gpu):
+    """A captured append + attention, replayed as the sequences grow; two
+    graphs captured from one batch, replayed in turn."""
+    b = Batch(27, [1, 1, 1], [100, 37, 2000], 2, 64, 16, "bf16", spare=8)
+    cache, _ = make(gpu, b, 4)
+    qs, kv, table = b.device()
+    table = torch.cat([table, torch.arange(b.pages - 3, b.pages, dtype=torch.int32).cuda()[:, None]], 1)
+    for s in range(3):  # a spare page after each sequence's last
+        table[s, -(-b.kv[s] // 16)] = b.pages - 3 + s
+    batch = cache.batch(qs, kv, table, 3, max_q=1, max_kv=2016)
+    x = torch.randn(3, 512, device="cuda")
+    cos, sin = (t.cuda() for t in tables(2100, 64))
+
+    def step():
+        q = cache.append(batch, x, cos, sin)
+        return cache.attend(batch, q)[0]
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = step()
+        graphs.append((g, o))
+    for i in range(4):
+        kv += 1
+        x.copy_(torch.randn(3, 512, device="cuda"))
+        for g, o in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, step()), i
+    batch.check()
+
+
+def test_a_step_with_the_quantised_path(gpu):
+    """qkv from vgx_gemm (q16), append, attention, and its q16 output into
+    vgx_gemm: a chunk at once equals the same tokens one after another."""
+    import oracle as o
+    from vgx import mmcf
+    rng = np.random.default_rng(5)
+    heads, kvh, hd, dim = 8, 4, 96, 768
+
+    def mat(r, c):
+        q, unit, plane = mmcf.q8_per_row(rng.standard_normal((r, c)).astype(np.float32) * 0.03)
+        return gpu.upload(mmcf.Matrix("q8", r, c, (q.view(np.uint8) ^ 0x80).ravel(), unit, True, plane))
+
+    wqkv, wo = mat((heads + 2 * kvh) * hd, dim), mat(dim, heads * hd)
+    x = torch.from_numpy(np.stack([o.quantize_act(rng.standard_normal(dim).astype(np.float32)) for _ in range(40)])).cuda()
+    cos, sin = (t.cuda() for t in tables(64, hd))
+    qn = torch.rand(hd, device="cuda") + 0.5
+    res = {}
+    for mode in ("chunk", "tokens"):
+        b = Batch(28, [40], [40], kvh, hd, 16, "bf16")
+        cache, batch = make(gpu, b, heads)
+        qs, kv, table = b.device()
+        if mode == "chunk":
+            q = cache.append(batch, gpu.gemm(wqkv, x), cos, sin, q_norm=qn, k_norm=qn)
+            att = cache.attend(batch, q, out=torch.empty(40, heads * hd, dtype=torch.int16, device="cuda"))[0]
+            res[mode] = gpu.gemm(wo, att, x)
+        else:
+            outs = []
+            for t in range(40):
+                one = cache.batch(torch.tensor([0, 1], dtype=torch.int32).cuda(),
+                                  torch.tensor([t + 1], dtype=torch.int32).cuda(), table, 1)
+                q = cache.append(one, gpu.gemm(wqkv, x[t:t + 1].contiguous()), cos, sin, q_norm=qn, k_norm=qn)
+                att = cache.attend(one, q, out=torch.empty(1, heads * hd, dtype=torch.int16, device="cuda"))[0]
+                outs.append(gpu.gemm(wo, att, x[t:t + 1].contiguous()))
+            res[mode] = torch.cat(outs)
+        pool = cache.k.clone(), cache.v.clone()
+        res[mode + "kv"] = pool
+    assert all(torch.equal(a, c) for a, c in zip(res["chunkkv"], res["tokenskv"]))
+    # attention's values are averages of V (|V| below 5 here), each side off by
+    # at most 2^-8 of that: the projection sums 768 of them times 0.03-sized
+    # weights, in root mean square 2^-8 * 5 * 0.03 * sqrt(768) / sqrt(3) < 0.01
+    d = (res["chunk"].float() - res["tokens"].float()) / 256
+    assert float(d.square().mean().sqrt()) < 0.02 and float(d.abs().max()) < 0.15

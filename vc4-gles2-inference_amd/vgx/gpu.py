@@ -18,6 +18,10 @@ def _ptr(t):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _np_ptr(a):
     return ctypes.c_void_p(0 if a is None else a.ctypes.data)
 
@@ -239,6 +243,131 @@ class Attention:
             pass
 
 
+_ELEM = {torch.float32: _l.E_F32, torch.bfloat16: _l.E_BF16, torch.float16: _l.E_F16, torch.int16: _l.E_Q16}
+_CACHE = {"bf16": (_l.E_BF16, torch.bfloat16, torch.bfloat16), "f16": (_l.E_F16, torch.float16, torch.float16),
+          "q8": (_l.E_Q8, torch.int8, torch.float16)}
+
+
+class RaggedBatch:
+    """A ragged batch over a paged cache: sequence s has rows qstart[s] ..
+    qstart[s+1]-1 of the ntok new ones, kvlen[s] positions counting them, and
+    its pages in table[s].  The arrays are read when a call runs, so they may
+    change between calls (and between replays of a captured one); max_q and
+    max_kv bound one sequence's rows and positions.  check() waits for the
+    device and raises if a call met a length or page outside its bounds."""
+
+    def __init__(self, gpu, qstart, kvlen, table, ntok, max_q=0, max_kv=0):
+        gpu.need(qstart, torch.int32, 1, "qstart")
+        gpu.need(kvlen, torch.int32, 1, "kvlen")
+        gpu.need(table, torch.int32, 2, "table")
+        nseq = kvlen.shape[0]
+        if qstart.shape[0] != nseq + 1 or table.shape[0] != nseq:
+            raise ValueError("a batch of %d sequences needs qstart of %d and a table of %d rows"
+                             % (nseq, nseq + 1, nseq))
+        if qstart.stride(0) != 1 or (nseq > 1 and kvlen.stride(0) != 1) or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("qstart, kvlen and a table's rows must be contiguous")
+        self.gpu, self.nseq, self.ntok = gpu, nseq, int(ntok)
+        self.fault = torch.zeros(1, dtype=torch.int32, device=gpu.device)
+        self._keep = (qstart, kvlen, table)
+        self.d = _l.Ragged(nseq, self.ntok, int(max_q), int(max_kv), qstart.data_ptr(), kvlen.data_ptr(),
+                           table.data_ptr(), table.shape[1], max(table.stride(0), table.shape[1]),
+                           self.fault.data_ptr())
+        self.ref = ctypes.byref(self.d)
+        self.ws = {}  # workspace bytes by (cache, window)
+
+    def check(self):
+        bits = int(self.fault.item())
+        if bits:
+            self.fault.zero_()
+            what = [w for b, w in ((_l.FAULT_LENGTH, "a length outside its bounds"),
+                                   (_l.FAULT_PAGE, "a page outside the pool")) if bits & b]
+            raise _l.VgxError(_l.VGX_ERANGE, "ragged batch: " + " and ".join(what))
+
+
+class PagedCache:
+    """One layer's paged KV cache over the caller's tensors k and v, each
+    (pages, kv_heads, page_size, head_dim) of any strides whose last is 1 (a
+    position-major pool is passed as its transposed view).  kind "bf16",
+    "f16" or "q8" (int8, the grids k_step and v_step, 1/16 by default); the
+    queries and outputs are bfloat16 for "bf16" and float16 for the others.
+    The calls run on torch's current stream."""
+
+    def __init__(self, gpu, heads, kv_heads, head_dim, kind, k, v, k_step=0.0, v_step=0.0):
+        elem, ctype, self.qtype = _CACHE[kind]
+        for t, name in ((k, "k"), (v, "v")):
+            gpu.need(t, ctype, 4, name)
+            if t.shape[1] != kv_heads or t.shape[3] != head_dim or t.stride(3) != 1 or t.shape != k.shape:
+                raise ValueError("%s must be (pages, %d, page_size, %d), head vectors contiguous" % (name, kv_heads,
+                                                                                                   head_dim))
+        self.gpu, self.heads, self.kv_heads, self.head_dim, self.kind = gpu, heads, kv_heads, head_dim, kind
+        self.k, self.v, self.width = k, v, heads * head_dim
+        self.d = _l.Paged(heads, kv_heads, head_dim, k.shape[2], k.shape[0], elem, k_step, v_step, k.data_ptr(),
+                          v.data_ptr(), *k.stride()[:3], *v.stride()[:3])
+        self.ref = ctypes.byref(self.d)
+
+    def batch(self, qstart, kvlen, table, ntok, max_q=0, max_kv=0):
+        return RaggedBatch(self.gpu, qstart, kvlen, table, ntok, max_q, max_kv)
+
+    def append(self, batch, qkv, cos=None, sin=None, rope_half=True, q_norm=None, k_norm=None, eps=1e-5, out=None):
+        """The rows qkv (ntok, (heads + 2 kv_heads) * head_dim; float32,
+        bfloat16, float16 or q16) normed, rotated (cos, sin: positions x rot/2)
+        and written into the cache; returns the queries (ntok, heads, head_dim)."""
+        g = self.gpu
+        g.need_rows(qkv, None, batch.ntok, self.width + 2 * self.kv_heads * self.head_dim, "qkv")
+        if qkv.dtype not in _ELEM:
+            raise ValueError("qkv must be float32, bfloat16, float16 or int16 (q16)")
+        npos = rot = 0
+        if cos is not None:
+            for t, name in ((cos, "cos"), (sin, "sin")):
+                g.need(t, torch.float32, 2, name)
+                if not t.is_contiguous() or t.shape != cos.shape:
+                    raise ValueError("cos and sin must be contiguous and of one shape")
+            npos, rot = cos.shape[0], 2 * cos.shape[1]
+        for t in (q_norm, k_norm):
+            if t is not None:
+                g.need(t, torch.float32, 1, "a norm weight")
+                if t.shape[0] != self.head_dim or t.stride(0) != 1:
+                    raise ValueError("a norm weight must be %d contiguous values" % self.head_dim)
+        q = out if out is not None else torch.empty((batch.ntok, self.heads, self.head_dim), dtype=self.qtype,
+                                                    device=g.device)
+        qs = self._rows(q, self.qtype, batch.ntok, "out")
+        r = _l.PagedRows(_ELEM[qkv.dtype], qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), _at(cos), _at(sin), npos,
+                         rot, int(rope_half), _at(q_norm), _at(k_norm), eps, q.data_ptr(), qs)
+        g.on_current(_l.load().vgx_paged_append, self.ref, batch.ref, ctypes.byref(r))
+        return q
+
+    def attend(self, batch, q, scale=0.0, window=0, out=None, lse=False):
+        """The attention of the rows q (ntok, heads, head_dim) over their
+        sequences: (out (ntok, heads * head_dim), lse (ntok, heads) or None).
+        out: a tensor to write, of the compute type or int16 (q16)."""
+        g = self.gpu
+        qs = self._rows(q, self.qtype, batch.ntok, "q")
+        if out is None:
+            out = torch.empty((batch.ntok, self.width), dtype=self.qtype, device=g.device)
+        kind = _l.E_Q16 if out.dtype == torch.int16 else _ELEM[self.qtype]
+        os_ = self._rows(out, out.dtype if kind == _l.E_Q16 else self.qtype, batch.ntok, "out")
+        key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window)
+        need = batch.ws.get(key)
+        L = _l.load()
+        if need is None:
+            need = batch.ws[key] = int(L.vgx_paged_attn_ws(g.ctx, self.ref, batch.ref, window))
+        ws = torch.empty(need, dtype=torch.uint8, device=g.device) if need else None
+        z = torch.empty((batch.ntok, self.heads), dtype=torch.float32, device=g.device) if lse else None
+        r = _l.PagedQuery(q.data_ptr(), qs, scale, window, kind, out.data_ptr(), os_, _at(z), _at(ws), need)
+        g.on_current(L.vgx_paged_attn, self.ref, batch.ref, ctypes.byref(r))
+        return out, z
+
+    def _rows(self, t, dtype, n, name):
+        """The stride of n rows of heads x head_dim values, (n, heads, head_dim) or (n, heads * head_dim)."""
+        if t.dim() == 3:
+            if t.shape[1] != self.heads or t.shape[2] != self.head_dim or t.stride(1) != self.head_dim:
+                raise ValueError("%s must be (%d, %d, %d), a row's heads contiguous" % (name, n, self.heads,
+                                                                                      self.head_dim))
+            t = t.flatten(1)
+        self.gpu.need_rows(t, dtype, n, self.width, name)
+        return max(t.stride(0), self.width)
+
+
 class GPU:
     """One libvgx context on one device, issuing on torch's current stream."""
 
@@ -255,6 +384,32 @@ class GPU:
 
     def sync(self):
         _l.check(_l.load().vgx_ctx_sync(self.ctx))
+
+    def on_current(self, call, *args):
+        """call(ctx, *args) on torch's current stream of this device, where
+        its tensors were made; the context's stream is put back after."""
+        L = _l.load()
+        now, was = torch.cuda.current_stream(self.device).cuda_stream, L.vgx_ctx_stream(self.ctx) or 0
+        if now == was:
+            _l.check(call(self.ctx, *args))
+            return
+        _l.check(L.vgx_ctx_set_stream(self.ctx, now))
+        try:
+            _l.check(call(self.ctx, *args))
+        finally:
+            L.vgx_ctx_set_stream(self.ctx, was)
+
+    def need(self, t, dtype, dims, name):
+        """Refuses a tensor of another device, type or number of dimensions."""
+        if t.device != self.device or t.dim() != dims or t.dtype != (dtype or t.dtype):
+            raise ValueError("%s must be a %d-dimensional %s tensor on %s, not %s on %s" % (
+                name, dims, dtype or t.dtype, self.device, t.dtype, t.device))
+
+    def need_rows(self, t, dtype, n, width, name):
+        """Refuses all but n rows of width contiguous values."""
+        self.need(t, dtype, 2, name)
+        if t.shape[0] < n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+            raise ValueError("%s must be %d rows of %d contiguous values, not %s" % (name, n, width, tuple(t.shape)))
 
     # -- weights
     def upload(self, m: Matrix):
@@ -440,6 +595,9 @@ class GPU:
 
     def attention(self, **kw):
         return Attention(self, **kw)
+
+    def paged_cache(self, heads, kv_heads, head_dim, kind, k, v, k_step=0.0, v_step=0.0):
+        return PagedCache(self, heads, kv_heads, head_dim, kind, k, v, k_step, v_step)
 
     def conv(self, w, layer_is_conv=None):
         return Conv(self, w, layer_is_conv)

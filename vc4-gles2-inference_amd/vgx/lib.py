@@ -39,6 +39,36 @@ class AttnDesc(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_I64 = ctypes.c_int64
+
+# element types of the paged cache's calls (enum vgx_elem)
+E_F32, E_BF16, E_F16, E_Q16, E_Q8 = 1, 2, 3, 4, 5
+FAULT_LENGTH, FAULT_PAGE = 1, 2
+
+
+class Paged(ctypes.Structure):
+    _fields_ = [("heads", _I), ("kv_heads", _I), ("head_dim", _I), ("page_size", _I), ("num_pages", _I),
+                ("kind", _I), ("k_step", ctypes.c_float), ("v_step", ctypes.c_float), ("k", _P), ("v", _P),
+                ("k_page", _I64), ("k_head", _I64), ("k_row", _I64),
+                ("v_page", _I64), ("v_head", _I64), ("v_row", _I64)]
+
+
+class Ragged(ctypes.Structure):
+    _fields_ = [("nseq", _I), ("ntok", _I), ("max_q", _I), ("max_kv", _I), ("qstart", _P), ("kvlen", _P),
+                ("table", _P), ("table_cols", _I), ("table_stride", _I64), ("fault", _P)]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [("kind", _I), ("qkv", _P), ("stride", _I64), ("cos", _P), ("sin", _P), ("npos", _I), ("rot", _I),
+                ("rope_half", _I), ("q_norm", _P), ("k_norm", _P), ("eps", ctypes.c_float), ("q", _P),
+                ("q_stride", _I64)]
+
+
+class PagedQuery(ctypes.Structure):
+    _fields_ = [("q", _P), ("q_stride", _I64), ("scale", ctypes.c_float), ("window", _I), ("out_kind", _I),
+                ("out", _P), ("out_stride", _I64), ("lse", _P), ("ws", _P), ("ws_bytes", ctypes.c_size_t)]
+
+
 _SIGS = {
     "vgx_abi_version": (_I, []),
     "vgx_strerror": (ctypes.c_char_p, [_I]),
@@ -108,6 +138,9 @@ _SIGS = {
     "vgx_kv_row_bytes": (_I, [_P]),
     "vgx_kv_read_rows": (_I, [_P, _I, _I, _I, _P]),
     "vgx_kv_write_rows": (_I, [_P, _I, _I, _I, _P]),
+    "vgx_paged_append": (_I, [_P, _P, _P, _P]),
+    "vgx_paged_attn_ws": (ctypes.c_size_t, [_P, _P, _P, _I]),
+    "vgx_paged_attn": (_I, [_P, _P, _P, _P]),
     "vgx_quantize_act": (None, [_P, _I, _P]),
     "vgx_x_pack_i16_2": (None, [_P, _I, _P]),
 }
