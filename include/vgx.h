@@ -468,6 +468,49 @@ typedef struct vgx_paged_query {
 size_t vgx_paged_attn_ws(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, int window);
 int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_query* query);
 
+/* vgx_draft_verify: the drafted tokens of a ragged batch against the target's
+ * logits.  The batch is vgx_ragged's: sequence s has rows qstart[s] ..
+ * qstart[s+1]-1 of ntok (the token it ended with, then its drafts), tokens[r]
+ * is row r's token, logits row r the target's for the token after it, so row r
+ * checks tokens[r + 1] and a sequence's last row has no draft.  With
+ * p_r = softmax(logits_r / T), T = temp[s] (device f32, NULL: 1), and q_r the
+ * same of draft row r (draft: the logits tokens[r + 1] was drawn from, same
+ * kind; NULL: drafts without a distribution, q_r = 1 at the token):
+ *   the draft of row r is accepted if u_accept[r] * q_r < p_r at the token;
+ *   at the first row refused, next is drawn from max(p - q, 0) (where that is
+ *   0 everywhere, from p; draft NULL: from p without the token), and with none
+ *   refused from p of the last row: the least j whose running sum passes u_next[s] times the whole sum.
+ * T <= 0 or NaN: greedy, the draft accepted if it is the row's first maximum,
+ * which is next.  Random numbers are in [0, 1); exponentials and sums run in
+ * 64 bits.  -infinity masks a token, NaN counts as -infinity, +infinity as the
+ * largest float; a drafted token outside 0 .. vocab-1 is refused.
+ * accepted[s]: drafts accepted; next[s]: -1 for a sequence without rows and
+ * where no token has a weight.  prob (may be NULL): f32[ntok], p_r at the
+ * drafted token (greedy: 1 or 0), 0 at a sequence's last row; rows of no
+ * sequence are left as they are.
+ * kind F32, BF16, F16 or Q16; strides in values, any alignment of the type.
+ * ws: vgx_draft_verify_ws bytes of device memory, as vgx_paged_attn's. */
+typedef struct vgx_draft {
+    int nseq, ntok, vocab;
+    const int* qstart;
+    const int* tokens;
+    int kind;
+    const void* logits;
+    int64_t stride;
+    const void* draft;
+    int64_t draft_stride;
+    const float* temp;
+    const float* u_accept;
+    const float* u_next;
+    int* accepted;
+    int* next;
+    float* prob;
+    void* ws;
+    size_t ws_bytes;
+} vgx_draft;
+size_t vgx_draft_verify_ws(int nseq, int ntok, int vocab, int kind, int with_draft);
+int vgx_draft_verify(vgx_ctx* ctx, const vgx_draft* args);
+
 /* ---- LFM2 gated short convolution: replaces GPU::init_conv, set_conv_kernel,
  * conv_block's gate/conv3/gate passes and clear_conv_state
  * (engine/src/gpu_conv.cpp:10-225), between the in_proj GEMV (3*dim rows:

@@ -1,0 +1,562 @@
+// Checking drafted tokens against the target's logits.
+//
+// p_r = softmax(l_r / T) of the target's row r, q_r of the draft's (1 at the
+// drafted token where its logits are not given).  The row's draft t is taken
+// when u q_r(t) < p_r(t); the first row that does not (or the sequence's last
+// row, which has no draft) gives the next token: the least j whose running
+// sum of w passes u' times the sum of all, w = max(p - q, 0) of a refused row
+// and p of the last.  Integers come out, so the exponentials and sums run in
+// 64 bits: a draw next to a border of the running sum has thousands of
+// borders to be wrong at.
+//
+// Launch 1 reads every logit once (a workgroup a row and chunk): the chunk's
+// maximum, its first index and its sum of exponentials.  With draft logits
+// launch 2 sums the chunks of w for the refused rows.  The last launch (a
+// workgroup a sequence) joins the rows' chunks, takes or refuses, finds the
+// chunk the draw falls into from the chunks' sums and the token in it from a
+// scan of that chunk alone.
+//
+// The exponential: e^x = 2^k 2^(i/64) e^r with 64 x / ln 2 = 64 k + i + f,
+// r = f ln 2 / 64, |r| < 0.0055: a table of 64 powers in LDS and a polynomial
+// of degree 5 (error r^6 / 720 < 4e-17); a table lookup instead of a
+// polynomial of degree 11 or more (P. T. P. Tang, ACM TOMS 15, 1989).
+#include <cfloat>
+#include <cmath>
+#include <string>
+
+#include "vgx_internal.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+struct VerifyArgs {
+    int nseq, ntok, vocab;
+    const int* qstart;
+    const int* tokens;
+    const uint8_t* x;
+    const uint8_t* d;     // the draft's logits, or nullptr
+    int64_t xs, ds;       // bytes between rows
+    const float* temp;
+    const float* ua;
+    const float* un;
+    int* accepted;
+    int* next;
+    float* prob;
+    struct Part* px;      // ntok x nch
+    struct Part* pd;
+    double* w;            // nseq x nch: sums of w of the refused rows
+    int nch;
+};
+
+struct Part {
+    float m;   // the chunk's maximum (-inf: nothing)
+    int arg;   // its first index
+    double z;  // sum of exp((x - m) / T)
+};
+
+template <int KIND>
+constexpr int kBytes = KIND == VGX_E_F32 ? 4 : 2;
+template <int KIND>
+constexpr int kPer = 16 / kBytes<KIND>;  // values of a 16-byte piece
+constexpr int kThreads = 256;
+constexpr int kPieces = 4;  // of 16 bytes a thread takes of a chunk
+constexpr int kChunk = kThreads * kPieces;  // pieces of a chunk
+
+// NaN counts as masked (-inf), +inf as the largest float.
+__device__ __forceinline__ float clean(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
+
+template <int KIND>
+__device__ __forceinline__ float one(const uint8_t* p, int i) {
+    if (KIND == VGX_E_F32) return clean(reinterpret_cast<const float*>(p)[i]);
+    const unsigned short u = reinterpret_cast<const unsigned short*>(p)[i];
+    if (KIND == VGX_E_Q16) return (float)(short)u * (1.0f / 256);
+    if (KIND == VGX_E_BF16) return clean(__uint_as_float((unsigned)u << 16));
+    return clean((float)__builtin_bit_cast(_Float16, u));
+}
+
+// A row as 16-byte pieces of the address space: piece g holds values
+// g * per - off .. + per - 1; the ends' pieces are read value by value.
+struct Row {
+    const uint8_t* p;
+    int off;
+};
+template <int KIND>
+__device__ __forceinline__ Row row_at(const uint8_t* x, int64_t stride, int r) {
+    Row q;
+    q.p = x + (int64_t)r * stride;
+    q.off = (int)(((uintptr_t)q.p & 15) / kBytes<KIND>);
+    return q;
+}
+template <int KIND>
+__device__ __forceinline__ void piece(const Row& q, int vocab, int g, float (&x)[kPer<KIND>]) {
+    constexpr int N = kPer<KIND>;
+    const int i0 = g * N - q.off;
+    if (i0 >= 0 && i0 + N <= vocab) {
+        const uint4 v = *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * kBytes<KIND>);
+        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (KIND == VGX_E_F32) {
+                x[i] = clean(__uint_as_float(u[i]));
+            } else if (KIND == VGX_E_Q16) {
+                x[2 * i] = (float)(short)(u[i] & 0xffff) * (1.0f / 256);
+                x[2 * i + 1] = (float)((int)u[i] >> 16) * (1.0f / 256);
+            } else if (KIND == VGX_E_BF16) {
+                x[2 * i] = clean(__uint_as_float(u[i] << 16));
+                x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
+            } else {
+                x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
+                x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = i0 + e >= 0 && i0 + e < vocab ? one<KIND>(q.p, i0 + e) : -INFINITY;
+    }
+}
+
+// 2^(i / 64), written into LDS by every workgroup.
+__device__ __forceinline__ void fill_table(double* t) {
+    for (int i = threadIdx.x; i < 64; i += blockDim.x) t[i] = exp2((double)i * (1.0 / 64));
+}
+// e^x for x <= 0 (0 below about -708: nothing a sum next to 1 would notice).
+__device__ __forceinline__ double exp_neg(double x, const double* tab) {
+    const double y = fmax(x, -745.0);
+    const double big = 6755399441055744.0;  // 1.5 * 2^52: the low bits hold the rounded value
+    const double kb = fma(y, 92.33248261689366, big);  // 64 / ln 2
+    const int n = (int)(unsigned)__builtin_bit_cast(unsigned long long, kb);
+    const double k = kb - big;
+    // ln 2 / 64 in two parts, the first of 31 bits: k times it is exact
+    double r = fma(k, -0.01083042468962958, y);
+    r = fma(k, -6.619564634077006e-12, r);
+    double e = fma(r, 1.0 / 120, 1.0 / 24);
+    e = fma(e, r, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    const double t = tab[n & 63];
+    e = fma(e * r, t, t);
+    return x < -700.0 ? 0.0 : ldexp(e, n >> 6);
+}
+
+struct Temp {
+    double inv;
+    bool greedy;
+};
+__device__ __forceinline__ Temp temp_of(const VerifyArgs& P, int s) {
+    const float t = P.temp ? P.temp[s] : 1.0f;
+    Temp r;
+    r.greedy = !(t > 0.0f);
+    r.inv = r.greedy ? 1.0 : fmin(1.0 / (double)t, 1e30);
+    return r;
+}
+__device__ __forceinline__ double weight(float x, float m, double inv, const double* tab) {
+    return x == -INFINITY ? 0.0 : exp_neg(((double)x - (double)m) * inv, tab);
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+// (value, index): the larger value, the smaller index of equals.
+__device__ __forceinline__ void wave_best(float& m, int& a) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m, o, 64);
+        const int a2 = __shfl_xor(a, o, 64);
+        if (m2 > m || (m2 == m && a2 < a)) { m = m2; a = a2; }
+    }
+}
+// The sequence of row t (every lane active); nseq behind the last.
+__device__ __forceinline__ int seq_of(const VerifyArgs& P, int t) {
+    int s = 0;
+    for (int b = 0; b < P.nseq; b += 64) {
+        const int j = b + (int)(threadIdx.x & 63);
+        s += __popcll(__ballot((j < P.nseq ? P.qstart[j + 1] : 0x7fffffff) <= t));
+    }
+    return s;
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
+    constexpr int N = kPer<KIND>;
+    __shared__ double tab[64], sz[4];
+    __shared__ float sm[4];
+    __shared__ int sa[4];
+    const int chunk = blockIdx.x, t = blockIdx.y;
+    const bool draft = blockIdx.z;
+    const int s = seq_of(P, t);
+    fill_table(tab);
+    if (s >= P.nseq) return;  // (uniform)
+    const Temp T = temp_of(P, s);
+    const Row q = row_at<KIND>(draft ? P.d : P.x, draft ? P.ds : P.xs, t);
+    float x[kPieces][N];
+    float m = -INFINITY;
+    int a = 0x7fffffff;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) piece<KIND>(q, P.vocab, chunk * kChunk + k * kThreads + threadIdx.x, x[k]);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (x[k][e] > m) {
+                m = x[k][e];
+                a = (chunk * kChunk + k * kThreads + (int)threadIdx.x) * N - q.off + e;
+            }
+    wave_best(m, a);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) { sm[wave] = m; sa[wave] = a; }
+    __syncthreads();
+    m = sm[0];
+    a = sa[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+        if (sm[w] > m || (sm[w] == m && sa[w] < a)) { m = sm[w]; a = sa[w]; }
+    double z = 0.0;
+    if (!T.greedy && m != -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) z += weight(x[k][e], m, T.inv, tab);
+    }
+    z = wave_sum(z);
+    if ((threadIdx.x & 63) == 0) sz[wave] = z;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Part r;
+        r.m = m;
+        r.arg = a;
+        r.z = sz[0] + sz[1] + sz[2] + sz[3];
+        (draft ? P.pd : P.px)[(int64_t)t * P.nch + chunk] = r;
+    }
+}
+
+// A row's chunks joined by one wave: its maximum, first index and sum.
+__device__ __forceinline__ Part join(const VerifyArgs& P, const Part* parts, int t, double inv, const double* tab) {
+    const int lane = threadIdx.x & 63;
+    const Part* p = parts + (int64_t)t * P.nch;
+    float m = -INFINITY;
+    int a = 0x7fffffff;
+    for (int c = lane; c < P.nch; c += 64) {
+        if (p[c].m > m || (p[c].m == m && p[c].arg < a)) { m = p[c].m; a = p[c].arg; }
+    }
+    wave_best(m, a);
+    double z = 0.0;
+    for (int c = lane; c < P.nch; c += 64) z += p[c].z * weight(p[c].m, m, inv, tab);
+    Part r;
+    r.m = m;
+    r.arg = a;
+    r.z = wave_sum(z);
+    return r;
+}
+
+// What a sequence's rows decide: the first row that refuses its draft (the
+// last row where none does), by every thread of the workgroup.
+struct Decision {
+    int q0, n, acc;
+    bool refused;
+};
+template <int KIND>
+__device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Temp& T, const double* tab, int* first,
+                                           bool write) {
+    Decision r;
+    r.q0 = min(max(P.qstart[s], 0), P.ntok);
+    r.n = max(min(P.qstart[s + 1], P.ntok) - r.q0, 0);
+    if (threadIdx.x == 0) *first = r.n - 1;
+    __syncthreads();
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int i = wave; i < r.n; i += waves) {
+        const int t = r.q0 + i;
+        if (i == r.n - 1) {
+            if (write && P.prob && (threadIdx.x & 63) == 0) P.prob[t] = 0.0f;
+            continue;
+        }
+        const int tok = P.tokens[t + 1];
+        const bool in = tok >= 0 && tok < P.vocab;
+        const Part x = join(P, P.px, t, T.inv, tab);
+        double pr, qr = 1.0;
+        if (T.greedy) {
+            pr = x.m != -INFINITY && tok == x.arg ? 1.0 : 0.0;
+        } else {
+            pr = in && x.z > 0.0 ? weight(one<KIND>(P.x + (int64_t)t * P.xs, in ? tok : 0), x.m, T.inv, tab) / x.z : 0.0;
+            if (P.d) {
+                const Part d = join(P, P.pd, t, T.inv, tab);
+                qr = in && d.z > 0.0 ? weight(one<KIND>(P.d + (int64_t)t * P.ds, in ? tok : 0), d.m, T.inv, tab) / d.z
+                                     : 0.0;
+            }
+        }
+        const bool ok = T.greedy ? pr > 0.0 : (double)P.ua[t] * qr < pr;
+        if ((threadIdx.x & 63) == 0) {
+            if (!ok) atomicMin(first, i);
+            if (write && P.prob) P.prob[t] = (float)pr;
+        }
+    }
+    __syncthreads();
+    r.acc = *first;
+    r.refused = r.acc < r.n - 1;
+    return r;
+}
+
+// w of one value of the refused row t.
+struct Residual {
+    float mx, md;
+    double zx, zd, inv;
+    int tok;  // without draft logits: the refused token
+};
+__device__ __forceinline__ double residual(const Residual& R, bool draft, float x, float d, int j, const double* tab) {
+    const double p = weight(x, R.mx, R.inv, tab) * R.zx;
+    if (!draft) return j == R.tok ? 0.0 : p;
+    return fmax(p - weight(d, R.md, R.inv, tab) * R.zd, 0.0);
+}
+
+// With draft logits: the sums of w over the chunks of the refused rows.
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) residual_kernel(const VerifyArgs P) {
+    constexpr int N = kPer<KIND>;
+    __shared__ double tab[64], sz[4];
+    __shared__ int first;
+    const int chunk = blockIdx.x, s = blockIdx.y;
+    fill_table(tab);
+    const Temp T = temp_of(P, s);
+    const Decision D = decide<KIND>(P, s, T, tab, &first, false);
+    if (!D.refused || T.greedy) return;
+    const int t = D.q0 + D.acc;
+    const Part x = join(P, P.px, t, T.inv, tab), d = join(P, P.pd, t, T.inv, tab);
+    const Residual R{x.m, d.m, x.z > 0.0 ? 1.0 / x.z : 0.0, d.z > 0.0 ? 1.0 / d.z : 0.0, T.inv, -1};
+    const Row qx = row_at<KIND>(P.x, P.xs, t), qd = row_at<KIND>(P.d, P.ds, t);
+    double w = 0.0;
+    for (int k = 0; k < kPieces; ++k) {
+        const int g = chunk * kChunk + k * kThreads + threadIdx.x;
+        float a[N], b[N];
+        piece<KIND>(qx, P.vocab, g, a);
+        if (qx.off == qd.off) {
+            piece<KIND>(qd, P.vocab, g, b);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int j = g * N - qx.off + e;
+                b[e] = j >= 0 && j < P.vocab ? one<KIND>(qd.p, j) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) w += residual(R, true, a[e], b[e], 0, tab);
+    }
+    w = wave_sum(w);
+    if ((threadIdx.x & 63) == 0) sz[threadIdx.x >> 6] = w;
+    __syncthreads();
+    if (threadIdx.x == 0) P.w[(int64_t)s * P.nch + chunk] = sz[0] + sz[1] + sz[2] + sz[3];
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) pick_kernel(const VerifyArgs P) {
+    constexpr int N = kPer<KIND>;
+    __shared__ double tab[64], sw[4], left;
+    __shared__ int first, chosen, found, last, plain;
+    const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    fill_table(tab);
+    const Temp T = temp_of(P, s);
+    const Decision D = decide<KIND>(P, s, T, tab, &first, true);
+    if (D.n <= 0) {
+        if (threadIdx.x == 0) { P.accepted[s] = 0; P.next[s] = -1; }
+        return;
+    }
+    const int t = D.q0 + D.acc;
+    const Part x = join(P, P.px, t, T.inv, tab);
+    if (threadIdx.x == 0) P.accepted[s] = D.acc;
+    if (T.greedy || x.m == -INFINITY) {
+        if (threadIdx.x == 0) P.next[s] = x.m == -INFINITY ? -1 : x.arg;
+        return;
+    }
+    bool draft = P.d && D.refused;
+    Part d{};
+    if (draft) d = join(P, P.pd, t, T.inv, tab);
+    const Residual R{x.m, d.m, 1.0 / x.z, d.z > 0.0 ? 1.0 / d.z : 0.0, T.inv, D.refused && !P.d ? P.tokens[t + 1] : -1};
+    const Row qx = row_at<KIND>(P.x, P.xs, t);
+    // the chunks' sums, walked by one wave; without draft logits they are
+    // launch 1's, less the refused token
+    const int tchunk = R.tok >= 0 && R.tok < P.vocab ? (R.tok + qx.off) / N / kChunk : -1;
+    if (wave == 0) {
+        auto sum_of = [&](int c) {
+            if (c >= P.nch) return 0.0;
+            if (draft) return P.w[(int64_t)s * P.nch + c];
+            const Part p = P.px[(int64_t)t * P.nch + c];
+            double z = p.z;
+            if (c == tchunk) z = fmax(z - weight(one<KIND>(qx.p, R.tok), p.m, T.inv, tab), 0.0);
+            return z * weight(p.m, x.m, T.inv, tab) * R.zx;
+        };
+        double total = 0.0;
+        for (int c = 0; c < P.nch; c += 64) total += sum_of(c + lane);
+        total = wave_sum(total);
+        if (lane == 0) plain = 0;
+        if (draft && !(total > 0.0)) {  // p = q: the draw is from p
+            draft = false;
+            if (lane == 0) plain = 1;
+            total = 0.0;
+            for (int c = 0; c < P.nch; c += 64) total += sum_of(c + lane);
+            total = wave_sum(total);
+        }
+        const double want = (double)P.un[s] * total;
+        double before = 0.0;
+        int pick = -1, some = -1;
+        double at = 0.0, some_at = 0.0;
+        for (int c = 0; c < P.nch && pick < 0; c += 64) {
+            const double v = sum_of(c + lane);
+            double run = v;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double y = __shfl_up(run, o, 64);
+                if (lane >= o) run += y;
+            }
+            const unsigned long long past = __ballot(before + run > want && v > 0.0);
+            const unsigned long long any = __ballot(v > 0.0);
+            if (past) {
+                const int l = __ffsll((unsigned long long)past) - 1;
+                pick = c + l;
+                at = before + __shfl(run, l, 64) - __shfl(v, l, 64);
+            } else if (any) {
+                const int l = 63 - __clzll((long long)any);
+                some = c + l;
+                some_at = before + __shfl(run, l, 64) - __shfl(v, l, 64);
+            }
+            before += __shfl(run, 63, 64);
+        }
+        if (lane == 0) {
+            chosen = pick >= 0 ? pick : some;
+            left = fmax(want - (pick >= 0 ? at : some_at), 0.0);
+            found = 0x7fffffff;
+            last = -1;
+        }
+    }
+    __syncthreads();
+    if (plain) draft = false;
+    if (chosen < 0) {  // nothing but the refused token has a weight
+        if (threadIdx.x == 0) P.next[s] = -1;
+        return;
+    }
+    // the chosen chunk, kPieces consecutive pieces a thread
+    const Row qd = draft ? row_at<KIND>(P.d, P.ds, t) : qx;
+    const int g0 = chosen * kChunk + threadIdx.x * kPieces;
+    double w[kPieces * N];
+    double sum = 0.0;
+    int mine = -1;  // the thread's last value with a weight
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+        float a[N], b[N];
+        piece<KIND>(qx, P.vocab, g0 + k, a);
+        if (draft) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int j = (g0 + k) * N - qx.off + e;
+                b[e] = j >= 0 && j < P.vocab ? one<KIND>(qd.p, j) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int j = (g0 + k) * N - qx.off + e;
+            w[k * N + e] = residual(R, draft, a[e], draft ? b[e] : 0.0f, j, tab);
+            sum += w[k * N + e];
+            if (w[k * N + e] > 0.0) mine = j;
+        }
+    }
+    double run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(run, o, 64);
+        if (lane >= o) run += y;
+    }
+    if (lane == 63) sw[wave] = run;
+    if (mine >= 0) atomicMax(&last, mine);
+    __syncthreads();
+    // before: the inclusive sum of the thread before this one, to the bit, so
+    // one thread's interval holds the draw
+    double before = __shfl_up(run, 1, 64);
+    if (lane == 0) before = 0.0;
+    double base = 0.0;
+    for (int v = 0; v < wave; ++v) base += sw[v];
+    before += base;
+    if (before <= left && base + run > left) {
+        int hit = -1;
+        double u = before;
+#pragma unroll
+        for (int i = 0; i < kPieces * N; ++i) {
+            u += w[i];
+            if (hit < 0 && u > left && w[i] > 0.0) hit = (g0 + i / N) * N - qx.off + i % N;
+        }
+        atomicMin(&found, hit >= 0 ? hit : mine);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) P.next[s] = found != 0x7fffffff ? found : last;
+}
+
+int chunks_of(int vocab, int kind) {
+    const int per = kind == VGX_E_F32 ? 4 : 8;
+    // (a row may begin inside a piece)
+    return (vocab + per - 1 + per * kChunk - 1) / (per * kChunk);
+}
+
+template <int KIND>
+void launch(const VerifyArgs& P, hipStream_t st) {
+    if (P.ntok) {
+        hipLaunchKernelGGL(stats_kernel<KIND>, dim3(P.nch, P.ntok, P.d ? 2 : 1), dim3(kThreads), 0, st, P);
+        if (P.d) hipLaunchKernelGGL(residual_kernel<KIND>, dim3(P.nch, P.nseq), dim3(kThreads), 0, st, P);
+    }
+    hipLaunchKernelGGL(pick_kernel<KIND>, dim3(P.nseq), dim3(kThreads), 0, st, P);
+}
+
+bool kind_ok(int k) { return k == VGX_E_F32 || k == VGX_E_BF16 || k == VGX_E_F16 || k == VGX_E_Q16; }
+
+}  // namespace
+
+extern "C" {
+
+size_t vgx_draft_verify_ws(int nseq, int ntok, int vocab, int kind, int with_draft) {
+    if (nseq < 0 || ntok < 0 || vocab <= 0 || vocab > (1 << 26) || !kind_ok(kind)) return 0;
+    const size_t nch = chunks_of(vocab, kind);
+    return nch * ((size_t)ntok * (with_draft ? 2 : 1) * sizeof(Part) + (size_t)(with_draft ? nseq : 0) * sizeof(double));
+}
+
+int vgx_draft_verify(vgx_ctx* ctx, const vgx_draft* a) {
+    if (!a) return vgx_fail(VGX_EINVAL, "vgx_draft_verify: NULL arguments");
+    if (a->nseq < 0 || a->ntok < 0 || a->nseq > 65535 || a->ntok > 65535)
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: nseq or ntok outside 0..65535");
+    if (a->vocab <= 0 || a->vocab > (1 << 26)) return vgx_fail(VGX_EINVAL, "vgx_draft_verify: vocab outside 1..2^26");
+    if (!kind_ok(a->kind)) return vgx_fail(VGX_EINVAL, "vgx_draft_verify: logits are f32, bf16, f16 or q16");
+    if (a->nseq && (!a->qstart || !a->accepted || !a->next || !a->u_next))
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: NULL qstart, u_next or output");
+    if (a->nseq && a->ntok && (!a->logits || !a->tokens || !a->u_accept))
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: NULL logits, tokens or u_accept");
+    const int eb = a->kind == VGX_E_F32 ? 4 : 2;
+    if (a->stride < a->vocab || (a->draft && a->draft_stride < a->vocab))
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: a row stride below vocab");
+    if (((uintptr_t)a->logits | (uintptr_t)a->draft) & (eb - 1))
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: logits not aligned to their type");
+    const size_t need = vgx_draft_verify_ws(a->nseq, a->ntok, a->vocab, a->kind, a->draft != nullptr);
+    if (a->nseq && need && (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 15)))
+        return vgx_fail(VGX_EINVAL, "vgx_draft_verify: the workspace is missing, too small or not 16-byte aligned");
+    if (!ctx) return vgx_fail(VGX_EINVAL, "vgx_draft_verify: no context");
+    if (a->nseq == 0) return VGX_OK;
+    VerifyArgs P{};
+    P.nseq = a->nseq; P.ntok = a->ntok; P.vocab = a->vocab;
+    P.qstart = a->qstart; P.tokens = a->tokens;
+    P.x = static_cast<const uint8_t*>(a->logits);
+    P.d = static_cast<const uint8_t*>(a->draft);
+    P.xs = a->stride * eb; P.ds = a->draft_stride * eb;
+    P.temp = a->temp; P.ua = a->u_accept; P.un = a->u_next;
+    P.accepted = a->accepted; P.next = a->next; P.prob = a->prob;
+    P.nch = chunks_of(a->vocab, a->kind);
+    P.px = static_cast<Part*>(a->ws);
+    P.pd = P.px + (size_t)a->ntok * P.nch;
+    P.w = reinterpret_cast<double*>(P.pd + (a->draft ? (size_t)a->ntok * P.nch : 0));
+    VGX_HIP(hipSetDevice(ctx->device));
+    switch (a->kind) {
+        case VGX_E_F32: launch<VGX_E_F32>(P, ctx->stream); break;
+        case VGX_E_BF16: launch<VGX_E_BF16>(P, ctx->stream); break;
+        case VGX_E_F16: launch<VGX_E_F16>(P, ctx->stream); break;
+        default: launch<VGX_E_Q16>(P, ctx->stream); break;
+    }
+    VGX_LAUNCH_CHECK("draft verify launch");
+    return VGX_OK;
+}
+
+}  // extern "C"

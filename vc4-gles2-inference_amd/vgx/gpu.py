@@ -599,6 +599,45 @@ class GPU:
     def paged_cache(self, heads, kv_heads, head_dim, kind, k, v, k_step=0.0, v_step=0.0):
         return PagedCache(self, heads, kv_heads, head_dim, kind, k, v, k_step, v_step)
 
+    def draft_verify(self, qstart, tokens, logits, u_accept, u_next, draft=None, temp=None):
+        """Drafted tokens against the target's logits (rows, vocab; float32,
+        bfloat16, float16 or q16): tokens[r + 1] against row r of its sequence
+        (rows qstart[s] .. qstart[s+1]-1).  draft: the logits the drafts were
+        drawn from; temp: a temperature a sequence (0: greedy).  Returns
+        (accepted drafts and next token of each sequence, the target's
+        probability of each drafted token)."""
+        self.need(qstart, torch.int32, 1, "qstart")
+        self.need(tokens, torch.int32, 1, "tokens")
+        nseq, n = qstart.shape[0] - 1, tokens.shape[0]
+        if nseq < 0:
+            raise ValueError("qstart must hold at least one entry")
+        if logits.dim() != 2 or logits.dtype not in _ELEM:
+            raise ValueError("logits must be rows of float32, bfloat16, float16 or int16 (q16)")
+        vocab = logits.shape[1]
+        for t, name in ((logits, "logits"), (draft, "draft")):
+            if t is not None:
+                self.need_rows(t, logits.dtype, n, vocab, name)
+        for t, size, name in ((u_accept, n, "u_accept"), (u_next, nseq, "u_next"), (temp, nseq, "temp")):
+            if t is not None:
+                self.need(t, torch.float32, 1, name)
+                if t.shape[0] != size:
+                    raise ValueError("%s must be %d values" % (name, size))
+        for t in (qstart, tokens, u_accept, u_next, temp):
+            if t is not None and t.numel() > 1 and t.stride(0) != 1:
+                raise ValueError("qstart, tokens, the random numbers and temp must be contiguous")
+        L, kind = _l.load(), _ELEM[logits.dtype]
+        acc_next = torch.empty((2, nseq), dtype=torch.int32, device=self.device)
+        # rows of no sequence keep a probability of 0
+        prob = torch.zeros(n, dtype=torch.float32, device=self.device)
+        need = int(L.vgx_draft_verify_ws(nseq, n, vocab, kind, int(draft is not None)))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        a = _l.Draft(nseq, n, vocab, qstart.data_ptr(), tokens.data_ptr(), kind, logits.data_ptr(),
+                     max(logits.stride(0), vocab), _at(draft), 0 if draft is None else max(draft.stride(0), vocab),
+                     _at(temp), u_accept.data_ptr(), u_next.data_ptr(), acc_next.data_ptr(),
+                     acc_next.data_ptr() + 4 * nseq, prob.data_ptr(), ws.data_ptr(), need)
+        self.on_current(L.vgx_draft_verify, ctypes.byref(a))
+        return acc_next[0], acc_next[1], prob
+
     def conv(self, w, layer_is_conv=None):
         return Conv(self, w, layer_is_conv)
 

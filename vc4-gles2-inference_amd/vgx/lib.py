@@ -69,6 +69,13 @@ class PagedQuery(ctypes.Structure):
                 ("out", _P), ("out_stride", _I64), ("lse", _P), ("ws", _P), ("ws_bytes", ctypes.c_size_t)]
 
 
+class Draft(ctypes.Structure):
+    _fields_ = [("nseq", _I), ("ntok", _I), ("vocab", _I), ("qstart", _P), ("tokens", _P), ("kind", _I),
+                ("logits", _P), ("stride", _I64), ("draft", _P), ("draft_stride", _I64), ("temp", _P),
+                ("u_accept", _P), ("u_next", _P), ("accepted", _P), ("next", _P), ("prob", _P), ("ws", _P),
+                ("ws_bytes", ctypes.c_size_t)]
+
+
 _SIGS = {
     "vgx_abi_version": (_I, []),
     "vgx_strerror": (ctypes.c_char_p, [_I]),
@@ -141,6 +148,8 @@ _SIGS = {
     "vgx_paged_append": (_I, [_P, _P, _P, _P]),
     "vgx_paged_attn_ws": (ctypes.c_size_t, [_P, _P, _P, _I]),
     "vgx_paged_attn": (_I, [_P, _P, _P, _P]),
+    "vgx_draft_verify_ws": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
+    "vgx_draft_verify": (_I, [_P, _P]),
     "vgx_quantize_act": (None, [_P, _I, _P]),
     "vgx_x_pack_i16_2": (None, [_P, _I, _P]),
 }
