@@ -26,6 +26,7 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -63,6 +64,15 @@ __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
                                                       0, 0);
 }
 template <int CK>
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
+    if constexpr (CK == VGX_E_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+template <int CK>
 __device__ __forceinline__ short to_ct(float x) {
     if constexpr (CK == VGX_E_BF16) return __builtin_bit_cast(short, (bf16_t)x);
     else return __builtin_bit_cast(short, (f16_t)x);
@@ -84,11 +94,29 @@ __device__ __forceinline__ uint2 q8_to_f16(unsigned w) {
     r.y = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, b) + off);
     return r;
 }
-// Whether a word of two 16-bit floats holds an infinity or NaN.
+// Infinities and NaN among V.  Where a row does not see a key its weight is 0,
+// but 0 * inf would reach it through the product, so tiles that some row does
+// not wholly see go into LDS with these set to 0 (the main loop stays free of
+// a second path, whose copies of the sums cost it up to 200 registers); if
+// there were any, a pass after the loop adds them to the rows that do see
+// them: a weight times an infinity or NaN is that value.
 template <int CK>
-__device__ __forceinline__ bool odd16(unsigned w) {
-    constexpr unsigned e = CK == VGX_E_BF16 ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || (w & (e << 16)) == (e << 16);
+__device__ __forceinline__ bool odd1(unsigned short x) {
+    constexpr unsigned short e = CK == VGX_E_BF16 ? 0x7f80u : 0x7c00u;
+    return (x & e) == e;
+}
+template <int CK>
+__device__ __forceinline__ bool clear_odd(unsigned& w) {
+    const bool lo = odd1<CK>((unsigned short)w), hi = odd1<CK>((unsigned short)(w >> 16));
+    w = (lo ? 0 : w & 0xffffu) | (hi ? 0 : w & 0xffff0000u);
+    return lo || hi;
+}
+template <int CK>
+__device__ __forceinline__ bool clear_odd(uint4& w) {
+    bool r = clear_odd<CK>(w.x);
+    r = clear_odd<CK>(w.y) || r;
+    r = clear_odd<CK>(w.z) || r;
+    return clear_odd<CK>(w.w) || r;
 }
 // LDS written by the wave's lanes, then read by others of the same wave.
 __device__ __forceinline__ void wave_sync() {
@@ -117,21 +145,25 @@ struct Geo {
 };
 static_assert(Geo<64>::pv == 192 && Geo<96>::pv == 192 && Geo<128>::pv == 320 && Geo<256>::pv == 576, "");
 
-// Staging of ROWS keys by THREADS threads: NL 16-byte pieces a thread of K and
-// as many of V.  Lane r of a wave holds the page of row r % ROWS.
-template <int KIND, int HD, bool EX, int ROWS, int THREADS>
+// Staging of a tile of 64 keys by a workgroup of 4 waves: wave w takes rows
+// 16 w .. 16 w + 15, NL 16-byte pieces a lane of K and as many of V.  Pages
+// whose size is a multiple of 16 (uni) give the wave one scalar address and
+// every lane an offset that stays; others are looked up row by row (lane r
+// holds the page of row r % 16).
+template <int KIND, int HD, bool EX>
 struct Stage {
     static constexpr int CK = KIND == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16;
     static constexpr int EB = KIND == VGX_E_Q8 ? 1 : 2;
     static constexpr int CPR = HD * EB / 16;  // pieces of a row
-    static constexpr int NL = (ROWS * CPR + THREADS - 1) / THREADS;
+    static constexpr int NL = (16 * CPR + 63) / 64;
+    static constexpr bool kAll = NL * 64 == 16 * CPR;
     uint4 k[NL], v[NL];
 
-    // The page of row j0 + lane % ROWS (the last row before `end` stands in
-    // for those behind); a page outside the pool counts as page 0, with the
+    // The page of row j0 + 16 w + lane % 16 (the last row before `end` stands
+    // in for those behind); a page outside the pool counts as page 0, with the
     // fault recorded.
     static __device__ __forceinline__ int page(const PagedDev& A, const int* tab, int j0, int end) {
-        const int j = min(j0 + (int)(threadIdx.x & (ROWS - 1)), end - 1);
+        const int j = min(j0 + 16 * (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 15), end - 1);
         int pg = tab[page_of(A, j)];
         if (pg < 0 || pg >= A.npages) {
             set_fault(A, VGX_FAULT_PAGE);
@@ -139,40 +171,37 @@ struct Stage {
         }
         return pg;
     }
-    // One of K and V (VALUE): a V row behind the end is zeros, whatever the
-    // page holds there; a K row there is the last one again (its scores are
-    // masked).
-    template <bool VALUE>
-    static __device__ __forceinline__ void load1(const PagedDev& A, const uint8_t* base, int pg, int j0, int end,
-                                                 int tid, uint4 (&w)[NL]) {
-        const int64_t ps = VALUE ? A.vpg : A.kpg, rs = VALUE ? A.vrow : A.krow;
+    // One of K and V; rows behind the end are whatever is there.
+    static __device__ __forceinline__ void load1(const PagedDev& A, const uint8_t* base, int64_t ps, int64_t rs, int pg,
+                                                 int j0, int end, bool uni, uint4 (&w)[NL]) {
+        const int lane = threadIdx.x & 63, jw = j0 + 16 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint8_t* sbase = base;
+        if (uni) {
+            const int j = min(jw, (end - 1) & ~15);
+            const int slot = j - page_of(A, j) * A.psize;
+            sbase += (int64_t)__builtin_amdgcn_readfirstlane(pg) * ps + (int64_t)slot * rs;
+        }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int sl = i * THREADS + tid;
-            const int row = sl / CPR, ch = sl - row * CPR;
-            const int p = __shfl(pg, row & (ROWS - 1), 64);
-            const bool use = (NL * THREADS == ROWS * CPR || row < ROWS) && (EX || ch * 16 < A.hd * EB);
-            const int j = min(j0 + row, end - 1);
-            const int slot = j - page_of(A, j) * A.psize;
+            const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
             w[i] = make_uint4(0, 0, 0, 0);
-            if (use && (!VALUE || j0 + row < end))
-                w[i] = *reinterpret_cast<const uint4*>(base + (int64_t)p * ps + (int64_t)slot * rs + ch * 16);
+            if ((!kAll && row >= 16) || (!EX && ch * 16 >= A.hd * EB)) continue;
+            const uint8_t* p;
+            if (uni) {
+                p = sbase + (unsigned)(row * (int)rs + ch * 16);
+            } else {
+                const int j = min(jw + row, end - 1);
+                const int slot = j - page_of(A, j) * A.psize;
+                p = base + (int64_t)__shfl(pg, row, 64) * ps + (int64_t)slot * rs + ch * 16;
+            }
+            w[i] = *reinterpret_cast<const uint4*>(p);
         }
     }
     __device__ __forceinline__ void load(const PagedDev& A, const uint8_t* kh, const uint8_t* vh, int pg, int j0,
-                                         int end, int tid) {
-        load1<false>(A, kh, pg, j0, end, tid, k);
-        load1<true>(A, vh, pg, j0, end, tid, v);
+                                         int end, bool uni) {
+        load1(A, kh, A.kpg, A.krow, pg, j0, end, uni, k);
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, v);
     }
-    static __device__ __forceinline__ bool odd1(const uint4 (&w)[NL]) {
-        bool r = false;
-        if (KIND != VGX_E_Q8)
-#pragma unroll
-            for (int i = 0; i < NL; ++i)
-                r = r || odd16<CK>(w[i].x) || odd16<CK>(w[i].y) || odd16<CK>(w[i].z) || odd16<CK>(w[i].w);
-        return r;
-    }
-    __device__ __forceinline__ bool odd() const { return odd1(v); }
     static __device__ __forceinline__ void put(uint8_t* p, const uint4& w) {
         if (KIND == VGX_E_Q8) {
             const uint2 a = q8_to_f16(w.x), b = q8_to_f16(w.y), c = q8_to_f16(w.z), d = q8_to_f16(w.w);
@@ -182,30 +211,78 @@ struct Stage {
             *reinterpret_cast<uint4*>(p) = w;
         }
     }
-    static __device__ __forceinline__ void store1(uint8_t* l, int pitch, int tid, const uint4 (&w)[NL]) {
+    static __device__ __forceinline__ void store1(uint8_t* l, int pitch, const uint4 (&w)[NL]) {
+        const int lane = threadIdx.x & 63;
+        l += 16 * (threadIdx.x >> 6) * pitch;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int sl = i * THREADS + tid;
-            const int row = sl / CPR, ch = sl - row * CPR;
-            if (NL * THREADS == ROWS * CPR || row < ROWS) put(l + row * pitch + ch * (32 / EB), w[i]);
+            const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
+            if (kAll || row < 16) put(l + row * pitch + ch * (32 / EB), w[i]);
         }
     }
-    __device__ __forceinline__ void store(uint8_t* lk, uint8_t* lv, int tid) const {
-        store1(lk, Geo<HD>::pk, tid, k);
-        store1(lv, Geo<HD>::pv, tid, v);
+    // V rows at or behind the tile's `left`-th become zeros, whatever the page
+    // holds there.
+    static __device__ __forceinline__ void cut(uint4 (&w)[NL], int left) {
+        const int lane = threadIdx.x & 63, r0 = 16 * (threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (r0 + (i * 64 + lane) / CPR >= left) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    static __device__ __forceinline__ bool clean(uint4 (&w)[NL]) {
+        bool r = false;
+        if (KIND != VGX_E_Q8)
+#pragma unroll
+            for (int i = 0; i < NL; ++i) r = clear_odd<CK>(w[i]) || r;
+        return r;
+    }
+    // The loaded tile into LDS; wide: with V cut and cleaned.  Whether there
+    // was something to clean.
+    __device__ __forceinline__ bool store(uint8_t* lk, uint8_t* lv, int left, bool wide) {
+        bool r = false;
+        store1(lk, Geo<HD>::pk, k);
+        if (wide) {
+            cut(v, left);
+            r = clean(v);
+        }
+        store1(lv, Geo<HD>::pv, v);
+        return r;
     }
     // Load and store in one go, K then V through the same registers (heads of
-    // more than 128 values leave none for a tile ahead); V's odd() comes back.
+    // more than 128 values leave none for a tile ahead).
     static __device__ __forceinline__ bool fetch(const PagedDev& A, const uint8_t* kh, const uint8_t* vh, int pg,
-                                                 int j0, int end, int tid, uint8_t* lk, uint8_t* lv) {
+                                                 int j0, int end, bool uni, uint8_t* lk, uint8_t* lv, bool wide) {
         uint4 w[NL];
-        load1<false>(A, kh, pg, j0, end, tid, w);
-        store1(lk, Geo<HD>::pk, tid, w);
-        load1<true>(A, vh, pg, j0, end, tid, w);
-        store1(lv, Geo<HD>::pv, tid, w);
-        return odd1(w);
+        bool r = false;
+        load1(A, kh, A.kpg, A.krow, pg, j0, end, uni, w);
+        store1(lk, Geo<HD>::pk, w);
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, w);
+        if (wide) {
+            cut(w, end - j0);
+            r = clean(w);
+        }
+        store1(lv, Geo<HD>::pv, w);
+        return r;
+    }
+    static __device__ __forceinline__ void fetch_v(const PagedDev& A, const uint8_t* vh, int pg, int j0, int end,
+                                                   bool uni, uint8_t* lv) {
+        uint4 w[NL];
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, w);
+        cut(w, end - j0);
+        store1(lv, Geo<HD>::pv, w);
     }
 };
+
+// What the main loop left out of four sums of a column: the infinities and
+// NaN of keys lo .. hi-1 of a tile in LDS (p: the first key's four values).
+template <int CK>
+__device__ __forceinline__ void add_odd(float (&x)[4], const uint8_t* p, int pitch, int lo, int hi) {
+    for (int r = lo; r < hi; ++r) {
+        const s16x4 w = *reinterpret_cast<const s16x4*>(p + r * pitch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (odd1<CK>((unsigned short)w[e])) x[e] += from_ct<CK>(w[e]);
+    }
+}
 
 // The running state of a wave's 32 columns.
 template <int HD>
@@ -238,14 +315,10 @@ __device__ __forceinline__ void load_q(const PagedDev& A, const uint8_t* qp, boo
 
 // One step over 32 * KB keys in LDS (lk, lv: the first row), the first of them
 // key j0.  mask: some column does not see some key; vlo <= key < vhi are the
-// lane's column's.  odd: an infinity or NaN among V (checked where mask is
-// set): 0 * inf would reach the rows that do not see it, so the weighted sum
-// then runs key by key over the visible ones (lp: a free LDS area of 4 KB
-// a wave).
+// lane's column's.
 template <int CK, int HD, bool EX, int KB>
 __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16], Acc<HD>& a, const uint8_t* lk,
-                                     const uint8_t* lv, int j0, float c, bool mask, int vlo, int vhi, bool odd,
-                                     float* lp) {
+                                     const uint8_t* lv, int j0, float c, bool mask, int vlo, int vhi) {
     const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
     f32x16 s[KB];
 #pragma unroll
@@ -273,11 +346,22 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = fmaxf(half_max(mx), a.m);
+    mx = half_max(mx);
+    // The reference value m is any that keeps the weights in range: it moves,
+    // and the sums with it, only when some column's maximum has passed its m by
+    // 2^6 (a weight then stays below 64, exact in no fewer bits).
+    if (__any(mx * c > fmaf(a.m, c, 6.0f))) {
+        const float m2 = fmaxf(mx, a.m);
+        const float alpha = exp2_((a.m - (m2 == -INFINITY ? 0.0f : m2)) * c);
+        a.m = m2;
+        a.l *= alpha;
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a.o[b][i] *= alpha;
+    }
     // (no key yet: subtract 0, so the exponents stay -inf and the weights 0)
-    const float mc = (mx == -INFINITY ? 0.0f : mx) * c;
-    const float alpha = exp2_(fmaf(a.m, c, -mc));
-    a.m = mx;
+    const float mc = (a.m == -INFINITY ? 0.0f : a.m) * c;
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -286,42 +370,7 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
             s[kb][i] = exp2_(fmaf(s[kb][i], c, -mc));
             sum += s[kb][i];
         }
-    a.l = fmaf(a.l, alpha, sum);
-#pragma unroll
-    for (int b = 0; b < HD / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) a.o[b][i] *= alpha;
-    if (odd) {
-#pragma unroll 1
-        for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float p = s[0][i];
-#pragma unroll
-                for (int u = 1; u < KB; ++u) p = kb == u ? s[u][i] : p;
-                lp[(8 * (i / 4) + 4 * h + (i & 3)) * 32 + col] = p;
-            }
-            wave_sync();
-            for (int r = 0; r < 32; ++r) {
-                const int j = j0 + kb * 32 + r;
-                const float p = lp[r * 32 + col];
-                if (j >= vlo && j < vhi) {
-#pragma unroll
-                    for (int b = 0; b < HD / 32; ++b)
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const s16x4 w = *reinterpret_cast<const s16x4*>(lv + (kb * 32 + r) * Geo<HD>::pv +
-                                                                            (32 * b + 8 * g + 4 * h) * 2);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                a.o[b][4 * g + e] = fmaf(p, from_ct<CK>(w[e]), a.o[b][4 * g + e]);
-                        }
-                }
-            }
-            wave_sync();
-        }
-        return;
-    }
+    a.l += sum;
     // lane 16 g + i's address: key row i / 4 of the half, dims 16 (g & 1) + 4 (i & 3)
     const int i16 = lane & 15;
     const uint8_t* vb = lv + (4 * h + (i16 >> 2)) * Geo<HD>::pv + (16 * ((lane >> 4) & 1) + 4 * (i16 & 3)) * 2;
@@ -390,19 +439,170 @@ __device__ __forceinline__ Col col_of(const AttnArgs& P, const SeqAt& q, int h, 
     return r;
 }
 
-// Few rows a sequence (max_q * grp <= 32): a workgroup is one sequence, KV
-// head and split; its 4 waves hold the same 32 columns and take tiles of 32
-// keys in turn, each through LDS of its own without a barrier, and join at
-// the end.
+// max / sum over the four lanes that hold a column (lane % 16).
+__device__ __forceinline__ float quad_max(float x) {
+    x = half_max(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x = half_sum(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A wave's tile of 32 keys on its way: K as the pieces its lanes multiply (key
+// lane % 16 of each half, 16 bytes from byte 64 T + 16 (lane / 16) of the
+// row), V as pieces of rows for LDS.  Pages whose size is a multiple of 16
+// (uni) give each half one scalar address and every lane an offset that stays;
+// others are looked up row by row.
 template <int KIND, int HD, bool EX>
+struct Keys {
+    static constexpr int CK = KIND == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16;
+    static constexpr int EB = KIND == VGX_E_Q8 ? 1 : 2;
+    static constexpr int RB = HD * EB;             // bytes of a row
+    static constexpr int KP = (RB + 63) / 64;      // K pieces a lane and half
+    static constexpr int CPR = RB / 16;            // V pieces of a row
+    static constexpr int NL = 32 * CPR / 64;       // V pieces a lane
+    static_assert(32 * CPR % 64 == 0, "");
+    uint4 k[2][KP], v[NL];
+
+    // the page of row j0 + lane % 32, checked
+    static __device__ __forceinline__ int page(const PagedDev& A, const int* tab, int j0, int end) {
+        const int j = min(j0 + (int)(threadIdx.x & 31), end - 1);
+        int pg = tab[page_of(A, j)];
+        if (pg < 0 || pg >= A.npages) {
+            set_fault(A, VGX_FAULT_PAGE);
+            pg = 0;
+        }
+        return pg;
+    }
+    // byte of a row that piece T of lane group g starts at; in the tail of a
+    // q8 row of 32 mod 64 bytes, 8 bytes a lane
+    static __device__ __forceinline__ int kbyte(int T, int g) {
+        return RB - 64 * T >= 64 ? 64 * T + 16 * g : 64 * T + 8 * g;
+    }
+    template <class Addr>
+    __device__ __forceinline__ void load_k(int rb, int g, int u, Addr addr) {
+#pragma unroll
+        for (int T = 0; T < KP; ++T) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (RB - 64 * T >= 64) {
+                if (EX || 64 * T + 16 * g < rb) w = *reinterpret_cast<const uint4*>(addr + kbyte(T, g));
+            } else if (EX || 64 * T + 8 * g < rb) {
+                const uint2 x = *reinterpret_cast<const uint2*>(addr + kbyte(T, g));
+                w.x = x.x;
+                w.y = x.y;
+            }
+            k[u][T] = w;
+        }
+    }
+    __device__ __forceinline__ void load_k(const PagedDev& A, const uint8_t* kh, int pg, int j0, int end, bool uni) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, rb = A.hd * EB;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (uni) {
+                const int p = __builtin_amdgcn_readlane(pg, 16 * u);
+                const int j = min(j0 + 16 * u, (end - 1) & ~15);
+                const int slot = j - page_of(A, j) * A.psize;
+                load_k(rb, g, u, kh + (int64_t)p * A.kpg + (int64_t)slot * A.krow + (unsigned)(r * (int)A.krow));
+            } else {
+                const int p = __shfl(pg, 16 * u + r, 64);
+                const int j = min(j0 + 16 * u + r, end - 1);
+                const int slot = j - page_of(A, j) * A.psize;
+                load_k(rb, g, u, kh + (int64_t)p * A.kpg + (int64_t)slot * A.krow);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const PagedDev& A, const uint8_t* vh, int pg, int j0, int end, bool uni) {
+        const int lane = threadIdx.x & 63, rb = A.hd * EB;
+        const uint8_t* base[2];
+        if (uni) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int p = __builtin_amdgcn_readlane(pg, 16 * u);
+                const int j = min(j0 + 16 * u, (end - 1) & ~15);
+                const int slot = j - page_of(A, j) * A.psize;
+                base[u] = vh + (int64_t)p * A.vpg + (int64_t)slot * A.vrow;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
+            const uint8_t* p;
+            if (uni) {
+                // (pieces 0 .. NL/2 - 1 are the first half's rows)
+                p = base[i >= NL / 2] + (unsigned)((row & 15) * (int)A.vrow + ch * 16);
+                if (NL & 1) p = (row < 16 ? base[0] : base[1]) + (unsigned)((row & 15) * (int)A.vrow + ch * 16);
+            } else {
+                const int q = __shfl(pg, row, 64);
+                const int j = min(j0 + row, end - 1);
+                const int slot = j - page_of(A, j) * A.psize;
+                p = vh + (int64_t)q * A.vpg + (int64_t)slot * A.vrow + ch * 16;
+            }
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (EX || ch * 16 < rb) v[i] = *reinterpret_cast<const uint4*>(p);
+        }
+    }
+    // V into LDS; rows behind the end as zeros.  Whether, cleaned where asked,
+    // it had something to clean.
+    __device__ __forceinline__ bool store_v(uint8_t* lv, int left, bool wide) {
+        const int lane = threadIdx.x & 63;
+        bool r = false;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
+            if (left < 32 && row >= left) v[i] = make_uint4(0, 0, 0, 0);
+            if (KIND != VGX_E_Q8 && wide) r = clear_odd<CK>(v[i]) || r;
+            uint8_t* p = lv + row * Geo<HD>::pv + ch * (32 / EB);
+            if (KIND == VGX_E_Q8) {
+                const uint2 a = q8_to_f16(v[i].x), b = q8_to_f16(v[i].y), c = q8_to_f16(v[i].z), d = q8_to_f16(v[i].w);
+                reinterpret_cast<uint4*>(p)[0] = make_uint4(a.x, a.y, b.x, b.y);
+                reinterpret_cast<uint4*>(p)[1] = make_uint4(c.x, c.y, d.x, d.y);
+            } else {
+                *reinterpret_cast<uint4*>(p) = v[i];
+            }
+        }
+        return r;
+    }
+    // K's A operand of k-step t (half u): values as Q's B operand has them.
+    __device__ __forceinline__ s16x8 frag(int u, int t) const {
+        if constexpr (KIND == VGX_E_Q8) {
+            const uint4 w = k[u][t / 2];
+            const uint2 a = q8_to_f16(t & 1 ? w.z : w.x), b = q8_to_f16(t & 1 ? w.w : w.y);
+            return __builtin_bit_cast(s16x8, make_uint4(a.x, a.y, b.x, b.y));
+        } else {
+            return __builtin_bit_cast(s16x8, k[u][t]);
+        }
+    }
+    // The first value of k-step t that lane group g holds.
+    static __device__ __forceinline__ int qdim(int t, int g) {
+        if (KIND != VGX_E_Q8) return 32 * t + 8 * g;
+        return RB - 64 * (t / 2) >= 64 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 64 * (t / 2) + 8 * g;
+    }
+};
+
+// LDS of one wave: its V tile; at the end 16 columns of sums.
+constexpr int rows_lds(int hd) {
+    const int pv = (hd * 2 + 63) / 128 * 128 + 64;
+    return 32 * pv > hd * 64 ? 32 * pv : hd * 64;
+}
+
+// Few rows a sequence (max_q * grp <= 16 NB): a workgroup is one sequence, KV
+// head and split; its 4 waves hold the same NB blocks of 16 columns and take
+// tiles of 32 keys in turn, without a barrier, and join at the end.  The 16x16x32
+// product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
+// the lane; two of them are the next product's B operand.
+template <int KIND, int HD, bool EX, int NB>
 __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
-    using St = Stage<KIND, HD, EX, 32, 64>;
-    constexpr int CK = St::CK;
-    constexpr int kWave = 32 * (Geo<HD>::pk + Geo<HD>::pv);
+    using Ks = Keys<KIND, HD, EX>;
+    constexpr int CK = Ks::CK, KS = HD / 32, DB = HD / 16;
+    constexpr int kWave = rows_lds(HD);
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float sm[4][32], sl[4][32];
+    __shared__ float sm[4][16 * NB], sl[4][16 * NB];
     const PagedDev& A = P.A;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int s = blockIdx.x / A.kvh, h = blockIdx.x - s * A.kvh;
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
@@ -411,87 +611,185 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     const int split = blockIdx.y;
     if (split >= sp.nsp) return;
     const int start = sp.lo + split * P.split_len, end = min(sp.hi, start + P.split_len);
-    const Col cl = col_of(P, q, h, col, end);
-    s16x8 qf[HD / 16];
-    load_q<HD, EX>(A, P.q + ((int64_t)cl.row * P.qstride + (int64_t)cl.head * A.hd) * 2, cl.valid, qf);
-    uint8_t* lk = smem + wave * kWave;
-    uint8_t* lv = lk + 32 * Geo<HD>::pk;
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     const int* tab = A.table + (int64_t)s * A.tstride;
+    const bool uni = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
+    uint8_t* lv = smem + wave * kWave;
+    Ks t;
+    int j0 = start + wave * 32;
+    int pg = 0, pn = 0;
+    if (j0 < end) {
+        pg = Ks::page(A, tab, j0, end);
+        if (j0 + 128 < end) pn = Ks::page(A, tab, j0 + 128, end);
+    }
+    Col cl[NB];
+    s16x8 qf[NB][KS];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        cl[b] = col_of(P, q, h, b * 16 + col, end);
+        const uint8_t* qp = P.q + ((int64_t)cl[b].row * P.qstride + (int64_t)cl[b].head * A.hd) * 2;
+#pragma unroll
+        for (int u = 0; u < KS; ++u) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            const int d = Ks::qdim(u, g);
+            if (cl[b].valid && (EX || d < A.hd)) w = *reinterpret_cast<const uint4*>(qp + d * 2);
+            qf[b][u] = __builtin_bit_cast(s16x8, w);
+        }
+    }
+    if (j0 < end) {
+        t.load_v(A, vh, pg, j0, end, uni);
+        t.load_k(A, kh, pg, j0, end, uni);
+    }
     // keys every column sees: [all_lo, all_hi)
     const int all_hi = min(q.kv - q.n + 1, end);
     const int all_lo = P.window > 0 ? q.kv - P.window : 0;
-    Acc<HD> a;
-    a.clear();
-    St st;
-    int j0 = start + wave * 32;
-    int pg = j0 < end ? St::page(A, tab, j0, end) : 0;
-    if (HD <= 128 && j0 < end) st.load(A, kh, vh, pg, j0, end, lane);
-    int pn = j0 + 128 < end ? St::page(A, tab, j0 + 128, end) : 0;
+    f32x4 o[NB][DB];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        m[b] = -INFINITY;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[b][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // a lane's address for the transposing read: key 4 g + i / 4, dims 4 (i & 3)
+    const uint8_t* vb = lv + (4 * g + (col >> 2)) * Geo<HD>::pv + 8 * (col & 3);
+    bool odd = false;
     while (j0 < end) {
         const bool mask = j0 + 32 > all_hi || j0 < all_lo;
-        bool odd;
-        wave_sync();
-        if (HD <= 128) {
-            odd = mask && __any(st.odd());
-            st.store(lk, lv, lane);
-        } else {
-            odd = __any(St::fetch(A, kh, vh, pg, j0, end, lane, lk, lv)) && mask;
-        }
         const int jn = j0 + 128;
+        wave_sync();
+        odd = t.store_v(lv, end - j0, mask) || odd;
+        if (jn < end) t.load_v(A, vh, pn, jn, end, uni);
+        f32x4 sc[NB][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) sc[b][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const s16x8 kf = t.frag(u, k);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) sc[b][u] = mfma16<CK>(kf, qf[b][k], sc[b][u]);
+            }
+        }
         if (jn < end) {
-            if (HD <= 128) st.load(A, kh, vh, pn, jn, end, lane);
-            pg = pn;
-            if (jn + 128 < end) pn = St::page(A, tab, jn + 128, end);
+            t.load_k(A, kh, pn, jn, end, uni);
+            if (jn + 128 < end) pn = Ks::page(A, tab, jn + 128, end);
+        }
+        s16x8 pf[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (mask) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = j0 + 16 * u + 4 * g + i;
+                        sc[b][u][i] = j >= cl[b].vlo && j < cl[b].vhi ? sc[b][u][i] : -INFINITY;
+                    }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(sc[b][0][0], sc[b][0][1]), fmaxf(sc[b][0][2], sc[b][0][3])),
+                             fmaxf(fmaxf(sc[b][1][0], sc[b][1][1]), fmaxf(sc[b][1][2], sc[b][1][3])));
+            mx = fmaxf(quad_max(mx), m[b]);
+            // (no key yet: subtract 0, so the exponents stay -inf and the weights 0)
+            const float mc = (mx == -INFINITY ? 0.0f : mx) * P.c;
+            const float alpha = exp2_(fmaf(m[b], P.c, -mc));
+            m[b] = mx;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[b][u][i] = exp2_(fmaf(sc[b][u][i], P.c, -mc));
+                    sum += sc[b][u][i];
+                    pf[b][4 * u + i] = to_ct<CK>(sc[b][u][i]);
+                }
+            l[b] = fmaf(l[b], alpha, sum);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[b][d] *= alpha;
         }
         wave_sync();
-        step<CK, HD, EX, 1>(A, qf, a, lk, lv, j0, P.c, mask, cl.vlo, cl.vhi, odd, reinterpret_cast<float*>(lk));
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            if (!EX && 16 * d >= A.hd) continue;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + 32 * d));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vb + 32 * d + 16 * Geo<HD>::pv));
+            const s16x8 vf = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b][d] = mfma16<CK>(vf, pf[b], o[b][d]);
+        }
         j0 = jn;
     }
-    // the waves' sums on a common maximum, joined in wave order
-    const float l = half_sum(a.l);
-    if (lane < 32) { sm[wave][col] = a.m; sl[wave][col] = l; }
-    __syncthreads();
-    float M = sm[0][col];
+    if (KIND != VGX_E_Q8 && __any(odd)) {
+        for (j0 = start + wave * 32; j0 < end; j0 += 128) {
+            if (j0 + 32 <= all_hi && j0 >= all_lo) continue;
+            t.load_v(A, vh, Ks::page(A, tab, j0, end), j0, end, uni);
+            wave_sync();
+            t.store_v(lv, end - j0, false);
+            wave_sync();
 #pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, sm[w][col]);
-    const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
-    float L = 0.0f;
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L = fmaf(sl[w][col], exp2_(fmaf(sm[w][col], P.c, -mc)), L);
-    const float f = exp2_(fmaf(a.m, P.c, -mc));
-    float* part = reinterpret_cast<float*>(smem + wave * kWave);
-    const int hh = lane >> 5;
-#pragma unroll
-    for (int b = 0; b < HD / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[(32 * b + 8 * (i / 4) + 4 * hh + (i & 3)) * 32 + col] = a.o[b][i] * f;
-    __syncthreads();
-    if (!cl.valid) return;
-    // thread: column lane % 32, every eighth group of 4 dims
-    const int64_t at = ((int64_t)split * A.ntok + cl.row) * A.heads + cl.head;
-    const bool whole = sp.nsp == 1;
-    const float r = whole ? inv_l(P, L) : 1.0f;
-    for (int d = 4 * (threadIdx.x >> 5); d < A.hd; d += 32) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) x[e] += reinterpret_cast<const float*>(smem + w * kWave)[(d + e) * 32 + col];
-            x[e] *= r;
+                for (int d = 0; d < DB; ++d) {
+                    float x[4] = {o[b][d][0], o[b][d][1], o[b][d][2], o[b][d][3]};
+                    add_odd<CK>(x, lv + (16 * d + 4 * g) * 2, Geo<HD>::pv, max(cl[b].vlo - j0, 0),
+                                min(cl[b].vhi - j0, 32));
+                    o[b][d] = f32x4{x[0], x[1], x[2], x[3]};
+                }
         }
-        const float4 v = make_float4(x[0], x[1], x[2], x[3]);
-        if (whole) put_out<CK>(P, cl.row, cl.head, d, v);
-        else *reinterpret_cast<float4*>(P.po + at * A.hd + d) = v;
     }
-    if (threadIdx.x < 32) {
-        if (!whole) {
-            P.pml[2 * at] = M;
-            P.pml[2 * at + 1] = L;
-        } else if (P.lse) {
-            P.lse[(int64_t)cl.row * A.heads + cl.head] = lse_of(P, M, L);
+    // the waves' sums on a common maximum, joined in wave order, 16 columns at
+    // a time through LDS
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const float x = quad_sum(l[b]);
+        if (lane < 16) { sm[wave][16 * b + col] = m[b]; sl[wave][16 * b + col] = x; }
+    }
+    __syncthreads();
+    const bool whole = sp.nsp == 1;
+    float* part = reinterpret_cast<float*>(smem + wave * kWave);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        float M = sm[0][16 * b + col];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) M = fmaxf(M, sm[w][16 * b + col]);
+        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+        float L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) L = fmaf(sl[w][16 * b + col], exp2_(fmaf(sm[w][16 * b + col], P.c, -mc)), L);
+        const float f = exp2_(fmaf(m[b], P.c, -mc));
+        if (b) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[(16 * d + 4 * g + i) * 16 + col] = o[b][d][i] * f;
+        __syncthreads();
+        if (!cl[b].valid) continue;
+        // thread: column lane % 16, every sixteenth group of 4 dims
+        const int64_t at = ((int64_t)split * A.ntok + cl[b].row) * A.heads + cl[b].head;
+        const float r = whole ? inv_l(P, L) : 1.0f;
+        for (int d = 4 * (threadIdx.x >> 4); d < A.hd; d += 64) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x[e] += reinterpret_cast<const float*>(smem + w * kWave)[(d + e) * 16 + col];
+                x[e] *= r;
+            }
+            const float4 v = make_float4(x[0], x[1], x[2], x[3]);
+            if (whole) put_out<CK>(P, cl[b].row, cl[b].head, d, v);
+            else *reinterpret_cast<float4*>(P.po + at * A.hd + d) = v;
+        }
+        if (threadIdx.x < 16) {
+            if (!whole) {
+                P.pml[2 * at] = M;
+                P.pml[2 * at + 1] = L;
+            } else if (P.lse) {
+                P.lse[(int64_t)cl[b].row * A.heads + cl[b].head] = lse_of(P, M, L);
+            }
         }
     }
 }
@@ -526,9 +824,9 @@ __device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int tile, int
 // Many rows a sequence: a workgroup is a tile of 128 columns (4 waves x 32) of
 // one KV head; the waves share tiles of 64 keys.
 template <int KIND, int HD, bool EX>
-__global__ void __launch_bounds__(256) paged_tile_kernel(const AttnArgs P) {
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
     constexpr int ROWS = 64;
-    using St = Stage<KIND, HD, EX, ROWS, 256>;
+    using St = Stage<KIND, HD, EX>;
     constexpr int CK = St::CK;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int any_odd;
@@ -537,6 +835,8 @@ __global__ void __launch_bounds__(256) paged_tile_kernel(const AttnArgs P) {
     const int tile = blockIdx.x / A.kvh, h = blockIdx.x - tile * A.kvh;
     int s, local;
     if (!tile_at(A, 128, tile, s, local)) return;
+    s = __builtin_amdgcn_readfirstlane(s);
+    local = __builtin_amdgcn_readfirstlane(local);
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
     const int m0 = local * 128, m1 = min(m0 + 128, q.n * A.grp) - 1;
@@ -557,16 +857,16 @@ __global__ void __launch_bounds__(256) paged_tile_kernel(const AttnArgs P) {
     const int any_lo = P.window > 0 ? base + r0 - P.window + 1 : 0;
     uint8_t* lk = smem;
     uint8_t* lv = smem + ROWS * Geo<HD>::pk;
-    float* lp = reinterpret_cast<float*>(smem + ROWS * (Geo<HD>::pk + Geo<HD>::pv)) + wave * 1024;
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     const int* tab = A.table + (int64_t)s * A.tstride;
+    const bool uni = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     Acc<HD> a;
     a.clear();
     St st;
     if (threadIdx.x == 0) any_odd = 0;
     int pg = start < end ? St::page(A, tab, start, end) : 0;
-    if (HD <= 128 && start < end) st.load(A, kh, vh, pg, start, end, threadIdx.x);
+    if (HD <= 128 && start < end) st.load(A, kh, vh, pg, start, end, uni);
     int pn = start + ROWS < end ? St::page(A, tab, start + ROWS, end) : 0;
     // tiles of keys that some column of the workgroup does not wholly see
     const int tile_hi = min(base + m0 / A.grp + 1, end);
@@ -574,23 +874,47 @@ __global__ void __launch_bounds__(256) paged_tile_kernel(const AttnArgs P) {
     for (int j0 = start; j0 < end; j0 += ROWS) {
         const bool wide = j0 + ROWS > tile_hi || j0 < tile_lo;
         __syncthreads();  // the last tile's reads are done
-        if (HD <= 128) {
-            if (wide && st.odd()) any_odd = 1;
-            st.store(lk, lv, threadIdx.x);
-        } else if (St::fetch(A, kh, vh, pg, j0, end, threadIdx.x, lk, lv) && wide) {
-            any_odd = 1;
-        }
+        const bool odd = HD <= 128 ? st.store(lk, lv, end - j0, wide)
+                                   : St::fetch(A, kh, vh, pg, j0, end, uni, lk, lv, wide);
+        if (odd) any_odd = 1;
         __syncthreads();
-        const bool odd = wide && any_odd;
         const int jn = j0 + ROWS;
         if (jn < end) {
-            if (HD <= 128) st.load(A, kh, vh, pn, jn, end, threadIdx.x);
+            if (HD <= 128) st.load(A, kh, vh, pn, jn, end, uni);
             pg = pn;
             if (jn + ROWS < end) pn = St::page(A, tab, jn + ROWS, end);
         }
         if (j0 < any_hi && j0 + ROWS > any_lo) {
             const bool mask = j0 + ROWS > all_hi || j0 < all_lo;
-            step<CK, HD, EX, 2>(A, qf, a, lk, lv, j0, P.c, mask, cl.vlo, cl.vhi, odd && mask, lp);
+            if constexpr (HD <= 128) {
+                step<CK, HD, EX, 2>(A, qf, a, lk, lv, j0, P.c, mask, cl.vlo, cl.vhi);
+            } else {  // (registers)
+#pragma unroll 1
+                for (int u = 0; u < 64; u += 32)
+                    step<CK, HD, EX, 1>(A, qf, a, lk + u * Geo<HD>::pk, lv + u * Geo<HD>::pv, j0 + u, P.c, mask, cl.vlo,
+                                        cl.vhi);
+            }
+        }
+    }
+    __syncthreads();
+    if (KIND != VGX_E_Q8 && any_odd) {
+        for (int j0 = start; j0 < end; j0 += ROWS) {
+            if (j0 + ROWS <= tile_hi && j0 >= tile_lo) continue;
+            __syncthreads();
+            St::fetch_v(A, vh, St::page(A, tab, j0, end), j0, end, uni, lv);
+            __syncthreads();
+            // (as the loop above skips and masks)
+            if (j0 >= any_hi || j0 + ROWS <= any_lo) continue;
+#pragma unroll
+            for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float x[4] = {a.o[b][4 * g], a.o[b][4 * g + 1], a.o[b][4 * g + 2], a.o[b][4 * g + 3]};
+                    add_odd<CK>(x, lv + (32 * b + 8 * g + 4 * (lane >> 5)) * 2, Geo<HD>::pv, max(cl.vlo - j0, 0),
+                                min(cl.vhi - j0, ROWS));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a.o[b][4 * g + e] = x[e];
+                }
         }
     }
     const float L = half_sum(a.l);
@@ -620,79 +944,141 @@ __global__ void __launch_bounds__(256) paged_tile_kernel(const AttnArgs P) {
     }
 }
 
-// Joins a row's splits, in split order: a wave a row and head.
-template <int CK>
-__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P) {
+// The splits of row t and head, as the kernels cut its tile (every lane
+// active); 0: not a row of the batch.
+__device__ __forceinline__ int splits_of(const AttnArgs& P, int t, int head) {
     const PagedDev& A = P.A;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(w / A.heads), head = (int)(w - (int64_t)t * A.heads);
-    if (t >= A.ntok) return;
-    const int lane = threadIdx.x & 63;
     const int s = seq_of_row(A, t);
-    if (s >= A.nseq) return;
+    if (s >= A.nseq) return 0;
     const SeqAt q = seq_at(A, s);
     const int i = t - q.q0;
-    if (i < 0 || i >= q.n) return;
-    // the row's tile, as the kernels cut it
+    if (i < 0 || i >= q.n) return 0;
     const int m = i * A.grp + head % A.grp;
     const int m0 = m / P.tm * P.tm, m1 = min(m0 + P.tm, q.n * A.grp) - 1;
-    const Span sp = span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len);
-    if (sp.nsp == 1) return;
+    return span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len).nsp;
+}
+
+// Joins a row's splits.  Few splits (WIDE false): a wave a row and head, in
+// split order.  Many: a workgroup a row and head, the splits dealt to groups
+// of hd / 4 threads, each in split order, the groups in theirs.
+template <int CK, bool WIDE>
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P) {
+    const PagedDev& A = P.A;
+    __shared__ float sw[4], sl[4];
+    __shared__ float4 so[256];
+    const int lane = threadIdx.x & 63;
+    const int64_t w = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int t = (int)(w / A.heads), head = (int)(w - (int64_t)t * A.heads);
+    if (t >= A.ntok) return;
+    const int nsp = splits_of(P, t, head);
+    if (nsp <= 1) return;
     const int64_t step = (int64_t)A.ntok * A.heads, at = (int64_t)t * A.heads + head;
-    float M = -INFINITY;
-    for (int k = 0; k < sp.nsp; ++k) M = fmaxf(M, P.pml[2 * (at + k * step)]);
-    const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
-    float L = 0.0f;
-    const int d = lane * 4;
+    const float2* ml = reinterpret_cast<const float2*>(P.pml) + at;
+    const float4* po = reinterpret_cast<const float4*>(P.po);
+    const int n4 = A.hd / 4;
     float4 o = make_float4(0, 0, 0, 0);
-    for (int k = 0; k < sp.nsp; ++k) {
-        const float f = exp2_(fmaf(P.pml[2 * (at + k * step)], P.c, -mc));
-        L = fmaf(P.pml[2 * (at + k * step) + 1], f, L);
-        if (d < A.hd) {
-            const float4 x = *reinterpret_cast<const float4*>(P.po + (at + k * step) * A.hd + d);
-            o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    float M = -INFINITY, L = 0.0f;
+    if (!WIDE) {
+        for (int k = 0; k < nsp; ++k) M = fmaxf(M, ml[k * step].x);
+        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+#pragma unroll 4
+        for (int k = 0; k < nsp; ++k) {
+            const float2 x = ml[k * step];
+            const float f = exp2_(fmaf(x.x, P.c, -mc));
+            L = fmaf(x.y, f, L);
+            const float4 y = po[(at + k * step) * n4 + min(lane, n4 - 1)];
+            o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+        }
+    } else {
+        for (int k = threadIdx.x; k < nsp; k += 256) M = fmaxf(M, ml[k * step].x);
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+        if (lane == 0) sw[threadIdx.x >> 6] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(sw[0], sw[1]), fmaxf(sw[2], sw[3]));
+        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+        const int ng = 256 / n4, gr = threadIdx.x / n4, d = threadIdx.x - gr * n4;
+        if (gr < ng) {
+#pragma unroll 8
+            for (int k = gr; k < nsp; k += ng) {
+                const float2 x = ml[k * step];
+                const float f = exp2_(fmaf(x.x, P.c, -mc));
+                const float4 y = po[(at + k * step) * n4 + d];
+                o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+            }
+        }
+        for (int k = threadIdx.x; k < nsp; k += 256) {
+            const float2 x = ml[k * step];
+            L = fmaf(x.y, exp2_(fmaf(x.x, P.c, -mc)), L);
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x, 64);
+        if (lane == 0) sl[threadIdx.x >> 6] = L;
+        so[threadIdx.x] = o;
+        __syncthreads();
+        L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+        if ((int)threadIdx.x >= n4) return;
+        for (int x = 1; x < ng; ++x) {
+            const float4 y = so[x * n4 + threadIdx.x];
+            o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
         }
     }
+    const int d = WIDE ? threadIdx.x : lane;
     const float r = inv_l(P, L);
-    if (d < A.hd) put_out<CK>(P, t, head, d, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
-    if (lane == 0 && P.lse) P.lse[at] = lse_of(P, M, L);
+    if (d < n4) put_out<CK>(P, t, head, 4 * d, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+    if (d == 0 && P.lse) P.lse[at] = lse_of(P, M, L);
 }
 
 typedef void (*AttnFn)(const AttnArgs);
 struct Plan {
     AttnFn fn;
     int lds, tm;
+    bool rows;
     int64_t wgs;       // workgroups of one split
     int split_len, nsplit;
     size_t ws;
 };
 
+// cols: the columns a sequence may have in a KV head.  Up to 48 the rows kernel
+// (16 for heads of more than 128 values; more columns fill the registers).
 template <int KIND, int HD, bool EX>
-void fn_of(bool rows, Plan& p) {
-    const int row = Geo<HD>::pk + Geo<HD>::pv;
-    p.fn = rows ? paged_rows_kernel<KIND, HD, EX> : paged_tile_kernel<KIND, HD, EX>;
-    p.lds = rows ? 4 * 32 * row : 64 * row + 4 * 4096;
+void fn_of(int64_t cols, Plan& p) {
+    if (cols <= (HD <= 128 ? 48 : 16)) {
+        const int nb = (int)(cols + 15) / 16;
+        p.fn = paged_rows_kernel<KIND, HD, EX, 1>;
+        if constexpr (HD <= 128) {
+            if (nb == 2) p.fn = paged_rows_kernel<KIND, HD, EX, 2>;
+            if (nb == 3) p.fn = paged_rows_kernel<KIND, HD, EX, 3>;
+        }
+        p.lds = 4 * rows_lds(HD);
+        p.tm = 16 * nb;
+        p.rows = true;
+    } else {
+        p.fn = paged_tile_kernel<KIND, HD, EX>;
+        p.lds = 64 * (Geo<HD>::pk + Geo<HD>::pv);
+        p.tm = 128;
+        p.rows = false;
+    }
 }
 template <int KIND>
-void fn_of(int hd, bool rows, Plan& p) {
+void fn_of(int hd, int64_t cols, Plan& p) {
     switch (hd) {
-        case 64: return fn_of<KIND, 64, true>(rows, p);
-        case 96: return fn_of<KIND, 96, true>(rows, p);
-        case 128: return fn_of<KIND, 128, true>(rows, p);
-        case 256: return fn_of<KIND, 256, true>(rows, p);
+        case 64: return fn_of<KIND, 64, true>(cols, p);
+        case 96: return fn_of<KIND, 96, true>(cols, p);
+        case 128: return fn_of<KIND, 128, true>(cols, p);
+        case 256: return fn_of<KIND, 256, true>(cols, p);
     }
-    return hd < 128 ? fn_of<KIND, 128, false>(rows, p) : fn_of<KIND, 256, false>(rows, p);
+    return hd < 128 ? fn_of<KIND, 128, false>(cols, p) : fn_of<KIND, 256, false>(cols, p);
 }
 
 Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     Plan p{};
-    const bool rows = (int64_t)A.max_q * A.grp <= 32;
-    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A.hd, rows, p);
-    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A.hd, rows, p);
-    else fn_of<VGX_E_Q8>(A.hd, rows, p);
-    p.tm = rows ? 32 : 128;
+    const int64_t cols = (int64_t)A.max_q * A.grp;
+    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A.hd, cols, p);
+    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A.hd, cols, p);
+    else fn_of<VGX_E_Q8>(A.hd, cols, p);
     // (a sequence with rows has at most rows * grp / tm + 1 tiles)
-    const int64_t tiles = rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
+    const int64_t tiles = p.rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
     p.wgs = tiles * A.kvh;
     int64_t span = A.max_kv;
     if (window > 0) span = std::min<int64_t>(span, (int64_t)window + p.tm + 64);
@@ -766,9 +1152,14 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     VGX_LAUNCH_CHECK("paged attention launch");
     if (p.nsplit > 1) {
         const int64_t jobs = (int64_t)A.ntok * A.heads;
-        hipLaunchKernelGGL(compute_kind(cache->kind) == VGX_E_BF16 ? paged_join_kernel<VGX_E_BF16>
-                                                                   : paged_join_kernel<VGX_E_F16>,
-                           dim3((unsigned)((jobs + 3) / 4)), dim3(256), 0, ctx->stream, P);
+        // (a row's partials one after the other cost a round trip each four)
+        const bool wide = p.nsplit > 8 && jobs < (1 << 24);
+        const bool bf = compute_kind(cache->kind) == VGX_E_BF16;
+        const AttnFn join = wide ? (bf ? paged_join_kernel<VGX_E_BF16, true> : paged_join_kernel<VGX_E_F16, true>)
+                                 : (bf ? paged_join_kernel<VGX_E_BF16, false> : paged_join_kernel<VGX_E_F16, false>);
+        const int64_t grid = wide ? jobs : (jobs + 3) / 4;
+        if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
+        hipLaunchKernelGGL(join, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P);
         VGX_LAUNCH_CHECK("paged attention join launch");
     }
     return VGX_OK;
