@@ -145,10 +145,25 @@ struct Geo {
 };
 static_assert(Geo<64>::pv == 192 && Geo<96>::pv == 192 && Geo<128>::pv == 320 && Geo<256>::pv == 576, "");
 
+// The page of position j (of the last one where j is past it) as the table has
+// it, and the page to read: 0 with the fault noted where the table's is outside
+// the pool.  Apart, so that a load does not wait for the table's before it.
+__device__ __forceinline__ int page_at(const PagedDev& A, const int* tab, int j, int end) {
+    return tab[page_of(A, min(j, end - 1))];
+}
+__device__ __forceinline__ int page_ok(const PagedDev& A, int pg, bool& bad) {
+    const bool in = (unsigned)pg < (unsigned)A.npages;
+    bad = bad || !in;
+    return in ? pg : 0;
+}
+
+// EX: heads of exactly HD values in pages whose size is a multiple of 16: 16
+// rows then lie one after the other and a wave's address is one scalar and an
+// offset a lane that stays.  Otherwise (EX false) HD is the room for a head and
+// every row is looked up.
+
 // Staging of a tile of 64 keys by a workgroup of 4 waves: wave w takes rows
-// 16 w .. 16 w + 15, NL 16-byte pieces a lane of K and as many of V.  Pages
-// whose size is a multiple of 16 (uni) give the wave one scalar address and
-// every lane an offset that stays; others are looked up row by row (lane r
+// 16 w .. 16 w + 15, NL 16-byte pieces a lane of K and as many of V (lane r
 // holds the page of row r % 16).
 template <int KIND, int HD, bool EX>
 struct Stage {
@@ -159,24 +174,16 @@ struct Stage {
     static constexpr bool kAll = NL * 64 == 16 * CPR;
     uint4 k[NL], v[NL];
 
-    // The page of row j0 + 16 w + lane % 16 (the last row before `end` stands
-    // in for those behind); a page outside the pool counts as page 0, with the
-    // fault recorded.
+    // the page of row j0 + 16 w + lane % 16
     static __device__ __forceinline__ int page(const PagedDev& A, const int* tab, int j0, int end) {
-        const int j = min(j0 + 16 * (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 15), end - 1);
-        int pg = tab[page_of(A, j)];
-        if (pg < 0 || pg >= A.npages) {
-            set_fault(A, VGX_FAULT_PAGE);
-            pg = 0;
-        }
-        return pg;
+        return page_at(A, tab, j0 + 16 * (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 15), end);
     }
     // One of K and V; rows behind the end are whatever is there.
     static __device__ __forceinline__ void load1(const PagedDev& A, const uint8_t* base, int64_t ps, int64_t rs, int pg,
-                                                 int j0, int end, bool uni, uint4 (&w)[NL]) {
+                                                 int j0, int end, uint4 (&w)[NL]) {
         const int lane = threadIdx.x & 63, jw = j0 + 16 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint8_t* sbase = base;
-        if (uni) {
+        if (EX) {
             const int j = min(jw, (end - 1) & ~15);
             const int slot = j - page_of(A, j) * A.psize;
             sbase += (int64_t)__builtin_amdgcn_readfirstlane(pg) * ps + (int64_t)slot * rs;
@@ -184,23 +191,23 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if ((!kAll && row >= 16) || (!EX && ch * 16 >= A.hd * EB)) continue;
             const uint8_t* p;
-            if (uni) {
+            if (EX) {
                 p = sbase + (unsigned)(row * (int)rs + ch * 16);
             } else {
+                const int q = __shfl(pg, row & 15, 64);  // (every lane takes part)
                 const int j = min(jw + row, end - 1);
                 const int slot = j - page_of(A, j) * A.psize;
-                p = base + (int64_t)__shfl(pg, row, 64) * ps + (int64_t)slot * rs + ch * 16;
+                p = base + (int64_t)q * ps + (int64_t)slot * rs + ch * 16;
             }
-            w[i] = *reinterpret_cast<const uint4*>(p);
+            w[i] = make_uint4(0, 0, 0, 0);
+            if ((kAll || row < 16) && (EX || ch * 16 < A.hd * EB)) w[i] = *reinterpret_cast<const uint4*>(p);
         }
     }
     __device__ __forceinline__ void load(const PagedDev& A, const uint8_t* kh, const uint8_t* vh, int pg, int j0,
-                                         int end, bool uni) {
-        load1(A, kh, A.kpg, A.krow, pg, j0, end, uni, k);
-        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, v);
+                                         int end) {
+        load1(A, kh, A.kpg, A.krow, pg, j0, end, k);
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, v);
     }
     static __device__ __forceinline__ void put(uint8_t* p, const uint4& w) {
         if (KIND == VGX_E_Q8) {
@@ -250,12 +257,12 @@ struct Stage {
     // Load and store in one go, K then V through the same registers (heads of
     // more than 128 values leave none for a tile ahead).
     static __device__ __forceinline__ bool fetch(const PagedDev& A, const uint8_t* kh, const uint8_t* vh, int pg,
-                                                 int j0, int end, bool uni, uint8_t* lk, uint8_t* lv, bool wide) {
+                                                 int j0, int end, uint8_t* lk, uint8_t* lv, bool wide) {
         uint4 w[NL];
         bool r = false;
-        load1(A, kh, A.kpg, A.krow, pg, j0, end, uni, w);
+        load1(A, kh, A.kpg, A.krow, pg, j0, end, w);
         store1(lk, Geo<HD>::pk, w);
-        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, w);
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, w);
         if (wide) {
             cut(w, end - j0);
             r = clean(w);
@@ -264,9 +271,9 @@ struct Stage {
         return r;
     }
     static __device__ __forceinline__ void fetch_v(const PagedDev& A, const uint8_t* vh, int pg, int j0, int end,
-                                                   bool uni, uint8_t* lv) {
+                                                   uint8_t* lv) {
         uint4 w[NL];
-        load1(A, vh, A.vpg, A.vrow, pg, j0, end, uni, w);
+        load1(A, vh, A.vpg, A.vrow, pg, j0, end, w);
         cut(w, end - j0);
         store1(lv, Geo<HD>::pv, w);
     }
@@ -453,9 +460,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 
 // A wave's tile of 32 keys on its way: K as the pieces its lanes multiply (key
 // lane % 16 of each half, 16 bytes from byte 64 T + 16 (lane / 16) of the
-// row), V as pieces of rows for LDS.  Pages whose size is a multiple of 16
-// (uni) give each half one scalar address and every lane an offset that stays;
-// others are looked up row by row.
+// row), V as pieces of rows for LDS.
 template <int KIND, int HD, bool EX>
 struct Keys {
     static constexpr int CK = KIND == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16;
@@ -467,15 +472,9 @@ struct Keys {
     static_assert(32 * CPR % 64 == 0, "");
     uint4 k[2][KP], v[NL];
 
-    // the page of row j0 + lane % 32, checked
+    // the page of row j0 + lane % 32
     static __device__ __forceinline__ int page(const PagedDev& A, const int* tab, int j0, int end) {
-        const int j = min(j0 + (int)(threadIdx.x & 31), end - 1);
-        int pg = tab[page_of(A, j)];
-        if (pg < 0 || pg >= A.npages) {
-            set_fault(A, VGX_FAULT_PAGE);
-            pg = 0;
-        }
-        return pg;
+        return page_at(A, tab, j0 + (int)(threadIdx.x & 31), end);
     }
     // byte of a row that piece T of lane group g starts at; in the tail of a
     // q8 row of 32 mod 64 bytes, 8 bytes a lane
@@ -497,11 +496,11 @@ struct Keys {
             k[u][T] = w;
         }
     }
-    __device__ __forceinline__ void load_k(const PagedDev& A, const uint8_t* kh, int pg, int j0, int end, bool uni) {
+    __device__ __forceinline__ void load_k(const PagedDev& A, const uint8_t* kh, int pg, int j0, int end) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, rb = A.hd * EB;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            if (uni) {
+            if (EX) {
                 const int p = __builtin_amdgcn_readlane(pg, 16 * u);
                 const int j = min(j0 + 16 * u, (end - 1) & ~15);
                 const int slot = j - page_of(A, j) * A.psize;
@@ -514,10 +513,10 @@ struct Keys {
             }
         }
     }
-    __device__ __forceinline__ void load_v(const PagedDev& A, const uint8_t* vh, int pg, int j0, int end, bool uni) {
+    __device__ __forceinline__ void load_v(const PagedDev& A, const uint8_t* vh, int pg, int j0, int end) {
         const int lane = threadIdx.x & 63, rb = A.hd * EB;
         const uint8_t* base[2];
-        if (uni) {
+        if (EX) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int p = __builtin_amdgcn_readlane(pg, 16 * u);
@@ -530,7 +529,7 @@ struct Keys {
         for (int i = 0; i < NL; ++i) {
             const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
             const uint8_t* p;
-            if (uni) {
+            if (EX) {
                 // (pieces 0 .. NL/2 - 1 are the first half's rows)
                 p = base[i >= NL / 2] + (unsigned)((row & 15) * (int)A.vrow + ch * 16);
                 if (NL & 1) p = (row < 16 ? base[0] : base[1]) + (unsigned)((row & 15) * (int)A.vrow + ch * 16);
@@ -544,16 +543,21 @@ struct Keys {
             if (EX || ch * 16 < rb) v[i] = *reinterpret_cast<const uint4*>(p);
         }
     }
-    // V into LDS; rows behind the end as zeros.  Whether, cleaned where asked,
-    // it had something to clean.
-    __device__ __forceinline__ bool store_v(uint8_t* lv, int left, bool wide) {
+    // V into LDS; wide: rows behind the end (the tile's `left`-th on) as zeros,
+    // and cleaned.  Whether there was something to clean.
+    __device__ __forceinline__ bool store_v(uint8_t* lv, int left, bool wide, bool keep_odd = false) {
         const int lane = threadIdx.x & 63;
         bool r = false;
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                if ((i * 64 + lane) / CPR >= left) v[i] = make_uint4(0, 0, 0, 0);
+                if (KIND != VGX_E_Q8 && !keep_odd) r = clear_odd<CK>(v[i]) || r;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int sl = i * 64 + lane, row = sl / CPR, ch = sl - row * CPR;
-            if (left < 32 && row >= left) v[i] = make_uint4(0, 0, 0, 0);
-            if (KIND != VGX_E_Q8 && wide) r = clear_odd<CK>(v[i]) || r;
             uint8_t* p = lv + row * Geo<HD>::pv + ch * (32 / EB);
             if (KIND == VGX_E_Q8) {
                 const uint2 a = q8_to_f16(v[i].x), b = q8_to_f16(v[i].y), c = q8_to_f16(v[i].z), d = q8_to_f16(v[i].w);
@@ -614,14 +618,14 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     const int* tab = A.table + (int64_t)s * A.tstride;
-    const bool uni = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     uint8_t* lv = smem + wave * kWave;
     Ks t;
     int j0 = start + wave * 32;
     int pg = 0, pn = 0;
+    bool bad = false, odd = false;
     if (j0 < end) {
         pg = Ks::page(A, tab, j0, end);
-        if (j0 + 128 < end) pn = Ks::page(A, tab, j0 + 128, end);
+        pn = Ks::page(A, tab, j0 + 128, end);
     }
     Col cl[NB];
     s16x8 qf[NB][KS];
@@ -638,8 +642,9 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
         }
     }
     if (j0 < end) {
-        t.load_v(A, vh, pg, j0, end, uni);
-        t.load_k(A, kh, pg, j0, end, uni);
+        pg = page_ok(A, pg, bad);
+        t.load_v(A, vh, pg, j0, end);
+        t.load_k(A, kh, pg, j0, end);
     }
     // keys every column sees: [all_lo, all_hi)
     const int all_hi = min(q.kv - q.n + 1, end);
@@ -655,13 +660,16 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     }
     // a lane's address for the transposing read: key 4 g + i / 4, dims 4 (i & 3)
     const uint8_t* vb = lv + (4 * g + (col >> 2)) * Geo<HD>::pv + 8 * (col & 3);
-    bool odd = false;
+    // (past the end the loads repeat the last rows: without a branch between
+    // them each product waits for its own loads only)
     while (j0 < end) {
         const bool mask = j0 + 32 > all_hi || j0 < all_lo;
         const int jn = j0 + 128;
         wave_sync();
         odd = t.store_v(lv, end - j0, mask) || odd;
-        if (jn < end) t.load_v(A, vh, pn, jn, end, uni);
+        pg = page_ok(A, pn, bad);
+        pn = Ks::page(A, tab, jn + 128, end);
+        t.load_v(A, vh, pg, jn, end);
         f32x4 sc[NB][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -674,10 +682,7 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
                 for (int b = 0; b < NB; ++b) sc[b][u] = mfma16<CK>(kf, qf[b][k], sc[b][u]);
             }
         }
-        if (jn < end) {
-            t.load_k(A, kh, pn, jn, end, uni);
-            if (jn + 128 < end) pn = Ks::page(A, tab, jn + 128, end);
-        }
+        t.load_k(A, kh, pg, jn, end);
         s16x8 pf[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -725,9 +730,9 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     if (KIND != VGX_E_Q8 && __any(odd)) {
         for (j0 = start + wave * 32; j0 < end; j0 += 128) {
             if (j0 + 32 <= all_hi && j0 >= all_lo) continue;
-            t.load_v(A, vh, Ks::page(A, tab, j0, end), j0, end, uni);
+            t.load_v(A, vh, page_ok(A, Ks::page(A, tab, j0, end), bad), j0, end);
             wave_sync();
-            t.store_v(lv, end - j0, false);
+            t.store_v(lv, end - j0, true, true);
             wave_sync();
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -740,6 +745,7 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
                 }
         }
     }
+    if (bad) set_fault(A, VGX_FAULT_PAGE);
     // the waves' sums on a common maximum, joined in wave order, 16 columns at
     // a time through LDS
 #pragma unroll
@@ -825,14 +831,16 @@ __device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int tile, int
 // one KV head; the waves share tiles of 64 keys.
 template <int KIND, int HD, bool EX>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
-    constexpr int ROWS = 64;
+    constexpr int ROWS = 64, kTile = 64 * (Geo<HD>::pk + Geo<HD>::pv);
     using St = Stage<KIND, HD, EX>;
     constexpr int CK = St::CK;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int any_odd;
     const PagedDev& A = P.A;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31;
-    const int tile = blockIdx.x / A.kvh, h = blockIdx.x - tile * A.kvh;
+    // the last tiles, which see the most keys, first
+    const int rev = blockIdx.x / A.kvh, h = blockIdx.x - rev * A.kvh;
+    const int tile = gridDim.x / A.kvh - 1 - rev;
     int s, local;
     if (!tile_at(A, 128, tile, s, local)) return;
     s = __builtin_amdgcn_readfirstlane(s);
@@ -860,48 +868,66 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(cons
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     const int* tab = A.table + (int64_t)s * A.tstride;
-    const bool uni = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     Acc<HD> a;
     a.clear();
     St st;
-    if (threadIdx.x == 0) any_odd = 0;
-    int pg = start < end ? St::page(A, tab, start, end) : 0;
-    if (HD <= 128 && start < end) st.load(A, kh, vh, pg, start, end, uni);
-    int pn = start + ROWS < end ? St::page(A, tab, start + ROWS, end) : 0;
+    if (threadIdx.x == 0) any_odd = 0;  // (read after the loop's barriers)
     // tiles of keys that some column of the workgroup does not wholly see
     const int tile_hi = min(base + m0 / A.grp + 1, end);
     const int tile_lo = P.window > 0 ? base + m1 / A.grp - P.window + 1 : 0;
-    for (int j0 = start; j0 < end; j0 += ROWS) {
-        const bool wide = j0 + ROWS > tile_hi || j0 < tile_lo;
-        __syncthreads();  // the last tile's reads are done
-        const bool odd = HD <= 128 ? st.store(lk, lv, end - j0, wide)
-                                   : St::fetch(A, kh, vh, pg, j0, end, uni, lk, lv, wide);
-        if (odd) any_odd = 1;
-        __syncthreads();
-        const int jn = j0 + ROWS;
-        if (jn < end) {
-            if (HD <= 128) st.load(A, kh, vh, pn, jn, end, uni);
-            pg = pn;
-            if (jn + ROWS < end) pn = St::page(A, tab, jn + ROWS, end);
+    auto wide = [&](int j) { return j + ROWS > tile_hi || j < tile_lo; };
+    // Two tiles in LDS (one for heads of more than 128 values): the next one is
+    // loaded into registers before this one's products and stored after them,
+    // so a tile costs one barrier.
+    constexpr bool kTwo = HD <= 128;
+    int pg = 0, pn = 0;
+    bool odd = false, bad = false;
+    if (start < end) {
+        pg = St::page(A, tab, start, end);
+        pn = St::page(A, tab, start + ROWS, end);
+        pg = page_ok(A, pg, bad);
+        if (kTwo) {
+            st.load(A, kh, vh, pg, start, end);
+            odd = st.store(lk, lv, end - start, wide(start));
         }
+    }
+    int buf = 0;
+    for (int j0 = start; j0 < end; j0 += ROWS) {
+        const int jn = j0 + ROWS;
+        if (!kTwo) {
+            __syncthreads();  // the last tile's reads are done
+            odd = St::fetch(A, kh, vh, pg, j0, end, lk, lv, wide(j0)) || odd;
+        }
+        __syncthreads();
+        const uint8_t* ck = lk + buf * kTile;
+        const uint8_t* cv = lv + buf * kTile;
+        // (past the end the loads repeat the last rows)
+        pg = page_ok(A, pn, bad);
+        if (kTwo) st.load(A, kh, vh, pg, jn, end);
+        pn = St::page(A, tab, jn + ROWS, end);
         if (j0 < any_hi && j0 + ROWS > any_lo) {
             const bool mask = j0 + ROWS > all_hi || j0 < all_lo;
             if constexpr (HD <= 128) {
-                step<CK, HD, EX, 2>(A, qf, a, lk, lv, j0, P.c, mask, cl.vlo, cl.vhi);
+                step<CK, HD, EX, 2>(A, qf, a, ck, cv, j0, P.c, mask, cl.vlo, cl.vhi);
             } else {  // (registers)
 #pragma unroll 1
                 for (int u = 0; u < 64; u += 32)
-                    step<CK, HD, EX, 1>(A, qf, a, lk + u * Geo<HD>::pk, lv + u * Geo<HD>::pv, j0 + u, P.c, mask, cl.vlo,
+                    step<CK, HD, EX, 1>(A, qf, a, ck + u * Geo<HD>::pk, cv + u * Geo<HD>::pv, j0 + u, P.c, mask, cl.vlo,
                                         cl.vhi);
             }
         }
+        if (kTwo && jn < end) {
+            buf ^= 1;
+            odd = st.store(lk + buf * kTile, lv + buf * kTile, end - jn, wide(jn)) || odd;
+        }
     }
+    if (odd) any_odd = 1;
     __syncthreads();
     if (KIND != VGX_E_Q8 && any_odd) {
         for (int j0 = start; j0 < end; j0 += ROWS) {
-            if (j0 + ROWS <= tile_hi && j0 >= tile_lo) continue;
+            if (!wide(j0)) continue;
             __syncthreads();
-            St::fetch_v(A, vh, St::page(A, tab, j0, end), j0, end, uni, lv);
+            St::fetch_v(A, vh, page_ok(A, St::page(A, tab, j0, end), bad), j0, end, lv);
             __syncthreads();
             // (as the loop above skips and masks)
             if (j0 >= any_hi || j0 + ROWS <= any_lo) continue;
@@ -917,6 +943,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(cons
                 }
         }
     }
+    if (bad) set_fault(A, VGX_FAULT_PAGE);
     const float L = half_sum(a.l);
     if (!cl.valid) return;
     const int hh = lane >> 5;
@@ -1055,37 +1082,42 @@ void fn_of(int64_t cols, Plan& p) {
         p.rows = true;
     } else {
         p.fn = paged_tile_kernel<KIND, HD, EX>;
-        p.lds = 64 * (Geo<HD>::pk + Geo<HD>::pv);
+        p.lds = (HD <= 128 ? 2 : 1) * 64 * (Geo<HD>::pk + Geo<HD>::pv);
         p.tm = 128;
         p.rows = false;
     }
 }
 template <int KIND>
-void fn_of(int hd, int64_t cols, Plan& p) {
-    switch (hd) {
+void fn_of(const PagedDev& A, int64_t cols, Plan& p) {
+    const int hd = A.hd;
+    const bool whole = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
+    if (whole) switch (hd) {
         case 64: return fn_of<KIND, 64, true>(cols, p);
         case 96: return fn_of<KIND, 96, true>(cols, p);
         case 128: return fn_of<KIND, 128, true>(cols, p);
         case 256: return fn_of<KIND, 256, true>(cols, p);
     }
-    return hd < 128 ? fn_of<KIND, 128, false>(cols, p) : fn_of<KIND, 256, false>(cols, p);
+    return hd <= 128 ? fn_of<KIND, 128, false>(cols, p) : fn_of<KIND, 256, false>(cols, p);
 }
 
 Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     Plan p{};
     const int64_t cols = (int64_t)A.max_q * A.grp;
-    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A.hd, cols, p);
-    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A.hd, cols, p);
-    else fn_of<VGX_E_Q8>(A.hd, cols, p);
+    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, p);
+    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, p);
+    else fn_of<VGX_E_Q8>(A, cols, p);
     // (a sequence with rows has at most rows * grp / tm + 1 tiles)
     const int64_t tiles = p.rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
     p.wgs = tiles * A.kvh;
     int64_t span = A.max_kv;
     if (window > 0) span = std::min<int64_t>(span, (int64_t)window + p.tm + 64);
-    // enough workgroups for four a CU, splits of 256 keys or more
-    const int64_t want = std::max<int64_t>(1, (int64_t)num_cu * 4 / p.wgs);
+    // Two workgroups a CU are resident; splits of 256 keys or more.  Sequences
+    // of different lengths: no split above 1024 keys, or the longest sequence's
+    // workgroups would run after all others.
+    const int64_t want = std::max<int64_t>(1, (int64_t)num_cu * (p.rows && A.nseq > 1 ? 6 : 2) / p.wgs);
     int64_t len = (span + want - 1) / want;
-    len = std::max<int64_t>((len + 255) / 256 * 256, 256);
+    if (p.rows && A.nseq > 1) len = std::min<int64_t>(len, 1024);
+    len = std::max<int64_t>((len + 127) / 128 * 128, 256);
     int64_t n = (span + len - 1) / len;
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX / 2);
     p.nsplit = (int)std::max<int64_t>(n, 1);
