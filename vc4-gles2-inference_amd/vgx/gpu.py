@@ -18,6 +18,11 @@ def _ptr(t):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+# the handle of torch's current stream on a device (an int)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _at(t):
     return 0 if t is None else t.data_ptr()
 
@@ -300,6 +305,7 @@ class PagedCache:
                 raise ValueError("%s must be (pages, %d, page_size, %d), head vectors contiguous" % (name, kv_heads,
                                                                                                    head_dim))
         self.gpu, self.heads, self.kv_heads, self.head_dim, self.kind = gpu, heads, kv_heads, head_dim, kind
+        self.ckind = _ELEM[self.qtype]
         self.k, self.v, self.width = k, v, heads * head_dim
         self.d = _l.Paged(heads, kv_heads, head_dim, k.shape[2], k.shape[0], elem, k_step, v_step, k.data_ptr(),
                           v.data_ptr(), *k.stride()[:3], *v.stride()[:3])
@@ -328,9 +334,10 @@ class PagedCache:
                 g.need(t, torch.float32, 1, "a norm weight")
                 if t.shape[0] != self.head_dim or t.stride(0) != 1:
                     raise ValueError("a norm weight must be %d contiguous values" % self.head_dim)
-        q = out if out is not None else torch.empty((batch.ntok, self.heads, self.head_dim), dtype=self.qtype,
-                                                    device=g.device)
-        qs = self._rows(q, self.qtype, batch.ntok, "out")
+        if out is None:
+            q, qs = torch.empty((batch.ntok, self.heads, self.head_dim), dtype=self.qtype, device=g.device), self.width
+        else:
+            q, qs = out, self._rows(out, self.qtype, batch.ntok, "out")
         r = _l.PagedRows(_ELEM[qkv.dtype], qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), _at(cos), _at(sin), npos,
                          rot, int(rope_half), _at(q_norm), _at(k_norm), eps, q.data_ptr(), qs)
         g.on_current(_l.load().vgx_paged_append, self.ref, batch.ref, ctypes.byref(r))
@@ -343,9 +350,10 @@ class PagedCache:
         g = self.gpu
         qs = self._rows(q, self.qtype, batch.ntok, "q")
         if out is None:
-            out = torch.empty((batch.ntok, self.width), dtype=self.qtype, device=g.device)
-        kind = _l.E_Q16 if out.dtype == torch.int16 else _ELEM[self.qtype]
-        os_ = self._rows(out, out.dtype if kind == _l.E_Q16 else self.qtype, batch.ntok, "out")
+            out, kind, os_ = torch.empty((batch.ntok, self.width), dtype=self.qtype, device=g.device), self.ckind, self.width
+        else:
+            kind = _l.E_Q16 if out.dtype == torch.int16 else self.ckind
+            os_ = self._rows(out, out.dtype if kind == _l.E_Q16 else self.qtype, batch.ntok, "out")
         key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window)
         need = batch.ws.get(key)
         L = _l.load()
@@ -359,13 +367,15 @@ class PagedCache:
 
     def _rows(self, t, dtype, n, name):
         """The stride of n rows of heads x head_dim values, (n, heads, head_dim) or (n, heads * head_dim)."""
-        if t.dim() == 3:
-            if t.shape[1] != self.heads or t.shape[2] != self.head_dim or t.stride(1) != self.head_dim:
-                raise ValueError("%s must be (%d, %d, %d), a row's heads contiguous" % (name, n, self.heads,
-                                                                                      self.head_dim))
-            t = t.flatten(1)
-        self.gpu.need_rows(t, dtype, n, self.width, name)
-        return max(t.stride(0), self.width)
+        if t.dim() != 3:
+            self.gpu.need_rows(t, dtype, n, self.width, name)
+            return max(t.stride(0), self.width)
+        self.gpu.need(t, dtype, 3, name)
+        rows, heads, hd = t.shape
+        st = t.stride()
+        if rows < n or heads != self.heads or hd != self.head_dim or st[2] != 1 or (heads > 1 and st[1] != hd):
+            raise ValueError("%s must be (%d, %d, %d), a row's heads contiguous" % (name, n, self.heads, self.head_dim))
+        return max(st[0], self.width)
 
 
 class GPU:
@@ -376,6 +386,7 @@ class GPU:
         h = ctypes.c_void_p()
         _l.check(L.vgx_ctx_create(device, ctypes.byref(h)))
         self.ctx, self.device = h, torch.device("cuda", device)
+        self._get_stream = L.vgx_ctx_stream
         self.use_torch_stream()
 
     def use_torch_stream(self):
@@ -388,20 +399,20 @@ class GPU:
     def on_current(self, call, *args):
         """call(ctx, *args) on torch's current stream of this device, where
         its tensors were made; the context's stream is put back after."""
-        L = _l.load()
-        now, was = torch.cuda.current_stream(self.device).cuda_stream, L.vgx_ctx_stream(self.ctx) or 0
+        now, was = _raw_stream(self.device.index), self._get_stream(self.ctx) or 0
         if now == was:
-            _l.check(call(self.ctx, *args))
-            return
-        _l.check(L.vgx_ctx_set_stream(self.ctx, now))
-        try:
-            _l.check(call(self.ctx, *args))
-        finally:
+            st = call(self.ctx, *args)
+        else:
+            L = _l.load()
+            _l.check(L.vgx_ctx_set_stream(self.ctx, now))
+            st = call(self.ctx, *args)
             L.vgx_ctx_set_stream(self.ctx, was)
+        if st:
+            _l.check(st)
 
     def need(self, t, dtype, dims, name):
         """Refuses a tensor of another device, type or number of dimensions."""
-        if t.device != self.device or t.dim() != dims or t.dtype != (dtype or t.dtype):
+        if t.dim() != dims or (dtype is not None and t.dtype is not dtype) or t.device != self.device:
             raise ValueError("%s must be a %d-dimensional %s tensor on %s, not %s on %s" % (
                 name, dims, dtype or t.dtype, self.device, t.dtype, t.device))
 
@@ -605,7 +616,7 @@ class GPU:
         (rows qstart[s] .. qstart[s+1]-1).  draft: the logits the drafts were
         drawn from; temp: a temperature a sequence (0: greedy).  Returns
         (accepted drafts and next token of each sequence, the target's
-        probability of each drafted token)."""
+        probability of each drafted token); rows of no sequence have none."""
         self.need(qstart, torch.int32, 1, "qstart")
         self.need(tokens, torch.int32, 1, "tokens")
         nseq, n = qstart.shape[0] - 1, tokens.shape[0]
@@ -627,8 +638,7 @@ class GPU:
                 raise ValueError("qstart, tokens, the random numbers and temp must be contiguous")
         L, kind = _l.load(), _ELEM[logits.dtype]
         acc_next = torch.empty((2, nseq), dtype=torch.int32, device=self.device)
-        # rows of no sequence keep a probability of 0
-        prob = torch.zeros(n, dtype=torch.float32, device=self.device)
+        prob = torch.empty(n, dtype=torch.float32, device=self.device)
         need = int(L.vgx_draft_verify_ws(nseq, n, vocab, kind, int(draft is not None)))
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         a = _l.Draft(nseq, n, vocab, qstart.data_ptr(), tokens.data_ptr(), kind, logits.data_ptr(),
