@@ -329,15 +329,28 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
     const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
     f32x16 s[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < HD / 16; ++t) {
-            if (!EX && 16 * t >= A.hd) continue;
+    for (int t = 0; t < HD / 16; ++t) {
+        if (!EX && 16 * t >= A.hd) continue;
+        // (reads far ahead of their products would spill)
+        if (HD > 128 && t % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
             const s16x8 kf = *reinterpret_cast<const s16x8*>(lk + (kb * 32 + col) * Geo<HD>::pk + (2 * t + h) * 16);
             s[kb] = mfma<CK>(kf, q[t], s[kb]);
         }
+    }
+    if constexpr (EX && HD <= 128) {  // four reads ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int t = 0; t < (KB * HD / 16 - 4) / 2; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
     if (mask) {
 #pragma unroll
@@ -593,17 +606,17 @@ constexpr int rows_lds(int hd) {
 }
 
 // Few rows a sequence (max_q * grp <= 16 NB): a workgroup is one sequence, KV
-// head and split; its 4 waves hold the same NB blocks of 16 columns and take
+// head and split; its WV waves hold the same NB blocks of 16 columns and take
 // tiles of 32 keys in turn, without a barrier, and join at the end.  The 16x16x32
 // product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
 // the lane; two of them are the next product's B operand.
-template <int KIND, int HD, bool EX, int NB>
-__global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
+template <int KIND, int HD, bool EX, int NB, int WV>
+__global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_rows_kernel(const AttnArgs P) {
     using Ks = Keys<KIND, HD, EX>;
     constexpr int CK = Ks::CK, KS = HD / 32, DB = HD / 16;
     constexpr int kWave = rows_lds(HD);
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float sm[4][16 * NB], sl[4][16 * NB];
+    __shared__ float sm[WV][16 * NB], sl[WV][16 * NB];
     const PagedDev& A = P.A;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
@@ -625,7 +638,7 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     bool bad = false, odd = false;
     if (j0 < end) {
         pg = Ks::page(A, tab, j0, end);
-        pn = Ks::page(A, tab, j0 + 128, end);
+        pn = Ks::page(A, tab, j0 + 32 * WV, end);
     }
     Col cl[NB];
     s16x8 qf[NB][KS];
@@ -664,11 +677,11 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     // them each product waits for its own loads only)
     while (j0 < end) {
         const bool mask = j0 + 32 > all_hi || j0 < all_lo;
-        const int jn = j0 + 128;
+        const int jn = j0 + 32 * WV;
         wave_sync();
         odd = t.store_v(lv, end - j0, mask) || odd;
         pg = page_ok(A, pn, bad);
-        pn = Ks::page(A, tab, jn + 128, end);
+        pn = Ks::page(A, tab, jn + 32 * WV, end);
         t.load_v(A, vh, pg, jn, end);
         f32x4 sc[NB][2];
 #pragma unroll
@@ -728,7 +741,7 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
         j0 = jn;
     }
     if (KIND != VGX_E_Q8 && __any(odd)) {
-        for (j0 = start + wave * 32; j0 < end; j0 += 128) {
+        for (j0 = start + wave * 32; j0 < end; j0 += 32 * WV) {
             if (j0 + 32 <= all_hi && j0 >= all_lo) continue;
             t.load_v(A, vh, page_ok(A, Ks::page(A, tab, j0, end), bad), j0, end);
             wave_sync();
@@ -760,11 +773,11 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
     for (int b = 0; b < NB; ++b) {
         float M = sm[0][16 * b + col];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) M = fmaxf(M, sm[w][16 * b + col]);
+        for (int w = 1; w < WV; ++w) M = fmaxf(M, sm[w][16 * b + col]);
         const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
         float L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) L = fmaf(sl[w][16 * b + col], exp2_(fmaf(sm[w][16 * b + col], P.c, -mc)), L);
+        for (int w = 0; w < WV; ++w) L = fmaf(sl[w][16 * b + col], exp2_(fmaf(sm[w][16 * b + col], P.c, -mc)), L);
         const float f = exp2_(fmaf(m[b], P.c, -mc));
         if (b) __syncthreads();
 #pragma unroll
@@ -776,13 +789,13 @@ __global__ void __launch_bounds__(256) paged_rows_kernel(const AttnArgs P) {
         // thread: column lane % 16, every sixteenth group of 4 dims
         const int64_t at = ((int64_t)split * A.ntok + cl[b].row) * A.heads + cl[b].head;
         const float r = whole ? inv_l(P, L) : 1.0f;
-        for (int d = 4 * (threadIdx.x >> 4); d < A.hd; d += 64) {
+        for (int d = 4 * (threadIdx.x >> 4); d < A.hd; d += 16 * WV) {
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 x[e] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) x[e] += reinterpret_cast<const float*>(smem + w * kWave)[(d + e) * 16 + col];
+                for (int w = 0; w < WV; ++w) x[e] += reinterpret_cast<const float*>(smem + w * kWave)[(d + e) * 16 + col];
                 x[e] *= r;
             }
             const float4 v = make_float4(x[0], x[1], x[2], x[3]);
@@ -837,7 +850,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(cons
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int any_odd;
     const PagedDev& A = P.A;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 31;
     // the last tiles, which see the most keys, first
     const int rev = blockIdx.x / A.kvh, h = blockIdx.x - rev * A.kvh;
     const int tile = gridDim.x / A.kvh - 1 - rev;
@@ -985,17 +999,20 @@ __device__ __forceinline__ int splits_of(const AttnArgs& P, int t, int head) {
     return span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len).nsp;
 }
 
-// Joins a row's splits.  Few splits (WIDE false): a wave a row and head, in
-// split order.  Many: a workgroup a row and head, the splits dealt to groups
-// of hd / 4 threads, each in split order, the groups in theirs.
+// Joins a row's splits.  Few splits (WIDE false): hd / 4 lanes (rounded up to a
+// power of two, lg) a row and head, in split order.  Many: a workgroup a row and
+// head, the splits dealt to groups of hd / 4 threads, each in split order, the
+// groups in theirs.
 template <int CK, bool WIDE>
-__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int lg) {
     const PagedDev& A = P.A;
     __shared__ float sw[4], sl[4];
     __shared__ float4 so[256];
     const int lane = threadIdx.x & 63;
-    const int64_t w = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(w / A.heads), head = (int)(w - (int64_t)t * A.heads);
+    // (a wave's lanes are of one row: lg divides so, or is 6)
+    const int64_t w0 = WIDE ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - lg);
+    const int t = (int)(w0 / A.heads);
+    const int head = (int)(w0 - (int64_t)t * A.heads) + (WIDE ? 0 : lane >> lg);
     if (t >= A.ntok) return;
     const int nsp = splits_of(P, t, head);
     if (nsp <= 1) return;
@@ -1013,7 +1030,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P) {
             const float2 x = ml[k * step];
             const float f = exp2_(fmaf(x.x, P.c, -mc));
             L = fmaf(x.y, f, L);
-            const float4 y = po[(at + k * step) * n4 + min(lane, n4 - 1)];
+            const float4 y = po[(at + k * step) * n4 + min(lane & ((1 << lg) - 1), n4 - 1)];
             o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
         }
     } else {
@@ -1050,16 +1067,20 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P) {
             o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
         }
     }
-    const int d = WIDE ? threadIdx.x : lane;
+    const int d = WIDE ? threadIdx.x : lane & ((1 << lg) - 1);
     const float r = inv_l(P, L);
     if (d < n4) put_out<CK>(P, t, head, 4 * d, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
     if (d == 0 && P.lse) P.lse[at] = lse_of(P, M, L);
 }
 
 typedef void (*AttnFn)(const AttnArgs);
+typedef void (*JoinFn)(const AttnArgs, int);
+// Positions up to which 8 waves of one workgroup take a sequence whole.
+constexpr int64_t kWhole = 1024;
+
 struct Plan {
     AttnFn fn;
-    int lds, tm;
+    int lds, tm, threads;
     bool rows;
     int64_t wgs;       // workgroups of one split
     int split_len, nsplit;
@@ -1067,17 +1088,23 @@ struct Plan {
 };
 
 // cols: the columns a sequence may have in a KV head.  Up to 48 the rows kernel
-// (16 for heads of more than 128 values; more columns fill the registers).
+// (16 for heads of more than 128 values; more columns fill the registers): 8
+// waves where one workgroup is to take a whole sequence.
 template <int KIND, int HD, bool EX>
-void fn_of(int64_t cols, Plan& p) {
+void fn_of(int64_t cols, int64_t span, Plan& p) {
+    p.threads = 256;
     if (cols <= (HD <= 128 ? 48 : 16)) {
         const int nb = (int)(cols + 15) / 16;
-        p.fn = paged_rows_kernel<KIND, HD, EX, 1>;
+        p.fn = paged_rows_kernel<KIND, HD, EX, 1, 4>;
         if constexpr (HD <= 128) {
-            if (nb == 2) p.fn = paged_rows_kernel<KIND, HD, EX, 2>;
-            if (nb == 3) p.fn = paged_rows_kernel<KIND, HD, EX, 3>;
+            if (nb == 1 && span <= kWhole) {
+                p.fn = paged_rows_kernel<KIND, HD, EX, 1, 8>;
+                p.threads = 512;
+            }
+            if (nb == 2) p.fn = paged_rows_kernel<KIND, HD, EX, 2, 4>;
+            if (nb == 3) p.fn = paged_rows_kernel<KIND, HD, EX, 3, 4>;
         }
-        p.lds = 4 * rows_lds(HD);
+        p.lds = p.threads / 64 * rows_lds(HD);
         p.tm = 16 * nb;
         p.rows = true;
     } else {
@@ -1088,36 +1115,40 @@ void fn_of(int64_t cols, Plan& p) {
     }
 }
 template <int KIND>
-void fn_of(const PagedDev& A, int64_t cols, Plan& p) {
+void fn_of(const PagedDev& A, int64_t cols, int64_t span, Plan& p) {
     const int hd = A.hd;
     const bool whole = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     if (whole) switch (hd) {
-        case 64: return fn_of<KIND, 64, true>(cols, p);
-        case 96: return fn_of<KIND, 96, true>(cols, p);
-        case 128: return fn_of<KIND, 128, true>(cols, p);
-        case 256: return fn_of<KIND, 256, true>(cols, p);
+        case 64: return fn_of<KIND, 64, true>(cols, span, p);
+        case 96: return fn_of<KIND, 96, true>(cols, span, p);
+        case 128: return fn_of<KIND, 128, true>(cols, span, p);
+        case 256:
+            if constexpr (KIND != VGX_E_Q8) return fn_of<KIND, 256, true>(cols, span, p);  // (q8: it would spill)
     }
-    return hd <= 128 ? fn_of<KIND, 128, false>(cols, p) : fn_of<KIND, 256, false>(cols, p);
+    return hd <= 128 ? fn_of<KIND, 128, false>(cols, span, p) : fn_of<KIND, 256, false>(cols, span, p);
 }
 
 Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     Plan p{};
     const int64_t cols = (int64_t)A.max_q * A.grp;
-    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, p);
-    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, p);
-    else fn_of<VGX_E_Q8>(A, cols, p);
+    int64_t span = A.max_kv;
+    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + 192);  // a tile's rows, lo's rounding
+    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, span, p);
+    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, span, p);
+    else fn_of<VGX_E_Q8>(A, cols, span, p);
     // (a sequence with rows has at most rows * grp / tm + 1 tiles)
     const int64_t tiles = p.rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
     p.wgs = tiles * A.kvh;
-    int64_t span = A.max_kv;
-    if (window > 0) span = std::min<int64_t>(span, (int64_t)window + p.tm + 64);
-    // Two workgroups a CU are resident; splits of 256 keys or more.  Sequences
-    // of different lengths: no split above 1024 keys, or the longest sequence's
-    // workgroups would run after all others.
-    const int64_t want = std::max<int64_t>(1, (int64_t)num_cu * (p.rows && A.nseq > 1 ? 6 : 2) / p.wgs);
+    // Two workgroups a CU are resident (three of the tile kernel at heads of up
+    // to 64); splits of 256 keys or more.  Sequences of different lengths: no
+    // split above 1024 keys, or the longest sequence's workgroups would run
+    // after all others.
+    const int fill = p.rows ? (A.nseq > 1 ? 6 : 2) : A.hd <= 64 ? 3 : 2;
+    const int64_t want = std::max<int64_t>(1, (int64_t)num_cu * fill / p.wgs);
     int64_t len = (span + want - 1) / want;
     if (p.rows && A.nseq > 1) len = std::min<int64_t>(len, 1024);
     len = std::max<int64_t>((len + 127) / 128 * 128, 256);
+    if (p.threads == 512) len = std::max<int64_t>(span, 1);
     int64_t n = (span + len - 1) / len;
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX / 2);
     p.nsplit = (int)std::max<int64_t>(n, 1);
@@ -1180,18 +1211,20 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     VGX_HIP(hipSetDevice(ctx->device));
     if (p.lds > 64 * 1024)
         VGX_HIP(hipFuncSetAttribute((const void*)p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds));
-    hipLaunchKernelGGL(p.fn, dim3((unsigned)p.wgs, (unsigned)p.nsplit), dim3(256), p.lds, ctx->stream, P);
+    hipLaunchKernelGGL(p.fn, dim3((unsigned)p.wgs, (unsigned)p.nsplit), dim3(p.threads), p.lds, ctx->stream, P);
     VGX_LAUNCH_CHECK("paged attention launch");
     if (p.nsplit > 1) {
         const int64_t jobs = (int64_t)A.ntok * A.heads;
         // (a row's partials one after the other cost a round trip each four)
         const bool wide = p.nsplit > 8 && jobs < (1 << 24);
         const bool bf = compute_kind(cache->kind) == VGX_E_BF16;
-        const AttnFn join = wide ? (bf ? paged_join_kernel<VGX_E_BF16, true> : paged_join_kernel<VGX_E_F16, true>)
+        const JoinFn join = wide ? (bf ? paged_join_kernel<VGX_E_BF16, true> : paged_join_kernel<VGX_E_F16, true>)
                                  : (bf ? paged_join_kernel<VGX_E_BF16, false> : paged_join_kernel<VGX_E_F16, false>);
-        const int64_t grid = wide ? jobs : (jobs + 3) / 4;
+        int lg = A.hd <= 64 ? 4 : A.hd <= 128 ? 5 : 6;
+        if (A.heads % (64 >> lg)) lg = 6;  // a wave's heads would be of two rows
+        const int64_t grid = wide ? jobs : ((jobs >> (6 - lg)) + 3) / 4;
         if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
-        hipLaunchKernelGGL(join, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P);
+        hipLaunchKernelGGL(join, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P, lg);
         VGX_LAUNCH_CHECK("paged attention join launch");
     }
     return VGX_OK;
