@@ -51,7 +51,7 @@ struct AttnArgs {
     float* lse;
     float* po;     // nsplit x ntok x heads x hd partial sums
     float* pml;    // nsplit x ntok x heads x (m, l)
-    int tm;        // columns of a tile (what combine needs to find a row's span)
+    int* pn;       // ntok x heads: a row's splits
 };
 
 template <int CK>
@@ -151,9 +151,9 @@ static_assert(Geo<64>::pv == 192 && Geo<96>::pv == 192 && Geo<128>::pv == 320 &&
 __device__ __forceinline__ int page_at(const PagedDev& A, const int* tab, int j, int end) {
     return tab[page_of(A, min(j, end - 1))];
 }
-__device__ __forceinline__ int page_ok(const PagedDev& A, int pg, bool& bad) {
+__device__ __forceinline__ int page_ok(const PagedDev& A, int pg, bool& bad, bool used = true) {
     const bool in = (unsigned)pg < (unsigned)A.npages;
-    bad = bad || !in;
+    bad = bad || (used && !in);
     return in ? pg : 0;
 }
 
@@ -599,10 +599,10 @@ struct Keys {
     }
 };
 
-// LDS of one wave: its V tile; at the end 16 columns of sums.
-constexpr int rows_lds(int hd) {
+// LDS of one wave: its V tile; at the end its columns' sums.
+constexpr int rows_lds(int hd, int nb) {
     const int pv = (hd * 2 + 63) / 128 * 128 + 64;
-    return 32 * pv > hd * 64 ? 32 * pv : hd * 64;
+    return 32 * pv > nb * (hd + 4) * 64 ? 32 * pv : nb * (hd + 4) * 64;
 }
 
 // Few rows a sequence (max_q * grp <= 16 NB): a workgroup is one sequence, KV
@@ -611,33 +611,46 @@ constexpr int rows_lds(int hd) {
 // product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
 // the lane; two of them are the next product's B operand.
 template <int KIND, int HD, bool EX, int NB, int WV>
-__global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_rows_kernel(const AttnArgs P) {
+__global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256) ? 2 : 1) paged_rows_kernel(const AttnArgs P) {
     using Ks = Keys<KIND, HD, EX>;
     constexpr int CK = Ks::CK, KS = HD / 32, DB = HD / 16;
-    constexpr int kWave = rows_lds(HD);
+    constexpr int kWave = rows_lds(HD, NB);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float sm[WV][16 * NB], sl[WV][16 * NB];
     const PagedDev& A = P.A;
+    // Every argument into scalar registers before the first use of one: the
+    // loads then go out as one batch instead of a round trip at each first use.
+    asm volatile("" ::"s"(A.k), "s"(A.v), "s"(A.kpg), "s"(A.khd), "s"(A.krow), "s"(A.vpg), "s"(A.vhd), "s"(A.vrow),
+                 "s"(A.tstride), "s"(A.qstart), "s"(A.kvlen), "s"(A.table), "s"(P.q), "s"(P.qstride), "s"(P.out),
+                 "s"(P.po), "s"(P.split_len), "s"(P.window), "s"(P.c), "s"(A.kvh), "s"(A.grp), "s"(A.psize),
+                 "s"(A.pmul), "s"(A.npages), "s"(A.max_kv), "s"(A.ntok), "s"(A.heads), "s"(A.max_q), "s"(A.tcols));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int s = blockIdx.x / A.kvh, h = blockIdx.x - s * A.kvh;
+    const int split = blockIdx.y;
+    const int* tab = A.table + (int64_t)s * A.tstride;
+    // Without a window the keys begin at 0, so the table's entries are asked
+    // for along with the lengths (an entry past the sequence's end is not used).
+    int pg = 0;
+    if (P.window <= 0) {
+        const int64_t j = (int64_t)split * P.split_len + wave * 32 + (lane & 31);
+        pg = tab[min(page_of(A, (int)min(j, (int64_t)A.max_kv)), A.tcols - 1)];
+    }
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
     if (q.n <= 0) return;
     const Span sp = span_of(q, 0, q.n - 1, P.window, P.split_len);
-    const int split = blockIdx.y;
     if (split >= sp.nsp) return;
     const int start = sp.lo + split * P.split_len, end = min(sp.hi, start + P.split_len);
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
-    const int* tab = A.table + (int64_t)s * A.tstride;
     uint8_t* lv = smem + wave * kWave;
     Ks t;
     int j0 = start + wave * 32;
-    int pg = 0, pn = 0;
+    int pn = 0;
     bool bad = false, odd = false;
     if (j0 < end) {
-        pg = Ks::page(A, tab, j0, end);
+        if (P.window > 0) pg = Ks::page(A, tab, j0, end);
         pn = Ks::page(A, tab, j0 + 32 * WV, end);
     }
     Col cl[NB];
@@ -655,7 +668,7 @@ __global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_r
         }
     }
     if (j0 < end) {
-        pg = page_ok(A, pg, bad);
+        pg = page_ok(A, pg, bad, j0 + (lane & 31) < end);
         t.load_v(A, vh, pg, j0, end);
         t.load_k(A, kh, pg, j0, end);
     }
@@ -740,7 +753,7 @@ __global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_r
         }
         j0 = jn;
     }
-    if (KIND != VGX_E_Q8 && __any(odd)) {
+    if (KIND != VGX_E_Q8 && __builtin_expect(__any(odd), 0)) {
         for (j0 = start + wave * 32; j0 < end; j0 += 32 * WV) {
             if (j0 + 32 <= all_hi && j0 >= all_lo) continue;
             t.load_v(A, vh, page_ok(A, Ks::page(A, tab, j0, end), bad), j0, end);
@@ -758,47 +771,47 @@ __global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_r
                 }
         }
     }
-    if (bad) set_fault(A, VGX_FAULT_PAGE);
-    // the waves' sums on a common maximum, joined in wave order, 16 columns at
-    // a time through LDS
+    if (__builtin_expect(bad, 0)) set_fault(A, VGX_FAULT_PAGE);
+    // the waves' columns through LDS, each thread then joining its outputs in
+    // wave order on their common maximum
+    float* part = reinterpret_cast<float*>(smem + wave * kWave);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const float x = quad_sum(l[b]);
         if (lane < 16) { sm[wave][16 * b + col] = m[b]; sl[wave][16 * b + col] = x; }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+            *reinterpret_cast<f32x4*>(part + (16 * b + col) * (HD + 4) + 16 * d + 4 * g) = o[b][d];
     }
     __syncthreads();
     const bool whole = sp.nsp == 1;
-    float* part = reinterpret_cast<float*>(smem + wave * kWave);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        float M = sm[0][16 * b + col];
-#pragma unroll
-        for (int w = 1; w < WV; ++w) M = fmaxf(M, sm[w][16 * b + col]);
-        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
-        float L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WV; ++w) L = fmaf(sl[w][16 * b + col], exp2_(fmaf(sm[w][16 * b + col], P.c, -mc)), L);
-        const float f = exp2_(fmaf(m[b], P.c, -mc));
-        if (b) __syncthreads();
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[(16 * d + 4 * g + i) * 16 + col] = o[b][d][i] * f;
-        __syncthreads();
         if (!cl[b].valid) continue;
-        // thread: column lane % 16, every sixteenth group of 4 dims
+        float f[WV], M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WV; ++w) {
+            f[w] = sm[w][16 * b + col];
+            M = fmaxf(M, f[w]);
+        }
+        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+#pragma unroll
+        for (int w = 0; w < WV; ++w) {
+            f[w] = exp2_(fmaf(f[w], P.c, -mc));
+            L = fmaf(sl[w][16 * b + col], f[w], L);
+        }
         const int64_t at = ((int64_t)split * A.ntok + cl[b].row) * A.heads + cl[b].head;
         const float r = whole ? inv_l(P, L) : 1.0f;
+        // thread: column lane % 16, every (4 WV)-th group of 4 dims
         for (int d = 4 * (threadIdx.x >> 4); d < A.hd; d += 16 * WV) {
-            float x[4];
+            f32x4 x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = 0.0f;
+            for (int w = 0; w < WV; ++w) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(smem + w * kWave + ((16 * b + col) * (HD + 4) + d) * 4);
 #pragma unroll
-                for (int w = 0; w < WV; ++w) x[e] += reinterpret_cast<const float*>(smem + w * kWave)[(d + e) * 16 + col];
-                x[e] *= r;
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f[w], x[e]);
             }
-            const float4 v = make_float4(x[0], x[1], x[2], x[3]);
+            const float4 v = make_float4(x[0] * r, x[1] * r, x[2] * r, x[3] * r);
             if (whole) put_out<CK>(P, cl[b].row, cl[b].head, d, v);
             else *reinterpret_cast<float4*>(P.po + at * A.hd + d) = v;
         }
@@ -806,8 +819,10 @@ __global__ void __launch_bounds__(64 * WV, NB == 1 && HD <= 128 ? 2 : 1) paged_r
             if (!whole) {
                 P.pml[2 * at] = M;
                 P.pml[2 * at + 1] = L;
-            } else if (P.lse) {
-                P.lse[(int64_t)cl[b].row * A.heads + cl[b].head] = lse_of(P, M, L);
+                if (split == 0) P.pn[at] = sp.nsp;
+            } else {
+                if (P.nsplit > 1) P.pn[at] = 1;
+                if (P.lse) P.lse[at] = lse_of(P, M, L);
             }
         }
     }
@@ -979,24 +994,12 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(cons
         if (!whole) {
             P.pml[2 * at] = a.m;
             P.pml[2 * at + 1] = L;
-        } else if (P.lse) {
-            P.lse[(int64_t)cl.row * A.heads + cl.head] = lse_of(P, a.m, L);
+            if (split == 0) P.pn[at] = sp.nsp;
+        } else {
+            if (P.nsplit > 1) P.pn[at] = 1;
+            if (P.lse) P.lse[at] = lse_of(P, a.m, L);
         }
     }
-}
-
-// The splits of row t and head, as the kernels cut its tile (every lane
-// active); 0: not a row of the batch.
-__device__ __forceinline__ int splits_of(const AttnArgs& P, int t, int head) {
-    const PagedDev& A = P.A;
-    const int s = seq_of_row(A, t);
-    if (s >= A.nseq) return 0;
-    const SeqAt q = seq_at(A, s);
-    const int i = t - q.q0;
-    if (i < 0 || i >= q.n) return 0;
-    const int m = i * A.grp + head % A.grp;
-    const int m0 = m / P.tm * P.tm, m1 = min(m0 + P.tm, q.n * A.grp) - 1;
-    return span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len).nsp;
 }
 
 // Joins a row's splits.  Few splits (WIDE false): hd / 4 lanes (rounded up to a
@@ -1014,9 +1017,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
     const int t = (int)(w0 / A.heads);
     const int head = (int)(w0 - (int64_t)t * A.heads) + (WIDE ? 0 : lane >> lg);
     if (t >= A.ntok) return;
-    const int nsp = splits_of(P, t, head);
-    if (nsp <= 1) return;
     const int64_t step = (int64_t)A.ntok * A.heads, at = (int64_t)t * A.heads + head;
+    // (the entry of a row behind the last sequence was written by nobody)
+    const int nsp = t < A.qstart[A.nseq] ? P.pn[at] : 0;
+    if (nsp <= 1 || nsp > P.nsplit) return;
     const float2* ml = reinterpret_cast<const float2*>(P.pml) + at;
     const float4* po = reinterpret_cast<const float4*>(P.po);
     const int n4 = A.hd / 4;
@@ -1075,7 +1079,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
 
 typedef void (*AttnFn)(const AttnArgs);
 typedef void (*JoinFn)(const AttnArgs, int);
-// Positions up to which 8 waves of one workgroup take a sequence whole.
+// Positions up to which one workgroup takes a sequence whole.
 constexpr int64_t kWhole = 1024;
 
 struct Plan {
@@ -1088,23 +1092,26 @@ struct Plan {
 };
 
 // cols: the columns a sequence may have in a KV head.  Up to 48 the rows kernel
-// (16 for heads of more than 128 values; more columns fill the registers): 8
-// waves where one workgroup is to take a whole sequence.
+// (16 for heads of more than 128 values; more columns fill the registers).  few:
+// under half a workgroup a CU, each of a whole sequence of up to 1024 positions:
+// 8 waves then finish it sooner (8 sequences of 900, 8 / 4 heads of 96: 11.2 us
+// against 12.1 with 4 waves, 11.9 with 4 splits; 128 workgroups: 20.0 against
+// 18.7).
 template <int KIND, int HD, bool EX>
-void fn_of(int64_t cols, int64_t span, Plan& p) {
+void fn_of(int64_t cols, bool few, Plan& p) {
     p.threads = 256;
     if (cols <= (HD <= 128 ? 48 : 16)) {
         const int nb = (int)(cols + 15) / 16;
         p.fn = paged_rows_kernel<KIND, HD, EX, 1, 4>;
         if constexpr (HD <= 128) {
-            if (nb == 1 && span <= kWhole) {
+            if (nb == 1 && few) {
                 p.fn = paged_rows_kernel<KIND, HD, EX, 1, 8>;
                 p.threads = 512;
             }
             if (nb == 2) p.fn = paged_rows_kernel<KIND, HD, EX, 2, 4>;
             if (nb == 3) p.fn = paged_rows_kernel<KIND, HD, EX, 3, 4>;
         }
-        p.lds = p.threads / 64 * rows_lds(HD);
+        p.lds = p.threads / 64 * rows_lds(HD, nb);
         p.tm = 16 * nb;
         p.rows = true;
     } else {
@@ -1115,17 +1122,17 @@ void fn_of(int64_t cols, int64_t span, Plan& p) {
     }
 }
 template <int KIND>
-void fn_of(const PagedDev& A, int64_t cols, int64_t span, Plan& p) {
+void fn_of(const PagedDev& A, int64_t cols, bool few, Plan& p) {
     const int hd = A.hd;
     const bool whole = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     if (whole) switch (hd) {
-        case 64: return fn_of<KIND, 64, true>(cols, span, p);
-        case 96: return fn_of<KIND, 96, true>(cols, span, p);
-        case 128: return fn_of<KIND, 128, true>(cols, span, p);
+        case 64: return fn_of<KIND, 64, true>(cols, few, p);
+        case 96: return fn_of<KIND, 96, true>(cols, few, p);
+        case 128: return fn_of<KIND, 128, true>(cols, few, p);
         case 256:
-            if constexpr (KIND != VGX_E_Q8) return fn_of<KIND, 256, true>(cols, span, p);  // (q8: it would spill)
+            if constexpr (KIND != VGX_E_Q8) return fn_of<KIND, 256, true>(cols, few, p);  // (q8: it would spill)
     }
-    return hd <= 128 ? fn_of<KIND, 128, false>(cols, span, p) : fn_of<KIND, 256, false>(cols, span, p);
+    return hd <= 128 ? fn_of<KIND, 128, false>(cols, few, p) : fn_of<KIND, 256, false>(cols, few, p);
 }
 
 Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
@@ -1133,26 +1140,34 @@ Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     const int64_t cols = (int64_t)A.max_q * A.grp;
     int64_t span = A.max_kv;
     if (window > 0) span = std::min<int64_t>(span, (int64_t)window + 192);  // a tile's rows, lo's rounding
-    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, span, p);
-    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, span, p);
-    else fn_of<VGX_E_Q8>(A, cols, span, p);
+    const bool few = span <= kWhole && (int64_t)A.nseq * A.kvh < num_cu / 2;
+    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, few, p);
+    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, few, p);
+    else fn_of<VGX_E_Q8>(A, cols, few, p);
     // (a sequence with rows has at most rows * grp / tm + 1 tiles)
     const int64_t tiles = p.rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
     p.wgs = tiles * A.kvh;
-    // Two workgroups a CU are resident (three of the tile kernel at heads of up
-    // to 64); splits of 256 keys or more.  Sequences of different lengths: no
-    // split above 1024 keys, or the longest sequence's workgroups would run
-    // after all others.
-    const int fill = p.rows ? (A.nseq > 1 ? 6 : 2) : A.hd <= 64 ? 3 : 2;
+    // Splits.  A workgroup of the rows kernel costs about 8 us before and after
+    // its keys (the tables' and first rows' round trips, the join of its waves),
+    // so splits go no further than filling the chip once (two workgroups a CU
+    // are resident, three of the tile kernel at heads of up to 64).  One
+    // sequence: down to 256 keys.  Several, whose lengths the host does not
+    // know: 512 keys or more (24 x 6 rows over 2800 positions, 16 / 2 heads of
+    // 64: 26.6 us at 256, 19.2 at 512, 18.9 at 768, 27.8 at 2048), and no more
+    // than 768 (1024 where the sequences alone fill the CUs), or the longest
+    // one's workgroups run after all others (64 sequences of 200 to 16000
+    // positions: 111 us at 1024, 124 at 512).
+    const int fill = !p.rows && A.hd <= 64 ? 3 : 2;
     const int64_t want = std::max<int64_t>(1, (int64_t)num_cu * fill / p.wgs);
-    int64_t len = (span + want - 1) / want;
-    if (p.rows && A.nseq > 1) len = std::min<int64_t>(len, 1024);
-    len = std::max<int64_t>((len + 127) / 128 * 128, 256);
+    int64_t len = std::max<int64_t>((span + want - 1) / want, 256);
+    if (p.rows && A.nseq > 1)
+        len = span <= kWhole ? span : std::min<int64_t>(std::max<int64_t>(len, 512), p.wgs >= num_cu ? 1024 : 768);
+    len = (len + 127) / 128 * 128;
     if (p.threads == 512) len = std::max<int64_t>(span, 1);
     int64_t n = (span + len - 1) / len;
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX / 2);
     p.nsplit = (int)std::max<int64_t>(n, 1);
-    p.ws = p.nsplit > 1 ? (size_t)p.nsplit * A.ntok * A.heads * (A.hd + 2) * 4 : 0;
+    p.ws = p.nsplit > 1 ? (size_t)p.nsplit * A.ntok * A.heads * (A.hd + 2) * 4 + (size_t)A.ntok * A.heads * 4 : 0;
     return p;
 }
 
@@ -1201,13 +1216,13 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     P.window = r->window;
     P.split_len = p.split_len;
     P.nsplit = p.nsplit;
-    P.tm = p.tm;
     P.out_q16 = r->out_kind == VGX_E_Q16;
     P.out = static_cast<uint8_t*>(r->out);
     P.ostride = r->out_stride;
     P.lse = r->lse;
     P.po = static_cast<float*>(r->ws);
     P.pml = P.po ? P.po + (size_t)p.nsplit * A.ntok * A.heads * A.hd : nullptr;
+    P.pn = P.po ? reinterpret_cast<int*>(P.pml + (size_t)p.nsplit * A.ntok * A.heads * 2) : nullptr;
     VGX_HIP(hipSetDevice(ctx->device));
     if (p.lds > 64 * 1024)
         VGX_HIP(hipFuncSetAttribute((const void*)p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds));
