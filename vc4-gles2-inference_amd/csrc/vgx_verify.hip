@@ -19,11 +19,12 @@
 // The exponential: e^y = 2^k 2^(i/64) e^(f ln 2 / 64) with 64 y / ln 2 = 64 k + i
 // + f, |f| <= 1/2: a table of 64 powers in LDS and a polynomial of degree 4 in f
 // (error (ln 2 / 128)^5 / 120 < 4e-14); a table lookup instead of a polynomial of degree 11 or more
-// (P. T. P. Tang, ACM TOMS 15, 1989).  14 operations of 64 bits a logit: what
+// (P. T. P. Tang, ACM TOMS 15, 1989).  12 operations of 64 bits a logit: what
 // bounds launch 1, 16-bit logits coming in faster than that.
 #include <cfloat>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "vgx_internal.h"
 
@@ -118,9 +119,13 @@ __device__ __forceinline__ void piece(const Row& q, int vocab, int g, float (&x)
     }
 }
 
-// 2^(i / 64), written into LDS by every workgroup.
+// 2^(i / 64), written into LDS by every workgroup, less i 2^14 in the high word:
+// adding n 2^14 for n = 64 k + i then adds k to the exponent alone.
 __device__ __forceinline__ void fill_table(double* t) {
-    for (int i = threadIdx.x; i < 64; i += blockDim.x) t[i] = exp2((double)i * (1.0 / 64));
+    for (int i = threadIdx.x; i < 64; i += blockDim.x) {
+        const unsigned long long u = __builtin_bit_cast(unsigned long long, exp2((double)i * (1.0 / 64)));
+        t[i] = __builtin_bit_cast(double, u - ((unsigned long long)i << 46));
+    }
 }
 // x, m -> e^((x - m) / T) for x <= m: a = 64 / (T ln 2).  Below e^-690 the
 // weight stays there: nothing a sum of 1 or more would notice.
@@ -130,9 +135,9 @@ struct Scale {
 __device__ __forceinline__ Scale scale_of(float m, double inv) {
     return {inv * 92.33248261689366, m == -INFINITY ? 0.0 : (double)m};
 }
-__device__ __forceinline__ double exp_of(float x, const Scale& S, const double* tab) {
+// sum + 2^(z / 64), z in [-63700, 0].
+__device__ __forceinline__ double add_pow(double z, double sum, const double* tab) {
     const double big = 6755399441055744.0;  // 1.5 * 2^52: the low bits hold the rounded value
-    const double z = fmax(((double)x - S.m) * S.a, -63700.0);
     const double kb = z + big;
     const int n = (int)(unsigned)__builtin_bit_cast(unsigned long long, kb);
     const double f = z - (kb - big);
@@ -142,8 +147,11 @@ __device__ __forceinline__ double exp_of(float x, const Scale& S, const double* 
     e = fma(e, f, 0.010830424696249145);
     e = fma(e, f, 1.0);
     const unsigned long long t = __builtin_bit_cast(unsigned long long, tab[n & 63]);
-    const double p = __builtin_bit_cast(double, t + ((unsigned long long)(unsigned)(n >> 6) << 52));
-    return e * p;
+    const unsigned hi = (unsigned)(t >> 32) + ((unsigned)n << 14);
+    return fma(e, __builtin_bit_cast(double, (unsigned long long)hi << 32 | (unsigned)t), sum);
+}
+__device__ __forceinline__ double exp_of(float x, const Scale& S, const double* tab) {
+    return add_pow(fmax(((double)x - S.m) * S.a, -63700.0), 0.0, tab);
 }
 
 struct Temp {
@@ -189,9 +197,19 @@ __device__ __forceinline__ int seq_of(const VerifyArgs& P, int t) {
     return s;
 }
 
+// Launch 1's values: floats, or q16's integers (their differences are exact in
+// 32 bits, which spares three operations a logit).
+template <int KIND>
+using Val = std::conditional_t<KIND == VGX_E_Q16, int, float>;
+template <int KIND>
+constexpr Val<KIND> kNothing = KIND == VGX_E_Q16 ? (Val<KIND>)(-(1 << 30)) : (Val<KIND>)(-INFINITY);
+__device__ __forceinline__ float bigger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ int bigger(int a, int b) { return max(a, b); }
+
 template <int KIND, int K>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
+    using V = Val<KIND>;
     __shared__ double tab[64], sz[4];
     __shared__ float sm[4];
     __shared__ int sa[4];
@@ -199,26 +217,49 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     const bool draft = blockIdx.z;
     const Row q = row_at<KIND>(draft ? P.d : P.x, draft ? P.ds : P.xs, t);
     const int g0 = chunk * K * kThreads + threadIdx.x;
-    float x[K][N];
+    V x[K][N];
+    bool full[K];  // (a row's first and last piece may be short)
 #pragma unroll
-    for (int k = 0; k < K; ++k) piece<KIND>(q, P.vocab, g0 + k * kThreads, x[k]);
+    for (int k = 0; k < K; ++k) {
+        const int i0 = (g0 + k * kThreads) * N - q.off;
+        full[k] = i0 >= 0 && i0 + N <= P.vocab;
+        if constexpr (KIND == VGX_E_Q16) {
+            if (full[k]) {
+                const uint4 v = *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * 2);
+                const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[k][2 * i] = (short)(u[i] & 0xffff);
+                    x[k][2 * i + 1] = (int)u[i] >> 16;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? (int)reinterpret_cast<const short*>(q.p)[i0 + e]
+                                                               : kNothing<KIND>;
+            }
+        } else {
+            piece<KIND>(q, P.vocab, g0 + k * kThreads, x[k]);
+        }
+    }
     const int s = seq_of(P, t);
     fill_table(tab);
     if (s >= P.nseq) return;  // (uniform)
     const Temp T = temp_of(P, s);
-    float m = -INFINITY;
+    V best = kNothing<KIND>;
     int a = 0x7fffffff;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < N; ++e) m = fmaxf(m, x[k][e]);
+        for (int e = 0; e < N; ++e) best = bigger(best, x[k][e]);
     if (T.greedy) {  // the first index of the maximum
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
-                if (x[k][e] == m) a = (g0 + k * kThreads) * N - q.off + e;
+                if (x[k][e] == best) a = (g0 + k * kThreads) * N - q.off + e;
     }
+    float m = KIND == VGX_E_Q16 ? (best == kNothing<KIND> ? -INFINITY : (float)best * (1.0f / 256)) : (float)best;
     wave_best(m, a);
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) { sm[wave] = m; sa[wave] = a; }
@@ -231,10 +272,28 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     double z[2] = {0.0, 0.0};
     if (!T.greedy && m != -INFINITY) {
         const Scale S = scale_of(m, T.inv);
+        if constexpr (KIND == VGX_E_Q16) {
+            const double a256 = S.a * (1.0 / 256);
+            const int mi = (int)(m * 256.0f);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k) {
+                if (full[k]) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e & 1] += exp_of(x[k][e], S, tab);
+                    for (int e = 0; e < N; ++e) z[e & 1] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[e & 1], tab);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (x[k][e] != kNothing<KIND>)
+                            z[0] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[0], tab);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+        }
     }
     const double zs = wave_sum(z[0] + z[1]);
     if ((threadIdx.x & 63) == 0) sz[wave] = zs;
