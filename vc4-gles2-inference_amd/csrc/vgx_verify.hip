@@ -32,6 +32,8 @@
 
 namespace {
 
+typedef unsigned uint32x2 __attribute__((ext_vector_type(2)));
+
 struct VerifyArgs {
     int nseq, ntok, vocab;
     const int* qstart;
@@ -146,9 +148,9 @@ __device__ __forceinline__ double add_pow(double z, double sum, const double* ta
     e = fma(e, f, 5.86490495505617e-05);
     e = fma(e, f, 0.010830424696249145);
     e = fma(e, f, 1.0);
-    const unsigned long long t = __builtin_bit_cast(unsigned long long, tab[n & 63]);
-    const unsigned hi = (unsigned)(t >> 32) + ((unsigned)n << 14);
-    return fma(e, __builtin_bit_cast(double, (unsigned long long)hi << 32 | (unsigned)t), sum);
+    uint32x2 t = __builtin_bit_cast(uint32x2, tab[n & 63]);
+    t.y += (unsigned)n << 14;
+    return fma(e, __builtin_bit_cast(double, t), sum);
 }
 __device__ __forceinline__ double exp_of(float x, const Scale& S, const double* tab) {
     return add_pow(fmax(((double)x - S.m) * S.a, -63700.0), 0.0, tab);
@@ -173,10 +175,39 @@ __device__ __forceinline__ double weight(float x, float m, double inv, const dou
     return weight(x, scale_of(m, inv), tab);
 }
 
+// Lane exchanges inside rows of 16 lanes (quad_perm [1,0,3,2], [2,3,0,1],
+// row_half_mirror, row_mirror), the four rows then joined through readlane.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false); }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    const uint32x2 u = __builtin_bit_cast(uint32x2, x);
+    const uint32x2 v = {(unsigned)dpp<CTRL>((int)u.x), (unsigned)dpp<CTRL>((int)u.y)};
+    return __builtin_bit_cast(double, v);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) { return __int_as_float(dpp<CTRL>(__float_as_int(x))); }
+__device__ __forceinline__ double lane_of(double x, int l) {
+    const uint32x2 u = __builtin_bit_cast(uint32x2, x);
+    const uint32x2 v = {(unsigned)__builtin_amdgcn_readlane((int)u.x, l), (unsigned)__builtin_amdgcn_readlane((int)u.y, l)};
+    return __builtin_bit_cast(double, v);
+}
+__device__ __forceinline__ float lane_of(float x, int l) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
+    x += dpp<0xB1>(x);
+    x += dpp<0x4E>(x);
+    x += dpp<0x141>(x);
+    x += dpp<0x140>(x);
+    return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));
+    x = fmaxf(x, dpp<0x140>(x));
+    return fmaxf(fmaxf(lane_of(x, 0), lane_of(x, 16)), fmaxf(lane_of(x, 32), lane_of(x, 48)));
 }
 // (value, index): the larger value, the smaller index of equals.
 __device__ __forceinline__ void wave_best(float& m, int& a) {
@@ -203,6 +234,30 @@ template <int KIND>
 using Val = std::conditional_t<KIND == VGX_E_Q16, int, float>;
 template <int KIND>
 constexpr Val<KIND> kNothing = KIND == VGX_E_Q16 ? (Val<KIND>)(-(1 << 30)) : (Val<KIND>)(-INFINITY);
+template <int KIND>
+__device__ __forceinline__ void unpack(const uint4& v, Val<KIND> (&x)[kPer<KIND>]) {
+    const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (KIND == VGX_E_F32) {
+            x[i] = clean(__uint_as_float(u[i]));
+        } else if constexpr (KIND == VGX_E_Q16) {
+            x[2 * i] = (short)(u[i] & 0xffff);
+            x[2 * i + 1] = (int)u[i] >> 16;
+        } else if constexpr (KIND == VGX_E_BF16) {
+            x[2 * i] = clean(__uint_as_float(u[i] << 16));
+            x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
+        } else {
+            x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
+            x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
+        }
+    }
+}
+template <int KIND>
+__device__ __forceinline__ Val<KIND> one_v(const uint8_t* p, int i) {
+    if constexpr (KIND == VGX_E_Q16) return reinterpret_cast<const short*>(p)[i];
+    else return one<KIND>(p, i);
+}
 __device__ __forceinline__ float bigger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ int bigger(int a, int b) { return max(a, b); }
 
@@ -216,52 +271,46 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     const int chunk = blockIdx.x, t = blockIdx.y;
     const bool draft = blockIdx.z;
     const Row q = row_at<KIND>(draft ? P.d : P.x, draft ? P.ds : P.xs, t);
-    const int g0 = chunk * K * kThreads + threadIdx.x;
-    V x[K][N];
-    bool full[K];  // (a row's first and last piece may be short)
+    auto first = [&](int k) { return ((chunk * K + k) * kThreads + (int)threadIdx.x) * N - q.off; };
+    // (a row's first and last piece may be short: read value by value)
+    auto full = [&](int i0) { return i0 >= 0 && i0 + N <= P.vocab; };
+    uint4 raw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int i0 = (g0 + k * kThreads) * N - q.off;
-        full[k] = i0 >= 0 && i0 + N <= P.vocab;
-        if constexpr (KIND == VGX_E_Q16) {
-            if (full[k]) {
-                const uint4 v = *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * 2);
-                const unsigned u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[k][2 * i] = (short)(u[i] & 0xffff);
-                    x[k][2 * i + 1] = (int)u[i] >> 16;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? (int)reinterpret_cast<const short*>(q.p)[i0 + e]
-                                                               : kNothing<KIND>;
-            }
-        } else {
-            piece<KIND>(q, P.vocab, g0 + k * kThreads, x[k]);
-        }
+        raw[k] = make_uint4(0, 0, 0, 0);
+        if (full(first(k))) raw[k] = *reinterpret_cast<const uint4*>(q.p + (int64_t)first(k) * kBytes<KIND>);
     }
     const int s = seq_of(P, t);
     fill_table(tab);
     if (s >= P.nseq) return;  // (uniform)
     const Temp T = temp_of(P, s);
+    const int wave = threadIdx.x >> 6;
+    V x[K][N];
     V best = kNothing<KIND>;
-    int a = 0x7fffffff;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        unpack<KIND>(raw[k], x[k]);
+        const int i0 = first(k);
+        if (!full(i0)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? one_v<KIND>(q.p, i0 + e) : kNothing<KIND>;
+        }
 #pragma unroll
         for (int e = 0; e < N; ++e) best = bigger(best, x[k][e]);
+    }
+    float m = KIND == VGX_E_Q16 ? (best == kNothing<KIND> ? -INFINITY : (float)best * (1.0f / 256)) : (float)best;
+    int a = 0x7fffffff;
     if (T.greedy) {  // the first index of the maximum
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
-                if (x[k][e] == best) a = (g0 + k * kThreads) * N - q.off + e;
+                if (x[k][e] == best) a = first(k) + e;
+        wave_best(m, a);
+    } else {
+        m = wave_max(m);
     }
-    float m = KIND == VGX_E_Q16 ? (best == kNothing<KIND> ? -INFINITY : (float)best * (1.0f / 256)) : (float)best;
-    wave_best(m, a);
-    const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) { sm[wave] = m; sa[wave] = a; }
     __syncthreads();
     m = sm[0];
@@ -272,27 +321,26 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     double z[2] = {0.0, 0.0};
     if (!T.greedy && m != -INFINITY) {
         const Scale S = scale_of(m, T.inv);
-        if constexpr (KIND == VGX_E_Q16) {
-            const double a256 = S.a * (1.0 / 256);
-            const int mi = (int)(m * 256.0f);
+        const double a256 = S.a * (1.0 / 256);
+        const int mi = (int)(m * 256.0f);
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (full[k]) {
+        for (int k = 0; k < K; ++k) {
+            if constexpr (KIND == VGX_E_Q16) {
+                if (full(first(k))) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) z[e & 1] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[e & 1], tab);
+                    for (int e = 0; e < N; ++e)
+                        z[e & 1] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[e & 1], tab);
                 } else {
 #pragma unroll
                     for (int e = 0; e < N; ++e)
                         if (x[k][e] != kNothing<KIND>)
                             z[0] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[0], tab);
                 }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k)
+            } else {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
                     z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+            }
         }
     }
     const double zs = wave_sum(z[0] + z[1]);
