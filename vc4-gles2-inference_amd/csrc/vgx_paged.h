@@ -82,6 +82,6 @@ __device__ __forceinline__ Span span_of(const SeqAt& q, int first, int last, int
     r.hi = max(min(q.kv, base + last + 1), 0);
     r.lo = window > 0 ? max(base + first - window + 1, 0) & ~63 : 0;
     r.lo = min(r.lo, r.hi);
-    r.nsp = max((r.hi - r.lo + split_len - 1) / split_len, 1);
+    r.nsp = (int)max(((unsigned)(r.hi - r.lo) + (unsigned)split_len - 1) / (unsigned)split_len, 1u);
     return r;
 }

@@ -165,16 +165,36 @@ __device__ __forceinline__ uint2 pack8_q8(const float (&x)[8], float inv) {
 }
 
 // A head vector is LPV = 8, 16 or 32 lanes of 8 values (the least that holds
-// head_dim), so a wave takes 64 / LPV head vectors and a workgroup of 4 waves
-// 256 / LPV.  The rotation's partner values are loaded a second time (the
-// cache line is the wave's own) instead of exchanged: the partner of a piece
-// of 8 is a piece of 8.
-template <int KIND, int ACT, int LPV>
+// head_dim), so a wave takes 64 / LPV head vectors at a time and a workgroup of 4
+// waves 256 / LPV, PASS times (all loads first): the row's place, a chain of
+// three round trips, is then looked up once for them.  The rotation's partner
+// values are loaded a second time (the cache line is the wave's own) instead of
+// exchanged: the partner of a piece of 8 is a piece of 8.  Bound by bytes where
+// rows are many: 32 / 8 heads of 128, 4233
+// bf16 rows, 24.3 us (4.3 TB/s; 26.5 us with one pass).
+template <int KIND, int ACT, int LPV, int PASS>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs P) {
     const PagedDev& A = P.A;
     const int t = blockIdx.x / P.wpt, part = blockIdx.x - t * P.wpt;
     const int sub = threadIdx.x & (LPV - 1);
-    const int vec = part * (256 / LPV) + threadIdx.x / LPV;
+    const int d0 = sub * 8;
+    constexpr int ab = ACT == VGX_E_F32 ? 4 : 2, VPP = 256 / LPV;  // head vectors a pass
+    const uint8_t* row = P.x + (int64_t)t * P.stride * ab;
+    const int half = P.rot / 2;
+    const bool turn = d0 < P.rot, first = d0 < half;
+    const int partner = P.half && turn ? (first ? d0 + half : d0 - half) : d0;
+    const int ti = P.half ? (first ? d0 : d0 - half) : d0 / 2;  // the angle of the first value
+    float x[PASS][8], y[PASS][8];
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+        const int vec = (part * PASS + p) * VPP + threadIdx.x / LPV;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[p][e] = y[p][e] = 0.0f;
+        if (vec < P.vecs && d0 < A.hd) {
+            load8<ACT>(row + ((int64_t)vec * A.hd + d0) * ab, x[p]);
+            if (P.half && turn && vec < A.heads + A.kvh) load8<ACT>(row + ((int64_t)vec * A.hd + partner) * ab, y[p]);
+        }
+    }
     const int s = seq_of_row(A, t);
     if (s >= A.nseq) return;  // behind the last sequence
     const SeqAt sq = seq_at(A, s);
@@ -185,95 +205,90 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs P) {
         return;
     }
     if (i < 0 || i >= sq.n || pos < 0) return;
-    const int d0 = sub * 8;
-    const bool in = vec < P.vecs && d0 < A.hd;
-    const int ab = ACT == VGX_E_F32 ? 4 : 2;
-    const uint8_t* row = P.x + (int64_t)t * P.stride * ab;
-    const bool isv = vec >= A.heads + A.kvh, isq = vec < A.heads;
-    float x[8], y[8];
-    bool turn = false, first = false;
-    int ti = 0;  // the angle of x[0]
-    if (in) load8<ACT>(row + ((int64_t)vec * A.hd + d0) * ab, x);
-    else for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    const float* nw = isv ? nullptr : isq ? P.qn : P.kn;
-    int partner = d0;
-    if (in && !isv && d0 < P.rot) {
-        turn = true;
-        if (P.half) {
-            const int h = P.rot / 2;
-            first = d0 < h;
-            ti = first ? d0 : d0 - h;
-            partner = first ? d0 + h : d0 - h;
-            load8<ACT>(row + ((int64_t)vec * A.hd + partner) * ab, y);
-        } else {
-            ti = d0 / 2;
-        }
-    }
-    // 32-bit sum of squares over the head's lanes
-    if (P.qn) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-        for (int o = 1; o < LPV; o <<= 1) ss += __shfl_xor(ss, o, 64);
-        if (in && nw) {
-            const float r = 1.0f / sqrtf(ss / (float)A.hd + P.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * nw[d0 + e];
-            if (turn && P.half)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = y[e] * r * nw[partner + e];
-        }
-    }
-    if (turn) {
-        const float* c = P.cs + (int64_t)pos * (P.rot / 2) + ti;
-        const float* n = P.sn + (int64_t)pos * (P.rot / 2) + ti;
-        if (P.half) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = first ? fmaf(-y[e], n[e], x[e] * c[e]) : fmaf(y[e], n[e], x[e] * c[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = x[2 * e], b = x[2 * e + 1];
-                x[2 * e] = fmaf(-b, n[e], a * c[e]);
-                x[2 * e + 1] = fmaf(a, n[e], b * c[e]);
-            }
-        }
-    }
-    if (!in) return;
-    constexpr int CK = KIND == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16;
-    if (isq) {
-        if (P.q) *reinterpret_cast<uint4*>(P.q + ((int64_t)t * P.qstride + vec * A.hd + d0) * 2) = pack8<CK>(x);
-        return;
-    }
     const int pi = page_of(A, pos), slot = pos - pi * A.psize;
     const int pg = A.table[(int64_t)s * A.tstride + pi];
-    if (pg < 0 || pg >= A.npages) {
-        if (sub == 0) set_fault(A, VGX_FAULT_PAGE);
-        return;
+    float c[8], n[8];
+    if (turn && d0 < A.hd) {
+        const float* cp = P.cs + (int64_t)pos * half + ti;
+        const float* np = P.sn + (int64_t)pos * half + ti;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool use = P.half || e < 4;  // (neighbours: four angles)
+            c[e] = use ? cp[e] : 1.0f;
+            n[e] = use ? np[e] : 0.0f;
+        }
     }
-    const int h = isv ? vec - A.heads - A.kvh : vec - A.heads;
-    uint8_t* o = isv ? A.v + (int64_t)pg * A.vpg + (int64_t)h * A.vhd + (int64_t)slot * A.vrow
-                     : A.k + (int64_t)pg * A.kpg + (int64_t)h * A.khd + (int64_t)slot * A.krow;
-    if (KIND == VGX_E_Q8)
-        *reinterpret_cast<uint2*>(o + d0) = pack8_q8(x, 1.0f / (isv ? A.vstep : A.kstep));
-    else
-        *reinterpret_cast<uint4*>(o + d0 * 2) = pack8<KIND>(x);
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+        const int vec = (part * PASS + p) * VPP + threadIdx.x / LPV;
+        const bool in = vec < P.vecs && d0 < A.hd;
+        const bool isv = vec >= A.heads + A.kvh, isq = vec < A.heads;
+        // 32-bit sum of squares over the head's lanes
+        if (P.qn) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[p][e], x[p][e], ss);
+#pragma unroll
+            for (int o = 1; o < LPV; o <<= 1) ss += __shfl_xor(ss, o, 64);
+            if (in && !isv) {
+                const float* nw = isq ? P.qn : P.kn;
+                const float r = 1.0f / sqrtf(ss / (float)A.hd + P.eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[p][e] = x[p][e] * r * nw[d0 + e];
+                if (turn && P.half)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[p][e] = y[p][e] * r * nw[partner + e];
+            }
+        }
+        if (!in) continue;
+        if (turn && !isv) {
+            if (P.half) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[p][e] = fmaf(first ? -y[p][e] : y[p][e], n[e], x[p][e] * c[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[p][2 * e], b = x[p][2 * e + 1];
+                    x[p][2 * e] = fmaf(-b, n[e], a * c[e]);
+                    x[p][2 * e + 1] = fmaf(a, n[e], b * c[e]);
+                }
+            }
+        }
+        constexpr int CK = KIND == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16;
+        if (isq) {
+            if (P.q) *reinterpret_cast<uint4*>(P.q + ((int64_t)t * P.qstride + vec * A.hd + d0) * 2) = pack8<CK>(x[p]);
+            continue;
+        }
+        if (pg < 0 || pg >= A.npages) {
+            if (sub == 0) set_fault(A, VGX_FAULT_PAGE);
+            continue;
+        }
+        const int h = isv ? vec - A.heads - A.kvh : vec - A.heads;
+        uint8_t* o = isv ? A.v + (int64_t)pg * A.vpg + (int64_t)h * A.vhd + (int64_t)slot * A.vrow
+                         : A.k + (int64_t)pg * A.kpg + (int64_t)h * A.khd + (int64_t)slot * A.krow;
+        if (KIND == VGX_E_Q8)
+            *reinterpret_cast<uint2*>(o + d0) = pack8_q8(x[p], 1.0f / (isv ? A.vstep : A.kstep));
+        else
+            *reinterpret_cast<uint4*>(o + d0 * 2) = pack8<KIND>(x[p]);
+    }
 }
 
 typedef void (*AppendFn)(const AppendArgs);
-template <int KIND, int ACT>
+template <int KIND, int ACT, int PASS>
 AppendFn append_lpv(int lpv) {
-    return lpv == 8 ? append_kernel<KIND, ACT, 8> : lpv == 16 ? append_kernel<KIND, ACT, 16> : append_kernel<KIND, ACT, 32>;
+    return lpv == 8    ? append_kernel<KIND, ACT, 8, PASS>
+           : lpv == 16 ? append_kernel<KIND, ACT, 16, PASS>
+                       : append_kernel<KIND, ACT, 32, PASS>;
 }
 template <int KIND>
-AppendFn append_act(int act, int lpv) {
+AppendFn append_act(int act, int lpv, bool three) {
     switch (act) {
-        case VGX_E_F32: return append_lpv<KIND, VGX_E_F32>(lpv);
-        case VGX_E_BF16: return append_lpv<KIND, VGX_E_BF16>(lpv);
-        case VGX_E_F16: return append_lpv<KIND, VGX_E_F16>(lpv);
+        case VGX_E_F32: return three ? append_lpv<KIND, VGX_E_F32, 3>(lpv) : append_lpv<KIND, VGX_E_F32, 1>(lpv);
+        case VGX_E_BF16: return three ? append_lpv<KIND, VGX_E_BF16, 3>(lpv) : append_lpv<KIND, VGX_E_BF16, 1>(lpv);
+        case VGX_E_F16: return three ? append_lpv<KIND, VGX_E_F16, 3>(lpv) : append_lpv<KIND, VGX_E_F16, 1>(lpv);
     }
-    return append_lpv<KIND, VGX_E_Q16>(lpv);
+    return three ? append_lpv<KIND, VGX_E_Q16, 3>(lpv) : append_lpv<KIND, VGX_E_Q16, 1>(lpv);
 }
 
 }  // namespace
@@ -313,12 +328,16 @@ extern "C" int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_
     P.qstride = r->q_stride;
     P.vecs = A.heads + 2 * A.kvh;
     const int lpv = A.hd <= 64 ? 8 : A.hd <= 128 ? 16 : 32;
-    P.wpt = (P.vecs * lpv + 255) / 256;
+    // three passes a workgroup where the rows alone fill the chip (8 workgroups
+    // a CU are resident)
+    const int passes = (P.vecs * lpv + 255) / 256;
+    const bool three = passes > 1 && A.ntok >= 8 * ctx->num_cu;
+    P.wpt = three ? (passes + 2) / 3 : passes;
     const int64_t grid = (int64_t)A.ntok * P.wpt;
     if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_append: too many rows");  // 2^32 threads
-    const AppendFn fn = cache->kind == VGX_E_BF16  ? append_act<VGX_E_BF16>(r->kind, lpv)
-                        : cache->kind == VGX_E_F16 ? append_act<VGX_E_F16>(r->kind, lpv)
-                                                   : append_act<VGX_E_Q8>(r->kind, lpv);
+    const AppendFn fn = cache->kind == VGX_E_BF16  ? append_act<VGX_E_BF16>(r->kind, lpv, three)
+                        : cache->kind == VGX_E_F16 ? append_act<VGX_E_F16>(r->kind, lpv, three)
+                                                   : append_act<VGX_E_Q8>(r->kind, lpv, three);
     VGX_HIP(hipSetDevice(ctx->device));
     hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P);
     VGX_LAUNCH_CHECK("paged append launch");

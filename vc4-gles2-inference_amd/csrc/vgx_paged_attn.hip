@@ -32,7 +32,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
-typedef f16_t f16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -82,16 +81,13 @@ __device__ __forceinline__ float from_ct(short x) {
     if constexpr (CK == VGX_E_BF16) return __uint_as_float((unsigned)(unsigned short)x << 16);
     else return (float)__builtin_bit_cast(f16_t, x);
 }
-// Four cache bytes as two pairs of half floats, exact: 0x6400 | (b ^ 0x80) is
-// 1024 + 128 + b.
+// Four cache bytes as two pairs of half floats, exact.
 __device__ __forceinline__ uint2 q8_to_f16(unsigned w) {
-    const unsigned u = w ^ 0x80808080u;
-    const unsigned a = __builtin_amdgcn_perm(0x64646464u, u, 0x05010500u);
-    const unsigned b = __builtin_amdgcn_perm(0x64646464u, u, 0x05030502u);
-    const f16x2 off = {(f16_t)-1152.0f, (f16_t)-1152.0f};
+    const float a = (float)(signed char)w, b = (float)(signed char)(w >> 8), c = (float)(signed char)(w >> 16),
+                d = (float)((int)w >> 24);
     uint2 r;
-    r.x = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, a) + off);
-    r.y = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, b) + off);
+    r.x = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+    r.y = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(c, d));
     return r;
 }
 // Infinities and NaN among V.  Where a row does not see a key its weight is 0,
@@ -641,7 +637,7 @@ __global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256
     if (q.n <= 0) return;
     const Span sp = span_of(q, 0, q.n - 1, P.window, P.split_len);
     if (split >= sp.nsp) return;
-    const int start = sp.lo + split * P.split_len, end = min(sp.hi, start + P.split_len);
+    const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     uint8_t* lv = smem + wave * kWave;
@@ -858,7 +854,7 @@ __device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int tile, int
 // Many rows a sequence: a workgroup is a tile of 128 columns (4 waves x 32) of
 // one KV head; the waves share tiles of 64 keys.
 template <int KIND, int HD, bool EX>
-__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
+__global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
     constexpr int ROWS = 64, kTile = 64 * (Geo<HD>::pk + Geo<HD>::pv);
     using St = Stage<KIND, HD, EX>;
     constexpr int CK = St::CK;
@@ -880,7 +876,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) paged_tile_kernel(cons
     const Span sp = span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len);
     const int split = blockIdx.y;
     if (split >= sp.nsp) return;
-    const int start = sp.lo + split * P.split_len, end = min(sp.hi, start + P.split_len);
+    const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
     const Col cl = col_of(P, q, h, m0 + wave * 32 + col, end);
     s16x8 qf[HD / 16];
     load_q<HD, EX>(A, P.q + ((int64_t)cl.row * P.qstride + (int64_t)cl.head * A.hd) * 2, cl.valid, qf);
@@ -1165,13 +1161,34 @@ Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     len = (len + 127) / 128 * 128;
     if (p.threads == 512) len = std::max<int64_t>(span, 1);
     int64_t n = (span + len - 1) / len;
-    p.split_len = (int)std::min<int64_t>(len, INT32_MAX / 2);
+    p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
     p.nsplit = (int)std::max<int64_t>(n, 1);
     p.ws = p.nsplit > 1 ? (size_t)p.nsplit * A.ntok * A.heads * (A.hd + 2) * 4 + (size_t)A.ntok * A.heads * 4 : 0;
     return p;
 }
 
 }  // namespace
+
+// LDS past 64 KB is granted per kernel, once a context (not on the launch path).
+hipError_t vgx_paged_attn_init() {
+    for (int hd : {64, 96, 128, 256, 80, 144})      // (the last two: the kernels without an exact head)
+        for (int64_t cols : {16, 32, 48, 49})
+            for (bool few : {false, true})
+                for (int kind : {VGX_E_BF16, VGX_E_F16, VGX_E_Q8}) {
+                    PagedDev A{};
+                    A.hd = hd;
+                    A.psize = 16;
+                    Plan p{};
+                    if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, few, p);
+                    else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, few, p);
+                    else fn_of<VGX_E_Q8>(A, cols, few, p);
+                    if (p.lds <= 64 * 1024) continue;
+                    const hipError_t e =
+                        hipFuncSetAttribute((const void*)p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds);
+                    if (e != hipSuccess) return e;
+                }
+    return hipSuccess;
+}
 
 extern "C" {
 
@@ -1204,7 +1221,7 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     Plan p = plan_of(A, cache->kind, r->window, ctx->num_cu);
     if (p.nsplit > 1 && (!r->ws || r->ws_bytes < p.ws)) {
         p.nsplit = 1;
-        p.split_len = INT32_MAX / 2;
+        p.split_len = INT32_MAX;
     }
     if (p.wgs >= (1 << 24) || p.nsplit > 65535) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
     P.q = static_cast<const uint8_t*>(r->q);
@@ -1224,8 +1241,6 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     P.pml = P.po ? P.po + (size_t)p.nsplit * A.ntok * A.heads * A.hd : nullptr;
     P.pn = P.po ? reinterpret_cast<int*>(P.pml + (size_t)p.nsplit * A.ntok * A.heads * 2) : nullptr;
     VGX_HIP(hipSetDevice(ctx->device));
-    if (p.lds > 64 * 1024)
-        VGX_HIP(hipFuncSetAttribute((const void*)p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds));
     hipLaunchKernelGGL(p.fn, dim3((unsigned)p.wgs, (unsigned)p.nsplit), dim3(p.threads), p.lds, ctx->stream, P);
     VGX_LAUNCH_CHECK("paged attention launch");
     if (p.nsplit > 1) {

@@ -249,6 +249,7 @@ class Attention:
 
 
 _ELEM = {torch.float32: _l.E_F32, torch.bfloat16: _l.E_BF16, torch.float16: _l.E_F16, torch.int16: _l.E_Q16}
+_F32, _I32 = torch.float32, torch.int32
 _CACHE = {"bf16": (_l.E_BF16, torch.bfloat16, torch.bfloat16), "f16": (_l.E_F16, torch.float16, torch.float16),
           "q8": (_l.E_Q8, torch.int8, torch.float16)}
 
@@ -307,6 +308,7 @@ class PagedCache:
         self.gpu, self.heads, self.kv_heads, self.head_dim, self.kind = gpu, heads, kv_heads, head_dim, kind
         self.ckind = _ELEM[self.qtype]
         self.k, self.v, self.width = k, v, heads * head_dim
+        self.qkv_width, self.norm_shape = (heads + 2 * kv_heads) * head_dim, torch.Size((head_dim,))
         self.d = _l.Paged(heads, kv_heads, head_dim, k.shape[2], k.shape[0], elem, k_step, v_step, k.data_ptr(),
                           v.data_ptr(), *k.stride()[:3], *v.stride()[:3])
         self.ref = ctypes.byref(self.d)
@@ -319,27 +321,27 @@ class PagedCache:
         bfloat16, float16 or q16) normed, rotated (cos, sin: positions x rot/2)
         and written into the cache; returns the queries (ntok, heads, head_dim)."""
         g = self.gpu
-        g.need_rows(qkv, None, batch.ntok, self.width + 2 * self.kv_heads * self.head_dim, "qkv")
-        if qkv.dtype not in _ELEM:
+        kind = _ELEM.get(qkv.dtype)
+        if kind is None:
             raise ValueError("qkv must be float32, bfloat16, float16 or int16 (q16)")
+        stride = g.need_rows(qkv, None, batch.ntok, self.qkv_width, "qkv")
         npos = rot = 0
         if cos is not None:
-            for t, name in ((cos, "cos"), (sin, "sin")):
-                g.need(t, torch.float32, 2, name)
-                if not t.is_contiguous() or t.shape != cos.shape:
-                    raise ValueError("cos and sin must be contiguous and of one shape")
-            npos, rot = cos.shape[0], 2 * cos.shape[1]
+            npos, half = cos.shape
+            rot = 2 * half
+            for t in (cos, sin):
+                if t.dtype is not _F32 or t.device != g.device or t.shape != cos.shape or not t.is_contiguous():
+                    raise ValueError("cos and sin must be contiguous float32 tensors of one shape on %s" % g.device)
         for t in (q_norm, k_norm):
-            if t is not None:
-                g.need(t, torch.float32, 1, "a norm weight")
-                if t.shape[0] != self.head_dim or t.stride(0) != 1:
-                    raise ValueError("a norm weight must be %d contiguous values" % self.head_dim)
+            if t is not None and (t.dtype is not _F32 or t.device != g.device or t.shape != self.norm_shape
+                                  or not t.is_contiguous()):
+                raise ValueError("a norm weight must be %d contiguous float32 values on %s" % (self.head_dim, g.device))
         if out is None:
             q, qs = torch.empty((batch.ntok, self.heads, self.head_dim), dtype=self.qtype, device=g.device), self.width
         else:
             q, qs = out, self._rows(out, self.qtype, batch.ntok, "out")
-        r = _l.PagedRows(_ELEM[qkv.dtype], qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), _at(cos), _at(sin), npos,
-                         rot, int(rope_half), _at(q_norm), _at(k_norm), eps, q.data_ptr(), qs)
+        r = _l.PagedRows(kind, qkv.data_ptr(), stride, _at(cos), _at(sin), npos, rot, int(rope_half), _at(q_norm),
+                         _at(k_norm), eps, q.data_ptr(), qs)
         g.on_current(_l.load().vgx_paged_append, self.ref, batch.ref, ctypes.byref(r))
         return q
 
@@ -368,8 +370,7 @@ class PagedCache:
     def _rows(self, t, dtype, n, name):
         """The stride of n rows of heads x head_dim values, (n, heads, head_dim) or (n, heads * head_dim)."""
         if t.dim() != 3:
-            self.gpu.need_rows(t, dtype, n, self.width, name)
-            return max(t.stride(0), self.width)
+            return self.gpu.need_rows(t, dtype, n, self.width, name)
         self.gpu.need(t, dtype, 3, name)
         rows, heads, hd = t.shape
         st = t.stride()
@@ -387,6 +388,7 @@ class GPU:
         _l.check(L.vgx_ctx_create(device, ctypes.byref(h)))
         self.ctx, self.device = h, torch.device("cuda", device)
         self._get_stream = L.vgx_ctx_stream
+        self._verify_ws = {}  # draft_verify's workspace bytes by its sizes
         self.use_torch_stream()
 
     def use_torch_stream(self):
@@ -417,10 +419,13 @@ class GPU:
                 name, dims, dtype or t.dtype, self.device, t.dtype, t.device))
 
     def need_rows(self, t, dtype, n, width, name):
-        """Refuses all but n rows of width contiguous values."""
+        """Refuses all but n rows of width contiguous values; their stride."""
         self.need(t, dtype, 2, name)
-        if t.shape[0] < n or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        rows, cols = t.shape
+        st = t.stride()
+        if rows < n or cols != width or (width > 1 and st[1] != 1):
             raise ValueError("%s must be %d rows of %d contiguous values, not %s" % (name, n, width, tuple(t.shape)))
+        return max(st[0], width)
 
     # -- weights
     def upload(self, m: Matrix):
@@ -617,36 +622,38 @@ class GPU:
         drawn from; temp: a temperature a sequence (0: greedy).  Returns
         (accepted drafts and next token of each sequence, the target's
         probability of each drafted token); rows of no sequence have none."""
-        self.need(qstart, torch.int32, 1, "qstart")
-        self.need(tokens, torch.int32, 1, "tokens")
         nseq, n = qstart.shape[0] - 1, tokens.shape[0]
         if nseq < 0:
             raise ValueError("qstart must hold at least one entry")
-        if logits.dim() != 2 or logits.dtype not in _ELEM:
+        for t, dtype, size, name in ((qstart, _I32, nseq + 1, "qstart"), (tokens, _I32, n, "tokens"),
+                                     (u_accept, _F32, n, "u_accept"), (u_next, _F32, nseq, "u_next"),
+                                     (temp, _F32, nseq, "temp")):
+            if t is not None and (t.dtype is not dtype or t.device != self.device or t.shape != (size,)
+                                  or not t.is_contiguous()):
+                raise ValueError("%s must be %d contiguous %s values on %s" % (name, size, dtype, self.device))
+        kind = _ELEM.get(logits.dtype)
+        if kind is None or logits.dim() != 2:
             raise ValueError("logits must be rows of float32, bfloat16, float16 or int16 (q16)")
         vocab = logits.shape[1]
-        for t, name in ((logits, "logits"), (draft, "draft")):
-            if t is not None:
-                self.need_rows(t, logits.dtype, n, vocab, name)
-        for t, size, name in ((u_accept, n, "u_accept"), (u_next, nseq, "u_next"), (temp, nseq, "temp")):
-            if t is not None:
-                self.need(t, torch.float32, 1, name)
-                if t.shape[0] != size:
-                    raise ValueError("%s must be %d values" % (name, size))
-        for t in (qstart, tokens, u_accept, u_next, temp):
-            if t is not None and t.numel() > 1 and t.stride(0) != 1:
-                raise ValueError("qstart, tokens, the random numbers and temp must be contiguous")
-        L, kind = _l.load(), _ELEM[logits.dtype]
-        acc_next = torch.empty((2, nseq), dtype=torch.int32, device=self.device)
-        prob = torch.empty(n, dtype=torch.float32, device=self.device)
-        need = int(L.vgx_draft_verify_ws(nseq, n, vocab, kind, int(draft is not None)))
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        a = _l.Draft(nseq, n, vocab, qstart.data_ptr(), tokens.data_ptr(), kind, logits.data_ptr(),
-                     max(logits.stride(0), vocab), _at(draft), 0 if draft is None else max(draft.stride(0), vocab),
-                     _at(temp), u_accept.data_ptr(), u_next.data_ptr(), acc_next.data_ptr(),
-                     acc_next.data_ptr() + 4 * nseq, prob.data_ptr(), ws.data_ptr(), need)
+        stride = self.need_rows(logits, None, n, vocab, "logits")
+        dstride = 0 if draft is None else self.need_rows(draft, logits.dtype, n, vocab, "draft")
+        L = _l.load()
+        key = (nseq, n, vocab, kind, draft is not None)
+        need = self._verify_ws.get(key)
+        if need is None:
+            if len(self._verify_ws) > 1000:
+                self._verify_ws.clear()
+            need = self._verify_ws[key] = int(L.vgx_draft_verify_ws(*key))
+        dev = self.device
+        accepted = torch.empty(nseq, dtype=_I32, device=dev)
+        nxt = torch.empty(nseq, dtype=_I32, device=dev)
+        prob = torch.empty(n, dtype=_F32, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        a = _l.Draft(nseq, n, vocab, qstart.data_ptr(), tokens.data_ptr(), kind, logits.data_ptr(), stride, _at(draft),
+                     dstride, _at(temp), u_accept.data_ptr(), u_next.data_ptr(), accepted.data_ptr(), nxt.data_ptr(),
+                     prob.data_ptr(), ws.data_ptr(), need)
         self.on_current(L.vgx_draft_verify, ctypes.byref(a))
-        return acc_next[0], acc_next[1], prob
+        return accepted, nxt, prob
 
     def conv(self, w, layer_is_conv=None):
         return Conv(self, w, layer_is_conv)
