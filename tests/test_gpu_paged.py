@@ -474,3 +474,165 @@ def test_a_step_with_the_quantised_path(gpu):
     # weights, in root mean square 2^-8 * 5 * 0.03 * sqrt(768) / sqrt(3) < 0.01
     d = (res["chunk"].float() - res["tokens"].float()) / 256
     assert float(d.square().mean().sqrt()) < 0.02 and float(d.abs().max()) < 0.15
+
+
+def test_shared_prefix(gpu):
+    """Two sequences whose tables name the same first pages."""
+    b = Batch(30, [1, 1], [100, 100], 2, 64, 16, "bf16")
+    b.table[1, :3] = b.table[0, :3]
+    check_attn(gpu, b, 8)
+    b = Batch(31, [40, 70], [120, 120], 2, 64, 16, "bf16")
+    b.table[1, :3] = b.table[0, :3]
+    check_attn(gpu, b, 4)
+
+
+def test_capture_without_a_call_before(gpu):
+    """The first calls of a context and of a batch inside a capture."""
+    from vgx import gpu as vg
+    b = Batch(32, [1, 2], [1500, 90], 2, 128, 16, "f16")
+    g = vg.GPU(0)
+    cache = g.paged_cache(8, 2, 128, "f16", b.k.cuda(), b.v.cuda())
+    batch = cache.batch(*b.device(), b.ntok)
+    x = torch.randn(b.ntok, 12 * 128, device="cuda")
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        q = cache.append(batch, x)
+        o = cache.attend(batch, q)[0]
+    for _ in range(3):
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, cache.attend(batch, cache.append(batch, x))[0])
+    batch.check()
+    g.close()
+
+
+@pytest.mark.parametrize("hd, kvh, heads", [(64, 2, 4), (128, 1, 4)])
+def test_results_repeat(gpu, hd, kvh, heads):
+    """The same call gives the same bits, split or not."""
+    b = Batch(33, [1, 3, 1], [5000, 700, 64], kvh, hd, 16, "q8")
+    cache, batch = make(gpu, b, heads)
+    q = torch.randn(b.ntok, heads, hd, device="cuda").half()
+    want = cache.attend(batch, q, lse=True)
+    for _ in range(20):
+        got = cache.attend(batch, q, lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_drafted_decode(gpu):
+    """A step as a server runs it: the rows' projections (vgx_gemm), append,
+    attend, the head and the drafts' check, with the lengths kept on the
+    device.  Greedy sequences give the tokens of decoding one at a time,
+    whatever was drafted."""
+    import oracle as o
+    from vgx import mmcf
+    rng = np.random.default_rng(9)
+    heads, kvh, hd, dim, vocab, nseq, steps = 4, 2, 64, 128, 512, 3, 14
+
+    def mat(r, c, s):
+        q, unit, plane = mmcf.q8_per_row(rng.standard_normal((r, c)).astype(np.float32) * s)
+        return gpu.upload(mmcf.Matrix("q8", r, c, (q.view(np.uint8) ^ 0x80).ravel(), unit, True, plane))
+
+    wqkv, wo, head = mat((heads + 2 * kvh) * hd, dim, 0.08), mat(dim, heads * hd, 0.08), mat(vocab, dim, 0.2)
+    emb = torch.from_numpy(np.stack([o.quantize_act(rng.standard_normal(dim).astype(np.float32))
+                                     for _ in range(vocab)])).cuda()
+    cos, sin = (t.cuda() for t in tables(64, hd))
+    table = torch.randperm(nseq * 4, generator=torch.Generator().manual_seed(1)).int().view(nseq, 4).cuda()
+    zeros = torch.zeros(nseq, device="cuda")  # greedy
+
+    def logits(cache, batch, tokens):
+        x = emb[tokens.long()].contiguous()
+        q = cache.append(batch, gpu.gemm(wqkv, x), cos, sin)
+        att = cache.attend(batch, q, out=torch.empty(len(tokens), heads * hd, dtype=torch.int16, device="cuda"))[0]
+        return gpu.gemm(head, gpu.gemm(wo, att, x))
+
+    def cache_of():
+        k = torch.zeros(nseq * 4, kvh, 16, hd, dtype=torch.bfloat16, device="cuda")
+        return gpu.paged_cache(heads, kvh, hd, "bf16", k, k.clone())
+
+    first = torch.tensor([5, 77, 300], dtype=torch.int32).cuda()
+    # one token at a time
+    cache, kv = cache_of(), torch.zeros(nseq, dtype=torch.int32).cuda()
+    qs = torch.arange(nseq + 1, dtype=torch.int32).cuda()
+    batch = cache.batch(qs, kv, table, nseq, max_q=1)
+    tok, want = first, [first.cpu()]
+    for _ in range(steps):
+        kv += 1
+        tok = gpu.argmax_rows(logits(cache, batch, tok))
+        want.append(tok.cpu())
+    want = torch.stack(want, 1)  # (nseq, steps + 1)
+    # drafts: the right tokens, spoilt at some places; ragged numbers of them
+    for spoil in (0.0, 0.4, 1.0):
+        cache, kv = cache_of(), torch.zeros(nseq, dtype=torch.int32).cuda()
+        got = [[int(t)] for t in first]
+        while min(len(g) for g in got) <= steps:
+            rows, starts = [], [0]
+            for s in range(nseq):
+                n = int(rng.integers(0, 5))
+                d = [int(want[s, min(len(got[s]) + i, steps)]) for i in range(n)]
+                d = [int(rng.integers(0, vocab)) if rng.random() < spoil else t for t in d]
+                rows += [got[s][-1]] + d
+                starts.append(len(rows))
+            qs = torch.tensor(starts, dtype=torch.int32).cuda()
+            tokens = torch.tensor(rows, dtype=torch.int32).cuda()
+            kv += qs[1:] - qs[:-1]
+            batch = cache.batch(qs, kv, table, len(rows), max_q=5)
+            l = logits(cache, batch, tokens)
+            u = torch.rand(len(rows), device="cuda")
+            acc, nxt, prob = gpu.draft_verify(qs, tokens, l, u, zeros, temp=zeros)
+            batch.check()
+            kv -= qs[1:] - qs[:-1] - 1 - acc  # refused drafts leave the cache
+            for s in range(nseq):
+                a = int(acc[s])
+                got[s] += rows[starts[s] + 1:starts[s] + 1 + a] + [int(nxt[s])]
+            if max(len(g) for g in got) > 56:
+                break
+        for s in range(nseq):
+            assert got[s][:steps + 1] == want[s].tolist()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("hd", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("nq", [[2, 4, 1, 0], [6, 3, 1, 5]])
+def test_attn_drafts(gpu, kind, hd, nq):
+    """17 to 48 columns a KV head (8 query heads each): two and three blocks of
+    columns, over one split and over several."""
+    check_attn(gpu, Batch(34, nq, [70, 33, 500, 9], 1, hd, 16, kind), 8)
+    b = Batch(35, nq, [70, 2100, 500, 9], 1, hd, 16, kind)
+    check_attn(gpu, b, 8, window=600 if kind == "q8" else 0)
+
+
+def test_attn_masked_values_drafts(gpu):
+    b = Batch(36, [6, 5], [140, 61], 1, 64, 16, "bf16")
+    q = (2 * b.randn(b.ntok, 8, 64)).to(torch.bfloat16)
+    want, _, mag, dots = ref.attend(b, q, 8)
+    bound = ref.attn_bound(b, torch.bfloat16, want, mag, dots)
+    b.v[int(b.table[0, 8]), :, 9, 3] = math.nan   # position 137 of 140
+    b.v[int(b.table[1, 3]), :, 10, 60] = -math.inf  # position 58 of 61
+    c, bt = make(gpu, b, 8)
+    got = c.attend(bt, q.cuda())[0].cpu().double().view_as(want)
+    for t in range(11):
+        dim, sees = (3, t >= 3) if t < 6 else (60, t >= 6 + 2)
+        if sees:
+            assert not torch.isfinite(got[t, :, dim]).any()
+        rest = [d for d in range(64) if d != dim or not sees]
+        assert ((got[t][:, rest] - want[t][:, rest]).abs() <= bound[t][:, rest]).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+def test_attn_many_sequences(gpu, kind):
+    """More workgroups than half the CUs, one a sequence and head."""
+    rng = np.random.default_rng(2)
+    kv = rng.integers(1, 400, 80).tolist()
+    check_attn(gpu, Batch(37, [1] * 80, kv, 2, 64, 16, kind), 4)
+    nq = rng.integers(0, 3, 80).tolist()
+    check_attn(gpu, Batch(38, nq, [k + 2 for k in kv], 2, 128, 32, kind), 8)
+
+
+def test_attn_chunks_split(gpu):
+    """A chunk of few tiles over a long cache: its keys are split too."""
+    b = Batch(39, [90, 70], [3000, 1200], 1, 128, 64, "f16")
+    cache, batch = make(gpu, b, 2)
+    check_attn(gpu, b, 2, cache=cache, batch=batch)
+    assert min(batch.ws.values()) > 0
+    check_attn(gpu, Batch(40, [150], [4000], 2, 64, 16, "q8"), 4, window=900)
