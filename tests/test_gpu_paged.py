@@ -636,3 +636,16 @@ def test_attn_chunks_split(gpu):
     check_attn(gpu, b, 2, cache=cache, batch=batch)
     assert min(batch.ws.values()) > 0
     check_attn(gpu, Batch(40, [150], [4000], 2, 64, 16, "q8"), 4, window=900)
+
+
+@pytest.mark.parametrize("kind, hd, heads, kvh", [("bf16", 64, 4, 2), ("q8", 128, 8, 1), ("f16", 80, 3, 3),
+                                                  ("bf16", 96, 36, 2), ("bf16", 256, 4, 2), ("f16", 32, 50, 1)])
+def test_attn_prompts_and_tokens(gpu, kind, hd, heads, kvh):
+    """Chunks and single tokens in one batch, with long caches among the short
+    rows' sequences: both kernels run, and both split."""
+    b = Batch(41, [100, 1, 2, 0, 1, 61], [150, 3000, 2500, 7, 9, 1700], kvh, hd, 16, kind)
+    cache, batch = make(gpu, b, heads)
+    check_attn(gpu, b, heads, cache=cache, batch=batch)
+    if heads // kvh <= 16:
+        assert min(batch.ws.values()) > 0
+    check_attn(gpu, b, heads, window=700)

@@ -43,14 +43,21 @@ struct AttnArgs {
     float c;       // scale * log2(e), the K step included: exponents of 2
     float scale;   // scale with the K step: scores
     int window;
-    int split_len, nsplit;
+    int split_len;
+    int cmin, cmax;  // the sequences of this launch: cmin < columns a KV head <= cmax
     int out_q16;
     uint8_t* out;
     int64_t ostride;
     float* lse;
-    float* po;     // nsplit x ntok x heads x hd partial sums
-    float* pml;    // nsplit x ntok x heads x (m, l)
-    int* pn;       // ntok x heads: a row's splits
+    // Partial results, numbered: hd sums and (m, l) each.  Split k of a row and
+    // head is number base + k * step; pn (ntok x heads) holds their splits and
+    // base.  Numbers go by row and head, or by sequence, KV head and column (the
+    // few rows of short sequences among many others').
+    float* po;
+    float2* pml;
+    uint2* pn;
+    unsigned pbase, pstep;
+    int by_seq;
 };
 
 template <int CK>
@@ -409,6 +416,13 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
         }
 }
 
+// Where a column's partial results begin.
+__device__ __forceinline__ unsigned part_of(const AttnArgs& P, int s, int h, int m, int row, int head) {
+    return P.pbase + (P.by_seq ? (unsigned)(s * P.A.kvh + h) * P.cmax + m : (unsigned)row * P.A.heads + head);
+}
+// A row's number of splits in the low half of pn.x, its numbering above.
+constexpr unsigned kBySeq = 1u << 16;
+
 // Four values of one output row: dims d .. d+3.
 template <int CK>
 __device__ __forceinline__ void put_out(const AttnArgs& P, int64_t row, int head, int d, float4 v) {
@@ -607,7 +621,7 @@ constexpr int rows_lds(int hd, int nb) {
 // product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
 // the lane; two of them are the next product's B operand.
 template <int KIND, int HD, bool EX, int NB, int WV>
-__global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256) ? 2 : 1) paged_rows_kernel(const AttnArgs P) {
+__device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) {
     using Ks = Keys<KIND, HD, EX>;
     constexpr int CK = Ks::CK, KS = HD / 32, DB = HD / 16;
     constexpr int kWave = rows_lds(HD, NB);
@@ -622,8 +636,7 @@ __global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256
                  "s"(A.pmul), "s"(A.npages), "s"(A.max_kv), "s"(A.ntok), "s"(A.heads), "s"(A.max_q), "s"(A.tcols));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int s = blockIdx.x / A.kvh, h = blockIdx.x - s * A.kvh;
-    const int split = blockIdx.y;
+    const int s = bx / A.kvh, h = bx - s * A.kvh;
     const int* tab = A.table + (int64_t)s * A.tstride;
     // Without a window the keys begin at 0, so the table's entries are asked
     // for along with the lengths (an entry past the sequence's end is not used).
@@ -634,7 +647,7 @@ __global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256
     }
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
-    if (q.n <= 0) return;
+    if (q.n <= 0 || q.n * A.grp > P.cmax) return;
     const Span sp = span_of(q, 0, q.n - 1, P.window, P.split_len);
     if (split >= sp.nsp) return;
     const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
@@ -796,7 +809,9 @@ __global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256
             f[w] = exp2_(fmaf(f[w], P.c, -mc));
             L = fmaf(sl[w][16 * b + col], f[w], L);
         }
-        const int64_t at = ((int64_t)split * A.ntok + cl[b].row) * A.heads + cl[b].head;
+        const int64_t at = (int64_t)cl[b].row * A.heads + cl[b].head;
+        const unsigned part0 = part_of(P, s, h, 16 * b + col, cl[b].row, cl[b].head);
+        const int64_t to = part0 + (int64_t)split * P.pstep;
         const float r = whole ? inv_l(P, L) : 1.0f;
         // thread: column lane % 16, every (4 WV)-th group of 4 dims
         for (int d = 4 * (threadIdx.x >> 4); d < A.hd; d += 16 * WV) {
@@ -809,30 +824,35 @@ __global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256
             }
             const float4 v = make_float4(x[0] * r, x[1] * r, x[2] * r, x[3] * r);
             if (whole) put_out<CK>(P, cl[b].row, cl[b].head, d, v);
-            else *reinterpret_cast<float4*>(P.po + at * A.hd + d) = v;
+            else *reinterpret_cast<float4*>(P.po + to * A.hd + d) = v;
         }
         if (threadIdx.x < 16) {
             if (!whole) {
-                P.pml[2 * at] = M;
-                P.pml[2 * at + 1] = L;
-                if (split == 0) P.pn[at] = sp.nsp;
+                P.pml[to] = make_float2(M, L);
+                if (split == 0) P.pn[at] = make_uint2(sp.nsp | (P.by_seq ? kBySeq : 0), part0);
             } else {
-                if (P.nsplit > 1) P.pn[at] = 1;
+                if (P.pn) P.pn[at] = make_uint2(1, 0);
                 if (P.lse) P.lse[at] = lse_of(P, M, L);
             }
         }
     }
 }
 
+template <int KIND, int HD, bool EX, int NB, int WV>
+__global__ void __launch_bounds__(64 * WV, (NB == 1 ? HD <= 128 : NB * HD <= 256) ? 2 : 1)
+    paged_rows_kernel(const AttnArgs P) {
+    rows_body<KIND, HD, EX, NB, WV>(P, blockIdx.x, blockIdx.y);
+}
+
 // The sequence and place of a tile of tm columns, tiles counted through the
 // batch: false past the last.  Every lane of the wave is active.
-__device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int tile, int& s, int& local) {
+__device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int cmin, int tile, int& s, int& local) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int b = 0; b < A.nseq; b += 64) {
         const int j = b + lane;
         const int n = j < A.nseq ? seq_at(A, j).n : 0;
-        const int cnt = (int)(((int64_t)n * A.grp + tm - 1) / tm);
+        const int cnt = n * A.grp > cmin ? (n * A.grp + tm - 1) / tm : 0;  // (the host bounds n * grp)
         int sum = cnt;  // the running sum over the lanes
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -854,7 +874,7 @@ __device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int tile, int
 // Many rows a sequence: a workgroup is a tile of 128 columns (4 waves x 32) of
 // one KV head; the waves share tiles of 64 keys.
 template <int KIND, int HD, bool EX>
-__global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
+__device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, int split) {
     constexpr int ROWS = 64, kTile = 64 * (Geo<HD>::pk + Geo<HD>::pv);
     using St = Stage<KIND, HD, EX>;
     constexpr int CK = St::CK;
@@ -864,17 +884,16 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 31;
     // the last tiles, which see the most keys, first
-    const int rev = blockIdx.x / A.kvh, h = blockIdx.x - rev * A.kvh;
-    const int tile = gridDim.x / A.kvh - 1 - rev;
+    const int rev = bx / A.kvh, h = bx - rev * A.kvh;
+    const int tile = wgs / A.kvh - 1 - rev;
     int s, local;
-    if (!tile_at(A, 128, tile, s, local)) return;
+    if (!tile_at(A, 128, P.cmin, tile, s, local)) return;
     s = __builtin_amdgcn_readfirstlane(s);
     local = __builtin_amdgcn_readfirstlane(local);
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
     const int m0 = local * 128, m1 = min(m0 + 128, q.n * A.grp) - 1;
     const Span sp = span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len);
-    const int split = blockIdx.y;
     if (split >= sp.nsp) return;
     const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
     const Col cl = col_of(P, q, h, m0 + wave * 32 + col, end);
@@ -972,7 +991,9 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
     const float L = half_sum(a.l);
     if (!cl.valid) return;
     const int hh = lane >> 5;
-    const int64_t at = ((int64_t)split * A.ntok + cl.row) * A.heads + cl.head;
+    const int64_t at = (int64_t)cl.row * A.heads + cl.head;
+    const unsigned part0 = part_of(P, s, h, 0, cl.row, cl.head);
+    const int64_t to = part0 + (int64_t)split * P.pstep;
     const bool whole = sp.nsp == 1;
     const float r = whole ? inv_l(P, L) : 1.0f;
 #pragma unroll
@@ -984,17 +1005,41 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
             const float4 v = make_float4(a.o[b][4 * g] * r, a.o[b][4 * g + 1] * r, a.o[b][4 * g + 2] * r,
                                          a.o[b][4 * g + 3] * r);
             if (whole) put_out<CK>(P, cl.row, cl.head, d, v);
-            else *reinterpret_cast<float4*>(P.po + at * A.hd + d) = v;
+            else *reinterpret_cast<float4*>(P.po + to * A.hd + d) = v;
         }
     if (hh == 0) {
         if (!whole) {
-            P.pml[2 * at] = a.m;
-            P.pml[2 * at + 1] = L;
-            if (split == 0) P.pn[at] = sp.nsp;
+            P.pml[to] = make_float2(a.m, L);
+            if (split == 0) P.pn[at] = make_uint2(sp.nsp, part0);
         } else {
-            if (P.nsplit > 1) P.pn[at] = 1;
+            if (P.pn) P.pn[at] = make_uint2(1, 0);
             if (P.lse) P.lse[at] = lse_of(P, a.m, L);
         }
+    }
+}
+
+template <int KIND, int HD, bool EX>
+__global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kernel(const AttnArgs P) {
+    tile_body<KIND, HD, EX>(P, blockIdx.x, gridDim.x, blockIdx.y);
+}
+
+// Prompts and single tokens in one batch: the sequences of at most 16 columns a
+// KV head as the rows kernel takes them, the others as tiles, in one launch (the
+// tiles first), so that the ones' bytes come in while the others multiply.
+struct BothArgs {
+    AttnArgs rows, tile;
+    int rows_wgs, tile_wgs;   // workgroups of one split
+    int tile_all;             // the tiles' workgroups of all splits
+};
+template <int KIND, int HD, bool EX>
+__global__ void __launch_bounds__(256, EX ? 2 : 1) paged_both_kernel(const BothArgs B) {
+    const int bx = blockIdx.x;
+    if (bx < B.tile_all) {
+        const int split = bx / B.tile_wgs;
+        tile_body<KIND, HD, EX>(B.tile, bx - split * B.tile_wgs, B.tile_wgs, split);
+    } else {
+        const int r = bx - B.tile_all, split = r / B.rows_wgs;
+        rows_body<KIND, HD, EX, 1, 4>(B.rows, r - split * B.rows_wgs, split);
     }
 }
 
@@ -1002,8 +1047,11 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
 // power of two, lg) a row and head, in split order.  Many: a workgroup a row and
 // head, the splits dealt to groups of hd / 4 threads, each in split order, the
 // groups in theirs.
+struct JoinArgs {
+    unsigned step_row, step_seq, total;  // between a row's splits, by its numbering; all partial results
+};
 template <int CK, bool WIDE>
-__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int lg) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int lg, const JoinArgs J) {
     const PagedDev& A = P.A;
     __shared__ float sw[4], sl[4];
     __shared__ float4 so[256];
@@ -1013,11 +1061,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
     const int t = (int)(w0 / A.heads);
     const int head = (int)(w0 - (int64_t)t * A.heads) + (WIDE ? 0 : lane >> lg);
     if (t >= A.ntok) return;
-    const int64_t step = (int64_t)A.ntok * A.heads, at = (int64_t)t * A.heads + head;
-    // (the entry of a row behind the last sequence was written by nobody)
-    const int nsp = t < A.qstart[A.nseq] ? P.pn[at] : 0;
-    if (nsp <= 1 || nsp > P.nsplit) return;
-    const float2* ml = reinterpret_cast<const float2*>(P.pml) + at;
+    // (the entry of a row behind the last sequence was written by nobody, nor
+    // that of a row past the bounds)
+    const uint2 e = t < A.qstart[A.nseq] ? P.pn[(int64_t)t * A.heads + head] : make_uint2(0, 0);
+    const int nsp = e.x & 0xffff;
+    const int64_t step = e.x & kBySeq ? J.step_seq : J.step_row, at = e.y;
+    if (nsp <= 1 || at + (nsp - 1) * step >= J.total) return;
+    const float2* ml = P.pml + at;
     const float4* po = reinterpret_cast<const float4*>(P.po);
     const int n4 = A.hd / 4;
     float4 o = make_float4(0, 0, 0, 0);
@@ -1070,21 +1120,33 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
     const int d = WIDE ? threadIdx.x : lane & ((1 << lg) - 1);
     const float r = inv_l(P, L);
     if (d < n4) put_out<CK>(P, t, head, 4 * d, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
-    if (d == 0 && P.lse) P.lse[at] = lse_of(P, M, L);
+    if (d == 0 && P.lse) P.lse[(int64_t)t * A.heads + head] = lse_of(P, M, L);
 }
 
 typedef void (*AttnFn)(const AttnArgs);
-typedef void (*JoinFn)(const AttnArgs, int);
+typedef void (*BothFn)(const BothArgs);
+typedef void (*JoinFn)(const AttnArgs, int, const JoinArgs);
 // Positions up to which one workgroup takes a sequence whole.
 constexpr int64_t kWhole = 1024;
 
-struct Plan {
+struct Launch {
     AttnFn fn;
+    BothFn both;
     int lds, tm, threads;
     bool rows;
+    int cmin, cmax;
     int64_t wgs;       // workgroups of one split
     int split_len, nsplit;
+};
+struct Plan {
+    Launch l[2];
+    int n;
+    int by_seq;        // the first one's partial results are numbered by sequence
+    size_t parts;      // partial results
     size_t ws;
+    unsigned step(const PagedDev& A, int i) const {
+        return i == 0 && by_seq ? (unsigned)A.nseq * A.kvh * l[0].cmax : (unsigned)A.ntok * A.heads;
+    }
 };
 
 // cols: the columns a sequence may have in a KV head.  Up to 48 the rows kernel
@@ -1094,8 +1156,10 @@ struct Plan {
 // against 12.1 with 4 waves, 11.9 with 4 splits; 128 workgroups: 20.0 against
 // 18.7).
 template <int KIND, int HD, bool EX>
-void fn_of(int64_t cols, bool few, Plan& p) {
+void fn_of(int64_t cols, bool few, Launch& p) {
     p.threads = 256;
+    p.both = nullptr;
+    if constexpr (HD <= 128) p.both = paged_both_kernel<KIND, HD, EX>;
     if (cols <= (HD <= 128 ? 48 : 16)) {
         const int nb = (int)(cols + 15) / 16;
         p.fn = paged_rows_kernel<KIND, HD, EX, 1, 4>;
@@ -1118,7 +1182,7 @@ void fn_of(int64_t cols, bool few, Plan& p) {
     }
 }
 template <int KIND>
-void fn_of(const PagedDev& A, int64_t cols, bool few, Plan& p) {
+void fn_of(const PagedDev& A, int64_t cols, bool few, Launch& p) {
     const int hd = A.hd;
     const bool whole = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
     if (whole) switch (hd) {
@@ -1131,17 +1195,22 @@ void fn_of(const PagedDev& A, int64_t cols, bool few, Plan& p) {
     return hd <= 128 ? fn_of<KIND, 128, false>(cols, few, p) : fn_of<KIND, 256, false>(cols, few, p);
 }
 
-Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
-    Plan p{};
-    const int64_t cols = (int64_t)A.max_q * A.grp;
+// The columns the rows kernel takes at most.
+int64_t max_cols(const PagedDev& A) { return A.hd <= 128 ? 48 : 16; }
+
+Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t cols, int cmin, bool alone) {
+    Launch p{};
     int64_t span = A.max_kv;
     if (window > 0) span = std::min<int64_t>(span, (int64_t)window + 192);  // a tile's rows, lo's rounding
-    const bool few = span <= kWhole && (int64_t)A.nseq * A.kvh < num_cu / 2;
+    const bool few = alone && span <= kWhole && (int64_t)A.nseq * A.kvh < num_cu / 2;
     if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, few, p);
     else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, few, p);
     else fn_of<VGX_E_Q8>(A, cols, few, p);
-    // (a sequence with rows has at most rows * grp / tm + 1 tiles)
-    const int64_t tiles = p.rows ? A.nseq : (int64_t)A.ntok * A.grp / p.tm + std::min(A.nseq, A.ntok);
+    p.cmin = cmin;
+    p.cmax = p.rows ? p.tm : INT32_MAX;
+    // (a sequence of more than cmin columns has at most columns / tm + 1 tiles)
+    const int64_t all = (int64_t)A.ntok * A.grp;
+    const int64_t tiles = p.rows ? A.nseq : all / p.tm + std::min<int64_t>(A.nseq, std::max<int64_t>(all / (cmin + 1), 1));
     p.wgs = tiles * A.kvh;
     // Splits.  A workgroup of the rows kernel costs about 8 us before and after
     // its keys (the tables' and first rows' round trips, the join of its waves),
@@ -1160,10 +1229,29 @@ Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
         len = span <= kWhole ? span : std::min<int64_t>(std::max<int64_t>(len, 512), p.wgs >= num_cu ? 1024 : 768);
     len = (len + 127) / 128 * 128;
     if (p.threads == 512) len = std::max<int64_t>(span, 1);
-    int64_t n = (span + len - 1) / len;
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
-    p.nsplit = (int)std::max<int64_t>(n, 1);
-    p.ws = p.nsplit > 1 ? (size_t)p.nsplit * A.ntok * A.heads * (A.hd + 2) * 4 + (size_t)A.ntok * A.heads * 4 : 0;
+    p.nsplit = (int)std::max<int64_t>((span + len - 1) / len, 1);
+    return p;
+}
+
+// One kind of sequences, or both where some may have many columns and others up
+// to 16: l[0] then takes these, whose long caches it splits, l[1] the others.
+Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
+    Plan p{};
+    const int64_t cols = (int64_t)A.max_q * A.grp;
+    const int64_t least = A.ntok - (int64_t)(A.nseq - 1) * A.max_q;  // rows of the shortest sequence, if all others are full
+    if (cols > max_cols(A) && A.hd <= 128 && A.grp <= 16 && A.nseq > 1 && least * A.grp <= 16) {
+        p.l[0] = launch_of(A, kind, window, num_cu, 16, 0, false);
+        p.l[1] = launch_of(A, kind, window, num_cu, cols, 16, false);
+        p.n = 2;
+        p.by_seq = 1;
+    } else {
+        p.l[0] = launch_of(A, kind, window, num_cu, cols, 0, true);
+        p.n = 1;
+    }
+    for (int i = 0; i < p.n; ++i)
+        if (p.l[i].nsplit > 1) p.parts += (size_t)p.l[i].nsplit * p.step(A, i);
+    p.ws = p.parts ? p.parts * (A.hd + 2) * 4 + (size_t)A.ntok * A.heads * 8 : 0;
     return p;
 }
 
@@ -1178,14 +1266,16 @@ hipError_t vgx_paged_attn_init() {
                     PagedDev A{};
                     A.hd = hd;
                     A.psize = 16;
-                    Plan p{};
+                    Launch p{};
                     if (kind == VGX_E_BF16) fn_of<VGX_E_BF16>(A, cols, few, p);
                     else if (kind == VGX_E_F16) fn_of<VGX_E_F16>(A, cols, few, p);
                     else fn_of<VGX_E_Q8>(A, cols, few, p);
                     if (p.lds <= 64 * 1024) continue;
-                    const hipError_t e =
-                        hipFuncSetAttribute((const void*)p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds);
-                    if (e != hipSuccess) return e;
+                    for (const void* fn : {(const void*)p.fn, (const void*)p.both}) {
+                        if (!fn || (fn == (const void*)p.both && p.rows)) continue;  // (the tiles' LDS is the larger)
+                        const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, p.lds);
+                        if (e != hipSuccess) return e;
+                    }
                 }
     return hipSuccess;
 }
@@ -1219,11 +1309,16 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     if (!ctx) return vgx_fail(VGX_EINVAL, "vgx_paged_attn: no context");
     if (A.ntok == 0 || A.nseq == 0) return VGX_OK;
     Plan p = plan_of(A, cache->kind, r->window, ctx->num_cu);
-    if (p.nsplit > 1 && (!r->ws || r->ws_bytes < p.ws)) {
-        p.nsplit = 1;
-        p.split_len = INT32_MAX;
+    const bool split = p.ws && r->ws && r->ws_bytes >= p.ws;
+    for (int i = 0; i < p.n && !split; ++i) {
+        p.l[i].nsplit = 1;
+        p.l[i].split_len = INT32_MAX;
     }
-    if (p.wgs >= (1 << 24) || p.nsplit > 65535) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
+    for (int i = 0; i < p.n; ++i)
+        if (p.l[i].wgs >= (1 << 24) || p.l[i].nsplit > 65535)
+            return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
+    if (p.parts > INT32_MAX || (int64_t)A.ntok * A.heads > INT32_MAX - 256)
+        return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
     P.q = static_cast<const uint8_t*>(r->q);
     P.qstride = r->q_stride;
     P.scale = (r->scale > 0 ? r->scale : 1.0f / std::sqrt((float)A.hd)) * A.kstep;
@@ -1231,22 +1326,47 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     if (!(P.c > 1e-30f) || std::isinf(P.c))
         return vgx_fail(VGX_EINVAL, "vgx_paged_attn: scale times the K step outside 1e-30 .. 1e38");
     P.window = r->window;
-    P.split_len = p.split_len;
-    P.nsplit = p.nsplit;
     P.out_q16 = r->out_kind == VGX_E_Q16;
     P.out = static_cast<uint8_t*>(r->out);
     P.ostride = r->out_stride;
     P.lse = r->lse;
-    P.po = static_cast<float*>(r->ws);
-    P.pml = P.po ? P.po + (size_t)p.nsplit * A.ntok * A.heads * A.hd : nullptr;
-    P.pn = P.po ? reinterpret_cast<int*>(P.pml + (size_t)p.nsplit * A.ntok * A.heads * 2) : nullptr;
+    if (split) {
+        P.po = static_cast<float*>(r->ws);
+        P.pml = reinterpret_cast<float2*>(P.po + p.parts * A.hd);
+        P.pn = reinterpret_cast<uint2*>(P.pml + p.parts);
+    }
     VGX_HIP(hipSetDevice(ctx->device));
-    hipLaunchKernelGGL(p.fn, dim3((unsigned)p.wgs, (unsigned)p.nsplit), dim3(p.threads), p.lds, ctx->stream, P);
+    JoinArgs J{(unsigned)A.ntok * A.heads, 0, (unsigned)p.parts};
+    BothArgs B;
+    int most = 1;
+    for (int i = 0; i < p.n; ++i) {
+        const Launch& l = p.l[i];
+        P.split_len = l.split_len;
+        P.cmin = l.cmin;
+        P.cmax = l.cmax;
+        P.by_seq = i == 0 && p.by_seq;
+        P.pstep = p.step(A, i);
+        if (P.by_seq) J.step_seq = P.pstep;
+        (i == 0 ? B.rows : B.tile) = P;
+        if (l.nsplit > 1) P.pbase += (unsigned)l.nsplit * P.pstep;
+        most = std::max(most, l.nsplit);
+    }
+    if (p.n == 1) {
+        const Launch& l = p.l[0];
+        hipLaunchKernelGGL(l.fn, dim3((unsigned)l.wgs, (unsigned)l.nsplit), dim3(l.threads), l.lds, ctx->stream, B.rows);
+    } else {
+        B.rows_wgs = (int)p.l[0].wgs;
+        B.tile_wgs = (int)p.l[1].wgs;
+        const int64_t tiles = p.l[1].wgs * p.l[1].nsplit, grid = tiles + p.l[0].wgs * p.l[0].nsplit;
+        if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
+        B.tile_all = (int)tiles;
+        hipLaunchKernelGGL(p.l[1].both, dim3((unsigned)grid), dim3(256), std::max(p.l[0].lds, p.l[1].lds), ctx->stream, B);
+    }
     VGX_LAUNCH_CHECK("paged attention launch");
-    if (p.nsplit > 1) {
+    if (most > 1) {
         const int64_t jobs = (int64_t)A.ntok * A.heads;
         // (a row's partials one after the other cost a round trip each four)
-        const bool wide = p.nsplit > 8 && jobs < (1 << 24);
+        const bool wide = most > 8 && p.n == 1 && jobs < (1 << 24);  // (both: few of the rows are split)
         const bool bf = compute_kind(cache->kind) == VGX_E_BF16;
         const JoinFn join = wide ? (bf ? paged_join_kernel<VGX_E_BF16, true> : paged_join_kernel<VGX_E_F16, true>)
                                  : (bf ? paged_join_kernel<VGX_E_BF16, false> : paged_join_kernel<VGX_E_F16, false>);
@@ -1254,7 +1374,7 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
         if (A.heads % (64 >> lg)) lg = 6;  // a wave's heads would be of two rows
         const int64_t grid = wide ? jobs : ((jobs >> (6 - lg)) + 3) / 4;
         if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
-        hipLaunchKernelGGL(join, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P, lg);
+        hipLaunchKernelGGL(join, dim3((unsigned)grid), dim3(256), 0, ctx->stream, P, lg, J);
         VGX_LAUNCH_CHECK("paged attention join launch");
     }
     return VGX_OK;
