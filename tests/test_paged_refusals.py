@@ -3,6 +3,7 @@ valid (the checks run before the device is touched: no GPU needed)."""
 import ctypes
 
 import pytest
+import torch
 
 from vgx import lib as vl
 
@@ -134,3 +135,50 @@ def test_null_descriptions():
         assert said(call, cache(), None, rows())[0] == vl.VGX_EINVAL
         assert said(call, cache(), batch(), None)[0] == vl.VGX_EINVAL
     assert L.vgx_paged_attn_ws(None, ctypes.byref(cache()), ctypes.byref(batch()), 0) == 0
+
+
+class _Cpu:
+    """What the binding's own checks need of a GPU (no device is touched before them)."""
+    device = torch.device("cpu")
+
+    def __init__(self):
+        from vgx import gpu as vg
+        self.need = lambda *a: vg.GPU.need(self, *a)
+        self.need_rows = lambda *a: vg.GPU.need_rows(self, *a)
+
+
+def _binding(ntok=3, table=None, nseq=2):
+    from vgx import gpu as vg
+    g = _Cpu()
+    k = torch.zeros(6, 2, 16, 32, dtype=torch.bfloat16)
+    cache = vg.PagedCache(g, 4, 2, 32, "bf16", k, k.clone())
+    i32 = torch.int32
+    return cache, cache.batch(torch.arange(nseq + 1, dtype=i32), torch.ones(nseq, dtype=i32),
+                              torch.zeros(nseq, 3, dtype=i32) if table is None else table, ntok)
+
+
+def test_binding_refuses_rows_that_overlap():
+    """An expanded tensor holds one row: as many as its shape says would be
+    read past its end."""
+    cache, batch = _binding()
+    row = torch.zeros(1, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        cache.append(batch, row.expand(3, -1))
+    with pytest.raises(ValueError, match="rows apart"):
+        cache.attend(batch, torch.zeros(1, 4, 32, dtype=torch.bfloat16).expand(3, -1, -1))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.attend(batch, torch.zeros(1, 128, dtype=torch.bfloat16).expand(3, -1))
+    with pytest.raises(ValueError, match="overlap"):
+        _binding(table=torch.zeros(1, 3, dtype=torch.int32).expand(2, -1))
+    with pytest.raises(ValueError, match="overlap"):
+        cache.append(batch, torch.zeros(3 * 256, dtype=torch.bfloat16).as_strided((3, 256), (128, 1)))
+
+
+def test_binding_refuses_half_a_pair():
+    cache, batch = _binding()
+    x, t = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(8, 16)
+    for kw in (dict(cos=t), dict(sin=t), dict(q_norm=torch.ones(32)), dict(k_norm=torch.ones(32))):
+        with pytest.raises(ValueError, match="both"):
+            cache.append(batch, x, **kw)
+    with pytest.raises(ValueError, match="rot/2"):
+        cache.append(batch, x, t[0], t[0])

@@ -270,13 +270,16 @@ class RaggedBatch:
         if qstart.shape[0] != nseq + 1 or table.shape[0] != nseq:
             raise ValueError("a batch of %d sequences needs qstart of %d and a table of %d rows"
                              % (nseq, nseq + 1, nseq))
-        if qstart.stride(0) != 1 or (nseq > 1 and kvlen.stride(0) != 1) or (table.shape[1] > 1 and table.stride(1) != 1):
+        if ((nseq > 0 and qstart.stride(0) != 1) or (nseq > 1 and kvlen.stride(0) != 1)
+                or (table.shape[1] > 1 and table.stride(1) != 1)):
             raise ValueError("qstart, kvlen and a table's rows must be contiguous")
+        if nseq > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError("a table's rows overlap (an expanded tensor: make it contiguous)")
         self.gpu, self.nseq, self.ntok = gpu, nseq, int(ntok)
         self.fault = torch.zeros(1, dtype=torch.int32, device=gpu.device)
         self._keep = (qstart, kvlen, table)
         self.d = _l.Ragged(nseq, self.ntok, int(max_q), int(max_kv), qstart.data_ptr(), kvlen.data_ptr(),
-                           table.data_ptr(), table.shape[1], max(table.stride(0), table.shape[1]),
+                           table.data_ptr(), table.shape[1], table.stride(0) if nseq > 1 else table.shape[1],
                            self.fault.data_ptr())
         self.ref = ctypes.byref(self.d)
         self.ws = {}  # workspace bytes by (cache, window)
@@ -326,7 +329,11 @@ class PagedCache:
             raise ValueError("qkv must be float32, bfloat16, float16 or int16 (q16)")
         stride = g.need_rows(qkv, None, batch.ntok, self.qkv_width, "qkv")
         npos = rot = 0
+        if (cos is None) != (sin is None) or (q_norm is None) != (k_norm is None):
+            raise ValueError("cos and sin, and the norm weights, come both or not at all")
         if cos is not None:
+            if cos.dim() != 2:
+                raise ValueError("cos and sin must be positions x rot/2")
             npos, half = cos.shape
             rot = 2 * half
             for t in (cos, sin):
@@ -374,9 +381,11 @@ class PagedCache:
         self.gpu.need(t, dtype, 3, name)
         rows, heads, hd = t.shape
         st = t.stride()
-        if rows < n or heads != self.heads or hd != self.head_dim or st[2] != 1 or (heads > 1 and st[1] != hd):
-            raise ValueError("%s must be (%d, %d, %d), a row's heads contiguous" % (name, n, self.heads, self.head_dim))
-        return max(st[0], self.width)
+        if (rows < n or heads != self.heads or hd != self.head_dim or st[2] != 1 or (heads > 1 and st[1] != hd)
+                or (n > 1 and st[0] < self.width)):
+            raise ValueError("%s must be (%d, %d, %d), a row's heads contiguous and its rows apart" % (
+                name, n, self.heads, self.head_dim))
+        return st[0] if n > 1 else self.width
 
 
 class GPU:
@@ -423,9 +432,10 @@ class GPU:
         self.need(t, dtype, 2, name)
         rows, cols = t.shape
         st = t.stride()
-        if rows < n or cols != width or (width > 1 and st[1] != 1):
-            raise ValueError("%s must be %d rows of %d contiguous values, not %s" % (name, n, width, tuple(t.shape)))
-        return max(st[0], width)
+        if rows < n or cols != width or (width > 1 and st[1] != 1) or (n > 1 and st[0] < width):
+            raise ValueError("%s must be %d rows of %d contiguous values that do not overlap, not %s with strides %s" % (
+                name, n, width, tuple(t.shape), st))
+        return st[0] if n > 1 else width
 
     # -- weights
     def upload(self, m: Matrix):
