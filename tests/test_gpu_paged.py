@@ -649,3 +649,15 @@ def test_attn_prompts_and_tokens(gpu, kind, hd, heads, kvh):
     if heads // kvh <= 16:
         assert min(batch.ws.values()) > 0
     check_attn(gpu, b, heads, window=700)
+
+
+@pytest.mark.parametrize("nq, kv", [([8, 3], [3, 9]), ([90, 70], [60, 200]), ([300, 1], [33, 40])])
+def test_attn_widest_window(gpu, nq, kv):
+    """The largest windows mask nothing, also where rows lie before position 0."""
+    b = Batch(34, nq, kv, 2, 64, 16, "bf16")
+    cache, batch = make(gpu, b, 4)
+    q = torch.randn(b.ntok, 4, 64, device="cuda").bfloat16()
+    want = cache.attend(batch, q)[0]
+    for w in (max(kv), 2 ** 31 - 40, 2 ** 31 - 1):
+        assert torch.equal(cache.attend(batch, q, window=w)[0], want)
+    check_attn(gpu, b, 4, window=2 ** 31 - 1)

@@ -64,8 +64,9 @@ int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, Pag
         if (!b->qstart || !b->kvlen || !b->table) return vgx_fail(VGX_EINVAL, w + "NULL qstart, kvlen or table");
         if (b->table_cols <= 0 || b->table_stride < b->table_cols)
             return vgx_fail(VGX_EINVAL, w + "a table without columns, or rows that overlap");
-        if ((int64_t)b->table_cols * c->page_size > INT32_MAX - (1 << 20))
-            return vgx_fail(VGX_ERANGE, w + "a table's row holds 2^31 - 2^20 positions or more");
+        // (positions, less a window and 2^24 rows, stay inside 32 bits)
+        if ((int64_t)b->table_cols * c->page_size > INT32_MAX - (1 << 25))
+            return vgx_fail(VGX_ERANGE, w + "a table's row holds 2^31 - 2^25 positions or more");
         if ((int64_t)b->max_kv > (int64_t)b->table_cols * c->page_size)
             return vgx_fail(VGX_ERANGE, w + "max_kv past what a table's row holds");
     }

@@ -1198,6 +1198,10 @@ void fn_of(const PagedDev& A, int64_t cols, bool few, Launch& p) {
 // The columns the rows kernel takes at most.
 int64_t max_cols(const PagedDev& A) { return A.hd <= 128 ? 48 : 16; }
 
+// A window of every position is none (and what is left keeps the kernels' sums
+// of positions and windows inside 32 bits).
+int window_of(const PagedDev& A, int window) { return window >= A.max_kv ? 0 : window; }
+
 Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t cols, int cmin, bool alone) {
     Launch p{};
     int64_t span = A.max_kv;
@@ -1286,7 +1290,7 @@ size_t vgx_paged_attn_ws(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged*
     PagedDev A;
     if (vgx_paged_fill("vgx_paged_attn_ws", cache, batch, &A) != VGX_OK || !ctx || window < 0) return 0;
     if (A.ntok == 0 || A.nseq == 0) return 0;
-    return plan_of(A, cache->kind, window, ctx->num_cu).ws;
+    return plan_of(A, cache->kind, window_of(A, window), ctx->num_cu).ws;
 }
 
 int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_query* r) {
@@ -1308,7 +1312,8 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
         return vgx_fail(VGX_EINVAL, "vgx_paged_attn: q, out or ws not 16-byte aligned");
     if (!ctx) return vgx_fail(VGX_EINVAL, "vgx_paged_attn: no context");
     if (A.ntok == 0 || A.nseq == 0) return VGX_OK;
-    Plan p = plan_of(A, cache->kind, r->window, ctx->num_cu);
+    P.window = window_of(A, r->window);
+    Plan p = plan_of(A, cache->kind, P.window, ctx->num_cu);
     const bool split = p.ws && r->ws && r->ws_bytes >= p.ws;
     for (int i = 0; i < p.n && !split; ++i) {
         p.l[i].nsplit = 1;
@@ -1325,7 +1330,6 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     P.c = P.scale * kLog2e;
     if (!(P.c > 1e-30f) || std::isinf(P.c))
         return vgx_fail(VGX_EINVAL, "vgx_paged_attn: scale times the K step outside 1e-30 .. 1e38");
-    P.window = r->window;
     P.out_q16 = r->out_kind == VGX_E_Q16;
     P.out = static_cast<uint8_t*>(r->out);
     P.ostride = r->out_stride;
