@@ -292,6 +292,16 @@ def test_refusals(bad, what):
     assert what in L.vgx_last_error().decode()
 
 
+def test_more_than_a_launch_holds():
+    """65535 rows of 2^26 logits: refused by the library, not by the launch."""
+    L = vl.load()
+    big = dict(ntok=65535, vocab=1 << 26, stride=1 << 26, ws_bytes=1 << 60)
+    assert L.vgx_draft_verify(None, ctypes.byref(args(**big))) == vl.VGX_ERANGE
+    assert "too many" in L.vgx_last_error().decode()
+    assert L.vgx_draft_verify(None, ctypes.byref(args(nseq=65535, vocab=1 << 24, stride=1 << 24,
+                                                      ws_bytes=1 << 60))) == vl.VGX_ERANGE
+
+
 def test_workspace_sizes():
     L = vl.load()
     assert L.vgx_draft_verify_ws(2, 6, 100, vl.E_F32, 0) == 6 * 16

@@ -182,3 +182,11 @@ def test_binding_refuses_half_a_pair():
             cache.append(batch, x, **kw)
     with pytest.raises(ValueError, match="rot/2"):
         cache.append(batch, x, t[0], t[0])
+
+
+@pytest.mark.parametrize("step", [2.0 ** -65, 1e-45, 2.0 ** 65, 3e38])
+def test_steps_whose_reciprocal_or_range_is_not_finite(step):
+    for which in ("k_step", "v_step"):
+        st, msg = append(c=cache(kind=vl.E_Q8, **{which: step}))
+        assert st == vl.VGX_EINVAL and "step" in msg, msg
+        assert append(c=cache(kind=vl.E_Q8, **{which: 2.0 ** -64}))[1].endswith("no context")

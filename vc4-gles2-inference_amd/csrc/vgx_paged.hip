@@ -55,8 +55,9 @@ int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, Pag
                 return vgx_fail(VGX_EINVAL, w + "a page, head or row stride is negative, above 2^40 or not a multiple of 16 bytes");
         if (!apart(c->head_dim, n, st)) return vgx_fail(VGX_EINVAL, w + "the page, head and row strides overlap");
     }
-    if (!(c->k_step >= 0) || !(c->v_step >= 0) || std::isinf(c->k_step) || std::isinf(c->v_step))
-        return vgx_fail(VGX_EINVAL, w + "a q8 step is negative or not a number");
+    for (float step : {c->k_step, c->v_step})  // (a NaN is refused; 1 / step and 128 step stay finite)
+        if (step != 0 && !(step >= 0x1p-64f && step <= 0x1p64f))
+            return vgx_fail(VGX_EINVAL, w + "a q8 step is neither 0 nor in 2^-64 .. 2^64");
     if (b->nseq < 0 || b->ntok < 0 || b->nseq > (1 << 20) || b->ntok > (1 << 24))
         return vgx_fail(VGX_EINVAL, w + "nseq outside 0..2^20 or ntok outside 0..2^24");
     if (b->max_q < 0 || b->max_kv < 0) return vgx_fail(VGX_EINVAL, w + "a negative bound");

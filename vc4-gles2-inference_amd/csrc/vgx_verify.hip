@@ -706,6 +706,9 @@ int vgx_draft_verify(vgx_ctx* ctx, const vgx_draft* a) {
     const size_t need = vgx_draft_verify_ws(a->nseq, a->ntok, a->vocab, a->kind, a->draft != nullptr);
     if (a->nseq && need && (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 15)))
         return vgx_fail(VGX_EINVAL, "vgx_draft_verify: the workspace is missing, too small or not 16-byte aligned");
+    const Cut cut = cut_of(a->ntok, a->vocab, a->kind, a->draft != nullptr);
+    if ((int64_t)cut.nch * a->ntok * (a->draft ? 2 : 1) >= (1 << 24) || (int64_t)cut.nch * a->nseq >= (1 << 23))
+        return vgx_fail(VGX_ERANGE, "vgx_draft_verify: too many logits for one call");  // 2^32 threads
     if (!ctx) return vgx_fail(VGX_EINVAL, "vgx_draft_verify: no context");
     if (a->nseq == 0) return VGX_OK;
     VerifyArgs P{};
@@ -716,7 +719,6 @@ int vgx_draft_verify(vgx_ctx* ctx, const vgx_draft* a) {
     P.xs = a->stride * eb; P.ds = a->draft_stride * eb;
     P.temp = a->temp; P.ua = a->u_accept; P.un = a->u_next;
     P.accepted = a->accepted; P.next = a->next; P.prob = a->prob;
-    const Cut cut = cut_of(a->ntok, a->vocab, a->kind, a->draft != nullptr);
     P.nch = cut.nch;
     P.chunk = cut.k * kThreads;
     P.px = static_cast<Part*>(a->ws);
