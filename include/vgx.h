@@ -389,12 +389,13 @@ typedef struct vgx_paged {
 
 /* The batch: nseq sequences whose new tokens are ntok consecutive rows.
  * Device arrays, read by the kernels (a captured call is replayed with new
- * contents): sequence s has rows qstart[s] .. qstart[s+1]-1 (qstart[0] = 0,
- * none is allowed), kvlen[s] positions counting those rows, and position p in
+ * contents): sequence s has rows qstart[s] .. qstart[s+1]-1 (none is
+ * allowed), kvlen[s] positions counting those rows, and position p in
  * page table[s * table_stride + p / page_size], slot p % page_size.  Its row
- * r is position kvlen[s] - rows + r.  Rows at or behind qstart[nseq] are left
- * as they are.  table_cols: entries a row of the table holds (entries past a
- * sequence's length are not read).
+ * r is position kvlen[s] - rows + r.  Rows before qstart[0] (so that a part
+ * of a larger batch can be named) and from qstart[nseq] on are left as they
+ * are.  table_cols: entries a row of the table holds (what stands past a
+ * sequence's length does not matter).
  * max_q, max_kv: the caller's bounds of the rows and positions of one
  * sequence, by which launches are sized (0: ntok, and what the table holds).
  * Bounds that the kernels check themselves, since the host cannot: a length
@@ -419,8 +420,8 @@ typedef struct vgx_ragged {
  * or neither) and the rotation of their first rot values by the angles of the
  * row's position (cos / sin: npos rows of rot/2 f32, device; rot a multiple of
  * 16, 0: none; rope_half as in vgx_attn_desc), then q rounded into q (ntok rows
- * of heads * head_dim, q_stride elements apart, compute type; may be NULL) and
- * K and V rounded into the pages.  qkv: ntok rows of (heads + 2 * kv_heads) *
+ * of heads * head_dim, q_stride elements apart, compute type, apart from qkv;
+ * may be NULL) and K and V rounded into the pages (a NaN is 0 on q8's grid).  qkv: ntok rows of (heads + 2 * kv_heads) *
  * head_dim values of kind F32, BF16, F16 or Q16 (vgx_gemm's output), stride
  * elements apart.  A row whose position is negative (more rows than kvlen) is
  * skipped. */
@@ -443,7 +444,8 @@ int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* bat
  * sequence's positions 0 .. its own (with window > 0 the last `window` of
  * them).  q: ntok rows of heads * head_dim, compute type, q_stride elements
  * apart; scale 0: 1/sqrt(head_dim).  out: rows of heads * head_dim, out_kind
- * the compute type or Q16 (vgx_gemm's input), out_stride elements apart.  lse
+ * the compute type or Q16 (vgx_gemm's input; a NaN is 0 on its grid),
+ * out_stride elements apart, apart from q.  lse
  * (may be NULL): f32, ntok x heads, the log of the softmax's denominator.  A
  * row without a visible position gives zeros and an lse of -infinity.
  * Positions a row does not see, and what a page holds behind its sequence's

@@ -661,3 +661,50 @@ def test_attn_widest_window(gpu, nq, kv):
     for w in (max(kv), 2 ** 31 - 40, 2 ** 31 - 1):
         assert torch.equal(cache.attend(batch, q, window=w)[0], want)
     check_attn(gpu, b, 4, window=2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("part", [(1, 3), (2, 4), (0, 2)])
+def test_part_of_a_batch(gpu, part):
+    """Some of a batch's sequences, named by their entries of qstart: the rows
+    before and behind them are left as they are."""
+    b = Batch(35, [70, 1, 3, 90], [100, 2500, 300, 1800], 2, 64, 16, "bf16")
+    cache, whole = make(gpu, b, 4)
+    qs, kv, table = b.device()
+    q = torch.randn(b.ntok, 4, 64, device="cuda").bfloat16()
+    lo, hi = part
+    for kw in (dict(), dict(max_q=90, max_kv=2500)):
+        some = cache.batch(qs[lo:hi + 1], kv[lo:hi], table[lo:hi], b.ntok, **kw)
+        out = torch.full((b.ntok, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+        z = cache.attend(some, q, out=out, lse=True)[1]
+        r0, r1 = int(b.qs[lo]), int(b.qs[hi])
+        assert (out[:r0] == 5).all() and (out[r1:] == 5).all()
+        sub = Batch(35, b.nq[lo:hi], b.kv[lo:hi], 2, 64, 16, "bf16")
+        sub.k, sub.v, sub.table, sub.pages = b.k, b.v, b.table[lo:hi], b.pages
+        want, wl, mag, dots = ref.attend(sub, q[r0:r1].cpu(), 4)
+        bound = ref.attn_bound(sub, torch.bfloat16, want, mag, dots)
+        assert ((out[r0:r1].cpu().double().view_as(want) - want).abs() <= bound).all()
+        assert torch.isfinite(z[r0:r1]).all()
+    x = torch.randn(b.ntok, 512, device="cuda")
+    before = cache.k.clone()
+    qo = torch.full((b.ntok, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    cache.append(some, x, out=qo)
+    assert (qo[:r0] == 5).all() and (qo[r1:] == 5).all()
+    assert int((cache.k != before).any(-1).any(1).sum()) == sum(b.nq[lo:hi])
+    some.check()
+
+
+def test_append_bad_page_writes_nothing_of_the_row(gpu):
+    from vgx import lib as vl
+    b = Batch(36, [2, 1], [20, 40], 2, 64, 16, "q8")
+    cache, _ = make(gpu, b, 4)
+    qs, kv, table = b.device()
+    table[1, 2] = b.pages
+    batch = cache.batch(qs, kv, table, 3)
+    qo = torch.full((3, 4, 64), 5.0, dtype=torch.float16, device="cuda")
+    before = cache.k.clone(), cache.v.clone()
+    cache.append(batch, torch.randn(3, 512, device="cuda"), out=qo)
+    with pytest.raises(vl.VgxError, match="page"):
+        batch.check()
+    assert (qo[2] == 5).all() and not (qo[:2] == 5).all(-1).any()
+    changed = (cache.k != before[0]).any(-1).any(1).nonzero()
+    assert {int(p) for p in changed[:, 0]} == {int(b.table[0, 1])}

@@ -1061,9 +1061,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
     const int t = (int)(w0 / A.heads);
     const int head = (int)(w0 - (int64_t)t * A.heads) + (WIDE ? 0 : lane >> lg);
     if (t >= A.ntok) return;
-    // (the entry of a row behind the last sequence was written by nobody, nor
-    // that of a row past the bounds)
-    const uint2 e = t < A.qstart[A.nseq] ? P.pn[(int64_t)t * A.heads + head] : make_uint2(0, 0);
+    // (the entry of a row before the first sequence or behind the last was
+    // written by nobody, nor that of a row past the bounds)
+    const uint2 e = t >= A.qstart[0] && t < A.qstart[A.nseq] ? P.pn[(int64_t)t * A.heads + head] : make_uint2(0, 0);
     const int nsp = e.x & 0xffff;
     const int64_t step = e.x & kBySeq ? J.step_seq : J.step_row, at = e.y;
     if (nsp <= 1 || at + (nsp - 1) * step >= J.total) return;
