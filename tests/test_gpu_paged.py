@@ -708,3 +708,18 @@ def test_append_bad_page_writes_nothing_of_the_row(gpu):
     assert (qo[2] == 5).all() and not (qo[:2] == 5).all(-1).any()
     changed = (cache.k != before[0]).any(-1).any(1).nonzero()
     assert {int(p) for p in changed[:, 0]} == {int(b.table[0, 1])}
+
+
+@pytest.mark.parametrize("kind, hd, page, window", [("bf16", 64, 16, 0), ("q8", 80, 5, 0), ("f16", 64, 16, 19000),
+                                                    ("f16", 128, 32, 0)])
+def test_attn_bounds_far_above(gpu, kind, hd, page, window):
+    """Bounds far above most lengths: few, longer splits, also of the one
+    sequence that reaches them."""
+    kv = [int(m) for m in torch.randint(0, 300, (40,), generator=torch.Generator().manual_seed(2))]
+    kv[3], kv[17], kv[39] = 24000, 1900, 17001
+    b = Batch(37, [1] * 39 + [3], kv, 8, hd, page, kind)
+    cache, batch = make(gpu, b, 8, max_q=4, max_kv=24000)
+    check_attn(gpu, b, 8, window=window, cache=cache, batch=batch)
+    # (the table's own size as the bound, and more rows than sequences have)
+    b.table = torch.cat([b.table, torch.full((40, 60000 // page), -1, dtype=torch.int32)], 1)
+    check_attn(gpu, b, 8, window=window, cache=cache, batch=cache.batch(*b.device(), b.ntok, 5))

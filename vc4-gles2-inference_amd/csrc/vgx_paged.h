@@ -69,19 +69,23 @@ __device__ __forceinline__ int seq_of_row(const PagedDev& A, int t) {
     return s;
 }
 
-// The positions a tile of a sequence's rows attends to, cut into splits of
-// split_len: [lo, hi) and the number of splits (at least 1).  first, last:
-// the tile's rows.  lo is a multiple of 64, so a tile of keys never starts
-// inside a page that its neighbour's tile also starts in.
+// The positions a tile of a sequence's rows attends to, cut into splits:
+// [lo, hi), a split's length and their number (at least 1).  first, last: the
+// tile's rows.  lo is a multiple of 64, so a tile of keys never starts inside a
+// page that its neighbour's tile also starts in.  Splits are split_len long, or
+// where that would make more than 2^sh, a multiple of 128 that does not (sh 31:
+// split_len is enough, and 128 or more).
 struct Span {
-    int lo, hi, nsp;
+    int lo, hi, len, nsp;
 };
-__device__ __forceinline__ Span span_of(const SeqAt& q, int first, int last, int window, int split_len) {
+__device__ __forceinline__ Span span_of(const SeqAt& q, int first, int last, int window, int split_len, int sh = 31) {
     Span r;
     const int base = q.kv - q.n;
     r.hi = max(min(q.kv, base + last + 1), 0);
     r.lo = window > 0 ? max(base + first - window + 1, 0) & ~63 : 0;
     r.lo = min(r.lo, r.hi);
-    r.nsp = (int)max(((unsigned)(r.hi - r.lo) + (unsigned)split_len - 1) / (unsigned)split_len, 1u);
+    const int n = max(r.hi - r.lo, 1);
+    r.len = max(split_len, (((n - 1) >> sh >> 7) + 1) << 7);
+    r.nsp = (int)(((unsigned)n + (unsigned)r.len - 1) / (unsigned)r.len);
     return r;
 }

@@ -43,7 +43,7 @@ struct AttnArgs {
     float c;       // scale * log2(e), the K step included: exponents of 2
     float scale;   // scale with the K step: scores
     int window;
-    int split_len;
+    int split_len, split_sh;
     int cmin, cmax;  // the sequences of this launch: cmin < columns a KV head <= cmax
     int out_q16;
     uint8_t* out;
@@ -632,7 +632,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
     // loads then go out as one batch instead of a round trip at each first use.
     asm volatile("" ::"s"(A.k), "s"(A.v), "s"(A.kpg), "s"(A.khd), "s"(A.krow), "s"(A.vpg), "s"(A.vhd), "s"(A.vrow),
                  "s"(A.tstride), "s"(A.qstart), "s"(A.kvlen), "s"(A.table), "s"(P.q), "s"(P.qstride), "s"(P.out),
-                 "s"(P.po), "s"(P.split_len), "s"(P.window), "s"(P.c), "s"(A.kvh), "s"(A.grp), "s"(A.psize),
+                 "s"(P.po), "s"(P.split_len), "s"(P.split_sh), "s"(P.window), "s"(P.c), "s"(A.kvh), "s"(A.grp), "s"(A.psize),
                  "s"(A.pmul), "s"(A.npages), "s"(A.max_kv), "s"(A.ntok), "s"(A.heads), "s"(A.max_q), "s"(A.tcols));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
@@ -648,9 +648,9 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
     const SeqAt q = seq_at(A, s);
     if (!q.ok && threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
     if (q.n <= 0 || q.n * A.grp > P.cmax) return;
-    const Span sp = span_of(q, 0, q.n - 1, P.window, P.split_len);
+    const Span sp = span_of(q, 0, q.n - 1, P.window, P.split_len, P.split_sh);
     if (split >= sp.nsp) return;
-    const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
+    const int start = sp.lo + split * sp.len, end = start + min(sp.hi - start, sp.len);
     const uint8_t* kh = A.k + (int64_t)h * A.khd;
     const uint8_t* vh = A.v + (int64_t)h * A.vhd;
     uint8_t* lv = smem + wave * kWave;
@@ -659,7 +659,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
     int pn = 0;
     bool bad = false, odd = false;
     if (j0 < end) {
-        if (P.window > 0) pg = Ks::page(A, tab, j0, end);
+        if (P.window > 0 || sp.len != P.split_len) pg = Ks::page(A, tab, j0, end);
         pn = Ks::page(A, tab, j0 + 32 * WV, end);
     }
     Col cl[NB];
@@ -895,7 +895,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, in
     const int m0 = local * 128, m1 = min(m0 + 128, q.n * A.grp) - 1;
     const Span sp = span_of(q, m0 / A.grp, m1 / A.grp, P.window, P.split_len);
     if (split >= sp.nsp) return;
-    const int start = sp.lo + split * P.split_len, end = start + min(sp.hi - start, P.split_len);
+    const int start = sp.lo + split * sp.len, end = start + min(sp.hi - start, sp.len);
     const Col cl = col_of(P, q, h, m0 + wave * 32 + col, end);
     s16x8 qf[HD / 16];
     load_q<HD, EX>(A, P.q + ((int64_t)cl.row * P.qstride + (int64_t)cl.head * A.hd) * 2, cl.valid, qf);
@@ -1136,7 +1136,7 @@ struct Launch {
     bool rows;
     int cmin, cmax;
     int64_t wgs;       // workgroups of one split
-    int split_len, nsplit;
+    int split_len, split_sh, nsplit;
 };
 struct Plan {
     Launch l[2];
@@ -1232,9 +1232,24 @@ Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t co
     if (p.rows && A.nseq > 1)
         len = span <= kWhole ? span : std::min<int64_t>(std::max<int64_t>(len, 512), p.wgs >= num_cu ? 1024 : 768);
     len = (len + 127) / 128 * 128;
-    if (p.threads == 512) len = std::max<int64_t>(span, 1);
+    if (p.threads == 512) len = std::max<int64_t>(span, 128);
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
     p.nsplit = (int)std::max<int64_t>((span + len - 1) / len, 1);
+    p.split_sh = 31;
+    // A bound far above the lengths costs an empty workgroup for each split
+    // that no sequence has, so their number ends at 8192 in all (8 splits at
+    // the least): longer sequences then take longer splits.  64 sequences of
+    // 500, 32 / 8 heads of 128: 42 us under bounds of 16384 to 10^6 positions
+    // (without this 81 at 65536, 889 at 10^6); one of 60000 positions among 24
+    // of 500, 16 / 8 heads of 64: 59 us (4096 in all: 79).
+    if (p.rows && A.nseq > 1) {
+        int sh = 3;
+        while (sh < 13 && (p.wgs << (sh + 1)) <= 8192) ++sh;
+        if (p.nsplit > 1 << sh) {
+            p.nsplit = 1 << sh;
+            p.split_sh = sh;
+        }
+    }
     return p;
 }
 
@@ -1318,6 +1333,7 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     for (int i = 0; i < p.n && !split; ++i) {
         p.l[i].nsplit = 1;
         p.l[i].split_len = INT32_MAX;
+        p.l[i].split_sh = 31;
     }
     for (int i = 0; i < p.n; ++i)
         if (p.l[i].wgs >= (1 << 24) || p.l[i].nsplit > 65535)
@@ -1346,6 +1362,7 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     for (int i = 0; i < p.n; ++i) {
         const Launch& l = p.l[i];
         P.split_len = l.split_len;
+        P.split_sh = l.split_sh;
         P.cmin = l.cmin;
         P.cmax = l.cmax;
         P.by_seq = i == 0 && p.by_seq;

@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
 
 // Pieces a thread and chunk (K) and chunks of a row.  A row may begin inside a
 // piece.  Chunks of 256 pieces (2048 16-bit logits) while they are fewer than
-// 1024; one row of 6400: 5.0 us against 8.5 with chunks of 1024.
+// 1024; one row of 6400: 3.8 us against 8.5 with chunks of 1024.
 struct Cut {
     int k, nch;
 };
