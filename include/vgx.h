@@ -401,9 +401,9 @@ typedef struct vgx_paged {
  * Bounds that the kernels check themselves, since the host cannot: a length
  * outside the table's, the bounds above or the rotation's, and a page outside
  * the pool, set bits (VGX_FAULT_*) in *fault (device int, may be NULL, never
- * cleared here).  The rows concerned are not written by vgx_paged_append, and
- * vgx_paged_attn leaves them with values that mean nothing; no access leaves
- * the buffers. */
+ * cleared here).  vgx_paged_append writes nothing of the rows concerned into
+ * the pages (nor, for a length, into q), and vgx_paged_attn leaves them with
+ * values that mean nothing; no access leaves the buffers. */
 enum vgx_fault { VGX_FAULT_LENGTH = 1, VGX_FAULT_PAGE = 2 };
 typedef struct vgx_ragged {
     int nseq, ntok, max_q, max_kv;
