@@ -388,12 +388,16 @@ constexpr int kKept = 32;  // joined rows kept in LDS
 struct Shared {
     double tab[64];
     Part x[kKept], d[kKept];
+    int tok[kKept];     // the drafted token, and its logit
+    float lx[kKept];
     int first;
 };
 struct Decision {
     int q0, n, acc;
     bool refused;
     Part x, d;
+    int tok;    // of a refused row: its draft, and that one's logit
+    float lx;
 };
 template <int KIND>
 __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Temp& T, Shared& H, bool write) {
@@ -416,7 +420,7 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
         const Part x = join(P, P.px, t, T.inv, H.tab);
         Part d{};
         if (dist) d = join(P, P.pd, t, T.inv, H.tab);
-        if (lead && i < kKept) { H.x[i] = x; H.d[i] = d; }
+        if (lead && i < kKept) { H.x[i] = x; H.d[i] = d; H.tok[i] = tok; H.lx[i] = lx; }
         if (!drafted) {
             if (write && P.prob && lead) P.prob[t] = 0.0f;
             continue;
@@ -441,9 +445,13 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
     if (r.acc < kKept) {
         r.x = H.x[r.acc];
         r.d = H.d[r.acc];
+        r.tok = H.tok[r.acc];
+        r.lx = H.lx[r.acc];
     } else {
         r.x = join(P, P.px, r.q0 + r.acc, T.inv, H.tab);
         if (P.d && !T.greedy) r.d = join(P, P.pd, r.q0 + r.acc, T.inv, H.tab);
+        r.tok = r.refused ? P.tokens[r.q0 + r.acc + 1] : -1;
+        r.lx = one<KIND>(P.x + (int64_t)(r.q0 + r.acc) * P.xs, r.tok >= 0 && r.tok < P.vocab ? r.tok : 0);
     }
     return r;
 }
@@ -515,6 +523,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
     __shared__ int chosen, found, last, plain;
     const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Temp T = temp_of(P, s);
+    const double un = P.un[s];  // (asked for before the chain below)
     const Decision D = decide<KIND>(P, s, T, H, true);
     if (D.n <= 0) {
         if (threadIdx.x == 0) { P.accepted[s] = 0; P.next[s] = -1; }
@@ -529,7 +538,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
         return;
     }
     bool draft = P.d && D.refused;
-    const Residual R = residual_of(D, T.inv, D.refused && !P.d ? P.tokens[t + 1] : -1);
+    const Residual R = residual_of(D, T.inv, D.refused && !P.d ? D.tok : -1);
     const Row qx = row_at<KIND>(P.x, P.xs, t);
     // the chunks' sums, walked by one wave; without draft logits they are
     // launch 1's, less the refused token
@@ -540,7 +549,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             if (draft) return P.w[(int64_t)s * P.nch + c];
             const Part p = P.px[(int64_t)t * P.nch + c];
             double z = p.z;
-            if (c == tchunk) z = fmax(z - weight(one<KIND>(qx.p, R.tok), p.m, T.inv, tab), 0.0);
+            if (c == tchunk) z = fmax(z - weight(D.lx, p.m, T.inv, tab), 0.0);
             return z * weight(p.m, R.sx, tab) * R.zx;
         };
         double total = 0.0;
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             for (int c = 0; c < P.nch; c += 64) total += sum_of(c + lane);
             total = wave_sum(total);
         }
-        const double want = (double)P.un[s] * total;
+        const double want = un * total;
         double before = 0.0;
         int pick = -1, some = -1;
         double at = 0.0, some_at = 0.0;
