@@ -209,6 +209,23 @@ __device__ __forceinline__ float wave_max(float x) {
     x = fmaxf(x, dpp<0x140>(x));
     return fmaxf(fmaxf(lane_of(x, 0), lane_of(x, 16)), fmaxf(lane_of(x, 32), lane_of(x, 48)));
 }
+// The running sum over the lanes: inside rows of 16 (row_shr), then the rows
+// before (row_bcast 15 and 31).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+    const uint32x2 u = __builtin_bit_cast(uint32x2, x);
+    const uint32x2 v = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, false),
+                        (unsigned)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, false)};
+    return x + __builtin_bit_cast(double, v);
+}
+__device__ __forceinline__ double wave_scan(double x) {
+    x = dpp_add<0x111, 0xF>(x);
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);
+    return dpp_add<0x143, 0xC>(x);
+}
 // (value, index): the larger value, the smaller index of equals.
 __device__ __forceinline__ void wave_best(float& m, int& a) {
 #pragma unroll
@@ -357,46 +374,49 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     }
 }
 
-// A row's chunks joined by one wave: its maximum, first index and sum.
-__device__ __forceinline__ Part join(const VerifyArgs& P, const Part* parts, int t, double inv, const double* tab) {
+// A row's chunks joined by one wave: its maximum, with best its first index, and
+// its sum.
+__device__ __forceinline__ Part join(const VerifyArgs& P, const Part* parts, int t, double inv, bool best,
+                                     const double* tab) {
     const int lane = threadIdx.x & 63;
     const Part* p = parts + (int64_t)t * P.nch;
-    Part x;
-    x.m = -INFINITY;
-    x.arg = 0x7fffffff;
-    x.z = 0.0;
-    if (lane < P.nch) x = p[lane];
-    float m = x.m;
-    int a = x.arg;
+    const Part none = {-INFINITY, 0x7fffffff, 0.0};
+    Part x = lane < P.nch ? p[lane] : none;
+    Part r = x;
+#pragma unroll 1
     for (int c = lane + 64; c < P.nch; c += 64)
-        if (p[c].m > m || (p[c].m == m && p[c].arg < a)) { m = p[c].m; a = p[c].arg; }
-    wave_best(m, a);
-    const Scale S = scale_of(m, inv);
-    double z = x.z * weight(x.m, S, tab);
-    for (int c = lane + 64; c < P.nch; c += 64) z += p[c].z * weight(p[c].m, S, tab);
-    Part r;
-    r.m = m;
-    r.arg = a;
-    r.z = wave_sum(z);
+        if (p[c].m > r.m || (p[c].m == r.m && p[c].arg < r.arg)) { r.m = p[c].m; r.arg = p[c].arg; }
+    if (best) wave_best(r.m, r.arg);
+    else r.m = wave_max(r.m);
+    const Scale S = scale_of(r.m, inv);
+    r.z = 0.0;
+#pragma unroll 1
+    for (int c = 0;;) {
+        r.z += x.z * weight(x.m, S, tab);
+        c += 64;
+        if (c >= P.nch) break;
+        x = c + lane < P.nch ? p[c + lane] : none;
+    }
+    r.z = wave_sum(r.z);
     return r;
 }
 
 // What a sequence's rows decide: the first row that refuses its draft (the
 // last row where none does), and that row joined, by every thread of the
-// workgroup.  A wave takes a row.
-constexpr int kKept = 32;  // joined rows kept in LDS
+// workgroup.  A wave takes a row's logits or its draft's, kGroup rows at a time.
+constexpr int kGroup = 32;
 struct Shared {
     double tab[64];
-    Part x[kKept], d[kKept];
-    int tok[kKept];     // the drafted token, and its logit
-    float lx[kKept];
-    int first;
+    Part x[2][kGroup];    // the target's rows, the draft's
+    double p[2][kGroup];  // what they give the drafted token
+    int tok[kGroup];      // the drafted token, and its logit
+    float lx[kGroup];
 };
 struct Decision {
     int q0, n, acc;
     bool refused;
     Part x, d;
-    int tok;    // of a refused row: its draft, and that one's logit
+    int tok;  // of a refused row: its draft, and that one's logit
     float lx;
 };
 template <int KIND>
@@ -405,53 +425,47 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
     r.q0 = min(max(P.qstart[s], 0), P.ntok);
     r.n = max(min(P.qstart[s + 1], P.ntok) - r.q0, 0);
     fill_table(H.tab);
-    if (threadIdx.x == 0) H.first = r.n - 1;
     __syncthreads();
-    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const bool lead = (threadIdx.x & 63) == 0;
-    for (int i = wave; i < r.n; i += waves) {
-        const int t = r.q0 + i;
-        const bool drafted = i + 1 < r.n, dist = P.d && !T.greedy;
-        const int tok = drafted ? P.tokens[t + 1] : -1;
-        const float ua = drafted ? P.ua[t] : 0.0f;
-        const bool in = tok >= 0 && tok < P.vocab;
-        const float lx = one<KIND>(P.x + (int64_t)t * P.xs, in ? tok : 0);
-        const float ld = dist ? one<KIND>(P.d + (int64_t)t * P.ds, in ? tok : 0) : 0.0f;
-        const Part x = join(P, P.px, t, T.inv, H.tab);
-        Part d{};
-        if (dist) d = join(P, P.pd, t, T.inv, H.tab);
-        if (lead && i < kKept) { H.x[i] = x; H.d[i] = d; H.tok[i] = tok; H.lx[i] = lx; }
-        if (!drafted) {
-            if (write && P.prob && lead) P.prob[t] = 0.0f;
-            continue;
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+    const int sides = P.d && !T.greedy ? 2 : 1;
+#pragma unroll 1
+    for (int g = 0; g < r.n; g += kGroup) {
+        const int m = min(r.n - g, kGroup);
+        const bool drafted = lane < m && g + lane + 1 < r.n;
+        const float ua = drafted ? P.ua[r.q0 + g + lane] : 0.0f;
+        if (g) __syncthreads();  // the last group's values are read
+#pragma unroll 1
+        for (int w = wave; w < m * sides; w += waves) {
+            const int side = w >= m, i = side ? w - m : w, t = r.q0 + g + i;
+            const int tok = g + i + 1 < r.n ? P.tokens[t + 1] : -1;
+            const bool in = tok >= 0 && tok < P.vocab;
+            const float l = one<KIND>(side ? P.d + (int64_t)t * P.ds : P.x + (int64_t)t * P.xs, in ? tok : 0);
+            const Part x = join(P, side ? P.pd : P.px, t, T.inv, T.greedy, H.tab);
+            double v;
+            if (T.greedy) v = x.m != -INFINITY && tok == x.arg ? 1.0 : 0.0;
+            else v = in && x.z > 0.0 ? weight(l, x.m, T.inv, H.tab) / x.z : 0.0;
+            if (lane == 0) {
+                H.x[side][i] = x;
+                H.p[side][i] = v;
+                if (!side) { H.tok[i] = tok; H.lx[i] = l; }
+            }
         }
-        double pr, qr = 1.0;
-        if (T.greedy) {
-            pr = x.m != -INFINITY && tok == x.arg ? 1.0 : 0.0;
-        } else {
-            pr = in && x.z > 0.0 ? weight(lx, x.m, T.inv, H.tab) / x.z : 0.0;
-            if (dist) qr = in && d.z > 0.0 ? weight(ld, d.m, T.inv, H.tab) / d.z : 0.0;
-        }
+        __syncthreads();
+        const double pr = drafted ? H.p[0][lane & (kGroup - 1)] : 0.0;
+        const double qr = drafted && sides == 2 ? H.p[1][lane & (kGroup - 1)] : 1.0;
         const bool ok = T.greedy ? pr > 0.0 : (double)ua * qr < pr;
-        if (lead) {
-            if (!ok) atomicMin(&H.first, i);
-            if (write && P.prob) P.prob[t] = (float)pr;
+        if (write && P.prob && wave == 0 && lane < m) P.prob[r.q0 + g + lane] = (float)pr;
+        const unsigned long long no = __ballot(drafted && !ok);
+        if (!r.refused && (no || g + m == r.n)) {
+            r.refused = no != 0;
+            const int i = no ? __ffsll(no) - 1 : m - 1;
+            r.acc = g + i;
+            r.x = H.x[0][i];
+            if (sides == 2) r.d = H.x[1][i];
+            r.tok = H.tok[i];
+            r.lx = H.lx[i];
         }
-    }
-    __syncthreads();
-    if (r.n <= 0) return r;
-    r.acc = H.first;
-    r.refused = r.acc < r.n - 1;
-    if (r.acc < kKept) {
-        r.x = H.x[r.acc];
-        r.d = H.d[r.acc];
-        r.tok = H.tok[r.acc];
-        r.lx = H.lx[r.acc];
-    } else {
-        r.x = join(P, P.px, r.q0 + r.acc, T.inv, H.tab);
-        if (P.d && !T.greedy) r.d = join(P, P.pd, r.q0 + r.acc, T.inv, H.tab);
-        r.tok = r.refused ? P.tokens[r.q0 + r.acc + 1] : -1;
-        r.lx = one<KIND>(P.x + (int64_t)(r.q0 + r.acc) * P.xs, r.tok >= 0 && r.tok < P.vocab ? r.tok : 0);
+        if (r.refused && !write) break;
     }
     return r;
 }
@@ -552,41 +566,42 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             if (c == tchunk) z = fmax(z - weight(D.lx, p.m, T.inv, tab), 0.0);
             return z * weight(p.m, R.sx, tab) * R.zx;
         };
-        double total = 0.0;
-        for (int c = 0; c < P.nch; c += 64) total += sum_of(c + lane);
-        total = wave_sum(total);
+        double total, v0;
         if (lane == 0) plain = 0;
-        if (draft && !(total > 0.0)) {  // p = q: the draw is from p
-            draft = false;
-            if (lane == 0) plain = 1;
+#pragma unroll 1
+        for (;;) {
             total = 0.0;
-            for (int c = 0; c < P.nch; c += 64) total += sum_of(c + lane);
+#pragma unroll 1
+            for (int c = 0; c < P.nch; c += 64) {
+                const double v = sum_of(c + lane);
+                if (c == 0) v0 = v;
+                total += v;
+            }
             total = wave_sum(total);
+            if (!draft || total > 0.0) break;
+            draft = false;  // p = q: the draw is from p
+            if (lane == 0) plain = 1;
         }
         const double want = un * total;
         double before = 0.0;
         int pick = -1, some = -1;
         double at = 0.0, some_at = 0.0;
+#pragma unroll 1
         for (int c = 0; c < P.nch && pick < 0; c += 64) {
-            const double v = sum_of(c + lane);
-            double run = v;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(run, o, 64);
-                if (lane >= o) run += y;
-            }
+            const double v = c ? sum_of(c + lane) : v0;
+            const double run = wave_scan(v);
             const unsigned long long past = __ballot(before + run > want && v > 0.0);
             const unsigned long long any = __ballot(v > 0.0);
             if (past) {
                 const int l = __ffsll((unsigned long long)past) - 1;
                 pick = c + l;
-                at = before + __shfl(run, l, 64) - __shfl(v, l, 64);
+                at = before + lane_of(run, l) - lane_of(v, l);
             } else if (any) {
                 const int l = 63 - __clzll((long long)any);
                 some = c + l;
-                some_at = before + __shfl(run, l, 64) - __shfl(v, l, 64);
+                some_at = before + lane_of(run, l) - lane_of(v, l);
             }
-            before += __shfl(run, 63, 64);
+            before += lane_of(run, 63);
         }
         if (lane == 0) {
             chosen = pick >= 0 ? pick : some;
@@ -633,12 +648,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             if (w[k * N + e] > 0.0) mine = j;
         }
     }
-    double run = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(run, o, 64);
-        if (lane >= o) run += y;
-    }
+    const double run = wave_scan(sum);
     if (lane == 63) sw[wave] = run;
     if (mine >= 0) atomicMax(&last, mine);
     __syncthreads();
