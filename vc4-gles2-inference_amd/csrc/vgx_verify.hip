@@ -374,14 +374,14 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     }
 }
 
-// A row's chunks joined by one wave: its maximum, with best its first index, and
-// its sum.
-__device__ __forceinline__ Part join(const VerifyArgs& P, const Part* parts, int t, double inv, bool best,
+__device__ __forceinline__ Part part_of(const VerifyArgs& P, const Part* p, int c) {
+    return c < P.nch ? p[c] : Part{-INFINITY, 0x7fffffff, 0.0};
+}
+// A row's chunks (p; x: the first 64, a lane each) joined by one wave: its
+// maximum, with best its first index, and its sum.
+__device__ __forceinline__ Part join(const VerifyArgs& P, const Part* p, Part x, double inv, bool best,
                                      const double* tab) {
     const int lane = threadIdx.x & 63;
-    const Part* p = parts + (int64_t)t * P.nch;
-    const Part none = {-INFINITY, 0x7fffffff, 0.0};
-    Part x = lane < P.nch ? p[lane] : none;
     Part r = x;
 #pragma unroll 1
     for (int c = lane + 64; c < P.nch; c += 64)
@@ -395,7 +395,7 @@ __device__ __forceinline__ Part join(const VerifyArgs& P, const Part* parts, int
         r.z += x.z * weight(x.m, S, tab);
         c += 64;
         if (c >= P.nch) break;
-        x = c + lane < P.nch ? p[c + lane] : none;
+        x = part_of(P, p, c + lane);
     }
     r.z = wave_sum(r.z);
     return r;
@@ -424,10 +424,23 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
     Decision r{};
     r.q0 = min(max(P.qstart[s], 0), P.ntok);
     r.n = max(min(P.qstart[s + 1], P.ntok) - r.q0, 0);
-    fill_table(H.tab);
-    __syncthreads();
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
     const int sides = P.d && !T.greedy ? 2 : 1;
+    // (the first row's loads are on their way while the table is made)
+    int side, i, tok;
+    const Part* p;
+    Part x;
+    auto load = [&](int g, int m, int w) {
+        side = w >= m;
+        i = side ? w - m : w;
+        const int t = r.q0 + g + i;
+        p = (side ? P.pd : P.px) + (int64_t)t * P.nch;
+        x = part_of(P, p, lane);
+        tok = g + i + 1 < r.n ? P.tokens[t + 1] : -1;
+    };
+    if (wave < min(r.n, kGroup) * sides) load(0, min(r.n, kGroup), wave);
+    fill_table(H.tab);
+    __syncthreads();
 #pragma unroll 1
     for (int g = 0; g < r.n; g += kGroup) {
         const int m = min(r.n - g, kGroup);
@@ -436,16 +449,16 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
         if (g) __syncthreads();  // the last group's values are read
 #pragma unroll 1
         for (int w = wave; w < m * sides; w += waves) {
-            const int side = w >= m, i = side ? w - m : w, t = r.q0 + g + i;
-            const int tok = g + i + 1 < r.n ? P.tokens[t + 1] : -1;
+            if (g || w != wave) load(g, m, w);
+            const int t = r.q0 + g + i;
             const bool in = tok >= 0 && tok < P.vocab;
             const float l = one<KIND>(side ? P.d + (int64_t)t * P.ds : P.x + (int64_t)t * P.xs, in ? tok : 0);
-            const Part x = join(P, side ? P.pd : P.px, t, T.inv, T.greedy, H.tab);
+            const Part y = join(P, p, x, T.inv, T.greedy, H.tab);
             double v;
-            if (T.greedy) v = x.m != -INFINITY && tok == x.arg ? 1.0 : 0.0;
-            else v = in && x.z > 0.0 ? weight(l, x.m, T.inv, H.tab) / x.z : 0.0;
+            if (T.greedy) v = y.m != -INFINITY && tok == y.arg ? 1.0 : 0.0;
+            else v = in && y.z > 0.0 ? weight(l, y.m, T.inv, H.tab) / y.z : 0.0;
             if (lane == 0) {
-                H.x[side][i] = x;
+                H.x[side][i] = y;
                 H.p[side][i] = v;
                 if (!side) { H.tok[i] = tok; H.lx[i] = l; }
             }
@@ -458,12 +471,12 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& P, int s, const Tem
         const unsigned long long no = __ballot(drafted && !ok);
         if (!r.refused && (no || g + m == r.n)) {
             r.refused = no != 0;
-            const int i = no ? __ffsll(no) - 1 : m - 1;
-            r.acc = g + i;
-            r.x = H.x[0][i];
-            if (sides == 2) r.d = H.x[1][i];
-            r.tok = H.tok[i];
-            r.lx = H.lx[i];
+            const int k = no ? __ffsll(no) - 1 : m - 1;
+            r.acc = g + k;
+            r.x = H.x[0][k];
+            if (sides == 2) r.d = H.x[1][k];
+            r.tok = H.tok[k];
+            r.lx = H.lx[k];
         }
         if (r.refused && !write) break;
     }
@@ -488,7 +501,7 @@ __device__ __forceinline__ double residual(const Residual& R, bool draft, float 
 
 // With draft logits: the sums of w over the chunks of the refused rows.  Every
 // workgroup decides for itself, which a launch between would cost more than: 32
-// sequences of 73448, 10 us, most of it that chain.
+// sequences of 73448, 8.8 us, most of it that chain.
 template <int KIND>
 __global__ void __launch_bounds__(kPick) residual_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
@@ -527,7 +540,7 @@ __global__ void __launch_bounds__(kPick) residual_kernel(const VerifyArgs P) {
     }
 }
 
-// 10 us for one sequence of 6400 logits, 14 for 128 of 64402: a chain of about ten
+// 9 us for one sequence of 6400 logits, 12 for 128 of 64402: a chain of about ten
 // dependent steps (chunks' statistics, decision, their walk, one chunk's logits).
 template <int KIND, int K>
 __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
