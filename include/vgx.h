@@ -421,10 +421,11 @@ typedef struct vgx_ragged {
  * row's position (cos / sin: npos rows of rot/2 f32, device; rot a multiple of
  * 16, 0: none; rope_half as in vgx_attn_desc), then q rounded into q (ntok rows
  * of heads * head_dim, q_stride elements apart, compute type, apart from qkv;
- * may be NULL) and K and V rounded into the pages (a NaN is 0 on q8's grid).  qkv: ntok rows of (heads + 2 * kv_heads) *
- * head_dim values of kind F32, BF16, F16 or Q16 (vgx_gemm's output), stride
- * elements apart.  A row whose position is negative (more rows than kvlen) is
- * skipped. */
+ * may be NULL) and K and V rounded into the pages (a NaN is 0 on q8's grid).
+ * Sequences may share pages, but not the positions that a call writes.  qkv:
+ * ntok rows of (heads + 2 * kv_heads) * head_dim values of kind F32, BF16, F16
+ * or Q16 (vgx_gemm's output), stride elements apart.  A row whose position is
+ * negative (more rows than kvlen) is skipped. */
 typedef struct vgx_paged_rows {
     int kind;
     const void* qkv;

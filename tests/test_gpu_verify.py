@@ -146,6 +146,41 @@ def test_empty_and_long_sequences(gpu, with_draft):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("kind, vocab", [(torch.float32, 300007), (torch.int16, 600011), (torch.bfloat16, 530001)])
+def test_more_chunks_than_lanes(gpu, kind, vocab, with_draft):
+    """Rows of over 64 chunks; also the last of them alone holding the weight."""
+    c = case(21, [3, 1, 4], vocab, kind, with_draft, [0.9, 0.0, 1.2])
+    check(gpu, *c)
+    if kind != torch.int16:
+        c[2][:, :vocab - 5] = -math.inf
+        check(gpu, *c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_rows(gpu, kind, with_draft):
+    """Enough rows that a thread takes four pieces of a chunk."""
+    check(gpu, *case(22, [9] * 14 + [5], 20011, kind, with_draft, [0.8, 0.0, 1.0] * 5, pad=1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [31, 32, 33, 50, 63, 64, 68])
+@pytest.mark.parametrize("with_draft, temp", [(False, 0.0), (False, 1.0), (True, 1.0)])
+def test_refused_far_into_a_sequence(gpu, at, with_draft, temp):
+    """Drafts that are the rows' maxima and pass, up to one that cannot."""
+    qs, tok, x, ua, un, d, _ = case(23, [2, 70], 300, torch.float32, with_draft)
+    tok[1:] = x[:-1].argmax(1).to(torch.int32)
+    ua.zero_()
+    tok[2 + at + 1] = 299
+    x[2 + at, 299] = -math.inf
+    t = torch.tensor([temp, temp])
+    got = check(gpu, qs, tok, x, ua, un, d, t)
+    assert got[0][1] == at
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("with_draft", [False, True])
 def test_masked_and_odd_logits(gpu, kind, with_draft):
