@@ -20,7 +20,7 @@
 // + f, |f| <= 1/2: a table of 64 powers in LDS and a polynomial of degree 4 in f
 // (error (ln 2 / 128)^5 / 120 < 4e-14); a table lookup instead of a polynomial of degree 11 or more
 // (P. T. P. Tang, ACM TOMS 15, 1989).  12 operations of 64 bits a logit: what
-// bounds launch 1, 16-bit logits coming in faster than that.
+// bounds launch 1 of floating-point logits; q16's go by two tables (stats16_kernel).
 #include <cfloat>
 #include <cmath>
 #include <string>
@@ -80,6 +80,26 @@ __device__ __forceinline__ float one(const uint8_t* p, int i) {
     return clean((float)__builtin_bit_cast(_Float16, u));
 }
 
+template <int KIND>
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[kPer<KIND>]) {
+    const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (KIND == VGX_E_F32) {
+            x[i] = clean(__uint_as_float(u[i]));
+        } else if constexpr (KIND == VGX_E_Q16) {
+            x[2 * i] = (float)(short)(u[i] & 0xffff) * (1.0f / 256);
+            x[2 * i + 1] = (float)((int)u[i] >> 16) * (1.0f / 256);
+        } else if constexpr (KIND == VGX_E_BF16) {
+            x[2 * i] = clean(__uint_as_float(u[i] << 16));
+            x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
+        } else {
+            x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
+            x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
+        }
+    }
+}
+
 // A row as 16-byte pieces of the address space: piece g holds values
 // g * per - off .. + per - 1; the ends' pieces are read value by value.
 struct Row {
@@ -98,23 +118,7 @@ __device__ __forceinline__ void piece(const Row& q, int vocab, int g, float (&x)
     constexpr int N = kPer<KIND>;
     const int i0 = g * N - q.off;
     if (i0 >= 0 && i0 + N <= vocab) {
-        const uint4 v = *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * kBytes<KIND>);
-        const unsigned u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (KIND == VGX_E_F32) {
-                x[i] = clean(__uint_as_float(u[i]));
-            } else if (KIND == VGX_E_Q16) {
-                x[2 * i] = (float)(short)(u[i] & 0xffff) * (1.0f / 256);
-                x[2 * i + 1] = (float)((int)u[i] >> 16) * (1.0f / 256);
-            } else if (KIND == VGX_E_BF16) {
-                x[2 * i] = clean(__uint_as_float(u[i] << 16));
-                x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
-            } else {
-                x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
-                x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
-            }
-        }
+        unpack<KIND>(*reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * kBytes<KIND>), x);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) x[e] = i0 + e >= 0 && i0 + e < vocab ? one<KIND>(q.p, i0 + e) : -INFINITY;
@@ -245,48 +249,38 @@ __device__ __forceinline__ int seq_of(const VerifyArgs& P, int t) {
     return s;
 }
 
-// Launch 1's values: floats, or q16's integers (their differences are exact in
-// 32 bits, which spares three operations a logit).
-template <int KIND>
-using Val = std::conditional_t<KIND == VGX_E_Q16, int, float>;
-template <int KIND>
-constexpr Val<KIND> kNothing = KIND == VGX_E_Q16 ? (Val<KIND>)(-(1 << 30)) : (Val<KIND>)(-INFINITY);
-template <int KIND>
-__device__ __forceinline__ void unpack(const uint4& v, Val<KIND> (&x)[kPer<KIND>]) {
-    const unsigned u[4] = {v.x, v.y, v.z, v.w};
+// What every launch-1 kernel ends with: the waves' statistics joined.
+struct Joined {
+    float m[4];
+    int a[4];
+    double z[4];
+};
+__device__ __forceinline__ void stats_best(Joined& J, bool greedy, float& m, int& a) {
+    if (greedy) wave_best(m, a);
+    else m = wave_max(m);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) { J.m[wave] = m; J.a[wave] = a; }
+    __syncthreads();
+    m = J.m[0];
+    a = J.a[0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (KIND == VGX_E_F32) {
-            x[i] = clean(__uint_as_float(u[i]));
-        } else if constexpr (KIND == VGX_E_Q16) {
-            x[2 * i] = (short)(u[i] & 0xffff);
-            x[2 * i + 1] = (int)u[i] >> 16;
-        } else if constexpr (KIND == VGX_E_BF16) {
-            x[2 * i] = clean(__uint_as_float(u[i] << 16));
-            x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
-        } else {
-            x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
-            x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
-        }
-    }
+    for (int w = 1; w < 4; ++w)
+        if (J.m[w] > m || (J.m[w] == m && J.a[w] < a)) { m = J.m[w]; a = J.a[w]; }
 }
-template <int KIND>
-__device__ __forceinline__ Val<KIND> one_v(const uint8_t* p, int i) {
-    if constexpr (KIND == VGX_E_Q16) return reinterpret_cast<const short*>(p)[i];
-    else return one<KIND>(p, i);
+__device__ __forceinline__ void stats_put(Joined& J, Part* to, float m, int a, double z) {
+    z = wave_sum(z);
+    if ((threadIdx.x & 63) == 0) J.z[threadIdx.x >> 6] = z;
+    __syncthreads();
+    if (threadIdx.x == 0) *to = Part{m, a, J.z[0] + J.z[1] + J.z[2] + J.z[3]};
 }
-__device__ __forceinline__ float bigger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ int bigger(int a, int b) { return max(a, b); }
 
-// 654 rows of 64402 q16 logits, 31 us (20.8 vector instructions a logit); 126 of
-// 73448 f32 and the draft's, 19 us (3.9 TB/s).
+// 126 rows of 73448 f32 logits and the draft's, 19 us (3.9 TB/s): 12 operations
+// of 64 bits a logit.
 template <int KIND, int K>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
-    using V = Val<KIND>;
-    __shared__ double tab[64], sz[4];
-    __shared__ float sm[4];
-    __shared__ int sa[4];
+    __shared__ double tab[64];
+    __shared__ Joined J;
     const int chunk = blockIdx.x, t = blockIdx.y;
     const bool draft = blockIdx.z;
     const Row q = row_at<KIND>(draft ? P.d : P.x, draft ? P.ds : P.xs, t);
@@ -303,9 +297,8 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     fill_table(tab);
     if (s >= P.nseq) return;  // (uniform)
     const Temp T = temp_of(P, s);
-    const int wave = threadIdx.x >> 6;
-    V x[K][N];
-    V best = kNothing<KIND>;
+    float x[K][N];
+    float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         unpack<KIND>(raw[k], x[k]);
@@ -313,65 +306,138 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
         if (!full(i0)) {
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? one_v<KIND>(q.p, i0 + e) : kNothing<KIND>;
+                x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? one<KIND>(q.p, i0 + e) : -INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) best = bigger(best, x[k][e]);
+        for (int e = 0; e < N; ++e) m = fmaxf(m, x[k][e]);
     }
-    float m = KIND == VGX_E_Q16 ? (best == kNothing<KIND> ? -INFINITY : (float)best * (1.0f / 256)) : (float)best;
     int a = 0x7fffffff;
     if (T.greedy) {  // the first index of the maximum
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
 #pragma unroll
             for (int e = N - 1; e >= 0; --e)
-                if (x[k][e] == best) a = first(k) + e;
-        wave_best(m, a);
-    } else {
-        m = wave_max(m);
+                if (x[k][e] == m) a = first(k) + e;
     }
-    if ((threadIdx.x & 63) == 0) { sm[wave] = m; sa[wave] = a; }
-    __syncthreads();
-    m = sm[0];
-    a = sa[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w)
-        if (sm[w] > m || (sm[w] == m && sa[w] < a)) { m = sm[w]; a = sa[w]; }
+    stats_best(J, T.greedy, m, a);
     double z[2] = {0.0, 0.0};
     if (!T.greedy && m != -INFINITY) {
         const Scale S = scale_of(m, T.inv);
-        const double a256 = S.a * (1.0 / 256);
-        const int mi = (int)(m * 256.0f);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+    }
+    stats_put(J, (draft ? P.pd : P.px) + (int64_t)t * P.nch + chunk, m, a, z[0] + z[1]);
+}
+
+// q16 logits are integers, and the maximum less one of them, d, is one of
+// 0 .. 65535: e^(-d / 256 T) is a product of two table entries, of d's low byte
+// and of its high one.  exp16 is that product computed alone.
+__device__ __forceinline__ double exp_low(int i, double a256, const double* tab) {
+    return add_pow(fmax((double)-i * a256, -63700.0), 0.0, tab);
+}
+__device__ __forceinline__ double exp16(int d, const Scale& S, const double* tab) {
+    const double a256 = S.a * (1.0 / 256);
+    return exp_low(d & 255, a256, tab) * exp_low(d & 0xff00, a256, tab);
+}
+typedef short short2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+
+// Launch 1 for q16: two LDS reads and one operation of 64 bits a logit instead of
+// 12.  654 rows of 64402, 22 us (3.8 TB/s; 31 us by stats_kernel's way); the
+// tables cost a thread 2 exponentials beside its 8 or 32 logits.
+template <int K>
+__global__ void __launch_bounds__(kThreads) stats16_kernel(const VerifyArgs P) {
+    constexpr int KIND = VGX_E_Q16, N = 8;
+    __shared__ double tab[64], low[256], high[256];
+    __shared__ Joined J;
+    const int chunk = blockIdx.x, t = blockIdx.y, tid = threadIdx.x;
+    const bool draft = blockIdx.z;
+    const Row q = row_at<KIND>(draft ? P.d : P.x, draft ? P.ds : P.xs, t);
+    auto first = [&](int k) { return ((chunk * K + k) * kThreads + tid) * N - q.off; };
+    auto full = [&](int i0) { return i0 >= 0 && i0 + N <= P.vocab; };
+    auto in = [&](int i) { return i >= 0 && i < P.vocab; };
+    union Piece {
+        uint4 v;
+        unsigned u[4];
+        short x[8];
+    } raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        raw[k].v = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);  // (nothing: the least value)
+        if (full(first(k))) raw[k].v = *reinterpret_cast<const uint4*>(q.p + (int64_t)first(k) * 2);
+    }
+    const int s = seq_of(P, t);
+    fill_table(tab);
+    if (s >= P.nseq) return;  // (uniform)
+    const Temp T = temp_of(P, s);
+    const Scale S = scale_of(0.0f, T.inv);
+    __syncthreads();
+    if (!T.greedy) {
+        low[tid] = exp_low(tid, S.a * (1.0 / 256), tab);
+        high[tid] = exp_low(tid << 8, S.a * (1.0 / 256), tab);
+    }
+    short2v best = {-32768, -32768};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int i0 = first(k);
+        if (!full(i0)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (in(i0 + e)) raw[k].x[e] = reinterpret_cast<const short*>(q.p)[i0 + e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            best = __builtin_elementwise_max(best, __builtin_bit_cast(short2v, raw[k].u[e]));
+    }
+    const short top = best.x > best.y ? best.x : best.y;
+    int a = 0x7fffffff;
+    if (T.greedy) {
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k)
+#pragma unroll
+            for (int e = N - 1; e >= 0; --e)
+                if (raw[k].x[e] == top && in(first(k) + e)) a = first(k) + e;
+    }
+    // (a thread may have no value at all)
+    bool some = false;
+#pragma unroll
+    for (int k = 0; k < K; ++k) some = some || (first(k) + N > 0 && first(k) < P.vocab);
+    float m = some ? (float)top * (1.0f / 256) : -INFINITY;
+    stats_best(J, T.greedy, m, a);
+    double z[2] = {0.0, 0.0};
+    if (!T.greedy && m != -INFINITY) {
+        const unsigned short mi = (unsigned short)(short)(int)(m * 256.0f);
+        const ushort2v m2 = {mi, mi};
+        auto at = [](const double* p, unsigned byte8) {
+            return *reinterpret_cast<const double*>(reinterpret_cast<const char*>(p) + byte8);
+        };
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if constexpr (KIND == VGX_E_Q16) {
-                if (full(first(k))) {
+            const int i0 = first(k);
+            if (full(i0)) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        z[e & 1] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[e & 1], tab);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (x[k][e] != kNothing<KIND>)
-                            z[0] = add_pow(fmax((double)(x[k][e] - mi) * a256, -63700.0), z[0], tab);
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned d = __builtin_bit_cast(unsigned, m2 - __builtin_bit_cast(ushort2v, raw[k].u[e]));
+                    const double y0 = at(low, (d & 255) << 3), y1 = at(high, (d >> 8 & 255) << 3);
+                    const double y2 = at(low, (d >> 16 & 255) << 3), y3 = at(high, (d >> 24) << 3);
+                    z[0] = fma(y0, y1, z[0]);
+                    z[1] = fma(y2, y3, z[1]);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+                    if (in(i0 + e)) {
+                        const unsigned short d = mi - (unsigned short)raw[k].x[e];
+                        z[0] = fma(low[d & 255], high[d >> 8], z[0]);
+                    }
             }
+            __builtin_amdgcn_sched_barrier(0);  // (all pieces' reads at once would spill)
         }
     }
-    const double zs = wave_sum(z[0] + z[1]);
-    if ((threadIdx.x & 63) == 0) sz[wave] = zs;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        Part r;
-        r.m = m;
-        r.arg = a;
-        r.z = sz[0] + sz[1] + sz[2] + sz[3];
-        (draft ? P.pd : P.px)[(int64_t)t * P.nch + chunk] = r;
-    }
+    stats_put(J, (draft ? P.pd : P.px) + (int64_t)t * P.nch + chunk, m, a, z[0] + z[1]);
 }
 
 __device__ __forceinline__ Part part_of(const VerifyArgs& P, const Part* p, int c) {
@@ -571,12 +637,17 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
     // launch 1's, less the refused token
     const int tchunk = R.tok >= 0 && R.tok < P.vocab ? (R.tok + qx.off) / N / P.chunk : -1;
     if (wave == 0) {
+        // (what launch 1 has added for the refused token, to the bit)
+        auto taken = [&](float m) {
+            const Scale S = scale_of(m, T.inv);
+            return KIND == VGX_E_Q16 ? exp16((int)((m - D.lx) * 256.0f), S, tab) : weight(D.lx, S, tab);
+        };
         auto sum_of = [&](int c) {
             if (c >= P.nch) return 0.0;
             if (draft) return P.w[(int64_t)s * P.nch + c];
             const Part p = P.px[(int64_t)t * P.nch + c];
             double z = p.z;
-            if (c == tchunk) z = fmax(z - weight(D.lx, p.m, T.inv, tab), 0.0);
+            if (c == tchunk) z = fmax(z - taken(p.m), 0.0);
             return z * weight(p.m, R.sx, tab) * R.zx;
         };
         double total, v0;
@@ -707,8 +778,10 @@ Cut cut_of(int ntok, int vocab, int kind, bool draft) {
 template <int KIND>
 void launch(const VerifyArgs& P, int k, hipStream_t st) {
     if (P.ntok) {
-        hipLaunchKernelGGL((k == 1 ? stats_kernel<KIND, 1> : stats_kernel<KIND, 4>), dim3(P.nch, P.ntok, P.d ? 2 : 1),
-                           dim3(kThreads), 0, st, P);
+        void (*stats)(const VerifyArgs);
+        if constexpr (KIND == VGX_E_Q16) stats = k == 1 ? stats16_kernel<1> : stats16_kernel<4>;
+        else stats = k == 1 ? stats_kernel<KIND, 1> : stats_kernel<KIND, 4>;
+        hipLaunchKernelGGL(stats, dim3(P.nch, P.ntok, P.d ? 2 : 1), dim3(kThreads), 0, st, P);
         if (P.d) hipLaunchKernelGGL(residual_kernel<KIND>, dim3(P.nch, P.nseq), dim3(kPick), 0, st, P);
     }
     hipLaunchKernelGGL((k == 1 ? pick_kernel<KIND, 1> : pick_kernel<KIND, 4>), dim3(P.nseq), dim3(kPick), 0, st, P);
