@@ -725,3 +725,47 @@ def test_attn_bounds_far_above(gpu, kind, hd, page, window):
     # (the table's own size as the bound, and more rows than sequences have)
     b.table = torch.cat([b.table, torch.full((40, 60000 // page), -1, dtype=torch.int32)], 1)
     check_attn(gpu, b, 8, window=window, cache=cache, batch=cache.batch(*b.device(), b.ntok, 5))
+
+
+def test_two_streams_at_once(gpu):
+    """Calls in flight together, each with a workspace of its own."""
+    b = Batch(38, [1, 3, 1, 200], [9000, 700, 20000, 5000], 2, 64, 16, "bf16")
+    cache, batch = make(gpu, b, 8, max_q=200)
+    qs = [torch.randn(b.ntok, 8, 64, device="cuda").bfloat16() for _ in range(2)]
+    want = [cache.attend(batch, q, lse=True) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(cache.attend(batch, qs[i], lse=True))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(o, w[0]) and torch.equal(z, w[1]) for o, z in g)
+
+
+def test_two_graphs(gpu):
+    """Two captured steps replayed in turn and together, eager work between."""
+    b = Batch(39, [1, 2, 1], [6000, 40, 1500], 2, 64, 16, "q8")
+    cache, batch = make(gpu, b, 8, max_q=2)
+    qs = [torch.randn(b.ntok, 8, 64, device="cuda").half() for _ in range(2)]
+    want = [cache.attend(batch, q)[0] for q in qs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(cache.attend(batch, q)[0])
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in qs]
+    for i in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache.attend(batch, qs[0])[0], want[0])
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), i

@@ -147,6 +147,23 @@ def test_empty_and_long_sequences(gpu, with_draft):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("vocab", [3, 4001, 70001])
+def test_q16_rails(gpu, vocab, with_draft):
+    """Distances from the maximum up to 65535 steps, by rows that hold both
+    ends, only the lowest value, or a maximum of every low byte."""
+    t = [1.0, 40.0, 0.05, 0.0, 1e-30, 300.0]
+    qs, tok, x, ua, un, d, temp = case(24, [5] * 6, vocab, torch.int16, with_draft, t)
+    g = torch.Generator().manual_seed(25)
+    for y in (x, d) if with_draft else (x,):
+        y[::4] = torch.randint(-32768, 32768, y[::4].shape, generator=g).to(torch.int16)
+        y[1::4, ::2] = -32768
+        y[2::8] = -32768
+        y[3::8, vocab // 2:] = 32767
+    check(gpu, qs, tok, x, ua, un, d, temp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_draft", [False, True])
 @pytest.mark.parametrize("kind, vocab", [(torch.float32, 300007), (torch.int16, 600011), (torch.bfloat16, 530001)])
 def test_more_chunks_than_lanes(gpu, kind, vocab, with_draft):
     """Rows of over 64 chunks; also the last of them alone holding the weight."""
