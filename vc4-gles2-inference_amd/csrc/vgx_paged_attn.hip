@@ -621,8 +621,8 @@ constexpr int rows_lds(int hd, int nb) {
 // product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
 // the lane; two of them are the next product's B operand.  Long caches are bound
 // by their bytes: one token at 130001 positions, 32 / 8 heads of 128 in bf16,
-// 92 us (5.8 TB/s); 64 at 200 .. 16000 in q8, 106 us (4.7 TB/s, the conversions
-// between the loads).  Short ones by a chain of round trips (lengths and table,
+// 92 us (5.8 TB/s); 64 at 200 .. 16000 in q8 pages of 4 KB, 106 us (4.7 TB/s; no
+// more with four workgroups a CU).  Short ones by a chain of round trips (lengths and table,
 // rows, the join): one token at 700, 8 / 4 heads of 96, 8.4 us.
 template <int KIND, int HD, bool EX, int NB, int WV>
 __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) {
