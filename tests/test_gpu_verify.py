@@ -319,6 +319,60 @@ def test_stream_and_graph(gpu):
         assert all(torch.equal(a, b) for a, b in zip(o, e)), i
 
 
+TIED = [
+    # (vocabulary, u, the tokens of equal logits): a draw on the border of two
+    (1024, 0.875, [6, 12, 15, 44, 77, 126, 146, 151, 205, 307, 338, 360, 436, 442, 456, 468, 493, 529, 553, 569, 586, 597,
+                   613, 617, 630, 655, 693, 716, 779, 834, 837, 842, 861, 862, 865, 903, 918, 933, 977, 997]),
+    (256, 0.5, [28, 75, 90, 93, 100, 101, 108, 109, 110, 119, 124, 134, 141, 156, 157, 168, 178, 216, 217, 218]),
+]
+
+
+def tied_cases():
+    g = torch.Generator().manual_seed(31)
+    out = list(TIED)
+    for vocab in (1024, 5000, 70001):
+        for _ in range(100):
+            n = int(torch.randint(1, 60, (1,), generator=g))
+            at = torch.randperm(vocab, generator=g)[:n].sort().values.tolist()
+            out.append((vocab, int(torch.randint(0, 16, (1,), generator=g)) / 16, at))
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("how", ["last", "refused", "drafted"])
+def test_few_tokens_of_equal_weight(gpu, kind, how):
+    """Rows whose mask leaves n tokens of one logit, and draws on a border
+    between two: token floor(u n) of them, exactly.  "last": a row without a
+    draft; "refused": one whose draft is a further token of that logit;
+    "drafted": p = q, every draft a token without weight."""
+    for vocab in (256, 1024, 5000, 70001):
+        some = [c for c in tied_cases() if c[0] == vocab]
+        one = 1 if how == "last" else 2
+        x = torch.full((one * len(some), vocab), -128.0 if kind == torch.int16 else -math.inf)
+        tok = torch.zeros(one * len(some), dtype=torch.int32)
+        want = []
+        for i, (_, u, at) in enumerate(some):
+            x[one * i, at] = 3.0
+            want.append(at[int(u * len(at))])
+            if how == "refused":
+                w = next(j for j in range(i % vocab, 2 * vocab) if j % vocab not in at) % vocab
+                x[one * i, w] = 3.0
+                tok[one * i + 1] = w
+            elif how == "drafted":
+                tok[one * i + 1] = next(j for j in range(vocab) if j not in at)
+            if one == 2:
+                x[2 * i + 1, 0] = 0.0
+        x = (x * 256).to(torch.int16) if kind == torch.int16 else x.to(kind)
+        # (q16 has no mask: its lowest value at T = 1/16, e^-2096 of the others)
+        temp = torch.full((len(some),), 1.0 / 16 if kind == torch.int16 else 1.0)
+        ua = torch.full((len(tok),), 1 - 2.0 ** -24)
+        un = torch.tensor([c[1] for c in some])
+        qs = list(range(0, len(tok) + 1, one))
+        a, n, _ = run(gpu, qs, tok, x, ua, un, x.clone() if how == "drafted" else None, temp)
+        assert a == [0] * len(some) and n == want, vocab
+
+
 BUF = 1 << 20
 
 

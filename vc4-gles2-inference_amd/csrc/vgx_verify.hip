@@ -559,6 +559,11 @@ __device__ __forceinline__ Residual residual_of(const Decision& D, double inv, i
     return {scale_of(D.x.m, inv), scale_of(D.d.m, inv), D.x.z > 0.0 ? 1.0 / D.x.z : 0.0,
             D.d.z > 0.0 ? 1.0 / D.d.z : 0.0, tok};
 }
+// A draw from p alone needs no 1 / the sum: the weights of equal maxima are then
+// 1, their sums exact, and a draw at a border of theirs is decided as defined.
+__device__ __forceinline__ void unscaled(Residual& R) {
+    R.zx = 1.0;
+}
 __device__ __forceinline__ double residual(const Residual& R, bool draft, float x, float d, int j, const double* tab) {
     const double p = weight(x, R.sx, tab) * R.zx;
     if (!draft) return j == R.tok ? 0.0 : p;
@@ -631,7 +636,8 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
         return;
     }
     bool draft = P.d && D.refused;
-    const Residual R = residual_of(D, T.inv, D.refused && !P.d ? D.tok : -1);
+    Residual R = residual_of(D, T.inv, D.refused && !P.d ? D.tok : -1);
+    if (!draft) unscaled(R);
     const Row qx = row_at<KIND>(P.x, P.xs, t);
     // the chunks' sums, walked by one wave; without draft logits they are
     // launch 1's, less the refused token
@@ -664,6 +670,7 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             total = wave_sum(total);
             if (!draft || total > 0.0) break;
             draft = false;  // p = q: the draw is from p
+            unscaled(R);
             if (lane == 0) plain = 1;
         }
         const double want = un * total;
@@ -695,7 +702,10 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
         }
     }
     __syncthreads();
-    if (plain) draft = false;
+    if (plain) {
+        draft = false;
+        unscaled(R);
+    }
     if (chosen < 0) {  // nothing but the refused token has a weight
         if (threadIdx.x == 0) P.next[s] = -1;
         return;
@@ -736,14 +746,17 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
     if (lane == 63) sw[wave] = run;
     if (mine >= 0) atomicMax(&last, mine);
     __syncthreads();
-    // before: the inclusive sum of the thread before this one, to the bit, so
-    // one thread's interval holds the draw
+    // The first thread with a weight whose running sum has passed the draw.  (The
+    // lanes' sums are added in different orders, so a thread without a weight
+    // may have one a rounding above its neighbour's: it takes no part.)  Several
+    // waves may find one: the least index is the first's.
     double before = __shfl_up(run, 1, 64);
     if (lane == 0) before = 0.0;
     double base = 0.0;
     for (int v = 0; v < wave; ++v) base += sw[v];
     before += base;
-    if (before <= left && base + run > left) {
+    const unsigned long long past = __ballot(mine >= 0 && base + run > left);
+    if (past && lane == __ffsll(past) - 1) {
         int hit = -1;
         double u = before;
 #pragma unroll
