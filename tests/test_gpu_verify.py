@@ -373,6 +373,39 @@ def test_few_tokens_of_equal_weight(gpu, kind, how):
         assert a == [0] * len(some) and n == want, vocab
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [4100, 70001])
+def test_refused_draft_alone_in_its_chunk(gpu, kind, vocab):
+    """What is left beside a refused draft is next to nothing, or nothing: the
+    draw goes by the tokens that have a weight, in the draft's chunk or past it."""
+    x = torch.full((12, vocab), -math.inf)
+    tok = torch.zeros(12, dtype=torch.int32)
+    want = []
+    # the draft 689.5 below the maximum, its neighbours past the cut at e^-690
+    x[0, :900], x[0, 7], x[0, 4000:4010] = -691.0, -689.5, 0.0
+    # a neighbour well inside it
+    x[2, :900], x[2, 7], x[2, 30], x[2, 4000:4010] = -691.0, -689.5, -600.0, 0.0
+    # the draft the maximum, 1999 neighbours with 10^-6 of its weight together, and nothing else
+    x[4, :2000], x[4, 7] = -21.5, 0.0
+    # ... and as much in two chunks
+    x[6, :1000], x[6, 7], x[6, 3100:4100] = -21.5, 0.0, -21.5
+    # the draft the only token: it is taken, and row 9 has token 0 alone
+    x[8, 7] = 0.0
+    # the draft at the row's end, its chunk-mates masked
+    x[10, vocab - 1], x[10, 3] = 5.0, -8.0
+    un = torch.tensor([0.0, 0.0, 0.5, 0.75, 0.5, 0.0])
+    # row 4: 1999 equal weights, u 999.5 of them: the 1000th, at 1000 (behind the draft);
+    # row 6: 999 and 1000, u 1499.25: the 501st of the second, at 3600
+    want = [4000, 30, 1000, 3600, 0, 3]
+    tok[1::2] = 7
+    tok[11] = vocab - 1
+    x[1::2, 0] = 0.0
+    ua = torch.full((12,), 1 - 2.0 ** -24)
+    a, n, _ = run(gpu, list(range(0, 13, 2)), tok, x.to(kind), ua, un)
+    assert a == [0, 0, 0, 0, 1, 0] and n == want
+
+
 BUF = 1 << 20
 
 

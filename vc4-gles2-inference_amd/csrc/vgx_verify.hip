@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
     // launch 1's, less the refused token
     const int tchunk = R.tok >= 0 && R.tok < P.vocab ? (R.tok + qx.off) / N / P.chunk : -1;
     if (wave == 0) {
-        // (what launch 1 has added for the refused token, to the bit)
+        // (what launch 1 has added for the refused token, but for the rounding of
+        // its fused additions)
         auto taken = [&](float m) {
             const Scale S = scale_of(m, T.inv);
             return KIND == VGX_E_Q16 ? exp16((int)((m - D.lx) * 256.0f), S, tab) : weight(D.lx, S, tab);
@@ -652,9 +653,15 @@ __global__ void __launch_bounds__(kPick) pick_kernel(const VerifyArgs P) {
             if (c >= P.nch) return 0.0;
             if (draft) return P.w[(int64_t)s * P.nch + c];
             const Part p = P.px[(int64_t)t * P.nch + c];
+            const double w = weight(p.m, R.sx, tab);
             double z = p.z;
-            if (c == tchunk) z = fmax(z - taken(p.m), 0.0);
-            return z * weight(p.m, R.sx, tab) * R.zx;
+            // A chunk whose sum passes 0 has to hold a token that can be drawn: one
+            // whose maximum is all but cut beside the row's counts as nothing
+            // without the refused token, as its other weights may be cut.  (Otherwise
+            // what is left is 0 or above 2^-53, so some weight is above 2^-66 of
+            // the maximum's.)
+            if (c == tchunk) z = w < 0x1p-900 ? 0.0 : fmax(z - taken(p.m), 0.0);
+            return z * w * R.zx;
         };
         double total, v0;
         if (lane == 0) plain = 0;
