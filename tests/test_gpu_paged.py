@@ -769,3 +769,36 @@ def test_two_graphs(gpu):
         torch.cuda.synchronize()
         assert torch.equal(cache.attend(batch, qs[0])[0], want[0])
         assert all(torch.equal(o, w) for o, w in zip(outs, want)), i
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("nq, kv", [([1, 2], [800, 130]), ([1], [9000]), ([90, 40], [800, 130]), ([100, 1], [100, 3000])])
+@pytest.mark.parametrize("size", [1500, 6000, 20000])
+def test_attn_scores_far_from_zero(gpu, kind, nq, kv, size):
+    """Scores of up to 2^31 and their differences: where the two largest of a
+    row are further apart than their 32-bit sums can be off, it is the largest
+    one's value that comes out."""
+    b = Batch(43, nq, kv, 2, 64, 16, kind)
+    b.k = (size * b.k.float()).clamp(-60000, 60000).to(b.k.dtype)
+    q = (size * b.randn(b.ntok, 4, 64)).clamp(-60000, 60000).to(ref.CTYPE[kind])
+    cache, batch = make(gpu, b, 4)
+    o, lse = cache.attend(batch, q.cuda(), lse=True)
+    o, lse = o.cpu().double().view(b.ntok, 4, 64), lse.cpu().double()
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    clear = 0
+    for s, (n, m) in enumerate(zip(b.nq, b.kv)):
+        for r in range(n):
+            t = int(b.qs[s]) + r
+            for h in range(4):
+                k, v = (ref.value(b.rows(s, x, h // 2, m - n + r + 1)) for x in (b.k, b.v))
+                x = k @ q[t, h].double() / 8
+                # 64 additions of 32 bits each side, and 40 more: e^-40 of the values
+                off = 2 * 64 * 2.0 ** -24 * float((k.abs() @ q[t, h].double().abs()).max()) / 8 + 40
+                top = x.topk(min(2, len(x))).values
+                if len(x) > 1 and top[0] - top[1] < off:
+                    continue
+                clear += 1
+                want = v[int(x.argmax())]
+                assert ((o[t, h] - want).abs() <= want.abs() * 2.0 ** -8).all()
+                assert abs(lse[t, h] - top[0]) <= off
+    assert clear >= b.ntok

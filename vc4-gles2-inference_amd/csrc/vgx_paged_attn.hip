@@ -136,6 +136,13 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// What to subtract from the scores: 0 while there is no key, so that the
+// exponents stay -inf and the weights 0.
+__device__ __forceinline__ float ref_or_0(float m) { return m == -INFINITY ? 0.0f : m; }
+// An exponent is c s - c m in one operation, whose c m is rounded alone.  From
+// 2^12 on that rounding is more than 2^-12, and at 2^31 it passes what a float
+// can hold the power of: there m is subtracted from the scores first.
+__device__ __forceinline__ bool far(float m, float c) { return fabsf(m * c) > 4096.0f && m != -INFINITY; }
 
 // A tile of keys in LDS.  K rows of HD values with 16 bytes between them (a
 // lane's 16-byte pieces of 8 rows then lie in 8 different bank groups); V rows
@@ -300,6 +307,7 @@ struct Acc {
     static constexpr int NB = HD / 32;
     f32x16 o[NB];
     float m, l;
+    bool big;  // some column's m is far from 0
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -307,6 +315,7 @@ struct Acc {
             for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
         m = -INFINITY;
         l = 0.0f;
+        big = false;
     }
 };
 
@@ -373,18 +382,26 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
     // The reference value m is any that keeps the weights in range: it moves,
     // and the sums with it, only when some column's maximum has passed its m by
     // 2^6 (a weight then stays below 64, exact in no fewer bits).
-    if (__any(mx * c > fmaf(a.m, c, 6.0f))) {
+    if (__any((mx - a.m) * c > 6.0f)) {
         const float m2 = fmaxf(mx, a.m);
-        const float alpha = exp2_((a.m - (m2 == -INFINITY ? 0.0f : m2)) * c);
+        const float alpha = exp2_((a.m - ref_or_0(m2)) * c);
         a.m = m2;
+        a.big = __any(far(m2, c));
         a.l *= alpha;
 #pragma unroll
         for (int b = 0; b < HD / 32; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) a.o[b][i] *= alpha;
     }
-    // (no key yet: subtract 0, so the exponents stay -inf and the weights 0)
-    const float mc = (a.m == -INFINITY ? 0.0f : a.m) * c;
+    const float m0 = ref_or_0(a.m);
+    float mc = m0 * c;
+    if (__builtin_expect(a.big, 0)) {
+        mc = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] -= m0;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -737,10 +754,15 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
             float mx = fmaxf(fmaxf(fmaxf(sc[b][0][0], sc[b][0][1]), fmaxf(sc[b][0][2], sc[b][0][3])),
                              fmaxf(fmaxf(sc[b][1][0], sc[b][1][1]), fmaxf(sc[b][1][2], sc[b][1][3])));
             mx = fmaxf(quad_max(mx), m[b]);
-            // (no key yet: subtract 0, so the exponents stay -inf and the weights 0)
-            const float mc = (mx == -INFINITY ? 0.0f : mx) * P.c;
-            const float alpha = exp2_(fmaf(m[b], P.c, -mc));
+            const float m0 = ref_or_0(mx);
+            float mc = m0 * P.c;
+            const float alpha = exp2_((m[b] - m0) * P.c);
             m[b] = mx;
+            if (__builtin_expect(__any(far(mx, P.c)), 0)) {
+                mc = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) sc[b][u] -= m0;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -807,10 +829,10 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
             f[w] = sm[w][16 * b + col];
             M = fmaxf(M, f[w]);
         }
-        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+        const float m0 = ref_or_0(M);
 #pragma unroll
         for (int w = 0; w < WV; ++w) {
-            f[w] = exp2_(fmaf(f[w], P.c, -mc));
+            f[w] = exp2_((f[w] - m0) * P.c);
             L = fmaf(sl[w][16 * b + col], f[w], L);
         }
         const int64_t at = (int64_t)cl[b].row * A.heads + cl[b].head;
@@ -1084,11 +1106,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
     float M = -INFINITY, L = 0.0f;
     if (!WIDE) {
         for (int k = 0; k < nsp; ++k) M = fmaxf(M, ml[k * step].x);
-        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+        const float m0 = ref_or_0(M);
 #pragma unroll 4
         for (int k = 0; k < nsp; ++k) {
             const float2 x = ml[k * step];
-            const float f = exp2_(fmaf(x.x, P.c, -mc));
+            const float f = exp2_((x.x - m0) * P.c);
             L = fmaf(x.y, f, L);
             const float4 y = po[(at + k * step) * n4 + min(lane & ((1 << lg) - 1), n4 - 1)];
             o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
@@ -1100,20 +1122,20 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs P, int l
         if (lane == 0) sw[threadIdx.x >> 6] = M;
         __syncthreads();
         M = fmaxf(fmaxf(sw[0], sw[1]), fmaxf(sw[2], sw[3]));
-        const float mc = (M == -INFINITY ? 0.0f : M) * P.c;
+        const float m0 = ref_or_0(M);
         const int ng = 256 / n4, gr = threadIdx.x / n4, d = threadIdx.x - gr * n4;
         if (gr < ng) {
 #pragma unroll 8
             for (int k = gr; k < nsp; k += ng) {
                 const float2 x = ml[k * step];
-                const float f = exp2_(fmaf(x.x, P.c, -mc));
+                const float f = exp2_((x.x - m0) * P.c);
                 const float4 y = po[(at + k * step) * n4 + d];
                 o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
             }
         }
         for (int k = threadIdx.x; k < nsp; k += 256) {
             const float2 x = ml[k * step];
-            L = fmaf(x.y, exp2_(fmaf(x.x, P.c, -mc)), L);
+            L = fmaf(x.y, exp2_((x.x - m0) * P.c), L);
         }
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x, 64);
