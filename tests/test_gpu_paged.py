@@ -802,3 +802,42 @@ def test_attn_scores_far_from_zero(gpu, kind, nq, kv, size):
                 assert ((o[t, h] - want).abs() <= want.abs() * 2.0 ** -8).all()
                 assert abs(lse[t, h] - top[0]) <= off
     assert clear >= b.ntok
+
+
+def tail_batch(seed, nq, kv, hd, kind, kvh, score, sink):
+    """One key a sequence whose score is `score`, all others' being 0, and its
+    value 0: what comes out is the others' share.  The queries that go with it."""
+    b = Batch(seed, nq, kv, kvh, hd, 16, kind)
+    b.k.zero_()
+    b.v = ref.to_cache(5 + 0.4 * b.randn(b.pages, kvh, 16, hd), kind)
+    for s, m in enumerate(kv):
+        p = {"first": 0, "middle": m // 2, "last": m - max(nq[s], 1)}[sink]
+        pg, sl = int(b.table[s, p // 16]), p % 16
+        b.k[pg, :, sl, 0] = 64 if kind == "q8" else 4  # 4 on the grid of 1/16
+        b.v[pg, :, sl] = 0
+    q = torch.randn(b.ntok, 2 * kvh, hd, generator=b.rng)
+    q[..., 0] = score / 4 * hd ** 0.5
+    return b, q.to(ref.CTYPE[kind])
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+@pytest.mark.parametrize("score", [10.0, 14.0, 17.5, 20.0])
+@pytest.mark.parametrize("sink", ["first", "middle", "last"])
+@pytest.mark.parametrize("nq, kv, hd", [([1], [5000], 64), ([3, 1], [5000, 700], 128), ([7, 1], [2000, 900], 144),
+                                        ([150], [3000], 64), ([140, 1], [1500, 4000], 64), ([70], [1200], 256)])
+def test_attn_many_small_weights(gpu, kind, score, sink, nq, kv, hd):
+    """Thousands of equal weights far below the largest add up.  A weight is at
+    least 2^9 of f16's units of the largest (so it is off by at most half a step
+    of itself or 2^-25 of those), the denominator at least the largest weight."""
+    b, q = tail_batch(42, nq, kv, hd, kind, 1, score, sink)
+    want, wl, mag, dots = ref.attend(b, q, 2)
+    n, half = max(kv), ref.HALF_STEP[torch.float16]
+    e_s = dots[..., None] * (hd + 8) * 2.0 ** -22 + 2.0 ** -21
+    bound = half * mag + (2 * e_s + 2 * n * 2.0 ** -24) * mag + n * 2.0 ** -34 * float(ref.value(b.v).abs().max())
+    bound = bound + half * (want.abs() + bound) + 2.0 ** -25
+    cache, batch = make(gpu, b, 2)
+    o, lse = cache.attend(batch, q.cuda(), lse=True)
+    got = o.cpu().double().view_as(want)
+    assert ((got - want).abs() <= bound).all()
+    tol = dots * (hd + 8) * 2.0 ** -22 + (n + 32) * 2.0 ** -24 + wl.abs() * 2.0 ** -22
+    assert ((lse.cpu().double() - wl).abs() <= tol).all()

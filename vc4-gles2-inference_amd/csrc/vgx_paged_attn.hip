@@ -7,8 +7,16 @@
 //   m' = max(m, max_keys S), P = exp2(c S - c m'), l = l 2^(c(m - m')) + sum P
 //   O^T = O^T 2^(c(m - m')) + V^T P    A = V^T, B = P
 // with c = scale * log2(e); out = O / l.  Products in the compute type with
-// 32-bit sums; P is rounded to it (relative error at most half a step a
-// weight, as the inputs' own); m, l and O stay in 32 bits.
+// 32-bit sums; m, l and O stay in 32 bits.
+//
+// P is rounded to the compute type, which is what the second product multiplies;
+// l sums it unrounded.  A weight is then off by at most half a step of its own
+// (2^-8 of it in bf16, 2^-11 in f16), as K and V were when they were stored;
+// carrying the rest of it in a second operand would double that product.  bf16
+// has the exponents of 32 bits.  In f16 a weight below 2^-14 loses bits and one
+// below 2^-25 all of them, which many such keys behind one that has nearly all
+// the weight would notice: there the weights are 2^lift times as large, in P
+// and in l (lift_of).
 //
 // Why transposed: a 32x32 product leaves column q's scores in lanes q and
 // q + 32 (keys 8a + 4h + b in register 4a + b of half h), which is a B operand
@@ -49,7 +57,7 @@ struct AttnArgs {
     uint8_t* out;
     int64_t ostride;
     float* lse;
-    // Partial results, numbered: hd sums and (m, l) each.  Split k of a row and
+    // Partial results, numbered: hd sums and (m, l) each, without the lift.  Split k of a row and
     // head is number base + k * step; pn (ntok x heads) holds their splits and
     // base.  Numbers go by row and head, or by sequence, KV head and column (the
     // few rows of short sequences among many others').
@@ -136,6 +144,12 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// The exponent of the largest weight: f16 ends at 2^16, and the tile kernel lets
+// weights pass its reference by 2^6.
+template <int CK, bool TILE>
+constexpr float lift_of = CK != VGX_E_F16 ? 0.0f : TILE ? 9.0f : 15.0f;
+template <int CK, bool TILE>
+constexpr float unlift_of = CK != VGX_E_F16 ? 1.0f : TILE ? 0x1p-9f : 0x1p-15f;
 // What to subtract from the scores: 0 while there is no key, so that the
 // exponents stay -inf and the weights 0.
 __device__ __forceinline__ float ref_or_0(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -381,7 +395,7 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
     mx = half_max(mx);
     // The reference value m is any that keeps the weights in range: it moves,
     // and the sums with it, only when some column's maximum has passed its m by
-    // 2^6 (a weight then stays below 64, exact in no fewer bits).
+    // 2^6 (a weight then stays below 64 lifts, exact in no fewer bits).
     if (__any((mx - a.m) * c > 6.0f)) {
         const float m2 = fmaxf(mx, a.m);
         const float alpha = exp2_((a.m - ref_or_0(m2)) * c);
@@ -394,9 +408,10 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
             for (int i = 0; i < 16; ++i) a.o[b][i] *= alpha;
     }
     const float m0 = ref_or_0(a.m);
-    float mc = m0 * c;
+    constexpr float lift = lift_of<CK, true>;
+    float mc = lift == 0.0f ? m0 * c : fmaf(m0, c, -lift);
     if (__builtin_expect(a.big, 0)) {
-        mc = 0.0f;
+        mc = -lift;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -755,11 +770,12 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
                              fmaxf(fmaxf(sc[b][1][0], sc[b][1][1]), fmaxf(sc[b][1][2], sc[b][1][3])));
             mx = fmaxf(quad_max(mx), m[b]);
             const float m0 = ref_or_0(mx);
-            float mc = m0 * P.c;
+            constexpr float lift = lift_of<CK, false>;
+            float mc = lift == 0.0f ? m0 * P.c : fmaf(m0, P.c, -lift);
             const float alpha = exp2_((m[b] - m0) * P.c);
             m[b] = mx;
             if (__builtin_expect(__any(far(mx, P.c)), 0)) {
-                mc = 0.0f;
+                mc = -lift;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) sc[b][u] -= m0;
             }
@@ -832,7 +848,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
         const float m0 = ref_or_0(M);
 #pragma unroll
         for (int w = 0; w < WV; ++w) {
-            f[w] = exp2_((f[w] - m0) * P.c);
+            f[w] = exp2_((f[w] - m0) * P.c) * unlift_of<CK, false>;
             L = fmaf(sl[w][16 * b + col], f[w], L);
         }
         const int64_t at = (int64_t)cl[b].row * A.heads + cl[b].head;
@@ -1017,14 +1033,16 @@ __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, in
         }
     }
     if (bad) set_fault(A, VGX_FAULT_PAGE);
-    const float L = half_sum(a.l);
+    // (the lift leaves: powers of two, exact)
+    constexpr float unlift = unlift_of<CK, true>;
+    const float L = half_sum(a.l) * unlift;
     if (!cl.valid) return;
     const int hh = lane >> 5;
     const int64_t at = (int64_t)cl.row * A.heads + cl.head;
     const unsigned part0 = part_of(P, s, h, 0, cl.row, cl.head);
     const int64_t to = part0 + (int64_t)split * P.pstep;
     const bool whole = sp.nsp == 1;
-    const float r = whole ? inv_l(P, L) : 1.0f;
+    const float r = whole ? inv_l(P, L) * unlift : unlift;
 #pragma unroll
     for (int b = 0; b < HD / 32; ++b)
 #pragma unroll
