@@ -156,7 +156,7 @@ __device__ __forceinline__ float ref_or_0(float m) { return m == -INFINITY ? 0.0
 // An exponent is c s - c m in one operation, whose c m is rounded alone.  From
 // 2^12 on that rounding is more than 2^-12, and at 2^31 it passes what a float
 // can hold the power of: there m is subtracted from the scores first.
-__device__ __forceinline__ bool far(float m, float c) { return fabsf(m * c) > 4096.0f && m != -INFINITY; }
+__device__ __forceinline__ bool far(float mc) { return fabsf(mc) > 4096.0f; }
 
 // A tile of keys in LDS.  K rows of HD values with 16 bytes between them (a
 // lane's 16-byte pieces of 8 rows then lie in 8 different bank groups); V rows
@@ -400,7 +400,7 @@ __device__ __forceinline__ void step(const PagedDev& A, const s16x8 (&q)[HD / 16
         const float m2 = fmaxf(mx, a.m);
         const float alpha = exp2_((a.m - ref_or_0(m2)) * c);
         a.m = m2;
-        a.big = __any(far(m2, c));
+        a.big = __any(far(ref_or_0(m2) * c));
         a.l *= alpha;
 #pragma unroll
         for (int b = 0; b < HD / 32; ++b)
@@ -774,7 +774,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
             float mc = lift == 0.0f ? m0 * P.c : fmaf(m0, P.c, -lift);
             const float alpha = exp2_((m[b] - m0) * P.c);
             m[b] = mx;
-            if (__builtin_expect(__any(far(mx, P.c)), 0)) {
+            if (__builtin_expect(__any(far(mc)), 0)) {
                 mc = -lift;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) sc[b][u] -= m0;
