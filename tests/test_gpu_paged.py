@@ -841,3 +841,24 @@ def test_attn_many_small_weights(gpu, kind, score, sink, nq, kv, hd):
     assert ((got - want).abs() <= bound).all()
     tol = dots * (hd + 8) * 2.0 ** -22 + (n + 32) * 2.0 ** -24 + wl.abs() * 2.0 ** -22
     assert ((lse.cpu().double() - wl).abs() <= tol).all()
+
+
+def test_check_waits_for_every_stream(gpu):
+    """A fault on a busy side stream is seen by a check() from the default one,
+    and one raised right after it by the next."""
+    from vgx import lib as vl
+    b = Batch(44, [1, 1], [20, 40], 2, 64, 16, "bf16")
+    cache, _ = make(gpu, b, 4)
+    qs, kv, table = b.device()
+    kv[1] = 10 ** 6
+    batch = cache.batch(qs, kv, table, 2)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            cache.attend(batch, q)
+        with pytest.raises(vl.VgxError, match="length"):
+            batch.check()
+    batch.check()

@@ -260,7 +260,8 @@ class RaggedBatch:
     its pages in table[s].  The arrays are read when a call runs, so they may
     change between calls (and between replays of a captured one); max_q and
     max_kv bound one sequence's rows and positions.  check() waits for the
-    device and raises if a call met a length or page outside its bounds."""
+    device (all its streams, whichever the calls ran on) and raises if a call
+    met a length or page outside its bounds."""
 
     def __init__(self, gpu, qstart, kvlen, table, ntok, max_q=0, max_kv=0):
         gpu.need(qstart, torch.int32, 1, "qstart")
@@ -285,9 +286,11 @@ class RaggedBatch:
         self.ws = {}  # workspace bytes by (cache, window)
 
     def check(self):
+        torch.cuda.synchronize(self.gpu.device)
         bits = int(self.fault.item())
         if bits:
             self.fault.zero_()
+            torch.cuda.synchronize(self.gpu.device)  # (before another stream's next call can set one)
             what = [w for b, w in ((_l.FAULT_LENGTH, "a length outside its bounds"),
                                    (_l.FAULT_PAGE, "a page outside the pool")) if bits & b]
             raise _l.VgxError(_l.VGX_ERANGE, "ragged batch: " + " and ".join(what))
