@@ -190,3 +190,15 @@ def test_steps_whose_reciprocal_or_range_is_not_finite(step):
         st, msg = append(c=cache(kind=vl.E_Q8, **{which: step}))
         assert st == vl.VGX_EINVAL and "step" in msg, msg
         assert append(c=cache(kind=vl.E_Q8, **{which: 2.0 ** -64}))[1].endswith("no context")
+
+
+def test_binding_refuses_a_batch_of_another_device():
+    """Its arrays are read by the cache's device."""
+    cache, batch = _binding()
+    other = _Cpu()
+    other.device = torch.device("cuda", 1)
+    batch.gpu = other
+    with pytest.raises(ValueError, match="cuda:1"):
+        cache.append(batch, torch.zeros(3, 256, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="cuda:1"):
+        cache.attend(batch, torch.zeros(3, 128, dtype=torch.bfloat16))

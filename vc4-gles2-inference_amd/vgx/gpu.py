@@ -327,6 +327,7 @@ class PagedCache:
         bfloat16, float16 or q16) normed, rotated (cos, sin: positions x rot/2)
         and written into the cache; returns the queries (ntok, heads, head_dim)."""
         g = self.gpu
+        self._same_device(batch)
         kind = _ELEM.get(qkv.dtype)
         if kind is None:
             raise ValueError("qkv must be float32, bfloat16, float16 or int16 (q16)")
@@ -360,6 +361,7 @@ class PagedCache:
         sequences: (out (ntok, heads * head_dim), lse (ntok, heads) or None).
         out: a tensor to write, of the compute type or int16 (q16)."""
         g = self.gpu
+        self._same_device(batch)
         qs = self._rows(q, self.qtype, batch.ntok, "q")
         if out is None:
             out, kind, os_ = torch.empty((batch.ntok, self.width), dtype=self.qtype, device=g.device), self.ckind, self.width
@@ -376,6 +378,10 @@ class PagedCache:
         r = _l.PagedQuery(q.data_ptr(), qs, scale, window, kind, out.data_ptr(), os_, _at(z), _at(ws), need)
         g.on_current(L.vgx_paged_attn, self.ref, batch.ref, ctypes.byref(r))
         return out, z
+
+    def _same_device(self, batch):
+        if batch.gpu is not self.gpu and batch.gpu.device != self.gpu.device:
+            raise ValueError("the batch is on %s, the cache on %s" % (batch.gpu.device, self.gpu.device))
 
     def _rows(self, t, dtype, n, name):
         """The stride of n rows of heads x head_dim values, (n, heads, head_dim) or (n, heads * head_dim)."""
