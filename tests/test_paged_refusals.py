@@ -202,3 +202,17 @@ def test_binding_refuses_a_batch_of_another_device():
         cache.append(batch, torch.zeros(3, 256, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="cuda:1"):
         cache.attend(batch, torch.zeros(3, 128, dtype=torch.bfloat16))
+
+
+def test_binding_keeps_no_workspace_size_of_a_refused_call():
+    """0 bytes, as a refused call has, would leave the next cache's long
+    sequences whole."""
+    cache, batch = _binding()
+
+    def refuse(call, *args):
+        raise vl.VgxError(vl.VGX_EINVAL, "refused")
+
+    cache.gpu.on_current, cache.gpu.ctx = refuse, None
+    with pytest.raises(vl.VgxError):
+        cache.attend(batch, torch.zeros(3, 128, dtype=torch.bfloat16))
+    assert not batch.ws

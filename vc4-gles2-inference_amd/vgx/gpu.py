@@ -371,12 +371,15 @@ class PagedCache:
         key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window)
         need = batch.ws.get(key)
         L = _l.load()
-        if need is None:
-            need = batch.ws[key] = int(L.vgx_paged_attn_ws(g.ctx, self.ref, batch.ref, window))
+        known = need is not None
+        if not known:
+            need = int(L.vgx_paged_attn_ws(g.ctx, self.ref, batch.ref, window))
         ws = torch.empty(need, dtype=torch.uint8, device=g.device) if need else None
         z = torch.empty((batch.ntok, self.heads), dtype=torch.float32, device=g.device) if lse else None
         r = _l.PagedQuery(q.data_ptr(), qs, scale, window, kind, out.data_ptr(), os_, _at(z), _at(ws), need)
         g.on_current(L.vgx_paged_attn, self.ref, batch.ref, ctypes.byref(r))
+        if not known:  # (a refused call's size is 0)
+            batch.ws[key] = need
         return out, z
 
     def _same_device(self, batch):
