@@ -862,3 +862,16 @@ def test_check_waits_for_every_stream(gpu):
         with pytest.raises(vl.VgxError, match="length"):
             batch.check()
     batch.check()
+
+
+def test_more_splits_than_a_number_holds(gpu):
+    """A batch whose splits would pass 2^31 partial results needs no workspace:
+    its sequences stay whole (it was refused before)."""
+    import ctypes
+    from vgx import lib as vl
+    at = 1 << 20  # (nothing is read)
+    c = vl.Paged(256, 8, 16, 16, 1 << 20, vl.E_BF16, 0.0, 0.0, at, at, 2048, 256, 16, 2048, 256, 16)
+    for nseq, split in ((1 << 16, True), (1 << 20, False)):
+        b = vl.Ragged(nseq, nseq, 1, 1 << 20, at, at, at, 1 << 16, 1 << 16, 0)
+        need = vl.load().vgx_paged_attn_ws(gpu.ctx, ctypes.byref(c), ctypes.byref(b), 0)
+        assert (need > 0) == split and need < 1 << 39

@@ -1320,6 +1320,7 @@ Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     }
     for (int i = 0; i < p.n; ++i)
         if (p.l[i].nsplit > 1) p.parts += (size_t)p.l[i].nsplit * p.step(A, i);
+    if (p.parts > INT32_MAX) p.parts = 0;  // (their numbers have 32 bits: such a batch fills the chip unsplit)
     p.ws = p.parts ? p.parts * (A.hd + 2) * 4 + (size_t)A.ntok * A.heads * 8 : 0;
     return p;
 }
@@ -1388,7 +1389,7 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
     for (int i = 0; i < p.n; ++i)
         if (p.l[i].wgs >= (1 << 24) || p.l[i].nsplit > 65535)
             return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
-    if (p.parts > INT32_MAX || (int64_t)A.ntok * A.heads > INT32_MAX - 256)
+    if ((int64_t)A.ntok * A.heads > INT32_MAX - 256)
         return vgx_fail(VGX_ERANGE, "vgx_paged_attn: too many rows");
     P.q = static_cast<const uint8_t*>(r->q);
     P.qstride = r->q_stride;
