@@ -875,3 +875,93 @@ def test_more_splits_than_a_number_holds(gpu):
         b = vl.Ragged(nseq, nseq, 1, 1 << 20, at, at, at, 1 << 16, 1 << 16, 0)
         need = vl.load().vgx_paged_attn_ws(gpu.ctx, ctypes.byref(c), ctypes.byref(b), 0)
         assert (need > 0) == split and need < 1 << 39
+
+
+def guarded(n, dtype, fill):
+    """n values of device memory between two runs of 4096 bytes of a pattern;
+    the whole as bytes, and the n."""
+    size = torch.tensor([], dtype=dtype).element_size()
+    raw = torch.full((8192 + (n * size + 15) // 16 * 16,), 0xA5, dtype=torch.uint8, device="cuda")
+    mid = raw[4096:4096 + n * size]
+    mid.fill_(fill)
+    return raw, mid.view(dtype)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q8"])
+@pytest.mark.parametrize("nq, kv, max_q, max_kv", [
+    ([3, 40], [20, 90], 4, 0), ([40, 3], [90, 20], 0, 64),          # whole, more rows or positions than promised
+    ([2, 9], [5000, 7000], 3, 0), ([2, 2], [3000, 9000], 2, 4096),  # split
+    ([1, 90], [6000, 5000], 60, 0), ([100, 1], [7000, 300], 100, 2000),  # prompts beside single tokens
+])
+def test_bounds_are_held_in_every_buffer(gpu, kind, nq, kv, max_q, max_kv):
+    """Beside a sequence past its bounds the other one's rows are right, and
+    nothing is written around out, lse and the workspace, whose partial
+    results hold 0xff where no workgroup writes them."""
+    import ctypes
+    from vgx import lib as vl
+    hd, heads = 64, 4
+    b = Batch(45, nq, kv, 2, hd, 16, kind)
+    cache, _ = make(gpu, b, heads)
+    batch = cache.batch(*b.device(), b.ntok, max_q=max_q, max_kv=max_kv)
+    q = (2 * b.randn(b.ntok, heads, hd)).to(ref.CTYPE[kind])
+    L = vl.load()
+    need = int(L.vgx_paged_attn_ws(gpu.ctx, cache.ref, batch.ref, 0))
+    ws_raw, ws = guarded(max(need, 16), torch.uint8, 0xFF)
+    out_raw, out = guarded(b.ntok * heads * hd, cache.qtype, 0xFF)
+    lse_raw, lse = guarded(b.ntok * heads, torch.float32, 0xFF)
+    qd = q.cuda()
+    r = vl.PagedQuery(qd.data_ptr(), heads * hd, 0.0, 0, cache.ckind, out.data_ptr(), heads * hd, lse.data_ptr(),
+                      ws.data_ptr() if need else 0, need)
+    vl.check(L.vgx_paged_attn(gpu.ctx, cache.ref, batch.ref, ctypes.byref(r)))
+    with pytest.raises(vl.VgxError, match="length"):
+        batch.check()
+    for raw, t in ((ws_raw, ws), (out_raw, out), (lse_raw, lse)):
+        n = t.numel() * t.element_size()
+        assert (raw[:4096] == 0xA5).all() and (raw[4096 + n:] == 0xA5).all()
+    want, wl, mag, dots = ref.attend(b, q, heads)
+    bound = ref.attn_bound(b, ref.CTYPE[kind], want, mag, dots)
+    got = ref.value(out.cpu()).view_as(want)
+    kept = [s for s in range(2) if (not max_q or nq[s] <= max_q) and (not max_kv or kv[s] <= max_kv)]
+    assert len(kept) == 1
+    rows = slice(int(b.qs[kept[0]]), int(b.qs[kept[0] + 1]))
+    assert ((got[rows] - want[rows]).abs() <= bound[rows]).all()
+    assert torch.isfinite(lse.view(b.ntok, heads)[rows]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_a_step_on_a_side_stream(gpu, kind):
+    """The projections, append, attention and the next projection on a side
+    stream behind other work of it: use_torch_stream() puts the calls of the
+    context there too, and back."""
+    from vgx import mmcf
+    rng = np.random.default_rng(11)
+    heads, kvh, hd, dim = 4, 2, 64, 256
+
+    def mat(r, c):
+        w, unit, plane = mmcf.q8_per_row(rng.standard_normal((r, c)).astype(np.float32) * 0.05)
+        return gpu.upload(mmcf.Matrix("q8", r, c, (w.view(np.uint8) ^ 0x80).ravel(), unit, True, plane))
+
+    wqkv, wo = mat((heads + 2 * kvh) * hd, dim), mat(dim, heads * hd)
+    b = Batch(46, [9, 1, 30], [70, 500, 30], kvh, hd, 16, kind)
+    cos, sin = (t.cuda() for t in tables(500, hd))
+    given = (torch.randn(b.ntok, dim, generator=b.rng) * 256).to(torch.int16).cuda()
+
+    def step(x):
+        cache, batch = make(gpu, b, heads)
+        q = cache.append(batch, gpu.gemm(wqkv, x), cos, sin)
+        att = cache.attend(batch, q, out=torch.empty(b.ntok, heads * hd, dtype=torch.int16, device="cuda"))[0]
+        return gpu.gemm(wo, att, x), batch
+
+    want = step(given)[0]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            gpu.use_torch_stream()
+            x = torch.zeros_like(given)
+            torch.cuda._sleep(20_000_000)
+            x.copy_(given)
+            got, batch = step(x)
+        gpu.use_torch_stream()
+        batch.check()
+        assert torch.equal(got, want)

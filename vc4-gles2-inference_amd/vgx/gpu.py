@@ -302,7 +302,8 @@ class PagedCache:
     position-major pool is passed as its transposed view).  kind "bf16",
     "f16" or "q8" (int8, the grids k_step and v_step, 1/16 by default); the
     queries and outputs are bfloat16 for "bf16" and float16 for the others.
-    The calls run on torch's current stream."""
+    The calls run on torch's current stream (GPU's others on the one set
+    last: see GPU)."""
 
     def __init__(self, gpu, heads, kv_heads, head_dim, kind, k, v, k_step=0.0, v_step=0.0):
         elem, ctype, self.qtype = _CACHE[kind]
@@ -401,7 +402,12 @@ class PagedCache:
 
 
 class GPU:
-    """One libvgx context on one device, issuing on torch's current stream."""
+    """One libvgx context on one device.  It issues on the stream that was
+    torch's current one when it was made or use_torch_stream() was last called;
+    the calls over a paged cache and draft_verify issue on torch's current
+    stream at the call.  Under torch.cuda.stream(...) call use_torch_stream()
+    first, and again after, wherever both kinds are mixed: calls on different
+    streams are not ordered with one another."""
 
     def __init__(self, device=0):
         L = _l.load()
@@ -413,6 +419,7 @@ class GPU:
         self.use_torch_stream()
 
     def use_torch_stream(self):
+        """Later calls issue on torch's stream of now."""
         s = torch.cuda.current_stream(self.device).cuda_stream
         _l.check(_l.load().vgx_ctx_set_stream(self.ctx, ctypes.c_void_p(s)))
 
