@@ -395,7 +395,8 @@ typedef struct vgx_paged {
  * r is position kvlen[s] - rows + r.  Rows before qstart[0] (so that a part
  * of a larger batch can be named) and from qstart[nseq] on are left as they
  * are.  table_cols: entries a row of the table holds (what stands past a
- * sequence's length does not matter).
+ * sequence's length, or for vgx_paged_attn before its rows' windows, does not
+ * matter).
  * max_q, max_kv: the caller's bounds of the rows and positions of one
  * sequence, by which launches are sized (0: ntok, and what the table holds).
  * Bounds that the kernels check themselves, since the host cannot: a length

@@ -965,3 +965,51 @@ def test_a_step_on_a_side_stream(gpu, kind):
         gpu.use_torch_stream()
         batch.check()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+@pytest.mark.parametrize("page", [5, 16, 64])
+@pytest.mark.parametrize("nq, window", [([1, 3, 2], 100), ([1], 600), ([90, 40, 1], 100), ([130, 70], 33), ([7, 9], 1)])
+def test_pages_behind_the_window_are_gone(gpu, kind, page, nq, window):
+    """Entries of pages that no row sees any more are anything; one of a page
+    that the first row still sees is a fault."""
+    from vgx import lib as vl
+    kv = [n + m for n, m in zip(nq, [700, 333, 1100])]
+    b = Batch(47, nq, kv, 2, 64, page, kind)
+    full = b.table.clone()
+    cache, batch = make(gpu, b, 8)
+    q = (2 * b.randn(b.ntok, 8, 64)).to(ref.CTYPE[kind])
+    want = cache.attend(batch, q.cuda(), window=window)[0]
+    batch.check()
+    first = [(m - n - window + 1) // page for n, m in zip(nq, kv)]  # the page of the first key seen
+    for gone in (-1, b.pages, 2 ** 31 - 1):
+        for s, f in enumerate(first):
+            b.table[s, :f] = gone
+        cache, batch = make(gpu, b, 8)
+        assert torch.equal(cache.attend(batch, q.cuda(), window=window)[0], want)
+        batch.check()
+    for s, f in enumerate(first):
+        b.table.copy_(full)
+        b.table[s, f] = -1
+        cache, batch = make(gpu, b, 8)
+        cache.attend(batch, q.cuda(), window=window)
+        with pytest.raises(vl.VgxError, match="page"):
+            batch.check()
+
+
+def test_infinite_values_and_pages_behind_the_window(gpu):
+    """The pass that adds them to the rows that see them, over tiles that begin
+    before the window."""
+    for nq in ([2, 1], [90, 60]):
+        b = Batch(48, nq, [n + 500 for n in nq], 2, 64, 16, "bf16")
+        for s in range(2):
+            pos = 500 - 40
+            b.v[int(b.table[s, pos // 16]), :, pos % 16, 7] = math.inf
+        cache, batch = make(gpu, b, 4)
+        q = torch.randn(b.ntok, 4, 64).bfloat16()
+        want = cache.attend(batch, q.cuda(), window=100)[0]
+        b.table[:, :(500 - 99) // 16] = -1
+        cache, batch = make(gpu, b, 4)
+        got = cache.attend(batch, q.cuda(), window=100)[0]
+        batch.check()
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.isinf(got).any()

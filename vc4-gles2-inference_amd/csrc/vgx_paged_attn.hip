@@ -170,8 +170,10 @@ struct Geo {
 static_assert(Geo<64>::pv == 192 && Geo<96>::pv == 192 && Geo<128>::pv == 320 && Geo<256>::pv == 576, "");
 
 // The page of position j (of the last one where j is past it) as the table has
-// it, and the page to read: 0 with the fault noted where the table's is outside
-// the pool.  Apart, so that a load does not wait for the table's before it.
+// it, and the page to read: 0 where the table's is outside the pool, with the
+// fault noted if some row sees the position (tiles begin at multiples of 64, up
+// to 63 positions before a window: pages behind it may be gone).  Apart, so that
+// a load does not wait for the table's before it.
 __device__ __forceinline__ int page_at(const PagedDev& A, const int* tab, int j, int end) {
     return tab[page_of(A, min(j, end - 1))];
 }
@@ -712,8 +714,9 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
             qf[b][u] = __builtin_bit_cast(s16x8, w);
         }
     }
+    const int seen = P.window > 0 ? q.kv - q.n - P.window + 1 : 0;  // the first key of any row
     if (j0 < end) {
-        pg = page_ok(A, pg, bad, j0 + (lane & 31) < end);
+        pg = page_ok(A, pg, bad, j0 + (lane & 31) < end && j0 + (lane & 31) >= seen);
         t.load_v(A, vh, pg, j0, end);
         t.load_k(A, kh, pg, j0, end);
     }
@@ -807,7 +810,7 @@ __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) 
     if (KIND != VGX_E_Q8 && __builtin_expect(__any(odd), 0)) {
         for (j0 = start + wave * 32; j0 < end; j0 += 32 * WV) {
             if (j0 + 32 <= all_hi && j0 >= all_lo) continue;
-            t.load_v(A, vh, page_ok(A, Ks::page(A, tab, j0, end), bad), j0, end);
+            t.load_v(A, vh, page_ok(A, Ks::page(A, tab, j0, end), bad, j0 + (lane & 31) >= seen), j0, end);
             wave_sync();
             t.store_v(lv, end - j0, true, true);
             wave_sync();
@@ -965,6 +968,9 @@ __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, in
     const int tile_hi = min(base + m0 / A.grp + 1, end);
     const int tile_lo = P.window > 0 ? base + m1 / A.grp - P.window + 1 : 0;
     auto wide = [&](int j) { return j + ROWS > tile_hi || j < tile_lo; };
+    // the first key of any row, and the row of a tile that the lane looks up
+    const int seen = P.window > 0 ? base + m0 / A.grp - P.window + 1 : 0;
+    const int row = 16 * wave + (lane & 15);
     // Two tiles in LDS (one for heads of more than 128 values): the next one is
     // loaded into registers before this one's products and stored after them,
     // so a tile costs one barrier.
@@ -974,7 +980,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, in
     if (start < end) {
         pg = St::page(A, tab, start, end);
         pn = St::page(A, tab, start + ROWS, end);
-        pg = page_ok(A, pg, bad);
+        pg = page_ok(A, pg, bad, start + row >= seen);
         if (kTwo) {
             st.load(A, kh, vh, pg, start, end);
             odd = st.store(lk, lv, end - start, wide(start));
@@ -1016,7 +1022,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, in
         for (int j0 = start; j0 < end; j0 += ROWS) {
             if (!wide(j0)) continue;
             __syncthreads();
-            St::fetch_v(A, vh, page_ok(A, St::page(A, tab, j0, end), bad), j0, end, lv);
+            St::fetch_v(A, vh, page_ok(A, St::page(A, tab, j0, end), bad, j0 + row >= seen), j0, end, lv);
             __syncthreads();
             // (as the loop above skips and masks)
             if (j0 >= any_hi || j0 + ROWS <= any_lo) continue;
