@@ -1013,3 +1013,70 @@ def test_infinite_values_and_pages_behind_the_window(gpu):
         got = cache.attend(batch, q.cuda(), window=100)[0]
         batch.check()
         assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.isinf(got).any()
+
+
+@pytest.mark.parametrize("k_step, v_step", [(0.03, 0.5), (1.0, 1.0 / 128), (2.0 ** -10, 3.0)])
+@pytest.mark.parametrize("nq, kv", [([1, 2], [700, 41]), ([1], [6000]), ([90, 70], [300, 70]), ([80, 1], [90, 3000])])
+def test_q8_steps_and_scales(gpu, k_step, v_step, nq, kv):
+    """Grids of K and V of their own, and a scale: append and attention."""
+    heads, kvh, hd = 4, 2, 64
+    b = Batch(49, nq, kv, kvh, hd, 16, "q8")
+    k, v = b.k.cuda(), b.v.cuda()
+    cache = gpu.paged_cache(heads, kvh, hd, "q8", k, v, k_step=k_step, v_step=v_step)
+    batch = cache.batch(*b.device(), b.ntok)
+    x = b.randn(b.ntok, (heads + 2 * kvh) * hd)
+    x[:, heads * hd:] *= torch.cat([torch.full((kvh * hd,), 40 * k_step), torch.full((kvh * hd,), 40 * v_step)])
+    q = cache.append(batch, x.cuda())
+    for t, new, step in ((k, x[:, heads * hd:(heads + kvh) * hd], k_step), (v, x[:, (heads + kvh) * hd:], v_step)):
+        new = new.view(b.ntok, kvh, hd).double()
+        for s, (n, m) in enumerate(zip(nq, kv)):
+            for r in range(n):
+                pos, row = m - n + r, int(b.qs[s]) + r
+                got = t[int(b.table[s, pos // 16]), :, pos % 16].cpu().double() * step
+                want = new[row].clamp(-128 * step, 127 * step)
+                # half a step, and the 32-bit quotient's and sum's rounding of 128 steps
+                assert ((got - want).abs() <= step * (0.5 + 256 * 2.0 ** -24)).all()
+    b.k, b.v = k.cpu(), v.cpu()
+    for scale in (0.0, 0.02 / k_step / hd ** 0.5):
+        o, lse = cache.attend(batch, q, scale=scale, lse=True)
+        batch.check()
+        want, wl, mag, dots = ref.attend(b, q.cpu(), heads, scale or None, 0, k_step, v_step)
+        # (the bound's floor for small weights is in V's own grid)
+        bound = ref.attn_bound(b, torch.float16, want, mag, dots) + max(kv) * 2.0 ** -25 * 128 * v_step
+        assert ((o.cpu().double().view_as(want) - want).abs() <= bound).all()
+        tol = dots * (hd + 8) * 2.0 ** -22 + (max(kv) + 32) * 2.0 ** -24 + wl.abs() * 2.0 ** -22
+        assert ((lse.cpu().double() - wl).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind, hd", [("bf16", 64), ("q8", 96), ("f16", 112)])
+def test_attn_many_sequences_of_chunks(gpu, kind, hd):
+    """More sequences than a wave has lanes, of none to 60 rows: tiles are
+    counted over all of them; and the same beside single tokens' kernel."""
+    rng = np.random.default_rng(6)
+    nq = rng.integers(0, 61, 150)
+    nq[rng.random(150) < 0.3] = 1
+    kv = [int(n) + int(m) for n, m in zip(nq, rng.integers(0, 120, 150))]
+    b = Batch(50, nq.tolist(), kv, 1, hd, 16, kind)
+    cache, batch = make(gpu, b, 2)
+    check_attn(gpu, b, 2, cache=cache, batch=batch)
+    check_attn(gpu, b, 2, window=50)
+
+
+@pytest.mark.parametrize("heads, kvh", [(300, 1), (258, 2), (1024, 4)])
+@pytest.mark.parametrize("nq", [[1, 1], [2, 5]])
+def test_many_heads(gpu, heads, kvh, nq):
+    """More heads a KV head than a tile has columns."""
+    b = Batch(51, nq, [40, 200], kvh, 16, 16, "bf16")
+    _, cache, batch = check_append(gpu, b, heads, torch.bfloat16, 16, True, True)
+    b.k, b.v = cache.k.cpu(), cache.v.cpu()
+    check_attn(gpu, b, heads, cache=cache, batch=batch)
+
+
+@pytest.mark.parametrize("hd", range(16, 257, 16))
+@pytest.mark.parametrize("kind", ["bf16", "q8"])
+def test_every_head_size(gpu, kind, hd):
+    for nq, kv in (([1, 3], [50, 33]), ([70, 1], [90, 300])):
+        b = Batch(52, nq, kv, 2, hd, 16, kind)
+        _, cache, batch = check_append(gpu, b, 6, torch.float16, hd, False, True)
+        b.k, b.v = cache.k.cpu(), cache.v.cpu()
+        check_attn(gpu, b, 6, cache=cache, batch=batch)

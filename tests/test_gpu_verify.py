@@ -406,6 +406,27 @@ def test_refused_draft_alone_in_its_chunk(gpu, kind, vocab):
     assert a == [0, 0, 0, 0, 1, 0] and n == want
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab", [5, 6401, 40003])
+def test_rows_that_begin_anywhere(gpu, kind, vocab):
+    """Logits and the draft's of other strides and first addresses: their rows
+    begin at different places of a 16-byte piece."""
+    qs, tok, x, ua, un, d, _ = case(26, [5, 1, 3, 8, 2, 6], vocab, kind, True)
+    dev = [t.cuda() for t in (torch.tensor(qs, dtype=torch.int32), tok, ua, un)]
+    want = expect(qs, tok, x, ua, un, d)
+
+    def placed(t, before, width):
+        base = torch.full((t.shape[0], width), 9, dtype=t.dtype, device="cuda")
+        base[:, before:before + vocab] = t.cuda()
+        return base[:, before:before + vocab]
+
+    for (bx, wx), (bd, wd) in (((0, vocab), (1, vocab + 3)), ((3, vocab + 5), (0, vocab + 1)), ((7, vocab + 7), (2, vocab + 9))):
+        a, n, p = gpu.draft_verify(dev[0], dev[1], placed(x, bx, wx), dev[2], dev[3], draft=placed(d, bd, wd))
+        assert a.cpu().tolist() == want[0] and n.cpu().tolist() == want[1]
+        assert ((p.cpu().double() - want[2]).abs() <= want[2] * 2.0 ** -23 + 2.0 ** -149).all()
+
+
 BUF = 1 << 20
 
 
