@@ -358,8 +358,9 @@ int vgx_attn_block_seqs(vgx_attn* a, int layer, int pos, int nseq, const int16_t
 /* ---- a ragged batch over a paged KV cache.  No counterpart in the reference,
  * which decodes one sequence into a contiguous cache; for servers whose
  * sequences have different lengths.  Numbers here are floating point (sums,
- * norms and softmax statistics in 32 bits or more), except where a type says
- * q16 or q8.  Element types: */
+ * norms and softmax statistics in 32 bits or more; the attention's softmax
+ * weights, once, in the compute type), except where a type says q16 or q8.
+ * Element types: */
 enum vgx_elem {
     VGX_E_F32 = 1,
     VGX_E_BF16 = 2,
@@ -447,8 +448,10 @@ int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* bat
  * them).  q: ntok rows of heads * head_dim, compute type, q_stride elements
  * apart; scale 0: 1/sqrt(head_dim).  out: rows of heads * head_dim, out_kind
  * the compute type or Q16 (vgx_gemm's input; a NaN is 0 on its grid),
- * out_stride elements apart, apart from q.  lse
- * (may be NULL): f32, ntok x heads, the log of the softmax's denominator.  A
+ * out_stride elements apart, apart from q.  The softmax weights are rounded to
+ * the compute type before they multiply V (each to half a step of itself; in
+ * F16 one below 2^-23 of the row's largest to 2^-34 of that); their sum is not.
+ * lse (may be NULL): f32, ntok x heads, the log of the softmax's denominator.  A
  * row without a visible position gives zeros and an lse of -infinity.
  * Positions a row does not see, and what a page holds behind its sequence's
  * end, do not reach it, whatever values are there.
@@ -487,7 +490,10 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
  * T <= 0 or NaN: greedy, the draft accepted if it is the row's first maximum,
  * which is next.  Random numbers are in [0, 1); exponentials and sums run in
  * 64 bits, and weights below e^-620 of a row's largest may count as 0.  -infinity masks a token, NaN counts as -infinity, +infinity as the
- * largest float; a drafted token outside 0 .. vocab-1 is refused.
+ * largest float; a drafted token outside 0 .. vocab-1 is refused.  p and q are
+ * of the whole vocabulary: where sampling cuts to some tokens (top-k, top-p)
+ * the caller masks the others, in the draft's logits too (q16 has no mask: take
+ * another type, or its lowest value).
  * accepted[s]: drafts accepted; next[s]: -1 for a sequence without rows and
  * where no token has a weight.  prob (may be NULL): f32[ntok], p_r at the
  * drafted token (greedy: 1 or 0), 0 at a sequence's last row; rows of no

@@ -655,8 +655,9 @@ constexpr int rows_lds(int hd, int nb) {
 // product leaves column lane % 16's scores of keys 4 g + i (g = lane / 16) in
 // the lane; two of them are the next product's B operand.  Long caches are bound
 // by their bytes: one token at 130001 positions, 32 / 8 heads of 128 in bf16,
-// 92 us (5.8 TB/s); 64 at 200 .. 16000 in q8 pages of 4 KB, 106 us (4.7 TB/s; no
-// more with four workgroups a CU).  Short ones by a chain of round trips (lengths and table,
+// 92 us (5.8 TB/s); 64 at 200 .. 16000 in q8, 106 us (4.7 TB/s; in bf16, with the
+// join, 200 us and 4.9: 2136 workgroups with keys are 4.2 rounds of those
+// resident; the same with four workgroups a CU, and with pages of 16 to 256).  Short ones by a chain of round trips (lengths and table,
 // rows, the join): one token at 700, 8 / 4 heads of 96, 8.4 us.
 template <int KIND, int HD, bool EX, int NB, int WV>
 __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) {
@@ -920,7 +921,8 @@ __device__ __forceinline__ bool tile_at(const PagedDev& A, int tm, int cmin, int
 // one KV head; the waves share tiles of 64 keys.  Bound by the products and, as
 // two waves a SIMD do not wholly hide it, the softmax between them (6.7 vector
 // instructions a product): 4000 rows at 8100 positions, 32 / 8 heads of 128 in
-// bf16, 419 us (955 TFLOP/s; a library product of 8192^3 reaches 1234).
+// bf16, 417 to 444 us by the card (900 to 959 TFLOP/s; a library product of
+// 8192^3 reaches 1234).
 template <int KIND, int HD, bool EX>
 __device__ __forceinline__ void tile_body(const AttnArgs& P, int bx, int wgs, int split) {
     constexpr int ROWS = 64, kTile = 64 * (Geo<HD>::pk + Geo<HD>::pv);

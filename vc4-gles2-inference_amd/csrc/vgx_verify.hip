@@ -19,8 +19,8 @@
 // The exponential: e^y = 2^k 2^(i/64) e^(f ln 2 / 64) with 64 y / ln 2 = 64 k + i
 // + f, |f| <= 1/2: a table of 64 powers in LDS and a polynomial of degree 4 in f
 // (error (ln 2 / 128)^5 / 120 < 4e-14); a table lookup instead of a polynomial of degree 11 or more
-// (P. T. P. Tang, ACM TOMS 15, 1989).  12 operations of 64 bits a logit: what
-// bounds launch 1 of floating-point logits; q16's go by two tables (stats16_kernel).
+// (P. T. P. Tang, ACM TOMS 15, 1989).  12 operations of 64 bits a logit, of 29
+// vector instructions in launch 1; q16's go by two tables (stats16_kernel).
 #include <cfloat>
 #include <cmath>
 #include <string>
@@ -274,8 +274,9 @@ __device__ __forceinline__ void stats_put(Joined& J, Part* to, float m, int a, d
     if (threadIdx.x == 0) *to = Part{m, a, J.z[0] + J.z[1] + J.z[2] + J.z[3]};
 }
 
-// 126 rows of 73448 f32 logits and the draft's, 19 us (3.9 TB/s): 12 operations
-// of 64 bits a logit.
+// 126 rows of 73448 f32 logits and the draft's, 20 us (3.7 TB/s): 14 us of vector
+// instructions (29 a logit, at 2.4 GHz) and 12 of bytes, which overlap in part
+// only: a workgroup loads its chunk, then computes.
 template <int KIND, int K>
 __global__ void __launch_bounds__(kThreads) stats_kernel(const VerifyArgs P) {
     constexpr int N = kPer<KIND>;
@@ -346,8 +347,9 @@ typedef short short2v __attribute__((ext_vector_type(2)));
 typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 // Launch 1 for q16: two LDS reads and one operation of 64 bits a logit instead of
-// 12.  654 rows of 64402, 22 us (3.8 TB/s; 31 us by stats_kernel's way); the
-// tables cost a thread 2 exponentials beside its 8 or 32 logits.
+// 12.  654 rows of 64402, 22 us (3.8 TB/s; 31 us by stats_kernel's way): 13 us of
+// vector instructions (12 a logit) and 13 of bytes; the tables cost a thread 2
+// exponentials beside its 8 or 32 logits.
 template <int K>
 __global__ void __launch_bounds__(kThreads) stats16_kernel(const VerifyArgs P) {
     constexpr int KIND = VGX_E_Q16, N = 8;
