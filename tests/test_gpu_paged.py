@@ -866,7 +866,7 @@ def test_check_waits_for_every_stream(gpu):
 
 def test_more_splits_than_a_number_holds(gpu):
     """A batch whose splits would pass 2^31 partial results needs no workspace:
-    its sequences stay whole (it was refused before)."""
+    its sequences stay whole."""
     import ctypes
     from vgx import lib as vl
     at = 1 << 20  # (nothing is read)

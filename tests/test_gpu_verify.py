@@ -427,6 +427,26 @@ def test_rows_that_begin_anywhere(gpu, kind, vocab):
         assert ((p.cpu().double() - want[2]).abs() <= want[2] * 2.0 ** -23 + 2.0 ** -149).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab", [300, 6401, 20003])
+def test_equal_distributions_that_begin_elsewhere(gpu, kind, vocab):
+    """p = q, rows at different places of a 16-byte piece (so their sums are
+    added in different orders), and a draft that no token is: the draw is from
+    p, as where the rows lie alike."""
+    n = 64
+    qs, tok, x, ua, un, _, _ = case(27, [2] * n, vocab, kind, False, hint=0.0)
+    tok[1::2] = vocab
+    want = expect(qs, tok, x, ua, un, x)
+    dev = [t.cuda() for t in (torch.tensor(qs, dtype=torch.int32), tok, ua, un)]
+    base = torch.zeros(2 * n, vocab + 9, dtype=x.dtype, device="cuda")
+    for before in (0, 1, 3, 5):
+        d = base[:, before:before + vocab]
+        d.copy_(x)
+        a, nx, _ = gpu.draft_verify(dev[0], dev[1], x.cuda(), dev[2], dev[3], draft=d)
+        assert a.cpu().tolist() == [0] * n and nx.cpu().tolist() == want[1], before
+
+
 BUF = 1 << 20
 
 

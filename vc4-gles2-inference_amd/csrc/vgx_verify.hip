@@ -569,7 +569,10 @@ __device__ __forceinline__ void unscaled(Residual& R) {
 __device__ __forceinline__ double residual(const Residual& R, bool draft, float x, float d, int j, const double* tab) {
     const double p = weight(x, R.sx, tab) * R.zx;
     if (!draft) return j == R.tok ? 0.0 : p;
-    return fmax(p - weight(d, R.sd, tab) * R.zd, 0.0);
+    // (sums of rows that lie differently are added in different orders, and the
+    // exponentials are good to 2^-44: less than 2^-40 of p is no difference)
+    const double r = p - weight(d, R.sd, tab) * R.zd;
+    return r > p * 0x1p-40 ? r : 0.0;
 }
 
 // With draft logits: the sums of w over the chunks of the refused rows.  Every
