@@ -490,9 +490,9 @@ int vgx_paged_attn(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch
  * T <= 0 or NaN: greedy, the draft accepted if it is the row's first maximum,
  * which is next.  Random numbers are in [0, 1); exponentials and sums run in
  * 64 bits; weights below e^-620 of a row's largest may count as 0, and p - q
- * below 2^-40 of p does.  -infinity masks a token, NaN counts as -infinity, +infinity as the
- * largest float; a drafted token outside 0 .. vocab-1 is refused.  p and q are
- * of the whole vocabulary: where sampling cuts to some tokens (top-k, top-p)
+ * below 2^-40 of p does.  -infinity masks a token, NaN counts as -infinity,
+ * +infinity as the largest float; a drafted token outside 0 .. vocab-1 is
+ * refused.  p and q are of the whole vocabulary: where sampling cuts to some tokens (top-k, top-p)
  * the caller masks the others, in the draft's logits too (q16 has no mask: take
  * another type, or its lowest value).
  * accepted[s]: drafts accepted; next[s]: -1 for a sequence without rows and

@@ -57,9 +57,9 @@ struct AttnArgs {
     uint8_t* out;
     int64_t ostride;
     float* lse;
-    // Partial results, numbered: hd sums and (m, l) each, without the lift.  Split k of a row and
-    // head is number base + k * step; pn (ntok x heads) holds their splits and
-    // base.  Numbers go by row and head, or by sequence, KV head and column (the
+    // Partial results, numbered: hd sums and (m, l) each, without the lift.  Split
+    // k of a row and head is number base + k * step; pn (ntok x heads) holds their
+    // splits and base.  Numbers go by row and head, or by sequence, KV head and column (the
     // few rows of short sequences among many others').
     float* po;
     float2* pml;
@@ -657,8 +657,9 @@ constexpr int rows_lds(int hd, int nb) {
 // by their bytes: one token at 130001 positions, 32 / 8 heads of 128 in bf16,
 // 92 us (5.8 TB/s); 64 at 200 .. 16000 in q8, 106 us (4.7 TB/s; in bf16, with the
 // join, 200 us and 4.9: 2136 workgroups with keys are 4.2 rounds of those
-// resident; the same with four workgroups a CU, and with pages of 16 to 256).  Short ones by a chain of round trips (lengths and table,
-// rows, the join): one token at 700, 8 / 4 heads of 96, 8.4 us.
+// resident; the same with four workgroups a CU, and with pages of 16 to 256).
+// Short ones by a chain of round trips (lengths and table, rows, the join): one
+// token at 700, 8 / 4 heads of 96, 8.4 us.
 template <int KIND, int HD, bool EX, int NB, int WV>
 __device__ __forceinline__ void rows_body(const AttnArgs& P, int bx, int split) {
     using Ks = Keys<KIND, HD, EX>;
