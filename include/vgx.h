@@ -522,6 +522,125 @@ typedef struct vgx_draft {
 size_t vgx_draft_verify_ws(int nseq, int ntok, int vocab, int kind, int with_draft);
 int vgx_draft_verify(vgx_ctx* ctx, const vgx_draft* args);
 
+/* ---- drafted trees.  The new rows of a sequence of a ragged batch may be a
+ * tree: row 0 is the token that the sequence ended with, and every other row
+ * has a parent among the rows before it.  A step of such rows is
+ * vgx_tree_masks once, vgx_paged_append_tree and vgx_paged_attn_tree in every
+ * layer, the head over all rows, vgx_sample on all rows' logits,
+ * vgx_tree_accept, and vgx_paged_keep for all layers at once.
+ *
+ * vgx_tree_masks: parent (device int[ntok]): the number, among its sequence's
+ * rows, of each row's parent; anything but a row before it (-1, say) makes a
+ * row a root.  depth (device int[ntok]): rows on the way up to its root.  see
+ * (device, ntok rows of `words` 64-bit words): bit j of row i is set where j
+ * is i itself or one of its ancestors, with window > 0 one of the last window
+ * - 1 of them.  words: 1 to 16, and batch->max_q (where 0, ntok) at most 64 *
+ * words.  Of the batch nseq, ntok, max_q, qstart and fault are read; a
+ * sequence of more rows than max_q sets VGX_FAULT_LENGTH.  Rows of no sequence
+ * are left as they are. */
+typedef struct vgx_tree {
+    const int* depth;
+    const uint64_t* see;
+    int words;
+} vgx_tree;
+int vgx_tree_masks(vgx_ctx* ctx, const vgx_ragged* batch, const int* parent, int window, int words, int* depth,
+                   uint64_t* see);
+
+/* vgx_paged_append with the rows in their sequence's slots as they come, but
+ * turned by the angles of position kvlen - rows + depth (device int[ntok]).  A
+ * depth that is negative or above the row's number sets VGX_FAULT_LENGTH, and
+ * the row is written nowhere. */
+int vgx_paged_append_tree(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_rows* rows,
+                          const int* depth);
+
+/* vgx_paged_attn over a tree: row i of a sequence sees its positions before the
+ * new rows (with window > 0 those from kvlen - rows + depth - window + 1 on)
+ * and the new rows j whose bit is set in its mask (any of the sequence's rows;
+ * the row itself only if its bit is).  Masks need not be vgx_tree_masks's; the
+ * window does not cut them.  depth may be NULL without a window (outside
+ * 0 .. rows - 1 it counts as the nearer end).  Pages from position kvlen -
+ * rows - window + 1 on are read.  Everything else is as at vgx_paged_attn,
+ * with a workspace of vgx_paged_attn_tree_ws bytes. */
+size_t vgx_paged_attn_tree_ws(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, int window);
+int vgx_paged_attn_tree(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_query* query,
+                        const vgx_tree* tree);
+
+/* vgx_tree_accept: the walk down each sequence's tree (parent as above, tokens:
+ * device int[ntok], each row's token) by the token that each row's logits gave
+ * (chosen: device int[ntok]): from row 0 on to the first child whose token is
+ * the chosen one, until there is none.  path (device int[ntok]): at
+ * qstart[s] + k the number of the k-th row of the way among the sequence's
+ * rows (the first is row 0), -1 behind its end; accepted[s]: rows of the way
+ * but the first; next[s]: the last one's chosen token.  A sequence without
+ * rows has 0 and -1.  A token drawn from each row's own distribution thus
+ * stays a draw from the target's.  Of the batch as at vgx_tree_masks, with
+ * max_q at most 1024. */
+int vgx_tree_accept(vgx_ctx* ctx, const vgx_ragged* batch, const int* parent, const int* tokens, const int* chosen,
+                    int* path, int* accepted, int* next);
+
+/* ---- pages of one or several layers' caches: caches[0 .. ncache-1] have one
+ * shape, type and strides (ncache 1 or more), and pages numbered alike.
+ * vgx_paged_keep: for k = 1 .. accepted[s] (device int[nseq]) the K and V of
+ *   position b + path[qstart[s] + k] go to position b + k, b = kvlen[s] - rows:
+ *   the rows of an accepted path become the sequence's next positions.  The
+ *   batch is the one that was appended.  A path entry below k or not below the
+ *   sequence's rows, or accepted[s] outside 0 .. rows - 1, sets
+ *   VGX_FAULT_LENGTH, a page outside the pool VGX_FAULT_PAGE; such a row, or
+ *   such a sequence, is left.  Positions that the call writes are in no page
+ *   that another sequence shares.
+ * vgx_paged_copy: pages dst[i] = pages src[i] (device int[n]), of each the
+ *   first rows[i] positions (device int[n]; NULL: all).  A fork copies the
+ *   last, partly filled page and shares the others; pages are moved together
+ *   by copying them and writing the new numbers into the tables.  No page may
+ *   be dst twice, nor src of one copy and dst of another of the same call; a
+ *   page copied to itself stays.  *fault (device int, may be NULL) takes
+ *   VGX_FAULT_PAGE for a page outside the pool and VGX_FAULT_LENGTH for rows
+ *   outside 0 .. page_size; nothing is copied there. */
+int vgx_paged_keep(vgx_ctx* ctx, int ncache, const vgx_paged* caches, const vgx_ragged* batch, const int* path,
+                   const int* accepted);
+int vgx_paged_copy(vgx_ctx* ctx, int ncache, const vgx_paged* caches, int n, const int* src, const int* dst,
+                   const int* rows, int* fault);
+
+/* vgx_sample: a token of each row of logits.  With m the row's largest logit
+ * and T = temp[r], a token's weight is e^((x - m) / T).  Tokens rank by their
+ * logits, equal ones by the lower index, and of the ranking stay
+ *   the first top_k[r]                               (<= 0: all);
+ *   of these those whose predecessors' weights sum to less than top_p[r] times
+ *   the sum of all of these                          (1 or more, or NaN: all);
+ *   of these those of a weight of min_p[r] or more   (<= 0 or NaN: all; above 1
+ *   counts as 1);
+ * the first in rank always stays.  token[r] is the least index whose running
+ * sum of weights, over the tokens that stay in index order, passes u[r] (in
+ * [0, 1)) times the whole sum.  kept[r]: how many stay; prob[r]: the token's
+ * weight over their sum (both may be NULL).  temp (NULL: 1), top_k, top_p and
+ * min_p (NULL: all stay) are device arrays of nrows.  T <= 0 or NaN: greedy,
+ * the first maximum with kept 1 and prob 1.  -infinity masks a token and NaN
+ * counts as it, +infinity as the largest float; a row without a token gives
+ * -1, 0 and 0.  Weights and sums have 64 bits; where many tokens stay, weights
+ * are rounded to a multiple of 2^-41 (vocabularies up to 2^17: 2^-45) of the
+ * largest, and a token that this leaves nothing is not drawn.  The result does
+ * not depend on the other rows.
+ * kind F32, BF16, F16 or Q16; stride in values, any alignment of the type;
+ * vocab up to 2^21.  ws: vgx_sample_ws bytes of device memory, as
+ * vgx_paged_attn's. */
+typedef struct vgx_sampling {
+    int nrows, vocab, kind;
+    const void* logits;
+    int64_t stride;
+    const float* u;
+    const float* temp;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    int* token;
+    int* kept;
+    float* prob;
+    void* ws;
+    size_t ws_bytes;
+} vgx_sampling;
+size_t vgx_sample_ws(int nrows, int vocab, int kind);
+int vgx_sample(vgx_ctx* ctx, const vgx_sampling* args);
+
 /* ---- LFM2 gated short convolution: replaces GPU::init_conv, set_conv_kernel,
  * conv_block's gate/conv3/gate passes and clear_conv_state
  * (engine/src/gpu_conv.cpp:10-225), between the in_proj GEMV (3*dim rows:

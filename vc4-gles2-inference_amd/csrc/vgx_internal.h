@@ -158,5 +158,6 @@ int vgx_gemv_plan(int kind, int rows, int cols, int num_cu, int* lpr, int* ri, i
 int vgx_gemv_launch(const GemvLaunch& L, hipStream_t s);
 hipError_t vgx_gemm_tile_init();   // vgx_gemm.hip, with the device current
 hipError_t vgx_paged_attn_init();  // vgx_paged_attn.hip, the same
+hipError_t vgx_paged_tree_init();  // vgx_paged_tree.hip, the same
 int vgx_argmax_launch(const int16_t* v, int n, int rows, int* out, hipStream_t s);
 int vgx_dequant_launch(const MatDev& d, float* out, hipStream_t s);

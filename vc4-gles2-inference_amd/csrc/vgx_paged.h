@@ -23,6 +23,10 @@ struct PagedDev {
 
 // Checks the two descriptions (no device needed) and fills d.
 int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, PagedDev* d);
+int vgx_cache_fill(const char* who, const vgx_paged* c, PagedDev* d);
+
+// 64-bit words of a tree row's mask, at most: rows of a drafted tree, by 64.
+constexpr int kTreeWords = 16;
 
 inline int elem_bytes(int kind) { return kind == VGX_E_F32 ? 4 : kind == VGX_E_Q8 ? 1 : 2; }
 inline int compute_kind(int cache_kind) { return cache_kind == VGX_E_BF16 ? VGX_E_BF16 : VGX_E_F16; }

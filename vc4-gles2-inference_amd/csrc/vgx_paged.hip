@@ -33,9 +33,9 @@ bool apart(int64_t ext, int64_t n[3], int64_t st[3]) {
 
 }  // namespace
 
-int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, PagedDev* d) {
+int vgx_cache_fill(const char* who, const vgx_paged* c, PagedDev* d) {
     const std::string w = std::string(who) + ": ";
-    if (!c || !b) return vgx_fail(VGX_EINVAL, w + "NULL cache or batch");
+    if (!c) return vgx_fail(VGX_EINVAL, w + "NULL cache or batch");
     if (c->kind != VGX_E_BF16 && c->kind != VGX_E_F16 && c->kind != VGX_E_Q8)
         return vgx_fail(VGX_EINVAL, w + "a cache is bf16, f16 or q8");
     if (c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || c->heads > 1024)
@@ -58,19 +58,6 @@ int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, Pag
     for (float step : {c->k_step, c->v_step})  // (a NaN is refused; 1 / step and 128 step stay finite)
         if (step != 0 && !(step >= 0x1p-64f && step <= 0x1p64f))
             return vgx_fail(VGX_EINVAL, w + "a q8 step is neither 0 nor in 2^-64 .. 2^64");
-    if (b->nseq < 0 || b->ntok < 0 || b->nseq > (1 << 20) || b->ntok > (1 << 24))
-        return vgx_fail(VGX_EINVAL, w + "nseq outside 0..2^20 or ntok outside 0..2^24");
-    if (b->max_q < 0 || b->max_kv < 0) return vgx_fail(VGX_EINVAL, w + "a negative bound");
-    if (b->nseq && b->ntok) {
-        if (!b->qstart || !b->kvlen || !b->table) return vgx_fail(VGX_EINVAL, w + "NULL qstart, kvlen or table");
-        if (b->table_cols <= 0 || b->table_stride < b->table_cols)
-            return vgx_fail(VGX_EINVAL, w + "a table without columns, or rows that overlap");
-        // (positions, less a window and 2^24 rows, stay inside 32 bits)
-        if ((int64_t)b->table_cols * c->page_size > INT32_MAX - (1 << 25))
-            return vgx_fail(VGX_ERANGE, w + "a table's row holds 2^31 - 2^25 positions or more");
-        if ((int64_t)b->max_kv > (int64_t)b->table_cols * c->page_size)
-            return vgx_fail(VGX_ERANGE, w + "max_kv past what a table's row holds");
-    }
     PagedDev& A = *d;
     A.k = static_cast<uint8_t*>(c->k);
     A.v = static_cast<uint8_t*>(c->v);
@@ -88,6 +75,28 @@ int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, Pag
     else { A.pmul = (unsigned)((((unsigned __int128)1 << (32 + s)) / p) + 1); A.psh = s; }
     A.kstep = c->kind == VGX_E_Q8 ? (c->k_step > 0 ? c->k_step : 1.0f / 16) : 1.0f;
     A.vstep = c->kind == VGX_E_Q8 ? (c->v_step > 0 ? c->v_step : 1.0f / 16) : 1.0f;
+    return VGX_OK;
+}
+
+int vgx_paged_fill(const char* who, const vgx_paged* c, const vgx_ragged* b, PagedDev* d) {
+    const std::string w = std::string(who) + ": ";
+    if (!b) return vgx_fail(VGX_EINVAL, w + "NULL cache or batch");
+    const int st = vgx_cache_fill(who, c, d);
+    if (st != VGX_OK) return st;
+    if (b->nseq < 0 || b->ntok < 0 || b->nseq > (1 << 20) || b->ntok > (1 << 24))
+        return vgx_fail(VGX_EINVAL, w + "nseq outside 0..2^20 or ntok outside 0..2^24");
+    if (b->max_q < 0 || b->max_kv < 0) return vgx_fail(VGX_EINVAL, w + "a negative bound");
+    if (b->nseq && b->ntok) {
+        if (!b->qstart || !b->kvlen || !b->table) return vgx_fail(VGX_EINVAL, w + "NULL qstart, kvlen or table");
+        if (b->table_cols <= 0 || b->table_stride < b->table_cols)
+            return vgx_fail(VGX_EINVAL, w + "a table without columns, or rows that overlap");
+        // (positions, less a window and 2^24 rows, stay inside 32 bits)
+        if ((int64_t)b->table_cols * c->page_size > INT32_MAX - (1 << 25))
+            return vgx_fail(VGX_ERANGE, w + "a table's row holds 2^31 - 2^25 positions or more");
+        if ((int64_t)b->max_kv > (int64_t)b->table_cols * c->page_size)
+            return vgx_fail(VGX_ERANGE, w + "max_kv past what a table's row holds");
+    }
+    PagedDev& A = *d;
     A.nseq = b->nseq; A.ntok = b->ntok; A.tcols = b->table_cols; A.tstride = b->table_stride;
     const int64_t held = (int64_t)b->table_cols * c->page_size;
     A.max_q = b->max_q > 0 ? std::min(b->max_q, b->ntok) : b->ntok;
@@ -110,6 +119,7 @@ struct AppendArgs {
     float eps;
     uint8_t* q;
     int64_t qstride;
+    const int* depth;  // of a tree's rows, or nullptr: a row's angles are its position's
     int vecs;        // heads + 2 * kvh
     int wpt;         // workgroups a row
 };
@@ -201,18 +211,18 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs P) {
     if (s >= A.nseq) return;  // behind the last sequence
     const SeqAt sq = seq_at(A, s);
     const int i = t - sq.q0, pos = sq.kv - sq.n + i;
-    const int cap = min(A.max_kv, P.rot ? P.npos : 0x7fffffff);
-    if (!sq.ok || pos >= cap) {
+    const int d = P.depth ? P.depth[t] : i, at = pos - i + d;  // the position of the row's angles
+    if (!sq.ok || pos >= A.max_kv || (P.rot && at >= P.npos) || d < 0 || d > i) {
         if (threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
         return;
     }
-    if (i < 0 || i >= sq.n || pos < 0) return;
+    if (i < 0 || i >= sq.n || pos < 0 || at < 0) return;
     const int pi = page_of(A, pos), slot = pos - pi * A.psize;
     const int pg = A.table[(int64_t)s * A.tstride + pi];
     float c[8], n[8];
     if (turn && d0 < A.hd) {
-        const float* cp = P.cs + (int64_t)pos * half + ti;
-        const float* np = P.sn + (int64_t)pos * half + ti;
+        const float* cp = P.cs + (int64_t)at * half + ti;
+        const float* np = P.sn + (int64_t)at * half + ti;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool use = P.half || e < 4;  // (neighbours: four angles)
@@ -295,34 +305,35 @@ AppendFn append_act(int act, int lpv, bool three) {
     return three ? append_lpv<KIND, VGX_E_Q16, 3>(lpv) : append_lpv<KIND, VGX_E_Q16, 1>(lpv);
 }
 
-}  // namespace
-
-extern "C" int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch,
-                                const vgx_paged_rows* r) {
+// vgx_paged_append and, of a tree's rows, vgx_paged_append_tree.
+int append_call(const char* who, vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch,
+                const vgx_paged_rows* r, bool tree, const int* depth) {
     AppendArgs P{};
-    const int st = vgx_paged_fill("vgx_paged_append", cache, batch, &P.A);
+    const int st = vgx_paged_fill(who, cache, batch, &P.A);
     if (st != VGX_OK) return st;
-    if (!r) return vgx_fail(VGX_EINVAL, "vgx_paged_append: NULL rows");
+    auto fail = [&](int status, const char* what) { return vgx_fail(status, std::string(who) + ": " + what); };
+    if (!r) return fail(VGX_EINVAL, "NULL rows");
     if (r->kind != VGX_E_F32 && r->kind != VGX_E_BF16 && r->kind != VGX_E_F16 && r->kind != VGX_E_Q16)
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: rows are f32, bf16, f16 or q16");
+        return fail(VGX_EINVAL, "rows are f32, bf16, f16 or q16");
     const PagedDev& A = P.A;
     const int64_t width = (int64_t)(A.heads + 2 * A.kvh) * A.hd;
     const int per16 = 16 / elem_bytes(r->kind);
     if (r->stride < width || r->stride % per16)
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: stride below a row's width or not a multiple of 16 bytes");
+        return fail(VGX_EINVAL, "stride below a row's width or not a multiple of 16 bytes");
     if (r->rot < 0 || r->rot % 16 || r->rot > A.hd)
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: rot must be a multiple of 16, at most head_dim");
+        return fail(VGX_EINVAL, "rot must be a multiple of 16, at most head_dim");
     if (r->rot && (!r->cos || !r->sin || r->npos <= 0))
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: a rotation without its table");
-    if (!r->q_norm != !r->k_norm) return vgx_fail(VGX_EINVAL, "vgx_paged_append: one norm weight of two");
+        return fail(VGX_EINVAL, "a rotation without its table");
+    if (!r->q_norm != !r->k_norm) return fail(VGX_EINVAL, "one norm weight of two");
     if (r->q_norm && !(r->eps >= 0 && std::isfinite(r->eps)))
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: eps is negative or not a number");
+        return fail(VGX_EINVAL, "eps is negative or not a number");
     if (r->q && (r->q_stride < (int64_t)A.heads * A.hd || r->q_stride % 8))
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: q_stride below a row's width or not a multiple of 16 bytes");
-    if (A.ntok && !r->qkv) return vgx_fail(VGX_EINVAL, "vgx_paged_append: NULL qkv");
+        return fail(VGX_EINVAL, "q_stride below a row's width or not a multiple of 16 bytes");
+    if (A.ntok && !r->qkv) return fail(VGX_EINVAL, "NULL qkv");
     if (((uintptr_t)r->qkv | (uintptr_t)r->q) & 15)
-        return vgx_fail(VGX_EINVAL, "vgx_paged_append: qkv or q not 16-byte aligned");
-    if (!ctx) return vgx_fail(VGX_EINVAL, "vgx_paged_append: no context");
+        return fail(VGX_EINVAL, "qkv or q not 16-byte aligned");
+    if (tree && A.ntok && !depth) return fail(VGX_EINVAL, "a tree without its rows' depths");
+    if (!ctx) return fail(VGX_EINVAL, "no context");
     if (A.ntok == 0 || A.nseq == 0) return VGX_OK;
     P.x = static_cast<const uint8_t*>(r->qkv);
     P.stride = r->stride;
@@ -330,6 +341,7 @@ extern "C" int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_
     P.qn = r->q_norm; P.kn = r->k_norm; P.eps = r->eps;
     P.q = static_cast<uint8_t*>(r->q);
     P.qstride = r->q_stride;
+    P.depth = depth;
     P.vecs = A.heads + 2 * A.kvh;
     const int lpv = A.hd <= 64 ? 8 : A.hd <= 128 ? 16 : 32;
     // three passes a workgroup where the rows alone fill the chip (8 workgroups
@@ -338,7 +350,7 @@ extern "C" int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_
     const bool three = passes > 1 && A.ntok >= 8 * ctx->num_cu;
     P.wpt = three ? (passes + 2) / 3 : passes;
     const int64_t grid = (int64_t)A.ntok * P.wpt;
-    if (grid >= (1 << 24)) return vgx_fail(VGX_ERANGE, "vgx_paged_append: too many rows");  // 2^32 threads
+    if (grid >= (1 << 24)) return fail(VGX_ERANGE, "too many rows");  // 2^32 threads
     const AppendFn fn = cache->kind == VGX_E_BF16  ? append_act<VGX_E_BF16>(r->kind, lpv, three)
                         : cache->kind == VGX_E_F16 ? append_act<VGX_E_F16>(r->kind, lpv, three)
                                                    : append_act<VGX_E_Q8>(r->kind, lpv, three);
@@ -347,3 +359,18 @@ extern "C" int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_
     VGX_LAUNCH_CHECK("paged append launch");
     return VGX_OK;
 }
+
+}  // namespace
+
+extern "C" {
+
+int vgx_paged_append(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_rows* r) {
+    return append_call("vgx_paged_append", ctx, cache, batch, r, false, nullptr);
+}
+
+int vgx_paged_append_tree(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_rows* r,
+                          const int* depth) {
+    return append_call("vgx_paged_append_tree", ctx, cache, batch, r, true, depth);
+}
+
+}  // extern "C"

@@ -254,6 +254,16 @@ _CACHE = {"bf16": (_l.E_BF16, torch.bfloat16, torch.bfloat16), "f16": (_l.E_F16,
           "q8": (_l.E_Q8, torch.int8, torch.float16)}
 
 
+def _raise_fault(gpu, fault, who, length):
+    torch.cuda.synchronize(gpu.device)
+    bits = int(fault.item())
+    if bits:
+        fault.zero_()
+        torch.cuda.synchronize(gpu.device)  # (before another stream's next call can set one)
+        what = [w for b, w in ((_l.FAULT_LENGTH, length), (_l.FAULT_PAGE, "a page outside the pool")) if bits & b]
+        raise _l.VgxError(_l.VGX_ERANGE, who + ": " + " and ".join(what))
+
+
 class RaggedBatch:
     """A ragged batch over a paged cache: sequence s has rows qstart[s] ..
     qstart[s+1]-1 of the ntok new ones, kvlen[s] positions counting them, and
@@ -285,15 +295,93 @@ class RaggedBatch:
         self.ref = ctypes.byref(self.d)
         self.ws = {}  # workspace bytes by (cache, window)
 
+    def tree(self, parent, window=0):
+        """The rows as drafted trees: parent[r] is the number of row r's parent
+        among its sequence's rows (-1: none)."""
+        return Tree(self, parent, window)
+
+    def accept(self, parent, tokens, chosen):
+        """The walk down each sequence's tree by the token that each row's
+        logits gave: (path: the rows of the way, at qstart[s] + k the k-th,
+        -1 behind its end; accepted: rows of the way but the first; next: the
+        last one's token)."""
+        g = self.gpu
+        for t, name in ((parent, "parent"), (tokens, "tokens"), (chosen, "chosen")):
+            g.need_values(t, _I32, self.ntok, name)
+        path = torch.empty(self.ntok, dtype=_I32, device=g.device)
+        accepted, nxt = (torch.empty(self.nseq, dtype=_I32, device=g.device) for _ in range(2))
+        g.on_current(_l.load().vgx_tree_accept, self.ref, parent.data_ptr(), tokens.data_ptr(), chosen.data_ptr(),
+                     path.data_ptr(), accepted.data_ptr(), nxt.data_ptr())
+        return path, accepted, nxt
+
     def check(self):
-        torch.cuda.synchronize(self.gpu.device)
-        bits = int(self.fault.item())
-        if bits:
-            self.fault.zero_()
-            torch.cuda.synchronize(self.gpu.device)  # (before another stream's next call can set one)
-            what = [w for b, w in ((_l.FAULT_LENGTH, "a length outside its bounds"),
-                                   (_l.FAULT_PAGE, "a page outside the pool")) if bits & b]
-            raise _l.VgxError(_l.VGX_ERANGE, "ragged batch: " + " and ".join(what))
+        _raise_fault(self.gpu, self.fault, "ragged batch", "a length outside its bounds")
+
+
+class Tree:
+    """A batch's rows as drafted trees: each row's depth and the mask of the
+    rows it sees, itself and its ancestors (with a window those inside it), from
+    its parent.  Made once for all layers; update() makes them anew from other
+    parents, in place (a captured step's)."""
+
+    def __init__(self, batch, parent, window=0):
+        g = batch.gpu
+        most = min(batch.d.max_q, batch.ntok) or batch.ntok
+        self.batch, self.window = batch, int(window)
+        self.words = max(1, -(-most // 64))
+        if self.words > 16:
+            raise ValueError("a tree has at most 1024 rows a sequence: give the batch its bound max_q")
+        self.depth = torch.empty(batch.ntok, dtype=_I32, device=g.device)
+        self.see = torch.empty((batch.ntok, self.words), dtype=torch.int64, device=g.device)
+        self.d = _l.Tree(self.depth.data_ptr(), self.see.data_ptr(), self.words)
+        self.ref = ctypes.byref(self.d)
+        self.update(parent)
+
+    def update(self, parent):
+        g = self.batch.gpu
+        g.need_values(parent, _I32, self.batch.ntok, "parent")
+        g.on_current(_l.load().vgx_tree_masks, self.batch.ref, parent.data_ptr(), self.window, self.words,
+                     self.depth.data_ptr(), self.see.data_ptr())
+
+
+class PagedLayers:
+    """The caches of a model's layers, alike in shape, type and strides, whose
+    pages are numbered alike: what moves pages moves them in all of them at
+    once."""
+
+    def __init__(self, caches):
+        if not caches:
+            raise ValueError("no caches")
+        self.gpu, self.caches = caches[0].gpu, list(caches)
+        if any(c.gpu.device != self.gpu.device for c in caches):
+            raise ValueError("the caches are on several devices")
+        self.d = (_l.Paged * len(caches))(*[c.d for c in caches])
+        self.fault = torch.zeros(1, dtype=_I32, device=self.gpu.device)
+
+    def keep(self, batch, path, accepted):
+        """The rows of an accepted path (RaggedBatch.accept) become their
+        sequences' next positions: kvlen[s] - rows + 1 + accepted[s] are held
+        then."""
+        g = self.gpu
+        self.caches[0]._same_device(batch)
+        g.need_values(path, _I32, batch.ntok, "path")
+        g.need_values(accepted, _I32, batch.nseq, "accepted")
+        g.on_current(_l.load().vgx_paged_keep, len(self.d), self.d, batch.ref, path.data_ptr(), accepted.data_ptr())
+
+    def copy(self, src, dst, rows=None):
+        """Pages dst[i] = pages src[i], of each the first rows[i] positions."""
+        g, n = self.gpu, src.shape[0]
+        g.need_values(src, _I32, n, "src")
+        g.need_values(dst, _I32, n, "dst")
+        if rows is not None:
+            g.need_values(rows, _I32, n, "rows")
+        g.on_current(_l.load().vgx_paged_copy, len(self.d), self.d, n, src.data_ptr(), dst.data_ptr(), _at(rows),
+                     self.fault.data_ptr())
+
+    def check(self):
+        """Waits for the device and raises if a copy met a page or a number of
+        rows outside its bounds (keep's are the batch's)."""
+        _raise_fault(self.gpu, self.fault, "paged copy", "a number of rows outside the page")
 
 
 class PagedCache:
@@ -323,10 +411,12 @@ class PagedCache:
     def batch(self, qstart, kvlen, table, ntok, max_q=0, max_kv=0):
         return RaggedBatch(self.gpu, qstart, kvlen, table, ntok, max_q, max_kv)
 
-    def append(self, batch, qkv, cos=None, sin=None, rope_half=True, q_norm=None, k_norm=None, eps=1e-5, out=None):
+    def append(self, batch, qkv, cos=None, sin=None, rope_half=True, q_norm=None, k_norm=None, eps=1e-5, out=None,
+               tree=None):
         """The rows qkv (ntok, (heads + 2 kv_heads) * head_dim; float32,
         bfloat16, float16 or q16) normed, rotated (cos, sin: positions x rot/2)
-        and written into the cache; returns the queries (ntok, heads, head_dim)."""
+        and written into the cache; returns the queries (ntok, heads, head_dim).
+        tree (RaggedBatch.tree): a row is rotated by its depth's position."""
         g = self.gpu
         self._same_device(batch)
         kind = _ELEM.get(qkv.dtype)
@@ -354,13 +444,19 @@ class PagedCache:
             q, qs = out, self._rows(out, self.qtype, batch.ntok, "out")
         r = _l.PagedRows(kind, qkv.data_ptr(), stride, _at(cos), _at(sin), npos, rot, int(rope_half), _at(q_norm),
                          _at(k_norm), eps, q.data_ptr(), qs)
-        g.on_current(_l.load().vgx_paged_append, self.ref, batch.ref, ctypes.byref(r))
+        if tree is None:
+            g.on_current(_l.load().vgx_paged_append, self.ref, batch.ref, ctypes.byref(r))
+        else:
+            self._same_batch(batch, tree)
+            g.on_current(_l.load().vgx_paged_append_tree, self.ref, batch.ref, ctypes.byref(r), tree.d.depth)
         return q
 
-    def attend(self, batch, q, scale=0.0, window=0, out=None, lse=False):
+    def attend(self, batch, q, scale=0.0, window=0, out=None, lse=False, tree=None):
         """The attention of the rows q (ntok, heads, head_dim) over their
         sequences: (out (ntok, heads * head_dim), lse (ntok, heads) or None).
-        out: a tensor to write, of the compute type or int16 (q16)."""
+        out: a tensor to write, of the compute type or int16 (q16).  tree
+        (RaggedBatch.tree, of the same window): of the new rows each sees
+        itself and its ancestors."""
         g = self.gpu
         self._same_device(batch)
         qs = self._rows(q, self.qtype, batch.ntok, "q")
@@ -369,19 +465,31 @@ class PagedCache:
         else:
             kind = _l.E_Q16 if out.dtype == torch.int16 else self.ckind
             os_ = self._rows(out, out.dtype if kind == _l.E_Q16 else self.qtype, batch.ntok, "out")
-        key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window)
+        if tree is not None:
+            self._same_batch(batch, tree)
+            if tree.window != window:
+                raise ValueError("the tree's window is %d, not %d" % (tree.window, window))
+        key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window, tree is None)
         need = batch.ws.get(key)
         L = _l.load()
         known = need is not None
         if not known:
-            need = int(L.vgx_paged_attn_ws(g.ctx, self.ref, batch.ref, window))
+            size = L.vgx_paged_attn_ws if tree is None else L.vgx_paged_attn_tree_ws
+            need = int(size(g.ctx, self.ref, batch.ref, window))
         ws = torch.empty(need, dtype=torch.uint8, device=g.device) if need else None
         z = torch.empty((batch.ntok, self.heads), dtype=torch.float32, device=g.device) if lse else None
         r = _l.PagedQuery(q.data_ptr(), qs, scale, window, kind, out.data_ptr(), os_, _at(z), _at(ws), need)
-        g.on_current(L.vgx_paged_attn, self.ref, batch.ref, ctypes.byref(r))
+        if tree is None:
+            g.on_current(L.vgx_paged_attn, self.ref, batch.ref, ctypes.byref(r))
+        else:
+            g.on_current(L.vgx_paged_attn_tree, self.ref, batch.ref, ctypes.byref(r), tree.ref)
         if not known:  # (a refused call's size is 0)
             batch.ws[key] = need
         return out, z
+
+    def _same_batch(self, batch, tree):
+        if tree.batch is not batch:
+            raise ValueError("the tree is of another batch")
 
     def _same_device(self, batch):
         if batch.gpu is not self.gpu and batch.gpu.device != self.gpu.device:
@@ -404,8 +512,8 @@ class PagedCache:
 class GPU:
     """One libvgx context on one device.  It issues on the stream that was
     torch's current one when it was made or use_torch_stream() was last called;
-    the calls over a paged cache and draft_verify issue on torch's current
-    stream at the call.  Under torch.cuda.stream(...) call use_torch_stream()
+    the calls over a paged cache, sample and draft_verify issue on torch's
+    current stream at the call.  Under torch.cuda.stream(...) call use_torch_stream()
     first, and again after, wherever both kinds are mixed: calls on different
     streams are not ordered with one another."""
 
@@ -455,6 +563,11 @@ class GPU:
             raise ValueError("%s must be %d rows of %d contiguous values that do not overlap, not %s with strides %s" % (
                 name, n, width, tuple(t.shape), st))
         return st[0] if n > 1 else width
+
+    def need_values(self, t, dtype, n, name):
+        """Refuses all but n contiguous values."""
+        if t.dtype is not dtype or t.device != self.device or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError("%s must be %d contiguous %s values on %s" % (name, n, dtype, self.device))
 
     # -- weights
     def upload(self, m: Matrix):
@@ -644,6 +757,35 @@ class GPU:
     def paged_cache(self, heads, kv_heads, head_dim, kind, k, v, k_step=0.0, v_step=0.0):
         return PagedCache(self, heads, kv_heads, head_dim, kind, k, v, k_step, v_step)
 
+    def paged_layers(self, caches):
+        return PagedLayers(caches)
+
+    def sample(self, logits, u, temp=None, top_k=None, top_p=None, min_p=None):
+        """A token of each row of logits (rows, vocab; float32, bfloat16,
+        float16 or q16) by the random numbers u in [0, 1), after the cuts that
+        are given, a value a row: temp (0: greedy), top_k (0: all), top_p (1:
+        all), min_p (0: all).  Returns (token, tokens that stay, the token's
+        probability among them).  On torch's current stream."""
+        kind = _ELEM.get(logits.dtype)
+        if kind is None or logits.dim() != 2:
+            raise ValueError("logits must be rows of float32, bfloat16, float16 or int16 (q16)")
+        n, vocab = logits.shape
+        stride = self.need_rows(logits, None, n, vocab, "logits")
+        self.need_values(u, _F32, n, "u")
+        for t, dtype, name in ((temp, _F32, "temp"), (top_k, _I32, "top_k"), (top_p, _F32, "top_p"),
+                               (min_p, _F32, "min_p")):
+            if t is not None:
+                self.need_values(t, dtype, n, name)
+        L, dev = _l.load(), self.device
+        need = int(L.vgx_sample_ws(n, vocab, kind))
+        token, kept = (torch.empty(n, dtype=_I32, device=dev) for _ in range(2))
+        prob = torch.empty(n, dtype=_F32, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        a = _l.Sampling(n, vocab, kind, logits.data_ptr(), stride, u.data_ptr(), _at(temp), _at(top_k), _at(top_p),
+                        _at(min_p), token.data_ptr(), kept.data_ptr(), prob.data_ptr(), _at(ws), need)
+        self.on_current(L.vgx_sample, ctypes.byref(a))
+        return token, kept, prob
+
     def draft_verify(self, qstart, tokens, logits, u_accept, u_next, draft=None, temp=None):
         """Drafted tokens against the target's logits (rows, vocab; float32,
         bfloat16, float16 or q16): tokens[r + 1] against row r of its sequence
@@ -657,9 +799,8 @@ class GPU:
         for t, dtype, size, name in ((qstart, _I32, nseq + 1, "qstart"), (tokens, _I32, n, "tokens"),
                                      (u_accept, _F32, n, "u_accept"), (u_next, _F32, nseq, "u_next"),
                                      (temp, _F32, nseq, "temp")):
-            if t is not None and (t.dtype is not dtype or t.device != self.device or t.shape != (size,)
-                                  or not t.is_contiguous()):
-                raise ValueError("%s must be %d contiguous %s values on %s" % (name, size, dtype, self.device))
+            if t is not None:
+                self.need_values(t, dtype, size, name)
         kind = _ELEM.get(logits.dtype)
         if kind is None or logits.dim() != 2:
             raise ValueError("logits must be rows of float32, bfloat16, float16 or int16 (q16)")

@@ -76,6 +76,16 @@ class Draft(ctypes.Structure):
                 ("ws_bytes", ctypes.c_size_t)]
 
 
+class Tree(ctypes.Structure):
+    _fields_ = [("depth", _P), ("see", _P), ("words", _I)]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [("nrows", _I), ("vocab", _I), ("kind", _I), ("logits", _P), ("stride", _I64), ("u", _P), ("temp", _P),
+                ("top_k", _P), ("top_p", _P), ("min_p", _P), ("token", _P), ("kept", _P), ("prob", _P), ("ws", _P),
+                ("ws_bytes", ctypes.c_size_t)]
+
+
 _SIGS = {
     "vgx_abi_version": (_I, []),
     "vgx_strerror": (ctypes.c_char_p, [_I]),
@@ -150,6 +160,15 @@ _SIGS = {
     "vgx_paged_attn": (_I, [_P, _P, _P, _P]),
     "vgx_draft_verify_ws": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
     "vgx_draft_verify": (_I, [_P, _P]),
+    "vgx_tree_masks": (_I, [_P, _P, _P, _I, _I, _P, _P]),
+    "vgx_paged_append_tree": (_I, [_P, _P, _P, _P, _P]),
+    "vgx_paged_attn_tree_ws": (ctypes.c_size_t, [_P, _P, _P, _I]),
+    "vgx_paged_attn_tree": (_I, [_P, _P, _P, _P, _P]),
+    "vgx_tree_accept": (_I, [_P, _P, _P, _P, _P, _P, _P, _P]),
+    "vgx_paged_keep": (_I, [_P, _I, _P, _P, _P, _P]),
+    "vgx_paged_copy": (_I, [_P, _I, _P, _I, _P, _P, _P, _P]),
+    "vgx_sample_ws": (ctypes.c_size_t, [_I, _I, _I]),
+    "vgx_sample": (_I, [_P, _P]),
     "vgx_quantize_act": (None, [_P, _I, _P]),
     "vgx_x_pack_i16_2": (None, [_P, _I, _P]),
 }
