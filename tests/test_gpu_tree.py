@@ -556,3 +556,26 @@ def test_two_streams_at_once(gpu, n):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_part_of_a_batch(gpu):
+    """Some of a batch's sequences, named by their entries of qstart: the rows
+    before and behind them are left as they are, and are no fault."""
+    nq, kv = [6, 3, 12, 5], [60, 30, 50, 90]
+    b = Batch(56, nq, kv, 1, 64, 16, "bf16")
+    parents = trees_of(nq, 57)
+    cache, _ = make(gpu, b, 2)
+    qs, kvlen, table = b.device()
+    some = cache.batch(qs[1:4], kvlen[1:3], table[1:3], b.ntok)
+    tree = some.tree(flat(parents))
+    cos, sin = (t.cuda() for t in tables(100, 64))
+    x = b.randn(b.ntok, 4 * 64).cuda()
+    q = torch.full((b.ntok, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    tree.depth[:6], tree.depth[21:] = 99, -5
+    cache.append(some, x, cos, sin, out=q, tree=tree)
+    out = torch.full((b.ntok, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    cache.attend(some, q, out=out, tree=tree)
+    some.check()
+    rest = list(range(6)) + list(range(21, 26))
+    assert (q[rest] == 7).all() and (out[rest] == 3).all()
+    assert not (q[6:21] == 7).all(-1).any() and not (out[6:21] == 3).all(-1).any()

@@ -211,8 +211,14 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs P) {
     if (s >= A.nseq) return;  // behind the last sequence
     const SeqAt sq = seq_at(A, s);
     const int i = t - sq.q0, pos = sq.kv - sq.n + i;
-    const int d = P.depth ? P.depth[t] : i, at = pos - i + d;  // the position of the row's angles
-    if (!sq.ok || pos >= A.max_kv || (P.rot && at >= P.npos) || d < 0 || d > i) {
+    int at = pos;  // the position of the row's angles
+    bool ok = sq.ok && pos < A.max_kv;
+    if (P.depth && i >= 0 && i < sq.n) {
+        const int d = P.depth[t];
+        ok = ok && d >= 0 && d <= i;
+        at = pos - i + d;
+    }
+    if (!ok || (P.rot && at >= P.npos)) {
         if (threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
         return;
     }
