@@ -621,7 +621,7 @@ int vgx_paged_copy(vgx_ctx* ctx, int ncache, const vgx_paged* caches, int n, con
  * largest, and a token that this leaves nothing is not drawn.  The result does
  * not depend on the other rows.
  * kind F32, BF16, F16 or Q16; stride in values, any alignment of the type;
- * vocab up to 2^21.  ws: vgx_sample_ws bytes of device memory, as
+ * vocab up to 2^21, nrows up to 65535.  ws: vgx_sample_ws bytes of device memory, as
  * vgx_paged_attn's. */
 typedef struct vgx_sampling {
     int nrows, vocab, kind;

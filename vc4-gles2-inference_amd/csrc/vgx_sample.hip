@@ -1,15 +1,23 @@
 // A token of each row of logits, by temperature, top-k, top-p and min-p.
 //
-// The tokens that stay are the first in a ranking by value and index, so a cut
-// is a place in it: (key, index), the key being the float's bits in an order of
-// integers.  top-k's is found by counting, top-p's by summing weights, in three
-// levels of a radix search; the draw then sums the weights of the tokens that
-// stay in index order.
+// The tokens that stay are the first in a ranking by value and index, so every
+// cut is a place in it, and so is the draw in the order of the indices: the token
+// at which a count or a sum of weights reaches a number.
+//
+// Launch 1 (a workgroup a row and chunk) reads every logit once: the chunk's
+// maximum, the maxima of its groups of 64 logits and, where the row needs it, the
+// sum of its weights.  Launch 2 (a workgroup a row) finds from the groups' maxima
+// a value that enough tokens reach (as many as groups whose maximum does), reads
+// the groups that reach it again and goes on with these tokens alone, a few
+// hundred of tens of thousands: up to 512 compare themselves with each other, up
+// to 4096 are counted into bins first.  Rows of which more stay are searched
+// whole, by bins over the row.
 //
 // Sums that are split at a place the data decides are taken in integers, which
 // have no order: a weight is rounded to a multiple of 2^-q of the largest, q as
 // large as the vocabulary's sum allows (2^-46 for 64402 tokens).  The tokens that
-// stay under top-p < 1 weigh 2^-24 / vocab of the sum or more.
+// stay under top-p < 1 weigh 2^-24 / vocab of the sum or more.  Without a cut the
+// sums are launch 1's, in 64-bit floats.
 #include <algorithm>
 #include <string>
 
@@ -21,6 +29,13 @@ namespace {
 
 typedef unsigned long long u64;
 
+struct Part {
+    float m;   // the chunk's maximum (-inf: nothing)
+    int arg;   // its first index (greedy rows)
+    int n;     // tokens that are not masked (rows without a cut)
+    int pad;
+    double z;  // sum of exp((x - m) / T) (rows that need it)
+};
 struct SampleArgs {
     int nrows, vocab;
     const uint8_t* x;
@@ -34,18 +49,154 @@ struct SampleArgs {
     int* kept;
     float* prob;
     int q;       // weights are multiples of 2^-q
+    Part* part;  // nrows x nch
+    float* gmax; // nrows x ng: the groups' maxima
+    int nch, k;  // chunks of a row; pieces of 16 bytes a thread and chunk
+    int ng;
 };
 
-constexpr int kRow = 1024;    // threads of a row
-constexpr int kBins = 2048;
+constexpr int kThreads = 256;  // of launch 1
+constexpr int kRow = 512;      // of launch 2
+constexpr int kWaves = kRow / 64;
+constexpr int kBins = 1024;
+constexpr int kFew = kRow;     // tokens that compare themselves with each other
+constexpr int kList = 4096;    // tokens gathered from a row
+constexpr int kGroup = 64;     // logits of a group
 constexpr int kMaxVocab = 1 << 21;
+
+// What a row asks for.
+struct Ask {
+    bool greedy, k, p, m;  // which cuts there are
+    int top_k;
+    double inv, top_p, min_p;
+    // the sum of all weights is needed
+    __device__ bool sum() const { return !greedy && !k && (p || !m); }
+    __device__ bool none() const { return !k && !p && !m; }
+};
+__device__ __forceinline__ Ask ask_of(const SampleArgs& P, int r) {
+    const float t = P.temp ? P.temp[r] : 1.0f;
+    const float tp = P.top_p ? P.top_p[r] : 1.0f, mp = P.min_p ? P.min_p[r] : 0.0f;
+    Ask a;
+    a.top_k = P.top_k ? P.top_k[r] : 0;
+    a.greedy = !(t > 0.0f) || a.top_k == 1 || tp <= 0.0f;
+    a.k = a.top_k > 0 && a.top_k < P.vocab;
+    a.p = tp < 1.0f;
+    a.m = mp > 0.0f;
+    a.inv = a.greedy ? 1.0 : fmin(1.0 / (double)t, 1e30);
+    a.top_p = tp;
+    a.min_p = a.m ? fmin((double)mp, 1.0) : 0.0;
+    return a;
+}
+
+// The largest of 16 lanes (rows of 32-bit logits: 16 pieces are a group) or 8.
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float x) {
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));
+    if (LANES == 16) x = fmaxf(x, dpp<0x140>(x));
+    return x;
+}
+
+template <int KIND, int K>
+__global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs P) {
+    constexpr int N = kPer<KIND>, LG = kGroup / N;  // lanes a group
+    __shared__ double tab[64];
+    __shared__ float sm[4];
+    __shared__ int sa[4], sn[4];
+    __shared__ double sz[4];
+    const int chunk = blockIdx.x, r = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const Row q = row_at<KIND>(P.x, P.xs, r);
+    auto first = [&](int k) { return ((chunk * K + k) * kThreads + t) * N - q.off; };
+    auto full = [&](int i0) { return i0 >= 0 && i0 + N <= P.vocab; };
+    uint4 raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        raw[k] = make_uint4(0, 0, 0, 0);
+        if (full(first(k))) raw[k] = *reinterpret_cast<const uint4*>(q.p + (int64_t)first(k) * kBytes<KIND>);
+    }
+    const Ask A = ask_of(P, r);
+    const bool sum = A.sum();
+    if (sum) fill_table(tab);
+    float x[K][N], gm[K];
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        unpack<KIND>(raw[k], x[k]);
+        const int i0 = first(k);
+        if (!full(i0)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                x[k][e] = i0 + e >= 0 && i0 + e < P.vocab ? one<KIND>(q.p, i0 + e) : -INFINITY;
+        }
+        gm[k] = x[k][0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) gm[k] = fmaxf(gm[k], x[k][e]);
+        m = fmaxf(m, gm[k]);
+    }
+    int a = 0x7fffffff;
+    if (A.greedy) {  // the first index of the maximum
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k)
+#pragma unroll
+            for (int e = N - 1; e >= 0; --e)
+                if (x[k][e] == m) a = first(k) + e;
+        wave_best(m, a);
+    } else {
+        m = wave_max(m);
+        if (!A.none()) {
+            float y = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const float g = lanes_max<LG>(gm[k]);
+                if ((lane & (LG - 1)) == k) y = g;
+            }
+            // lane k of a group stores its k-th piece's
+            const int k = lane & (LG - 1);
+            if (k < K) P.gmax[(int64_t)r * P.ng + (chunk * K + k) * (kThreads / LG) + t / LG] = y;
+        }
+    }
+    if (lane == 0) { sm[wave] = m; sa[wave] = a; }
+    __syncthreads();
+    m = sm[0];
+    a = sa[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+        if (sm[w] > m || (sm[w] == m && sa[w] < a)) { m = sm[w]; a = sa[w]; }
+    double z[2] = {0.0, 0.0};
+    int n = 0;
+    if (sum && m != -INFINITY) {
+        const Scale S = scale_of(m, A.inv);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                // (a masked one adds e^-690)
+                z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+                n += x[k][e] != -INFINITY;
+            }
+    }
+    if (sum) {
+        const double w = wave_sum(z[0] + z[1]);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
+        if (lane == 0) { sz[wave] = w; sn[wave] = n; }
+        __syncthreads();
+        z[0] = sz[0] + sz[1] + sz[2] + sz[3];
+        n = sn[0] + sn[1] + sn[2] + sn[3];
+    }
+    if (t == 0) P.part[(int64_t)r * P.nch + chunk] = Part{m, a, n, 0, z[0]};
+}
 
 // The order of floats as unsigned integers (-0 as 0; never 0).
 __device__ __forceinline__ unsigned key_of(float x) {
     const unsigned u = __float_as_uint(x + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// The tokens before a place in the ranking, and the one there.
+__device__ __forceinline__ float value_of(unsigned k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// A place in the ranking: the tokens up to it stay.
 struct Cut {
     unsigned key;
     int idx;
@@ -58,17 +209,32 @@ __device__ __forceinline__ bool stays(const Cut& c, unsigned key, int i) {
 __device__ __forceinline__ u64 fixed(double w, double scale) {
     return __builtin_bit_cast(u64, fma(w, scale, 4503599627370496.0)) - 0x4330000000000000ull;
 }
+__device__ __forceinline__ u64 wave_add(u64 x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
 
 struct RowShared {
     double tab[64];
-    float m[kRow / 64];
-    int a[kRow / 64];
-    unsigned cnt[kBins];
-    u64 sum[kBins];
-    u64 wave[kRow / 64];
-    int bin;
-    u64 above, value;
-    int idx;
+    u64 wave[kWaves];
+    float m[kWaves];
+    int a[kWaves];
+    union {
+        struct {
+            unsigned cnt[kBins];
+            u64 sum[kBins];
+        } h;
+        struct {
+            u64 order[kFew], w[kFew];
+        } few;
+    };
+    unsigned key[kList];
+    int idx[kList];
+    int bin, n, ngroups;
+    unsigned lo, hi;
+    u64 above, total;
+    Cut at;
 };
 
 // The running sum over the workgroup's threads; total: of all.
@@ -84,219 +250,538 @@ __device__ __forceinline__ u64 block_scan(u64 x, u64* sm, u64& total) {
     __syncthreads();
     u64 before = 0;
     total = 0;
-    for (int w = 0; w < kRow / 64; ++w) {
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
         if (w < wave) before += sm[w];
         total += sm[w];
     }
     return x + before;
 }
 
+// A row's piece g as it lies in memory; values outside the row are 0.
 template <int KIND>
-struct RowOf {
-    static constexpr int N = kPer<KIND>;
-    const SampleArgs& P;
-    RowShared& H;
-    Row q;
-    int slabs;     // of kRow pieces
-    Scale S;
-    double scale;  // 2^q
-    __device__ __forceinline__ RowOf(const SampleArgs& P_, RowShared& H_, int r)
-        : P(P_), H(H_), q(row_at<KIND>(P_.x, P_.xs, r)), S{}, scale(__longlong_as_double((long long)(1023 + P_.q) << 52)) {
-        slabs = (P.vocab + q.off + kRow * N - 1) / (kRow * N);
-    }
-    // f(x, index) of every token of a slab that is not masked
-    template <class F>
-    __device__ __forceinline__ void slab(int k, F f) const {
-        const int g = k * kRow + (int)threadIdx.x;
-        float x[N];
-        piece<KIND>(q, P.vocab, g, x);
+__device__ __forceinline__ uint4 raw_piece(const Row& q, int vocab, int g) {
+    constexpr int N = kPer<KIND>;
+    const int i0 = g * N - q.off;
+    if (i0 >= 0 && i0 + N <= vocab) return *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * kBytes<KIND>);
+    unsigned u[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (x[e] != -INFINITY) f(x[e], g * N - q.off + e);
-    }
-    __device__ __forceinline__ u64 weigh(float x) const { return fixed(weight(x, S, H.tab), scale); }
-
-    // The index of the n-th token (1 ..) of a value, inside a cut.
-    __device__ int nth(unsigned key, const Cut& in, u64 n) const {
-        u64 before = 0;
-        for (int k = 0; k < slabs; ++k) {
-            u64 c = 0;
-            slab(k, [&](float x, int i) {
-                const unsigned y = key_of(x);
-                c += y == key && stays(in, y, i);
-            });
-            u64 total;
-            const u64 run = before + block_scan(c, H.wave, total);
-            if (run >= n && run - c < n) {
-                u64 left = n - (run - c);
-                slab(k, [&](float x, int i) {
-                    const unsigned y = key_of(x);
-                    if (y == key && stays(in, y, i) && --left == 0) H.idx = i;
-                });
-            }
-            before += total;
-            if (before >= n) break;
+    for (int e = 0; e < N; ++e)
+        if (i0 + e >= 0 && i0 + e < vocab) {
+            if (KIND == VGX_E_F32) u[e] = reinterpret_cast<const unsigned*>(q.p)[i0 + e];
+            else u[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(q.p)[i0 + e] << 16 * (e & 1);
         }
-        __syncthreads();
-        const int r = H.idx;
-        __syncthreads();
-        return r;
-    }
-
-    // The cut after `want` tokens of those inside `in`, or (WEIGHTED) after the
-    // token at which the sum of weights reaches top_p of theirs.
-    template <bool WEIGHTED>
-    __device__ Cut select(const Cut& in, u64 want, double top_p) const {
-        u64 before = 0, value = 0;
-        unsigned prefix = 0;
-        const int t = threadIdx.x;
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+// f(value, index) of a piece's values inside the row, one after the other: a loop
+// that shifts them down, as many copies of a long f would not stay in the
+// instruction cache.
+template <int KIND, class F>
+__device__ __forceinline__ void each_of(uint4 v, int i0, int vocab, F f) {
+    constexpr int N = kPer<KIND>;
 #pragma unroll 1
-        for (int level = 0; level < 3; ++level) {
-            const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-            for (int i = t; i < kBins; i += kRow) { H.cnt[i] = 0; H.sum[i] = 0; }
-            if (t == 0) H.bin = -1;
-            __syncthreads();
-            for (int k = 0; k < slabs; ++k)
-                slab(k, [&](float x, int i) {
-                    const unsigned y = key_of(x);
-                    if (!stays(in, y, i) || (level && y >> (shift + bits) != prefix)) return;
-                    const int b = y >> shift & ((1 << bits) - 1);
-                    atomicAdd(&H.cnt[b], 1u);
-                    if (WEIGHTED) {
-                        const u64 w = weigh(x);
-                        if (w) atomicAdd(&H.sum[b], w);
-                    }
-                });
-            __syncthreads();
-            // bins from the largest down, two a thread
-            const int b0 = kBins - 1 - 2 * t;
-            const u64 v0 = WEIGHTED ? H.sum[b0] : H.cnt[b0], v1 = WEIGHTED ? H.sum[b0 - 1] : H.cnt[b0 - 1];
-            u64 total;
-            const u64 run = block_scan(v0 + v1, H.wave, total), at = before + run - v0 - v1;
-            if (WEIGHTED && level == 0) {
-                const double y = ceil(top_p * (double)total);
-                want = y < 1.0 ? 1 : (u64)y;
-            }
-            if (at < want && want <= before + run) {
-                const bool low = want > at + v0;
-                H.bin = low ? b0 - 1 : b0;
-                H.above = low ? at + v0 : at;
-                H.value = low ? v1 : v0;
-            }
-            __syncthreads();
-            const int bin = H.bin;
-            if (bin < 0) return in;  // fewer tokens than that
-            before = H.above;
-            value = H.value;
-            prefix = prefix << bits | (unsigned)bin;
-            if (level < 2) __syncthreads();
+    for (int e = 0; e < N; ++e) {
+        float x;
+        if (KIND == VGX_E_F32) x = clean(__uint_as_float(v.x));
+        else if (KIND == VGX_E_Q16) x = (float)(short)(v.x & 0xffff) * (1.0f / 256);
+        else if (KIND == VGX_E_BF16) x = clean(__uint_as_float(v.x << 16));
+        else x = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(v.x & 0xffff)));
+        if (i0 + e >= 0 && i0 + e < vocab) f(x, i0 + e);
+        if (KIND == VGX_E_F32) {
+            v.x = v.y; v.y = v.z; v.z = v.w;
+        } else {
+            v.x = v.y << 16 | v.x >> 16;
+            v.y = v.z << 16 | v.y >> 16;
+            v.z = v.w << 16 | v.z >> 16;
+            v.w >>= 16;
         }
-        const u64 ties = H.cnt[prefix & 1023];
-        __syncthreads();
-        u64 n = want - before;
-        if (WEIGHTED) {
-            const u64 w = value / ties;  // (equal ones)
-            n = (n + w - 1) / w;
+    }
+}
+// The tokens of a row (f(key, index) of each that is not masked) ...
+template <int KIND>
+struct WholeRow {
+    const SampleArgs& P;
+    Row q;
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        constexpr int N = kPer<KIND>;
+        const int pieces = (P.vocab + q.off + N - 1) / N;
+        int g = threadIdx.x;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (g < pieces) v = raw_piece<KIND>(q, P.vocab, g);
+        while (g < pieces) {
+            uint4 next = v;
+            if (g + kRow < pieces) next = raw_piece<KIND>(q, P.vocab, g + kRow);
+            each_of<KIND>(v, g * N - q.off, P.vocab, [&](float x, int i) {
+                if (x != -INFINITY) f(key_of(x), i);
+            });
+            v = next;
+            g += kRow;
         }
-        if (n >= ties) return Cut{prefix, prefix == in.key ? in.idx : 0x7fffffff};
-        return Cut{prefix, nth(prefix, in, n)};
+    }
+};
+// ... or those gathered from it.
+struct Gathered {
+    const RowShared& H;
+    int n;
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int i = threadIdx.x; i < n; i += kRow) f(H.key[i], H.idx[i]);
     }
 };
 
+// The tokens that stay inside a cut, with their weights.
+struct Weigh {
+    Scale S;
+    double scale, least;
+    const double* tab;
+    __device__ __forceinline__ double real(unsigned key) const { return weight(value_of(key), S, tab); }
+    __device__ __forceinline__ u64 operator()(unsigned key) const {
+        const double w = real(key);
+        return w < least ? 0 : fixed(w, scale);
+    }
+};
+
+// The token at which the tokens inside `in`, in the ranking's order or (BY_INDEX)
+// that of their indices, reach `want` (of their total, once that is known): of
+// tokens, or of weights (WEIGHTED).  False: they do not.  Bins over the values
+// first (floats' keys spread over them badly), then over the keys of the bin that
+// holds the place, then over the indices of one key, until few are left.
+template <bool WEIGHTED, bool BY_INDEX, class Source, class Want>
+__device__ __forceinline__ bool locate(RowShared& H, const Source& src, const Weigh& W, const Cut& in, float m, float range, int vocab,
+                       Want want_of) {
+    const int t = threadIdx.x;
+    const float step = (float)(kBins - 1) / range;
+    enum { VALUE, KEY, INDEX };
+    int mode = BY_INDEX ? INDEX : VALUE;
+    unsigned lo = BY_INDEX ? ~(unsigned)(vocab - 1) : 0, hi = ~0u, eq = 0;  // (INDEX: of the indices' complements)
+    u64 before = 0, want = 0;
+#pragma unroll 1
+    for (bool first = true;; first = false) {
+        const int sh = mode == VALUE ? 0 : max(0, 32 - __clz((int)(hi - lo)) - 10);
+        auto bin_of = [&](unsigned key, int i) -> int {
+            if (!stays(in, key, i)) return -1;
+            if (mode == VALUE) return kBins - 1 - (int)fminf((m - value_of(key)) * step, (float)(kBins - 1));
+            if (mode == INDEX && !BY_INDEX && key != eq) return -1;
+            const unsigned o = mode == KEY ? key : ~(unsigned)i;
+            return o < lo || o > hi ? -1 : (int)((o - lo) >> sh);
+        };
+        __syncthreads();
+        for (int i = t; i < kBins; i += kRow) { H.h.cnt[i] = 0; H.h.sum[i] = 0; }
+        if (t == 0) { H.bin = -1; H.n = 0; H.lo = ~0u; H.hi = 0; }
+        __syncthreads();
+        src.each([&](unsigned key, int i) {
+            const int b = bin_of(key, i);
+            if (b < 0) return;
+            if (WEIGHTED) {
+                const u64 w = W(key);
+                if (w) atomicAdd(&H.h.sum[b], w);
+            }
+            atomicAdd(&H.h.cnt[b], 1u);
+        });
+        __syncthreads();
+        const int b0 = kBins - 1 - 2 * t;
+        const unsigned c0 = H.h.cnt[b0], c1 = H.h.cnt[b0 - 1];
+        const u64 v0 = WEIGHTED ? H.h.sum[b0] : c0, v1 = WEIGHTED ? H.h.sum[b0 - 1] : c1;
+        u64 total;
+        const u64 run = block_scan(v0 + v1, H.wave, total), at = before + run - v0 - v1;
+        if (first) want = want_of(total);
+        if (at < want && want <= before + run) {
+            const bool low = want > at + v0;
+            H.bin = low ? b0 - 1 : b0;
+            H.above = low ? at + v0 : at;
+            H.total = low ? c1 : c0;
+        }
+        __syncthreads();
+        const int bin = H.bin;
+        if (bin < 0) return false;
+        before = H.above;
+        const int c = (int)H.total;
+        if (c <= kFew) {
+            __syncthreads();  // (the bins' memory is used again)
+            src.each([&](unsigned key, int i) {
+                if (bin_of(key, i) != bin) return;
+                const int at = atomicAdd(&H.n, 1);
+                H.few.order[at] = BY_INDEX ? (u64)(unsigned)i << 32 | key : (u64)~key << 32 | (unsigned)i;
+                H.few.w[at] = WEIGHTED ? W(key) : 1;
+            });
+            __syncthreads();
+            const u64 mine = t < c ? H.few.order[t] : 0, w = t < c ? H.few.w[t] : 0;
+            u64 s = before;
+            if (t < c)
+                for (int j = 0; j < c; ++j)
+                    if (H.few.order[j] < mine) s += H.few.w[j];
+            if (t < c && s < want && want <= s + w)
+                H.at = BY_INDEX ? Cut{(unsigned)mine, (int)(mine >> 32)} : Cut{~(unsigned)(mine >> 32), (int)(unsigned)mine};
+            __syncthreads();
+            return true;
+        }
+        if (mode == VALUE) {  // the keys of the bin
+            unsigned a = ~0u, b = 0;
+            src.each([&](unsigned key, int i) {
+                if (bin_of(key, i) != bin) return;
+                a = min(a, key);
+                b = max(b, key);
+            });
+            if (a <= b) { atomicMin(&H.lo, a); atomicMax(&H.hi, b); }
+            __syncthreads();
+            lo = H.lo;
+            hi = H.hi;
+            mode = KEY;
+        } else {
+            lo += (unsigned)bin << sh;
+            hi = min(hi, lo + ((1u << sh) - 1));
+        }
+        if (mode == KEY && lo == hi) {  // equal values: by their indices
+            eq = lo;
+            mode = INDEX;
+            lo = ~(unsigned)(vocab - 1);
+            hi = ~0u;
+        }
+    }
+}
+
+// The cuts and the draw over a source that holds all that may stay.  z: the sum
+// of all weights, negative where the source holds them all.
+template <class Source>
+__device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, const Source& src, int r, const Ask& A, Weigh W, float m,
+                             double z) {
+    const int t = threadIdx.x;
+    const double least = W.least;
+    W.least = 0.0;
+    Cut cut{0, 0x7fffffff};
+    // weights below 2^-q are 0
+    const float range = (float)fmin((double)(P.q + 1) * 0.7 / A.inv, 1e30);
+    if (A.k && locate<false, false>(H, src, W, cut, m, range, P.vocab, [&](u64) { return (u64)A.top_k; })) cut = H.at;
+    if (A.p) {
+        const bool some = locate<true, false>(H, src, W, cut, m, range, P.vocab, [&](u64 total) {
+            const double y = ceil(A.top_p * (A.k || z < 0.0 ? (double)total : z * W.scale));
+            return y < 1.0 ? 1ull : (u64)y;
+        });
+        if (some) cut = H.at;
+    }
+    __syncthreads();
+    W.least = least;
+    const double u = P.u[r];
+    // how many stay
+    unsigned n = 0;
+    if (t == 0) H.ngroups = 0;
+    __syncthreads();
+    src.each([&](unsigned key, int i) { n += stays(cut, key, i) && (least == 0.0 || W.real(key) >= least); });
+    n = (unsigned)wave_add(n);
+    if ((t & 63) == 0 && n) atomicAdd(&H.ngroups, (int)n);
+    u64 sum = 0;
+    // (a draw of 1 or more, or no number, takes the last token)
+    locate<true, true>(H, src, W, cut, m, range, P.vocab, [&](u64 total) {
+        sum = total;
+        return u >= 0.0 && u < 1.0 ? min((u64)(u * (double)total), total - 1) + 1 : u < 0.0 ? 1ull : total;
+    });
+    if (t == 0) {
+        P.token[r] = H.at.idx;
+        if (P.kept) P.kept[r] = H.ngroups;
+        if (P.prob) P.prob[r] = (float)(W.real(H.at.key) / ((double)sum / W.scale));
+    }
+}
+
+// The same for up to kRow gathered tokens, each with its thread: its rank and the
+// weights before it by comparing with all others, then the weights of those that
+// stay with a lower index.
+__device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared& H, int n, int r, const Ask& A, const Weigh& W, double z) {
+    const int t = threadIdx.x;
+    const bool in = t < n;
+    const unsigned key = in ? H.key[t] : 0;
+    const int idx = in ? H.idx[t] : 0;
+    const u64 mine = (u64)~key << 32 | (unsigned)idx;
+    const double real = in ? W.real(key) : 0.0;
+    u64 w = in ? fixed(real, W.scale) : 0;
+    H.few.order[t] = in ? mine : ~0ull;
+    H.few.w[t] = w;
+    __syncthreads();
+    u64 before = 0;
+    int rank = 0;
+    if (in)
+        for (int j = 0; j < n; ++j)
+            if (H.few.order[j] < mine) { ++rank; before += H.few.w[j]; }
+    bool stay = in && (!A.k || rank < A.top_k);
+    u64 total;
+    if (A.p) {
+        double all = z * W.scale;
+        if (A.k) {
+            block_scan(stay ? w : 0, H.wave, total);
+            all = (double)total;
+        }
+        const double y = ceil(A.top_p * all);
+        stay = stay && before < (y < 1.0 ? 1ull : (u64)y);
+    }
+    stay = stay && real >= W.least;
+    if (!stay) w = 0;
+    block_scan(w, H.wave, total);
+    const u64 sum = total;
+    block_scan(stay, H.wave, total);
+    H.few.order[t] = stay ? (u64)(unsigned)idx : ~0ull;
+    H.few.w[t] = w;
+    __syncthreads();
+    u64 c = 0;
+    if (stay)
+        for (int j = 0; j < n; ++j)
+            if (H.few.order[j] < (u64)(unsigned)idx) c += H.few.w[j];
+    const double u = P.u[r];
+    const u64 want = u >= 0.0 && u < 1.0 ? min((u64)(u * (double)sum), sum - 1) : u < 0.0 ? 0 : sum - 1;
+    if (stay && c <= want && want < c + w) {
+        P.token[r] = idx;
+        if (P.kept) P.kept[r] = (int)total;
+        if (P.prob) P.prob[r] = (float)(real / ((double)sum / W.scale));
+    }
+}
+
+// A draw without a cut: the chunk from launch 1's sums, the token in it from its
+// weights.
 template <int KIND>
-__global__ void __launch_bounds__(kRow) sample_kernel(const SampleArgs P) {
+__device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int r, const Row& q, const Ask& A, const Scale& S) {
+    constexpr int N = kPer<KIND>;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    __shared__ int chosen, found, last, kept;
+    __shared__ double left, sum, sw[kWaves];
+    __shared__ float lx;
+    const Part* part = P.part + (int64_t)r * P.nch;
+    if (wave == 0) {
+        auto sum_of = [&](int c) { return c < P.nch ? part[c].z * weight(part[c].m, S, H.tab) : 0.0; };
+        double total = 0.0;
+        int n = 0;
+        for (int c = lane; c < P.nch; c += 64) {
+            total += sum_of(c);
+            n += part[c].n;
+        }
+        total = wave_sum(total);
+        n = (int)wave_add((unsigned)n);
+        const double un = P.u[r];
+        const double want = un >= 0.0 ? un * total : un < 0.0 ? 0.0 : total;
+        double before = 0.0, at = 0.0, some_at = 0.0;
+        int pick = -1, some = -1;
+        for (int c = 0; c < P.nch && pick < 0; c += 64) {
+            const double v = sum_of(c + lane), run = wave_scan(v);
+            const u64 past = __ballot(before + run > want && v > 0.0), any = __ballot(v > 0.0);
+            if (past) {
+                const int l = __ffsll(past) - 1;
+                pick = c + l;
+                at = before + lane_of(run, l) - lane_of(v, l);
+            } else if (any) {
+                const int l = 63 - __clzll((long long)any);
+                some = c + l;
+                some_at = before + lane_of(run, l) - lane_of(v, l);
+            }
+            before += lane_of(run, 63);
+        }
+        if (lane == 0) {
+            chosen = pick >= 0 ? pick : some;
+            left = fmax(want - (pick >= 0 ? at : some_at), 0.0);
+            sum = total;
+            kept = n;
+            found = 0x7fffffff;
+            last = -1;
+        }
+    }
+    __syncthreads();
+    // the chunk's pieces, consecutive ones of a thread
+    const int pieces = P.k * kThreads, per = (pieces + kRow - 1) / kRow;
+    double s = 0.0;
+    int mine = -1;
+    float lastx = 0.0f;
+    auto each = [&](auto f) {
+        for (int k = 0; k < per; ++k) {
+            const int j = t * per + k;
+            if (j >= pieces) break;
+            const int g = chosen * pieces + j;
+            each_of<KIND>(raw_piece<KIND>(q, P.vocab, g), g * N - q.off, P.vocab,
+                          [&](float x, int i) { f(x, i, weight(x, S, H.tab)); });
+        }
+    };
+    each([&](float x, int i, double w) {
+        s += w;
+        if (w > 0.0) { mine = i; lastx = x; }
+    });
+    const double run = wave_scan(s);
+    if (lane == 63) sw[wave] = run;
+    if (mine >= 0) atomicMax(&last, mine);
+    __syncthreads();
+    // (as the draft check takes it: only a thread with a weight, and of several
+    // waves the first)
+    double before = __shfl_up(run, 1, 64);
+    if (lane == 0) before = 0.0;
+    double base = 0.0;
+    for (int v = 0; v < wave; ++v) base += sw[v];
+    before += base;
+    const u64 past = __ballot(mine >= 0 && base + run > left);
+    int hit = -1;
+    float hx = 0.0f;
+    if (past && lane == __ffsll(past) - 1) {
+        double c = before;
+        each([&](float x, int i, double w) {
+            c += w;
+            if (hit < 0 && c > left && w > 0.0) { hit = i; hx = x; }
+        });
+        if (hit < 0) { hit = mine; hx = lastx; }
+        atomicMin(&found, hit);
+    }
+    __syncthreads();
+    const int token = found != 0x7fffffff ? found : last;
+    if (hit == token) lx = hx;
+    else if (found == 0x7fffffff && mine == token) lx = lastx;
+    __syncthreads();
+    if (t == 0) {
+        P.token[r] = token;
+        if (P.kept) P.kept[r] = kept;
+        if (P.prob) P.prob[r] = (float)(weight(lx, S, H.tab) / sum);
+    }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
+    constexpr int N = kPer<KIND>, LG = kGroup / N;
     __shared__ RowShared H;
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    RowOf<KIND> R(P, H, r);
-    fill_table(H.tab);
+    const Row q = row_at<KIND>(P.x, P.xs, r);
+    const Part* part = P.part + (int64_t)r * P.nch;
+    const float* gmax = P.gmax + (int64_t)r * P.ng;
+    const Ask A = ask_of(P, r);
     float m = -INFINITY;
     int a = 0x7fffffff;
-    for (int k = 0; k < R.slabs; ++k)
-        R.slab(k, [&](float x, int i) {
-            if (x > m) { m = x; a = i; }
-        });
-    wave_best(m, a);
+    for (int c = t; c < P.nch; c += kRow)
+        if (part[c].m > m || (part[c].m == m && part[c].arg < a)) { m = part[c].m; a = part[c].arg; }
+    fill_table(H.tab);
+    if (A.greedy) wave_best(m, a);
+    else m = wave_max(m);
     if (lane == 0) { H.m[wave] = m; H.a[wave] = a; }
     __syncthreads();
     m = H.m[0];
     a = H.a[0];
-    for (int w = 1; w < kRow / 64; ++w)
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w)
         if (H.m[w] > m || (H.m[w] == m && H.a[w] < a)) { m = H.m[w]; a = H.a[w]; }
-    const float T = P.temp ? P.temp[r] : 1.0f;
-    const int top_k = P.top_k ? P.top_k[r] : 0;
-    const float top_p = P.top_p ? P.top_p[r] : 1.0f;
-    const float min_p = P.min_p ? P.min_p[r] : 0.0f;
-    const bool none = m == -INFINITY;
-    if (none || !(T > 0.0f) || top_k == 1 || top_p <= 0.0f) {
+    const bool nothing = m == -INFINITY;
+    if (nothing || A.greedy) {
         if (t == 0) {
-            P.token[r] = none ? -1 : a;
-            if (P.kept) P.kept[r] = !none;
-            if (P.prob) P.prob[r] = none ? 0.0f : 1.0f;
+            P.token[r] = nothing ? -1 : a;
+            if (P.kept) P.kept[r] = !nothing;
+            if (P.prob) P.prob[r] = nothing ? 0.0f : 1.0f;
         }
         return;
     }
-    R.S = scale_of(m, fmin(1.0 / (double)T, 1e30));
-    Cut cut{0, 0x7fffffff};
-    if (top_k > 0 && top_k < P.vocab) cut = R.template select<false>(cut, (u64)top_k, 0.0);
-    if (top_p < 1.0f) cut = R.template select<true>(cut, 0, (double)top_p);
-    const double least = min_p > 0.0f ? fmin((double)min_p, 1.0) : 0.0;
-    // the slabs' sums, and how many tokens stay
-    __shared__ u64 part[kMaxVocab / (kRow * 4) + 2];
-    __shared__ unsigned kept;
-    __shared__ int pick, last, found;
-    __shared__ u64 left;
-    __shared__ float lx;
-    for (int k = t; k < R.slabs; k += kRow) part[k] = 0;
-    if (t == 0) { kept = 0; found = 0x7fffffff; last = -1; }
-    __syncthreads();
-    unsigned n = 0;
-    for (int k = 0; k < R.slabs; ++k) {
-        u64 s = 0;
-        R.slab(k, [&](float x, int i) {
-            if (!stays(cut, key_of(x), i)) return;
-            const double w = weight(x, R.S, H.tab);
-            if (w < least) return;
-            ++n;
-            s += fixed(w, R.scale);
-        });
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
-        if (lane == 0 && s) atomicAdd(&part[k], s);
+    const Scale S = scale_of(m, A.inv);
+    if (A.none()) return draw_all<KIND>(P, H, r, q, A, S);
+    const Weigh W{S, __longlong_as_double((long long)(1023 + P.q) << 52), A.min_p, H.tab};
+    double z = 0.0;
+    if (A.sum()) {  // (one wave's order for every thread)
+        for (int c = lane; c < P.nch; c += 64) z += part[c].z * weight(part[c].m, S, H.tab);
+        z = wave_sum(z);
     }
+    // A value that min-p's tokens reach, a rounding below its border.
+    float floor_m = -INFINITY;
+    if (A.m && !A.k && A.inv > 0.0)
+        floor_m = (float)((double)m + log(A.min_p) / A.inv) - 1e-5f * (fabsf(m) + (float)(1.0 / A.inv));
+    // Groups by their maxima: bins of the distance from the row's.
+    float low = INFINITY;
+    for (int g = t; g < P.ng; g += kRow)
+        if (gmax[g] != -INFINITY) low = fminf(low, gmax[g]);
+    low = -wave_max(-low);
+    if (lane == 0) H.m[wave] = low;
+    for (int i = t; i < kBins; i += kRow) H.h.cnt[i] = 0;
+    __syncthreads();
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
-    if (lane == 0 && n) atomicAdd(&kept, n);
+    for (int w = 0; w < kWaves; ++w) low = fminf(low, H.m[w]);
+    const float step = (float)(kBins - 1) / fmaxf(m - low, 1e-30f);
+    auto bin_of = [&](float x) { return (int)fminf((m - x) * step, (float)(kBins - 1)); };
+    for (int g = t; g < P.ng; g += kRow)
+        if (gmax[g] != -INFINITY) atomicAdd(&H.h.cnt[bin_of(gmax[g])], 1u);
     __syncthreads();
-    u64 sum = 0;
-    for (int k = 0; k < R.slabs; ++k) sum += part[k];
-    // (a draw of 1 or more, or no number, takes the last token)
-    const double u = P.u[r];
-    const u64 want = u >= 0.0 && u < 1.0 ? min((u64)(u * (double)sum), sum - 1) : u < 0.0 ? 0 : sum - 1;
-    u64 before = 0;
-    int k = 0;
-    while (before + part[k] <= want) before += part[k++];
-    u64 s = 0;
-    auto each = [&](auto f) {
-        R.slab(k, [&](float x, int i) {
-            if (!stays(cut, key_of(x), i)) return;
-            const double w = weight(x, R.S, H.tab);
-            if (w >= least) f(x, i, fixed(w, R.scale));
-        });
-    };
-    each([&](float, int, u64 w) { s += w; });
-    u64 total;
-    u64 run = before + block_scan(s, H.wave, total) - s;
-    if (run <= want && want < run + s)
-        each([&](float x, int i, u64 w) {
-            if (run <= want && want < run + w) { found = i; lx = x; }
-            run += w;
-        });
-    __syncthreads();
-    if (t == 0) {
-        P.token[r] = found;
-        if (P.kept) P.kept[r] = (int)kept;
-        if (P.prob) P.prob[r] = (float)(weight(lx, R.S, H.tab) / ((double)sum / R.scale));
+    u64 groups;
+    const unsigned c0 = H.h.cnt[2 * t], c1 = H.h.cnt[2 * t + 1];
+    const u64 run = block_scan(c0 + c1, H.wave, groups);
+    // Tokens wanted: top-k's at the least; for top-p 64, and where their weights
+    // do not reach it 512.
+    u64 want = A.k ? (u64)A.top_k : A.p ? 64 : groups;
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+        if (want > groups) {
+            if (A.k && P.vocab > kList) break;  // (the groups' maxima do not bound that many)
+            want = groups;
+        }
+        __syncthreads();
+        if (t == 0) { H.n = 0; H.ngroups = 0; }
+        if (run >= want && run - c0 - c1 < want) H.bin = run - c1 >= want ? 2 * t : 2 * t + 1;
+        __syncthreads();
+        const int last = H.bin;  // tokens in bins up to it
+        const bool all = want == groups;
+        auto in = [&](float x) { return x >= floor_m && (all || bin_of(x) <= last); };
+        // the groups, into the list's memory, then their tokens
+        __syncthreads();
+        for (int g = t; g < P.ng; g += kRow)
+            if (gmax[g] != -INFINITY && in(gmax[g])) {
+                const int at = atomicAdd(&H.ngroups, 1);
+                if (at < 4 * kFew) reinterpret_cast<int*>(&H.few)[at] = g;
+            }
+        __syncthreads();
+        const int ngr = H.ngroups;
+        if (ngr > 4 * kFew) break;
+        for (int j = t; j < ngr * LG; j += kRow) {
+            const int g = reinterpret_cast<int*>(&H.few)[j / LG] * LG + j % LG;
+            float x[N];
+            piece<KIND>(q, P.vocab, g, x);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (x[e] != -INFINITY && in(x[e])) {
+                    const int at = atomicAdd(&H.n, 1);
+                    if (at < kList) {
+                        H.key[at] = key_of(x[e]);
+                        H.idx[at] = g * N - q.off + e;
+                    }
+                }
+        }
+        __syncthreads();
+        const int n = H.n;
+        if (n > kList) break;
+        bool enough = A.k || !A.p || all;
+        if (!enough) {
+            u64 s = 0, total;
+            for (int i = t; i < n; i += kRow) s += fixed(W.real(H.key[i]), W.scale);
+            block_scan(s, H.wave, total);
+            // (what is below min-p's border is not missing)
+            enough = (double)total >= A.top_p * z * W.scale + 1.0 || (floor_m > -INFINITY && bin_of(floor_m) <= last);
+        }
+        if (enough) {
+            if (n <= kFew) cut_and_draw_few(P, H, n, r, A, W, z);
+            else cut_and_draw(P, H, Gathered{H, n}, r, A, W, m, z);
+            return;
+        }
+        want = 512;
     }
+    __syncthreads();
+    cut_and_draw(P, H, WholeRow<KIND>{P, q}, r, A, W, m, -1.0);
+}
+
+// Pieces a thread and chunk (K) and chunks of a row; chunks of 256 pieces while
+// they are 1024 or fewer.
+struct Chunks {
+    int k, nch, ng;
+};
+Chunks chunks_of(int nrows, int vocab, int kind) {
+    const int per = kind == VGX_E_F32 ? 4 : 8;
+    Chunks c;
+    c.k = 1;
+    c.nch = (vocab + per - 1 + per * kThreads - 1) / (per * kThreads);
+    if ((int64_t)nrows * c.nch > 1024) {
+        c.k = 4;
+        c.nch = (vocab + per - 1 + per * kThreads * 4 - 1) / (per * kThreads * 4);
+    }
+    c.ng = c.nch * c.k * kThreads * per / kGroup;
+    return c;
+}
+
+template <int KIND>
+void launch(const SampleArgs& P, hipStream_t st) {
+    hipLaunchKernelGGL((P.k == 1 ? sample_stats_kernel<KIND, 1> : sample_stats_kernel<KIND, 4>), dim3(P.nch, P.nrows),
+                       dim3(kThreads), 0, st, P);
+    hipLaunchKernelGGL(sample_pick_kernel<KIND>, dim3(P.nrows), dim3(kRow), 0, st, P);
 }
 
 bool kind_ok(int k) { return k == VGX_E_F32 || k == VGX_E_BF16 || k == VGX_E_F16 || k == VGX_E_Q16; }
@@ -305,12 +790,16 @@ bool kind_ok(int k) { return k == VGX_E_F32 || k == VGX_E_BF16 || k == VGX_E_F16
 
 extern "C" {
 
-size_t vgx_sample_ws(int nrows, int vocab, int kind) { return 0; }
+size_t vgx_sample_ws(int nrows, int vocab, int kind) {
+    if (nrows < 0 || vocab <= 0 || vocab > kMaxVocab || !kind_ok(kind)) return 0;
+    const Chunks c = chunks_of(nrows, vocab, kind);
+    return (size_t)nrows * (c.nch * sizeof(Part) + c.ng * sizeof(float));
+}
 
 int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
     auto fail = [](int status, const char* what) { return vgx_fail(status, std::string("vgx_sample: ") + what); };
     if (!a) return fail(VGX_EINVAL, "NULL arguments");
-    if (a->nrows < 0 || a->nrows > (1 << 20)) return fail(VGX_EINVAL, "nrows outside 0..2^20");
+    if (a->nrows < 0 || a->nrows > 65535) return fail(VGX_EINVAL, "nrows outside 0..65535");
     if (a->vocab <= 0 || a->vocab > kMaxVocab) return fail(VGX_EINVAL, "vocab outside 1..2^21");
     if (!kind_ok(a->kind)) return fail(VGX_EINVAL, "logits are f32, bf16, f16 or q16");
     if (a->nrows && (!a->logits || !a->u || !a->token)) return fail(VGX_EINVAL, "NULL logits, u or token");
@@ -320,6 +809,8 @@ int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
     const size_t need = vgx_sample_ws(a->nrows, a->vocab, a->kind);
     if (need && (!a->ws || a->ws_bytes < need || ((uintptr_t)a->ws & 15)))
         return fail(VGX_EINVAL, "the workspace is missing, too small or not 16-byte aligned");
+    const Chunks c = chunks_of(a->nrows, a->vocab, a->kind);
+    if ((int64_t)c.nch * a->nrows >= (1 << 24)) return fail(VGX_ERANGE, "too many logits for one call");  // 2^32 threads
     if (!ctx) return fail(VGX_EINVAL, "no context");
     if (a->nrows == 0) return VGX_OK;
     SampleArgs P{};
@@ -332,12 +823,16 @@ int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
     int lg = 0;
     while ((1 << lg) < a->vocab) ++lg;
     P.q = std::min(50, 62 - lg);
+    P.nch = c.nch; P.k = c.k; P.ng = c.ng;
+    P.part = static_cast<Part*>(a->ws);
+    P.gmax = reinterpret_cast<float*>(P.part + (size_t)a->nrows * c.nch);
     VGX_HIP(hipSetDevice(ctx->device));
-    void (*fn)(const SampleArgs) = a->kind == VGX_E_F32    ? sample_kernel<VGX_E_F32>
-                                   : a->kind == VGX_E_BF16 ? sample_kernel<VGX_E_BF16>
-                                   : a->kind == VGX_E_F16  ? sample_kernel<VGX_E_F16>
-                                                           : sample_kernel<VGX_E_Q16>;
-    hipLaunchKernelGGL(fn, dim3(a->nrows), dim3(kRow), 0, ctx->stream, P);
+    switch (a->kind) {
+        case VGX_E_F32: launch<VGX_E_F32>(P, ctx->stream); break;
+        case VGX_E_BF16: launch<VGX_E_BF16>(P, ctx->stream); break;
+        case VGX_E_F16: launch<VGX_E_F16>(P, ctx->stream); break;
+        default: launch<VGX_E_Q16>(P, ctx->stream); break;
+    }
     VGX_LAUNCH_CHECK("sample launch");
     return VGX_OK;
 }
