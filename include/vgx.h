@@ -618,8 +618,8 @@ int vgx_paged_copy(vgx_ctx* ctx, int ncache, const vgx_paged* caches, int n, con
  * counts as it, +infinity as the largest float; a row without a token gives
  * -1, 0 and 0.  Weights and sums have 64 bits; where many tokens stay, weights
  * are rounded to a multiple of 2^-41 (vocabularies up to 2^17: 2^-45) of the
- * largest, and a token that this leaves nothing is not drawn.  The result does
- * not depend on the other rows.
+ * largest, and a token that this leaves nothing is not drawn.  A row's result
+ * does not depend on the others, but for the rounding of sums.
  * kind F32, BF16, F16 or Q16; stride in values, any alignment of the type;
  * vocab up to 2^21, nrows up to 65535.  ws: vgx_sample_ws bytes of device memory, as
  * vgx_paged_attn's. */

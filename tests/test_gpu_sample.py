@@ -226,3 +226,29 @@ def test_graph_and_streams(gpu):
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(a, g.sample(y, u, top_p=top_p)))
     g.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows, vocab", [(1, 30011), (40, 64402), (5, 400009)])
+def test_thousands_stay(gpu, kind, rows, vocab):
+    """Rows without a peak, by top-p alone: what stays is past what is gathered."""
+    x, u = rows_of(15, rows, vocab, kind, spread=2.0, top=9.0, pad=1)
+    p = [[0.9, 0.5, 0.99, 0.999, 0.7][i % 5] for i in range(rows)]
+    t = [[1.0, 1.5, 2.0, 1.3, 0.9, 4.0, 1e3][i % 7] for i in range(rows)]
+    kept = check(gpu, x, u, temp=t, top_p=p)[1]
+    assert int(kept.max()) > 4096
+    check(gpu, x, u, temp=t, min_p=[1e-4] * rows)
+    check(gpu, x, u, temp=t, top_p=p, min_p=[1e-6] * rows)
+    check(gpu, x, u, temp=t, top_k=[5000] * rows, top_p=p)
+
+
+@pytest.mark.parametrize("shift", [-1e30, -3e5, -1000.0, 1000.0, 3e5, 1e30])
+@pytest.mark.parametrize("temp", [1e-6, 0.7, 3.0])
+def test_far_from_zero(gpu, shift, temp):
+    """Logits whose bins are no whole numbers, or far from 0."""
+    x, u = rows_of(16, 4, 9001, torch.float32)
+    x = x + shift
+    check(gpu, x, u, temp=[temp] * 4, top_p=[0.9] * 4)
+    check(gpu, x, u, temp=[temp] * 4, top_k=[100] * 4)
+    check(gpu, x, u, temp=[temp] * 4, min_p=[0.1] * 4)
+    check(gpu, x, u, temp=[temp] * 4)

@@ -6,12 +6,14 @@
 //
 // Launch 1 (a workgroup a row and chunk) reads every logit once: the chunk's
 // maximum, the maxima of its groups of 64 logits and, where the row needs it, the
-// sum of its weights.  Launch 2 (a workgroup a row) finds from the groups' maxima
-// a value that enough tokens reach (as many as groups whose maximum does), reads
-// the groups that reach it again and goes on with these tokens alone, a few
-// hundred of tens of thousands: up to 512 compare themselves with each other, up
-// to 4096 are counted into bins first.  Rows of which more stay are searched
-// whole, by bins over the row.
+// sum of its weights, under top-p alone by bins of an eighth of the temperature.
+// Launch 2 (a workgroup a row) finds a value that all that may stay reach: from
+// the bins, from min-p, or from the groups' maxima (as many tokens reach it as
+// maxima do).  It reads the groups that reach it again and goes on with these
+// tokens alone, a few hundred of tens of thousands: up to 512 compare themselves
+// with each other, up to 4096 are counted into bins first.  Where top-p keeps
+// more, the bins give all sums but the cut's own bin.  What is left is searched
+// whole.
 //
 // Sums that are split at a place the data decides are taken in integers, which
 // have no order: a weight is rounded to a multiple of 2^-q of the largest, q as
@@ -32,7 +34,7 @@ typedef unsigned long long u64;
 struct Part {
     float m;   // the chunk's maximum (-inf: nothing)
     int arg;   // its first index (greedy rows)
-    int n;     // tokens that are not masked (rows without a cut)
+    int n;     // tokens that are not masked (rows without a cut), or the bin of m
     int pad;
     double z;  // sum of exp((x - m) / T) (rows that need it)
 };
@@ -51,6 +53,7 @@ struct SampleArgs {
     int q;       // weights are multiples of 2^-q
     Part* part;  // nrows x nch
     float* gmax; // nrows x ng: the groups' maxima
+    u64* hist;   // nrows x nch x kHist: sums of weights by bins (top-p alone)
     int nch, k;  // chunks of a row; pieces of 16 bytes a thread and chunk
     int ng;
 };
@@ -62,6 +65,8 @@ constexpr int kBins = 1024;
 constexpr int kFew = kRow;     // tokens that compare themselves with each other
 constexpr int kList = 4096;    // tokens gathered from a row
 constexpr int kGroup = 64;     // logits of a group
+constexpr int kHist = kThreads; // bins of a chunk; the last holds all below
+constexpr int kMaxChunks = 1024;
 constexpr int kMaxVocab = 1 << 21;
 
 // What a row asks for.
@@ -72,7 +77,13 @@ struct Ask {
     // the sum of all weights is needed
     __device__ bool sum() const { return !greedy && !k && (p || !m); }
     __device__ bool none() const { return !k && !p && !m; }
+    __device__ bool bins() const { return !greedy && p && !k && !m; }
+    // A value's bin from above, as a whole float; bins are as wide as weights of
+    // e^(1/8).
+    __device__ float step() const { return (float)(8.0 * inv); }
 };
+__device__ __forceinline__ float bin_at(float x, float step) { return floorf(x * step); }
+constexpr float kFar = 4194304.0f;  // bins past it are not whole numbers
 __device__ __forceinline__ Ask ask_of(const SampleArgs& P, int r) {
     const float t = P.temp ? P.temp[r] : 1.0f;
     const float tp = P.top_p ? P.top_p[r] : 1.0f, mp = P.min_p ? P.min_p[r] : 0.0f;
@@ -87,6 +98,34 @@ __device__ __forceinline__ Ask ask_of(const SampleArgs& P, int r) {
     a.min_p = a.m ? fmin((double)mp, 1.0) : 0.0;
     return a;
 }
+
+// A weight (0 .. 1) as a multiple of 2^-q, rounded to nearest: the low bits of a
+// sum with 2^52.
+__device__ __forceinline__ u64 fixed(double w, double scale) {
+    return __builtin_bit_cast(u64, fma(w, scale, 4503599627370496.0)) - 0x4330000000000000ull;
+}
+// Sums and running sums over the lanes, as wave_sum and wave_scan.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_shift(u64 x) {
+    const uint32x2 u = __builtin_bit_cast(uint32x2, x);
+    const uint32x2 v = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, false),
+                        (unsigned)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, false)};
+    return __builtin_bit_cast(u64, v);
+}
+__device__ __forceinline__ u64 wave_run(u64 x) {
+    x += dpp_shift<0x111, 0xF>(x);
+    x += dpp_shift<0x112, 0xF>(x);
+    x += dpp_shift<0x114, 0xF>(x);
+    x += dpp_shift<0x118, 0xF>(x);
+    x += dpp_shift<0x142, 0xA>(x);
+    return x + dpp_shift<0x143, 0xC>(x);
+}
+__device__ __forceinline__ u64 lane_of(u64 x, int l) {
+    const uint32x2 u = __builtin_bit_cast(uint32x2, x);
+    const uint32x2 v = {(unsigned)__builtin_amdgcn_readlane((int)u.x, l), (unsigned)__builtin_amdgcn_readlane((int)u.y, l)};
+    return __builtin_bit_cast(u64, v);
+}
+__device__ __forceinline__ u64 wave_add(u64 x) { return lane_of(wave_run(x), 63); }
 
 // The largest of 16 lanes (rows of 32-bit logits: 16 pieces are a group) or 8.
 template <int LANES>
@@ -105,6 +144,7 @@ __global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs
     __shared__ float sm[4];
     __shared__ int sa[4], sn[4];
     __shared__ double sz[4];
+    __shared__ u64 hist[kHist];
     const int chunk = blockIdx.x, r = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Row q = row_at<KIND>(P.x, P.xs, r);
     auto first = [&](int k) { return ((chunk * K + k) * kThreads + t) * N - q.off; };
@@ -116,8 +156,9 @@ __global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs
         if (full(first(k))) raw[k] = *reinterpret_cast<const uint4*>(q.p + (int64_t)first(k) * kBytes<KIND>);
     }
     const Ask A = ask_of(P, r);
-    const bool sum = A.sum();
+    const bool sum = A.sum(), bins = A.bins();
     if (sum) fill_table(tab);
+    if (bins) hist[t] = 0;
     float x[K][N], gm[K];
     float m = -INFINITY;
 #pragma unroll
@@ -165,21 +206,44 @@ __global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs
         if (sm[w] > m || (sm[w] == m && sa[w] < a)) { m = sm[w]; a = sa[w]; }
     double z[2] = {0.0, 0.0};
     int n = 0;
-    if (sum && m != -INFINITY) {
+    if (bins) {
+        // weights as multiples of 2^-50 of the chunk's largest: sums that do not
+        // depend on their order
         const Scale S = scale_of(m, A.inv);
+        const float step = A.step(), top = bin_at(m, step);
+        if (m != -INFINITY) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                // (a masked one adds e^-690)
-                z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
-                n += x[k][e] != -INFINITY;
-            }
-    }
-    if (sum) {
+                for (int e = 0; e < N; ++e) {
+                    const double w = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), 0.0, tab);
+                    const u64 f = fixed(w, 0x1p50);
+                    const int b = (int)fminf(top - bin_at(x[k][e], step), (float)(kHist - 1));
+                    if (f) atomicAdd(&hist[b], f);
+                }
+        }
+        __syncthreads();
+        const u64 f = hist[t];
+        P.hist[((int64_t)r * P.nch + chunk) * kHist + t] = f;
+        const u64 w = wave_add(f);
+        if (lane == 0) sz[wave] = (double)w;
+        __syncthreads();
+        z[0] = (sz[0] + sz[1] + sz[2] + sz[3]) * 0x1p-50;
+        n = m == -INFINITY ? -0x7fffffff : fabsf(m * step) < kFar ? (int)top : 0x7fffffff;
+    } else if (sum) {
+        if (m != -INFINITY) {
+            const Scale S = scale_of(m, A.inv);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    // (a masked one adds e^-690)
+                    z[e & 1] = add_pow(fmax(((double)x[k][e] - S.m) * S.a, -63700.0), z[e & 1], tab);
+                    n += x[k][e] != -INFINITY;
+                }
+        }
         const double w = wave_sum(z[0] + z[1]);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
+        n = (int)wave_add((u64)n);
         if (lane == 0) { sz[wave] = w; sn[wave] = n; }
         __syncthreads();
         z[0] = sz[0] + sz[1] + sz[2] + sz[3];
@@ -204,21 +268,10 @@ struct Cut {
 __device__ __forceinline__ bool stays(const Cut& c, unsigned key, int i) {
     return key > c.key || (key == c.key && i <= c.idx);
 }
-// A weight (0 .. 1) as a multiple of 2^-q, rounded to nearest: the low bits of a
-// sum with 2^52.
-__device__ __forceinline__ u64 fixed(double w, double scale) {
-    return __builtin_bit_cast(u64, fma(w, scale, 4503599627370496.0)) - 0x4330000000000000ull;
-}
-__device__ __forceinline__ u64 wave_add(u64 x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
-
 struct RowShared {
     double tab[64];
     u64 wave[kWaves];
-    float m[kWaves];
+    float m[kWaves], low[kWaves];
     int a[kWaves];
     union {
         struct {
@@ -226,25 +279,33 @@ struct RowShared {
             u64 sum[kBins];
         } h;
         struct {
-            u64 order[kFew], w[kFew];
+            u64 order[kFew], w[kFew], before[kFew];
+            unsigned rank[kFew];
         } few;
+        int groups[4 * kFew];
+        struct {
+            double sum[kMaxChunks];
+            u64 more[kMaxChunks];
+        } chunk;
+        struct {
+            double f[kFew], part[kHist], wave[4];
+            int down[kFew];
+        } merge;
     };
     unsigned key[kList];
     int idx[kList];
-    int bin, n, ngroups;
+    int bin, n, stay, found, last;
     unsigned lo, hi;
     u64 above, total;
+    double left, sum;
+    float x;
     Cut at;
 };
 
 // The running sum over the workgroup's threads; total: of all.
 __device__ __forceinline__ u64 block_scan(u64 x, u64* sm, u64& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
+    x = wave_run(x);
     __syncthreads();  // the last scan's sums are read
     if (lane == 63) sm[wave] = x;
     __syncthreads();
@@ -256,6 +317,40 @@ __device__ __forceinline__ u64 block_scan(u64 x, u64* sm, u64& total) {
         total += sm[w];
     }
     return x + before;
+}
+// A place for each lane that has something, in a list whose length is *n.
+__device__ __forceinline__ int place_of(bool some, int* n) {
+    const u64 all = __ballot(some);
+    if (!all) return 0;
+    const int lane = threadIdx.x & 63;
+    int at = 0;
+    if (lane == __ffsll(all) - 1) at = atomicAdd(n, __popcll(all));
+    return __builtin_amdgcn_readlane(at, __ffsll(all) - 1) + __popcll(all & ((1ull << lane) - 1));
+}
+// Of n tokens (few.order, few.w) each one's rank and the weights before it: all
+// threads take part, several a token where there are few.
+__device__ __forceinline__ void compare_all(RowShared& H, int n) {
+    const int t = threadIdx.x;
+    const int cols = n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512, parts = kRow / cols;
+    H.few.before[t] = 0;
+    H.few.rank[t] = 0;
+    __syncthreads();
+    const int i = t & (cols - 1), per = (n + parts - 1) / parts, j0 = t / cols * per, j1 = min(n, j0 + per);
+    const u64 mine = H.few.order[i];
+    u64 s = 0;
+    unsigned c = 0;
+#pragma unroll 4
+    for (int j = j0; j < j1; ++j) {
+        const u64 o = H.few.order[j], w = H.few.w[j];
+        const bool less = o < mine;
+        s += less ? w : 0;
+        c += less;
+    }
+    if (c) {
+        atomicAdd(&H.few.before[i], s);
+        atomicAdd(&H.few.rank[i], c);
+    }
+    __syncthreads();
 }
 
 // A row's piece g as it lies in memory; values outside the row are 0.
@@ -402,15 +497,13 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
             src.each([&](unsigned key, int i) {
                 if (bin_of(key, i) != bin) return;
                 const int at = atomicAdd(&H.n, 1);
+                if (at >= kFew) return;  // (never: c of them)
                 H.few.order[at] = BY_INDEX ? (u64)(unsigned)i << 32 | key : (u64)~key << 32 | (unsigned)i;
                 H.few.w[at] = WEIGHTED ? W(key) : 1;
             });
             __syncthreads();
-            const u64 mine = t < c ? H.few.order[t] : 0, w = t < c ? H.few.w[t] : 0;
-            u64 s = before;
-            if (t < c)
-                for (int j = 0; j < c; ++j)
-                    if (H.few.order[j] < mine) s += H.few.w[j];
+            compare_all(H, c);
+            const u64 mine = t < c ? H.few.order[t] : 0, w = t < c ? H.few.w[t] : 0, s = before + H.few.before[t];
             if (t < c && s < want && want <= s + w)
                 H.at = BY_INDEX ? Cut{(unsigned)mine, (int)(mine >> 32)} : Cut{~(unsigned)(mine >> 32), (int)(unsigned)mine};
             __syncthreads();
@@ -465,11 +558,11 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
     const double u = P.u[r];
     // how many stay
     unsigned n = 0;
-    if (t == 0) H.ngroups = 0;
+    if (t == 0) H.stay = 0;
     __syncthreads();
     src.each([&](unsigned key, int i) { n += stays(cut, key, i) && (least == 0.0 || W.real(key) >= least); });
     n = (unsigned)wave_add(n);
-    if ((t & 63) == 0 && n) atomicAdd(&H.ngroups, (int)n);
+    if ((t & 63) == 0 && n) atomicAdd(&H.stay, (int)n);
     u64 sum = 0;
     // (a draw of 1 or more, or no number, takes the last token)
     locate<true, true>(H, src, W, cut, m, range, P.vocab, [&](u64 total) {
@@ -478,7 +571,7 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
     });
     if (t == 0) {
         P.token[r] = H.at.idx;
-        if (P.kept) P.kept[r] = H.ngroups;
+        if (P.kept) P.kept[r] = H.stay;
         if (P.prob) P.prob[r] = (float)(W.real(H.at.key) / ((double)sum / W.scale));
     }
 }
@@ -496,13 +589,9 @@ __device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared&
     u64 w = in ? fixed(real, W.scale) : 0;
     H.few.order[t] = in ? mine : ~0ull;
     H.few.w[t] = w;
-    __syncthreads();
-    u64 before = 0;
-    int rank = 0;
-    if (in)
-        for (int j = 0; j < n; ++j)
-            if (H.few.order[j] < mine) { ++rank; before += H.few.w[j]; }
-    bool stay = in && (!A.k || rank < A.top_k);
+    compare_all(H, n);
+    const u64 before = H.few.before[t];
+    bool stay = in && (!A.k || (int)H.few.rank[t] < A.top_k);
     u64 total;
     if (A.p) {
         double all = z * W.scale;
@@ -520,11 +609,8 @@ __device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared&
     block_scan(stay, H.wave, total);
     H.few.order[t] = stay ? (u64)(unsigned)idx : ~0ull;
     H.few.w[t] = w;
-    __syncthreads();
-    u64 c = 0;
-    if (stay)
-        for (int j = 0; j < n; ++j)
-            if (H.few.order[j] < (u64)(unsigned)idx) c += H.few.w[j];
+    compare_all(H, n);
+    const u64 c = H.few.before[t];
     const double u = P.u[r];
     const u64 want = u >= 0.0 && u < 1.0 ? min((u64)(u * (double)sum), sum - 1) : u < 0.0 ? 0 : sum - 1;
     if (stay && c <= want && want < c + w) {
@@ -534,27 +620,21 @@ __device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared&
     }
 }
 
-// A draw without a cut: the chunk from launch 1's sums, the token in it from its
-// weights.
-template <int KIND>
-__device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int r, const Row& q, const Ask& A, const Scale& S) {
+// The draw from the chunks' sums (H.chunk.sum, in 64-bit floats): the chunk, then
+// the token in it from its weights.  stay(x, index): which of them count.
+template <int KIND, class Stay>
+__device__ __forceinline__ void draw_in_chunks(const SampleArgs& P, RowShared& H, int r, const Row& q, const Scale& S,
+                                               int kept, Stay stay) {
     constexpr int N = kPer<KIND>;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    __shared__ int chosen, found, last, kept;
-    __shared__ double left, sum, sw[kWaves];
-    __shared__ float lx;
-    const Part* part = P.part + (int64_t)r * P.nch;
+    __shared__ double sw[kWaves];
     if (wave == 0) {
-        auto sum_of = [&](int c) { return c < P.nch ? part[c].z * weight(part[c].m, S, H.tab) : 0.0; };
+        auto sum_of = [&](int c) { return c < P.nch ? H.chunk.sum[c] : 0.0; };
         double total = 0.0;
-        int n = 0;
-        for (int c = lane; c < P.nch; c += 64) {
-            total += sum_of(c);
-            n += part[c].n;
-        }
+        for (int c = lane; c < P.nch; c += 64) total += sum_of(c);
         total = wave_sum(total);
-        n = (int)wave_add((unsigned)n);
         const double un = P.u[r];
+        // (a draw of 1 or more, or no number, takes the last token)
         const double want = un >= 0.0 ? un * total : un < 0.0 ? 0.0 : total;
         double before = 0.0, at = 0.0, some_at = 0.0;
         int pick = -1, some = -1;
@@ -573,17 +653,17 @@ __device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int 
             before += lane_of(run, 63);
         }
         if (lane == 0) {
-            chosen = pick >= 0 ? pick : some;
-            left = fmax(want - (pick >= 0 ? at : some_at), 0.0);
-            sum = total;
-            kept = n;
-            found = 0x7fffffff;
-            last = -1;
+            H.bin = pick >= 0 ? pick : some;
+            H.left = fmax(want - (pick >= 0 ? at : some_at), 0.0);
+            H.sum = total;
+            H.found = 0x7fffffff;
+            H.last = -1;
         }
     }
     __syncthreads();
+    const double left = H.left;
     // the chunk's pieces, consecutive ones of a thread
-    const int pieces = P.k * kThreads, per = (pieces + kRow - 1) / kRow;
+    const int pieces = P.k * kThreads, per = (pieces + kRow - 1) / kRow, g0 = H.bin * pieces;
     double s = 0.0;
     int mine = -1;
     float lastx = 0.0f;
@@ -591,9 +671,9 @@ __device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int 
         for (int k = 0; k < per; ++k) {
             const int j = t * per + k;
             if (j >= pieces) break;
-            const int g = chosen * pieces + j;
-            each_of<KIND>(raw_piece<KIND>(q, P.vocab, g), g * N - q.off, P.vocab,
-                          [&](float x, int i) { f(x, i, weight(x, S, H.tab)); });
+            each_of<KIND>(raw_piece<KIND>(q, P.vocab, g0 + j), (g0 + j) * N - q.off, P.vocab, [&](float x, int i) {
+                if (x != -INFINITY && stay(x, i)) f(x, i, weight(x, S, H.tab));
+            });
         }
     };
     each([&](float x, int i, double w) {
@@ -602,7 +682,7 @@ __device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int 
     });
     const double run = wave_scan(s);
     if (lane == 63) sw[wave] = run;
-    if (mine >= 0) atomicMax(&last, mine);
+    if (mine >= 0) atomicMax(&H.last, mine);
     __syncthreads();
     // (as the draft check takes it: only a thread with a weight, and of several
     // waves the first)
@@ -621,141 +701,335 @@ __device__ __forceinline__ void draw_all(const SampleArgs& P, RowShared& H, int 
             if (hit < 0 && c > left && w > 0.0) { hit = i; hx = x; }
         });
         if (hit < 0) { hit = mine; hx = lastx; }
-        atomicMin(&found, hit);
+        atomicMin(&H.found, hit);
     }
     __syncthreads();
-    const int token = found != 0x7fffffff ? found : last;
-    if (hit == token) lx = hx;
-    else if (found == 0x7fffffff && mine == token) lx = lastx;
+    const bool none = H.found == 0x7fffffff;
+    const int token = none ? H.last : H.found;
+    if (!none && hit == token) H.x = hx;
+    if (none && mine == token) H.x = lastx;
     __syncthreads();
     if (t == 0) {
         P.token[r] = token;
         if (P.kept) P.kept[r] = kept;
-        if (P.prob) P.prob[r] = (float)(weight(lx, S, H.tab) / sum);
+        if (P.prob) P.prob[r] = (float)(weight(H.x, S, H.tab) / H.sum);
     }
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
-    constexpr int N = kPer<KIND>, LG = kGroup / N;
-    __shared__ RowShared H;
-    const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const Row q = row_at<KIND>(P.x, P.xs, r);
-    const Part* part = P.part + (int64_t)r * P.nch;
-    const float* gmax = P.gmax + (int64_t)r * P.ng;
-    const Ask A = ask_of(P, r);
+// The maximum of a row's chunks, and (greedy) its first index.
+__device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, const Part* part, bool first, int& a) {
+    const int t = threadIdx.x;
     float m = -INFINITY;
-    int a = 0x7fffffff;
+    a = 0x7fffffff;
     for (int c = t; c < P.nch; c += kRow)
         if (part[c].m > m || (part[c].m == m && part[c].arg < a)) { m = part[c].m; a = part[c].arg; }
-    fill_table(H.tab);
-    if (A.greedy) wave_best(m, a);
+    if (first) wave_best(m, a);
     else m = wave_max(m);
-    if (lane == 0) { H.m[wave] = m; H.a[wave] = a; }
+    if ((t & 63) == 0) { H.m[t >> 6] = m; H.a[t >> 6] = a; }
     __syncthreads();
     m = H.m[0];
     a = H.a[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w)
         if (H.m[w] > m || (H.m[w] == m && H.a[w] < a)) { m = H.m[w]; a = H.a[w]; }
-    const bool nothing = m == -INFINITY;
-    if (nothing || A.greedy) {
+    return m;
+}
+
+// Top-p's bin from the chunks' bins: H.bin (-1: none of them, or they are not
+// whole), the weights above it H.left, all weights H.sum.
+__device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, const Part* part, int r, const Ask& A,
+                                         const Scale& S, float top) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = t & (kHist - 1), half = t / kHist;
+    const u64* hist = P.hist + (int64_t)r * P.nch * kHist;
+    double v = 0.0, z = 0.0;
+    bool far = !(fabsf(top) < kFar);
+    for (int c0 = 0; c0 < P.nch; c0 += kRow) {
+        __syncthreads();
+        if (c0 + t < P.nch) {
+            const Part x = part[c0 + t];
+            const bool some = x.m != -INFINITY;
+            const double f = some ? weight(x.m, S, H.tab) : 0.0;
+            if (some && x.n == 0x7fffffff) far = true;
+            H.merge.f[t] = f;
+            H.merge.down[t] = some && !far ? (int)fminf(top - (float)x.n, (float)kHist) : kHist;
+            z += x.z * f;
+        }
+        __syncthreads();
+        const int n = min(P.nch - c0, kRow);
+#pragma unroll 4
+        for (int c = half; c < n; c += 2) {
+            const int at = b - H.merge.down[c];
+            if (at >= 0 && at < kHist - 1) v += (double)hist[(int64_t)(c0 + c) * kHist + at] * H.merge.f[c];
+        }
+    }
+    // (z: threads in order; a row of up to 512 chunks has one each)
+    z = wave_sum(z);
+    far = __any(far);
+    if (lane == 0) { H.wave[wave] = __builtin_bit_cast(u64, z); H.a[wave] = far; }
+    if (half) H.merge.part[b] = v;
+    if (t == 0) H.bin = -1;
+    __syncthreads();
+    z = 0.0;
+    far = false;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        z += __builtin_bit_cast(double, H.wave[w]);
+        far = far || H.a[w];
+    }
+    double run = 0.0;
+    v = half ? 0.0 : (v + H.merge.part[b]) * 0x1p-50;
+    run = wave_scan(v);
+    if (!half && lane == 63) H.merge.wave[wave] = run;
+    __syncthreads();
+    for (int w = 0; w < wave && !half; ++w) run += H.merge.wave[w];
+    const double want = A.top_p * z;
+    // (the least bin whose running sum reaches it: the scan's sums may be a
+    // rounding apart from lane to lane)
+    const u64 past = __ballot(!half && b < kHist - 1 && run >= want && v > 0.0);
+    if (t == 0) H.n = kHist;
+    __syncthreads();
+    if (past && lane == 0) atomicMin(&H.n, wave * 64 + __ffsll(past) - 1);
+    __syncthreads();
+    if (!half && b == H.n && !far) {
+        H.bin = b;
+        H.left = run - v;
+        H.sum = z;
+    }
+    if (t == 0 && (far || H.n == kHist)) H.sum = z;
+    __syncthreads();
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
+    constexpr int N = kPer<KIND>, LG = kGroup / N, kHold = 3;
+    __shared__ RowShared H;
+    const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const Row q = row_at<KIND>(P.x, P.xs, r);
+    const Part* part = P.part + (int64_t)r * P.nch;
+    const float* gmax = P.gmax + (int64_t)r * P.ng;
+    // the groups' maxima, a thread's first ones held (rows that have none: not used)
+    float held[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) held[i] = gmax[min(t + i * kRow, P.ng - 1)];
+    auto each_group = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kHold; ++i) {
+            const bool in = t + i * kRow < P.ng;
+            f(t + i * kRow, in ? held[i] : -INFINITY);
+        }
+        for (int g = t + kHold * kRow; g - t < P.ng; g += kRow) f(g, g < P.ng ? gmax[g] : -INFINITY);
+    };
+    const Ask A = ask_of(P, r);
+    fill_table(H.tab);
+    int a;
+    if (A.greedy || A.none()) {
+        const float m = join_max(P, H, part, A.greedy, a);
+        const bool nothing = m == -INFINITY;
+        if (nothing || A.greedy) {
+            if (t == 0) {
+                P.token[r] = nothing ? -1 : a;
+                if (P.kept) P.kept[r] = !nothing;
+                if (P.prob) P.prob[r] = nothing ? 0.0f : 1.0f;
+            }
+            return;
+        }
+        const Scale S = scale_of(m, A.inv);
+        int n = 0;
+        for (int c = t; c < P.nch; c += kRow) {
+            H.chunk.sum[c] = part[c].z * weight(part[c].m, S, H.tab);
+            n += part[c].n;
+        }
+        u64 kept;
+        block_scan((u64)n, H.wave, kept);
+        return draw_in_chunks<KIND>(P, H, r, q, S, (int)kept, [](float, int) { return true; });
+    }
+    float m = -INFINITY, low = INFINITY;
+    each_group([&](int, float x) {
+        m = fmaxf(m, x);
+        if (x != -INFINITY) low = fminf(low, x);
+    });
+    m = wave_max(m);
+    low = -wave_max(-low);
+    if (lane == 0) { H.m[wave] = m; H.low[wave] = low; }
+    for (int i = t; i < kBins; i += kRow) H.h.cnt[i] = 0;
+    if (t == 0) { H.n = 0; H.stay = 0; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        m = fmaxf(m, H.m[w]);
+        low = fminf(low, H.low[w]);
+    }
+    if (m == -INFINITY) {
         if (t == 0) {
-            P.token[r] = nothing ? -1 : a;
-            if (P.kept) P.kept[r] = !nothing;
-            if (P.prob) P.prob[r] = nothing ? 0.0f : 1.0f;
+            P.token[r] = -1;
+            if (P.kept) P.kept[r] = 0;
+            if (P.prob) P.prob[r] = 0.0f;
         }
         return;
     }
     const Scale S = scale_of(m, A.inv);
-    if (A.none()) return draw_all<KIND>(P, H, r, q, A, S);
     const Weigh W{S, __longlong_as_double((long long)(1023 + P.q) << 52), A.min_p, H.tab};
-    double z = 0.0;
-    if (A.sum()) {  // (one wave's order for every thread)
-        for (int c = lane; c < P.nch; c += 64) z += part[c].z * weight(part[c].m, S, H.tab);
-        z = wave_sum(z);
-    }
-    // A value that min-p's tokens reach, a rounding below its border.
-    float floor_m = -INFINITY;
-    if (A.m && !A.k && A.inv > 0.0)
-        floor_m = (float)((double)m + log(A.min_p) / A.inv) - 1e-5f * (fabsf(m) + (float)(1.0 / A.inv));
-    // Groups by their maxima: bins of the distance from the row's.
-    float low = INFINITY;
-    for (int g = t; g < P.ng; g += kRow)
-        if (gmax[g] != -INFINITY) low = fminf(low, gmax[g]);
-    low = -wave_max(-low);
-    if (lane == 0) H.m[wave] = low;
-    for (int i = t; i < kBins; i += kRow) H.h.cnt[i] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) low = fminf(low, H.m[w]);
-    const float step = (float)(kBins - 1) / fmaxf(m - low, 1e-30f);
-    auto bin_of = [&](float x) { return (int)fminf((m - x) * step, (float)(kBins - 1)); };
-    for (int g = t; g < P.ng; g += kRow)
-        if (gmax[g] != -INFINITY) atomicAdd(&H.h.cnt[bin_of(gmax[g])], 1u);
-    __syncthreads();
-    u64 groups;
-    const unsigned c0 = H.h.cnt[2 * t], c1 = H.h.cnt[2 * t + 1];
-    const u64 run = block_scan(c0 + c1, H.wave, groups);
-    // Tokens wanted: top-k's at the least; for top-p 64, and where their weights
-    // do not reach it 512.
-    u64 want = A.k ? (u64)A.top_k : A.p ? 64 : groups;
-#pragma unroll 1
-    for (int round = 0; round < 2; ++round) {
-        if (want > groups) {
-            if (A.k && P.vocab > kList) break;  // (the groups' maxima do not bound that many)
-            want = groups;
+    const float hstep = A.step(), top = bin_at(m, hstep);
+    double z = -1.0;
+    // All that may stay: x >= floor_m, and in bins of the distance from m up to
+    // last (not: every bin).
+    float floor_m = -INFINITY, step = 0.0f;
+    int last = kBins - 1;
+    bool open = true;  // nothing is known of the row
+    if (A.bins()) {
+        find_bin(P, H, part, r, A, S, top);
+        z = H.sum;
+        if (H.bin >= 0) {
+            open = false;
+            last = H.bin;
         }
+    } else if (A.m && !A.k) {
+        if (A.p) {  // (one wave's order for every thread)
+            z = 0.0;
+            for (int c = lane; c < P.nch; c += 64) z += part[c].z * weight(part[c].m, S, H.tab);
+            z = wave_sum(z);
+        }
+        // a rounding below min-p's border
+        if (A.inv > 0.0) {
+            floor_m = (float)((double)m + log(A.min_p) / A.inv) - 1e-5f * (fabsf(m) + (float)(1.0 / A.inv));
+            open = false;
+        }
+    } else {  // as many tokens as top-k keeps reach what as many groups' maxima do
+        step = (float)(kBins - 1) / fmaxf(m - low, 1e-30f);
+        each_group([&](int, float x) {
+            if (x != -INFINITY) atomicAdd(&H.h.cnt[(int)fminf((m - x) * step, (float)(kBins - 1))], 1u);
+        });
         __syncthreads();
-        if (t == 0) { H.n = 0; H.ngroups = 0; }
+        u64 groups;
+        const unsigned c0 = H.h.cnt[2 * t], c1 = H.h.cnt[2 * t + 1];
+        const u64 want = (u64)A.top_k, run = block_scan(c0 + c1, H.wave, groups);
         if (run >= want && run - c0 - c1 < want) H.bin = run - c1 >= want ? 2 * t : 2 * t + 1;
         __syncthreads();
-        const int last = H.bin;  // tokens in bins up to it
-        const bool all = want == groups;
-        auto in = [&](float x) { return x >= floor_m && (all || bin_of(x) <= last); };
-        // the groups, into the list's memory, then their tokens
+        if (want <= groups) {
+            open = false;
+            last = H.bin;
+        }
+    }
+    if (open && P.vocab <= kList) open = false;  // (then all of it is gathered)
+    const bool bins = A.bins();
+    auto in = [&](float x) {
+        if (bins) return top - bin_at(x, hstep) <= (float)last || last == kBins - 1;
+        return x >= floor_m && (last == kBins - 1 || (int)fminf((m - x) * step, (float)(kBins - 1)) <= last);
+    };
+    if (!open) {
         __syncthreads();
-        for (int g = t; g < P.ng; g += kRow)
-            if (gmax[g] != -INFINITY && in(gmax[g])) {
-                const int at = atomicAdd(&H.ngroups, 1);
-                if (at < 4 * kFew) reinterpret_cast<int*>(&H.few)[at] = g;
-            }
+        if (t == 0) H.n = 0;
         __syncthreads();
-        const int ngr = H.ngroups;
-        if (ngr > 4 * kFew) break;
-        for (int j = t; j < ngr * LG; j += kRow) {
-            const int g = reinterpret_cast<int*>(&H.few)[j / LG] * LG + j % LG;
-            float x[N];
-            piece<KIND>(q, P.vocab, g, x);
+        each_group([&](int g, float x) {
+            const bool some = x != -INFINITY && in(x);
+            const int at = place_of(some, &H.n);
+            if (some && at < 4 * kFew) H.groups[at] = g;
+        });
+        __syncthreads();
+        const int ngr = H.n;
+        __syncthreads();
+        if (t == 0) H.n = 0;
+        __syncthreads();
+        if (ngr <= 4 * kFew) {
+            for (int j0 = 0; j0 < ngr * LG; j0 += kRow) {
+                const int j = j0 + t;
+                float x[N];
+                int i0 = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (x[e] != -INFINITY && in(x[e])) {
-                    const int at = atomicAdd(&H.n, 1);
-                    if (at < kList) {
+                for (int e = 0; e < N; ++e) x[e] = -INFINITY;
+                if (j < ngr * LG) {
+                    const int g = H.groups[j / LG] * LG + j % LG;
+                    piece<KIND>(q, P.vocab, g, x);
+                    i0 = g * N - q.off;
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const bool some = x[e] != -INFINITY && in(x[e]);
+                    const int at = place_of(some, &H.n);
+                    if (some && at < kList) {
                         H.key[at] = key_of(x[e]);
-                        H.idx[at] = g * N - q.off + e;
+                        H.idx[at] = i0 + e;
                     }
                 }
+            }
+            __syncthreads();
+            const int n = H.n;
+            if (n <= kList) {
+                if (n <= kFew) cut_and_draw_few(P, H, n, r, A, W, z);
+                else cut_and_draw(P, H, Gathered{H, n}, r, A, W, m, z);
+                return;
+            }
         }
         __syncthreads();
-        const int n = H.n;
-        if (n > kList) break;
-        bool enough = A.k || !A.p || all;
-        if (!enough) {
-            u64 s = 0, total;
-            for (int i = t; i < n; i += kRow) s += fixed(W.real(H.key[i]), W.scale);
-            block_scan(s, H.wave, total);
-            // (what is below min-p's border is not missing)
-            enough = (double)total >= A.top_p * z * W.scale + 1.0 || (floor_m > -INFINITY && bin_of(floor_m) <= last);
-        }
-        if (enough) {
-            if (n <= kFew) cut_and_draw_few(P, H, n, r, A, W, z);
-            else cut_and_draw(P, H, Gathered{H, n}, r, A, W, m, z);
-            return;
-        }
-        want = 512;
     }
-    __syncthreads();
+    if (bins && last < kBins - 1) {
+        // Thousands stay: all above top-p's bin, whose own tokens are gathered.
+        if (t == 0) { H.n = 0; H.stay = 0; }
+        const double left = H.left;
+        __syncthreads();
+        const float edge = top - (float)last;
+        int above = 0;
+        const int pieces = (P.vocab + q.off + N - 1) / N;
+        for (int g0 = 0; g0 < pieces; g0 += kRow) {
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = -INFINITY;
+            if (g0 + t < pieces) piece<KIND>(q, P.vocab, g0 + t, x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float b = bin_at(x[e], hstep);
+                above += b > edge;
+                const bool some = b == edge && x[e] != -INFINITY;
+                const int at = place_of(some, &H.n);
+                if (some && at < kList) {
+                    H.key[at] = key_of(x[e]);
+                    H.idx[at] = (g0 + t) * N - q.off + e;
+                }
+            }
+        }
+        u64 kept;
+        block_scan((u64)above, H.wave, kept);
+        const int n = H.n;
+        if (n <= kList) {
+            Cut cut{0, 0x7fffffff};
+            const float range = (float)fmin((double)(P.q + 1) * 0.7 / A.inv, 1e30);
+            const double y = ceil((A.top_p * z - left) * W.scale);
+            if (locate<true, false>(H, Gathered{H, n}, W, cut, m, range, P.vocab,
+                                    [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
+                cut = H.at;
+            __syncthreads();
+            // the chunks' sums: a wave a chunk, its bins above the cut's, then those
+            // of the bin's tokens that stay
+            const int per = P.k * kThreads * N;
+            for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
+            __syncthreads();
+            int more = 0;
+            Gathered{H, n}.each([&](unsigned key, int i) {
+                if (!stays(cut, key, i)) return;
+                ++more;
+                atomicAdd(&H.chunk.more[(i + q.off) / per], W(key));
+            });
+            more = (int)wave_add((u64)more);
+            if (lane == 0) atomicAdd(&H.stay, more);
+            __syncthreads();
+            for (int c = wave; c < P.nch; c += kWaves) {
+                const Part x = part[c];
+                const int bins_in = x.m == -INFINITY ? 0 : last - (int)fminf(top - (float)x.n, (float)kHist);
+                u64 f = 0;
+                for (int b = lane; b < bins_in; b += 64) f += P.hist[((int64_t)r * P.nch + c) * kHist + b];
+                f = wave_add(f);
+                if (lane == 0)
+                    H.chunk.sum[c] = (x.m == -INFINITY ? 0.0 : (double)f * 0x1p-50 * weight(x.m, S, H.tab)) +
+                                     (double)H.chunk.more[c] / W.scale;
+            }
+            __syncthreads();
+            return draw_in_chunks<KIND>(P, H, r, q, S, (int)kept + H.stay, [&](float x, int i) {
+                const float b = bin_at(x, hstep);
+                return b > edge || (b == edge && stays(cut, key_of(x), i));
+            });
+        }
+        __syncthreads();
+    }
     cut_and_draw(P, H, WholeRow<KIND>{P, q}, r, A, W, m, -1.0);
 }
 
@@ -793,7 +1067,7 @@ extern "C" {
 size_t vgx_sample_ws(int nrows, int vocab, int kind) {
     if (nrows < 0 || vocab <= 0 || vocab > kMaxVocab || !kind_ok(kind)) return 0;
     const Chunks c = chunks_of(nrows, vocab, kind);
-    return (size_t)nrows * (c.nch * sizeof(Part) + c.ng * sizeof(float));
+    return (size_t)nrows * (c.nch * (sizeof(Part) + kHist * sizeof(u64)) + c.ng * sizeof(float));
 }
 
 int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
@@ -824,7 +1098,8 @@ int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
     while ((1 << lg) < a->vocab) ++lg;
     P.q = std::min(50, 62 - lg);
     P.nch = c.nch; P.k = c.k; P.ng = c.ng;
-    P.part = static_cast<Part*>(a->ws);
+    P.hist = static_cast<u64*>(a->ws);
+    P.part = reinterpret_cast<Part*>(P.hist + (size_t)a->nrows * c.nch * kHist);
     P.gmax = reinterpret_cast<float*>(P.part + (size_t)a->nrows * c.nch);
     VGX_HIP(hipSetDevice(ctx->device));
     switch (a->kind) {
