@@ -62,8 +62,9 @@ constexpr int kThreads = 256;  // of launch 1
 constexpr int kRow = 512;      // of launch 2
 constexpr int kWaves = kRow / 64;
 constexpr int kBins = 1024;
-constexpr int kFew = kRow;     // tokens that compare themselves with each other
-constexpr int kList = 4096;    // tokens gathered from a row
+constexpr int kFew = 192;      // tokens that compare themselves with each other
+constexpr int kList = 4096;    // tokens gathered from a row; under top-p alone
+constexpr int kAbove = 1024;   // the first of these are for those above its bin
 constexpr int kGroup = 64;     // logits of a group
 constexpr int kHist = kThreads; // bins of a chunk; the last holds all below
 constexpr int kMaxChunks = 1024;
@@ -84,6 +85,9 @@ struct Ask {
 };
 __device__ __forceinline__ float bin_at(float x, float step) { return floorf(x * step); }
 constexpr float kFar = 4194304.0f;  // bins past it are not whole numbers
+// Where a chunk of maximum's bin n keeps its d-th bin from there: by the bin
+// itself, so that a row's bins can be asked for before its maximum is known.
+__device__ __forceinline__ int slot_of(int n, int d) { return (n - d) & (kHist - 1); }
 __device__ __forceinline__ Ask ask_of(const SampleArgs& P, int r) {
     const float t = P.temp ? P.temp[r] : 1.0f;
     const float tp = P.top_p ? P.top_p[r] : 1.0f, mp = P.min_p ? P.min_p[r] : 0.0f;
@@ -224,12 +228,12 @@ __global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs
         }
         __syncthreads();
         const u64 f = hist[t];
-        P.hist[((int64_t)r * P.nch + chunk) * kHist + t] = f;
+        n = m == -INFINITY ? -0x7fffffff : fabsf(m * step) < kFar ? (int)top : 0x7fffffff;
+        P.hist[((int64_t)r * P.nch + chunk) * kHist + slot_of(n, t)] = f;
         const u64 w = wave_add(f);
         if (lane == 0) sz[wave] = (double)w;
         __syncthreads();
         z[0] = (sz[0] + sz[1] + sz[2] + sz[3]) * 0x1p-50;
-        n = m == -INFINITY ? -0x7fffffff : fabsf(m * step) < kFar ? (int)top : 0x7fffffff;
     } else if (sum) {
         if (m != -INFINITY) {
             const Scale S = scale_of(m, A.inv);
@@ -268,6 +272,8 @@ struct Cut {
 __device__ __forceinline__ bool stays(const Cut& c, unsigned key, int i) {
     return key > c.key || (key == c.key && i <= c.idx);
 }
+constexpr int kGroups = 2048;  // groups that are read again, at most
+
 struct RowShared {
     double tab[64];
     u64 wave[kWaves];
@@ -279,22 +285,22 @@ struct RowShared {
             u64 sum[kBins];
         } h;
         struct {
-            u64 order[kFew], w[kFew], before[kFew];
-            unsigned rank[kFew];
+            u64 order[kRow], w[kRow], before[kRow];
+            unsigned rank[kRow];
         } few;
-        int groups[4 * kFew];
+        int groups[kGroups];
         struct {
             double sum[kMaxChunks];
             u64 more[kMaxChunks];
         } chunk;
         struct {
-            double f[kFew], part[kHist], wave[4];
-            int down[kFew];
+            double f[kRow], part[2][kHist], wave[4];
+            int down[kRow];
         } merge;
     };
     unsigned key[kList];
     int idx[kList];
-    int bin, n, stay, found, last;
+    int bin, n, above_n, stay, found, last;
     unsigned lo, hi;
     u64 above, total;
     double left, sum;
@@ -318,14 +324,21 @@ __device__ __forceinline__ u64 block_scan(u64 x, u64* sm, u64& total) {
     }
     return x + before;
 }
-// A place for each lane that has something, in a list whose length is *n.
-__device__ __forceinline__ int place_of(bool some, int* n) {
-    const u64 all = __ballot(some);
-    if (!all) return 0;
-    const int lane = threadIdx.x & 63;
+// Places for the lanes' c things each in a list whose length is *n: the first of
+// a lane's.
+__device__ __forceinline__ int place_of(int c, int* n) {
+    int run = c;
+    run += __builtin_amdgcn_update_dpp(0, run, 0x111, 0xF, 0xF, false);
+    run += __builtin_amdgcn_update_dpp(0, run, 0x112, 0xF, 0xF, false);
+    run += __builtin_amdgcn_update_dpp(0, run, 0x114, 0xF, 0xF, false);
+    run += __builtin_amdgcn_update_dpp(0, run, 0x118, 0xF, 0xF, false);
+    run += __builtin_amdgcn_update_dpp(0, run, 0x142, 0xA, 0xF, false);
+    run += __builtin_amdgcn_update_dpp(0, run, 0x143, 0xC, 0xF, false);
+    const int all = __builtin_amdgcn_readlane(run, 63);
+    if (all == 0) return 0;
     int at = 0;
-    if (lane == __ffsll(all) - 1) at = atomicAdd(n, __popcll(all));
-    return __builtin_amdgcn_readlane(at, __ffsll(all) - 1) + __popcll(all & ((1ull << lane) - 1));
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
+    return __builtin_amdgcn_readfirstlane(at) + run - c;
 }
 // Of n tokens (few.order, few.w) each one's rank and the weights before it: all
 // threads take part, several a token where there are few.
@@ -368,6 +381,18 @@ __device__ __forceinline__ uint4 raw_piece(const Row& q, int vocab, int g) {
         }
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
+// The e-th value of a piece.
+template <int KIND>
+__device__ __forceinline__ float value_in(const uint4& v, int e) {
+    const int w = KIND == VGX_E_F32 ? e : e / 2;
+    const unsigned a = w & 1 ? v.y : v.x, b = w & 1 ? v.w : v.z;
+    unsigned u = w & 2 ? b : a;
+    if (KIND == VGX_E_F32) return clean(__uint_as_float(u));
+    u = u >> 16 * (e & 1) & 0xffff;
+    if (KIND == VGX_E_Q16) return (float)(short)u * (1.0f / 256);
+    if (KIND == VGX_E_BF16) return clean(__uint_as_float(u << 16));
+    return clean((float)__builtin_bit_cast(_Float16, (unsigned short)u));
+}
 // f(value, index) of a piece's values inside the row, one after the other: a loop
 // that shifts them down, as many copies of a long f would not stay in the
 // instruction cache.
@@ -401,27 +426,38 @@ struct WholeRow {
     __device__ __forceinline__ void each(F f) const {
         constexpr int N = kPer<KIND>;
         const int pieces = (P.vocab + q.off + N - 1) / N;
-        int g = threadIdx.x;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (g < pieces) v = raw_piece<KIND>(q, P.vocab, g);
-        while (g < pieces) {
-            uint4 next = v;
-            if (g + kRow < pieces) next = raw_piece<KIND>(q, P.vocab, g + kRow);
-            each_of<KIND>(v, g * N - q.off, P.vocab, [&](float x, int i) {
-                if (x != -INFINITY) f(key_of(x), i);
-            });
-            v = next;
-            g += kRow;
+        constexpr int U = 4;  // pieces a thread in one round trip
+#pragma unroll 1
+        for (int g0 = threadIdx.x; g0 < pieces; g0 += kRow * U) {
+            uint4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v[u] = make_uint4(0, 0, 0, 0);
+                if (g0 + u * kRow < pieces) v[u] = raw_piece<KIND>(q, P.vocab, g0 + u * kRow);
+            }
+#pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                each_of<KIND>(v[0], (g0 + u * kRow) * N - q.off, P.vocab, [&](float x, int i) {
+                    if (x != -INFINITY) f(key_of(x), i);
+                });
+#pragma unroll
+                for (int w = 0; w + 1 < U; ++w) v[w] = v[w + 1];
+            }
         }
     }
 };
-// ... or those gathered from it.
+// ... or those gathered from it: the list's places i0 .. i0 + n - 1, and the
+// first n0 ones.
 struct Gathered {
     const RowShared& H;
-    int n;
+    int n0, i0, n;
+    __device__ __forceinline__ int place(int i) const { return i < n0 ? i : i - n0 + i0; }
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        for (int i = threadIdx.x; i < n; i += kRow) f(H.key[i], H.idx[i]);
+        for (int i = threadIdx.x; i < n0 + n; i += kRow) {
+            const int at = place(i);
+            f(H.key[at], H.idx[at]);
+        }
     }
 };
 
@@ -456,7 +492,7 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
         const int sh = mode == VALUE ? 0 : max(0, 32 - __clz((int)(hi - lo)) - 10);
         auto bin_of = [&](unsigned key, int i) -> int {
             if (!stays(in, key, i)) return -1;
-            if (mode == VALUE) return kBins - 1 - (int)fminf((m - value_of(key)) * step, (float)(kBins - 1));
+            if (mode == VALUE) return kBins - 1 - (int)fminf(fmaxf((m - value_of(key)) * step, 0.0f), (float)(kBins - 1));
             if (mode == INDEX && !BY_INDEX && key != eq) return -1;
             const unsigned o = mode == KEY ? key : ~(unsigned)i;
             return o < lo || o > hi ? -1 : (int)((o - lo) >> sh);
@@ -497,7 +533,7 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
             src.each([&](unsigned key, int i) {
                 if (bin_of(key, i) != bin) return;
                 const int at = atomicAdd(&H.n, 1);
-                if (at >= kFew) return;  // (never: c of them)
+                if (at >= kFew) return;  // (never)
                 H.few.order[at] = BY_INDEX ? (u64)(unsigned)i << 32 | key : (u64)~key << 32 | (unsigned)i;
                 H.few.w[at] = WEIGHTED ? W(key) : 1;
             });
@@ -576,14 +612,15 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
     }
 }
 
-// The same for up to kRow gathered tokens, each with its thread: its rank and the
+// The same for up to kFew gathered tokens, each with its thread: its rank and the
 // weights before it by comparing with all others, then the weights of those that
 // stay with a lower index.
-__device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared& H, int n, int r, const Ask& A, const Weigh& W, double z) {
-    const int t = threadIdx.x;
+__device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared& H, const Gathered& src, int r,
+                                                 const Ask& A, const Weigh& W, double z) {
+    const int t = threadIdx.x, n = src.n0 + src.n;
     const bool in = t < n;
-    const unsigned key = in ? H.key[t] : 0;
-    const int idx = in ? H.idx[t] : 0;
+    const unsigned key = in ? H.key[src.place(t)] : 0;
+    const int idx = in ? H.idx[src.place(t)] : 0;
     const u64 mine = (u64)~key << 32 | (unsigned)idx;
     const double real = in ? W.real(key) : 0.0;
     u64 w = in ? fixed(real, W.scale) : 0;
@@ -694,19 +731,27 @@ __device__ __forceinline__ void draw_in_chunks(const SampleArgs& P, RowShared& H
     const u64 past = __ballot(mine >= 0 && base + run > left);
     int hit = -1;
     float hx = 0.0f;
-    if (past && lane == __ffsll(past) - 1) {
-        double c = before;
-        each([&](float x, int i, double w) {
-            c += w;
-            if (hit < 0 && c > left && w > 0.0) { hit = i; hx = x; }
-        });
-        if (hit < 0) { hit = mine; hx = lastx; }
-        atomicMin(&H.found, hit);
+    if (past) {
+        // the first such thread's values, one a lane
+        const int l = __ffsll(past) - 1;
+        const double b = lane_of(before, l);
+        const int fall = __builtin_amdgcn_readlane(mine, l);
+        const float fallx = lane_of(lastx, l);
+        const int i = (g0 + (wave * 64 + l) * per) * N - q.off + lane;
+        const bool in = lane < per * N && i >= 0 && i < P.vocab;
+        const float x = in ? one<KIND>(q.p, i) : -INFINITY;
+        const double w = in && x != -INFINITY && stay(x, i) ? weight(x, S, H.tab) : 0.0;
+        const double c = b + wave_scan(w);
+        const u64 at = __ballot(w > 0.0 && c > left);
+        const int k = __ffsll(at) - 1;
+        hit = at ? __builtin_amdgcn_readlane(i, max(k, 0)) : fall;
+        hx = at ? lane_of(x, max(k, 0)) : fallx;
+        if (lane == 0) atomicMin(&H.found, hit);
     }
     __syncthreads();
     const bool none = H.found == 0x7fffffff;
     const int token = none ? H.last : H.found;
-    if (!none && hit == token) H.x = hx;
+    if (!none && hit == token && lane == 0) H.x = hx;
     if (none && mine == token) H.x = lastx;
     __syncthreads();
     if (t == 0) {
@@ -715,6 +760,7 @@ __device__ __forceinline__ void draw_in_chunks(const SampleArgs& P, RowShared& H
         if (P.prob) P.prob[r] = (float)(weight(H.x, S, H.tab) / H.sum);
     }
 }
+static_assert(4 * kThreads / kRow * 8 <= 64, "a thread's values of a chunk: a lane each");
 
 // The maximum of a row's chunks, and (greedy) its first index.
 __device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, const Part* part, bool first, int& a) {
@@ -736,17 +782,20 @@ __device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, con
 }
 
 // Top-p's bin from the chunks' bins: H.bin (-1: none of them, or they are not
-// whole), the weights above it H.left, all weights H.sum.
-__device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, const Part* part, int r, const Ask& A,
-                                         const Scale& S, float top) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = t & (kHist - 1), half = t / kHist;
-    const u64* hist = P.hist + (int64_t)r * P.nch * kHist;
-    double v = 0.0, z = 0.0;
+// whole), the weights above it H.left, all weights H.sum.  held: the thread's slot
+// of its first chunks (every second one: half the threads take the others).
+constexpr int kHoldBins = 10;
+__device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, const Part* part, const Part& own,
+                                         const u64 (&held)[kHoldBins], int r, const Ask& A, const Scale& S, float top) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, slot = t & (kHist - 1), half = t / kHist;
+    const u64* hist = P.hist + (int64_t)r * P.nch * kHist + slot;
     bool far = !(fabsf(top) < kFar);
+    const int mine = ((far ? 0 : (int)top) - slot) & (kHist - 1);  // the row's bin that the slot is
+    double v = 0.0, z = 0.0;
     for (int c0 = 0; c0 < P.nch; c0 += kRow) {
         __syncthreads();
         if (c0 + t < P.nch) {
-            const Part x = part[c0 + t];
+            const Part x = c0 ? part[c0 + t] : own;
             const bool some = x.m != -INFINITY;
             const double f = some ? weight(x.m, S, H.tab) : 0.0;
             if (some && x.n == 0x7fffffff) far = true;
@@ -756,18 +805,24 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
         }
         __syncthreads();
         const int n = min(P.nch - c0, kRow);
-#pragma unroll 4
-        for (int c = half; c < n; c += 2) {
-            const int at = b - H.merge.down[c];
-            if (at >= 0 && at < kHist - 1) v += (double)hist[(int64_t)(c0 + c) * kHist + at] * H.merge.f[c];
+        auto add = [&](int c, u64 w) {
+            const int at = mine - H.merge.down[c];
+            v += at >= 0 && at < kHist - 1 ? (double)w * H.merge.f[c] : 0.0;
+        };
+        if (c0 == 0) {
+#pragma unroll
+            for (int k = 0; k < kHoldBins; ++k)
+                if (half + 2 * k < n) add(half + 2 * k, held[k]);
         }
+#pragma unroll 4
+        for (int c = half + (c0 ? 0 : 2 * kHoldBins); c < n; c += 2) add(c, hist[(int64_t)(c0 + c) * kHist]);
     }
     // (z: threads in order; a row of up to 512 chunks has one each)
     z = wave_sum(z);
     far = __any(far);
     if (lane == 0) { H.wave[wave] = __builtin_bit_cast(u64, z); H.a[wave] = far; }
-    if (half) H.merge.part[b] = v;
-    if (t == 0) H.bin = -1;
+    H.merge.part[half][mine] = v;
+    if (t == 0) { H.bin = -1; H.n = kHist; }
     __syncthreads();
     z = 0.0;
     far = false;
@@ -776,26 +831,21 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
         z += __builtin_bit_cast(double, H.wave[w]);
         far = far || H.a[w];
     }
-    double run = 0.0;
-    v = half ? 0.0 : (v + H.merge.part[b]) * 0x1p-50;
-    run = wave_scan(v);
+    v = half ? 0.0 : (H.merge.part[0][slot] + H.merge.part[1][slot]) * 0x1p-50;
+    double run = wave_scan(v);
     if (!half && lane == 63) H.merge.wave[wave] = run;
     __syncthreads();
     for (int w = 0; w < wave && !half; ++w) run += H.merge.wave[w];
-    const double want = A.top_p * z;
     // (the least bin whose running sum reaches it: the scan's sums may be a
     // rounding apart from lane to lane)
-    const u64 past = __ballot(!half && b < kHist - 1 && run >= want && v > 0.0);
-    if (t == 0) H.n = kHist;
-    __syncthreads();
+    const u64 past = __ballot(!half && slot < kHist - 1 && run >= A.top_p * z && v > 0.0);
     if (past && lane == 0) atomicMin(&H.n, wave * 64 + __ffsll(past) - 1);
     __syncthreads();
-    if (!half && b == H.n && !far) {
-        H.bin = b;
+    if (!half && slot == H.n && !far) {
+        H.bin = slot;
         H.left = run - v;
-        H.sum = z;
     }
-    if (t == 0 && (far || H.n == kHist)) H.sum = z;
+    if (t == 0) H.sum = z;
     __syncthreads();
 }
 
@@ -807,7 +857,9 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
     const Row q = row_at<KIND>(P.x, P.xs, r);
     const Part* part = P.part + (int64_t)r * P.nch;
     const float* gmax = P.gmax + (int64_t)r * P.ng;
-    // the groups' maxima, a thread's first ones held (rows that have none: not used)
+    // the thread's chunk, and the groups' maxima, the first ones held (not used where
+    // the row has none)
+    const Part own = part[min(t, P.nch - 1)];
     float held[kHold];
 #pragma unroll
     for (int i = 0; i < kHold; ++i) held[i] = gmax[min(t + i * kRow, P.ng - 1)];
@@ -820,6 +872,12 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         for (int g = t + kHold * kRow; g - t < P.ng; g += kRow) f(g, g < P.ng ? gmax[g] : -INFINITY);
     };
     const Ask A = ask_of(P, r);
+    u64 bins_of[kHoldBins];
+    if (A.bins()) {
+        const u64* hist = P.hist + (int64_t)r * P.nch * kHist + (t & (kHist - 1));
+#pragma unroll
+        for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + 2 * k, P.nch - 1) * kHist];
+    }
     fill_table(H.tab);
     int a;
     if (A.greedy || A.none()) {
@@ -877,7 +935,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
     int last = kBins - 1;
     bool open = true;  // nothing is known of the row
     if (A.bins()) {
-        find_bin(P, H, part, r, A, S, top);
+        find_bin(P, H, part, own, bins_of, r, A, S, top);
         z = H.sum;
         if (H.bin >= 0) {
             open = false;
@@ -911,122 +969,119 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         }
     }
     if (open && P.vocab <= kList) open = false;  // (then all of it is gathered)
-    const bool bins = A.bins();
-    auto in = [&](float x) {
-        if (bins) return top - bin_at(x, hstep) <= (float)last || last == kBins - 1;
-        return x >= floor_m && (last == kBins - 1 || (int)fminf((m - x) * step, (float)(kBins - 1)) <= last);
+    const bool bins = A.bins() && last < kHist - 1;  // top-p's bin is known
+    const float edge = top - (float)last;
+    // 0: cannot stay; 1: may; 2 (bins): stays
+    auto kind_of = [&](float x) {
+        if (bins) {
+            const float b = bin_at(x, hstep);
+            return b > edge ? 2 : b == edge ? 1 : 0;
+        }
+        return x >= floor_m && (last == kBins - 1 || (int)fminf((m - x) * step, (float)(kBins - 1)) <= last) ? 1 : 0;
     };
     if (!open) {
         __syncthreads();
-        if (t == 0) H.n = 0;
+        if (t == 0) { H.n = 0; H.above_n = 0; H.stay = 0; H.found = 0; }
         __syncthreads();
         each_group([&](int g, float x) {
-            const bool some = x != -INFINITY && in(x);
-            const int at = place_of(some, &H.n);
-            if (some && at < 4 * kFew) H.groups[at] = g;
+            const bool some = x != -INFINITY && kind_of(x);
+            const int at = place_of(some, &H.found);
+            if (some && at < kGroups) H.groups[at] = g;
         });
         __syncthreads();
-        const int ngr = H.n;
-        __syncthreads();
-        if (t == 0) H.n = 0;
-        __syncthreads();
-        if (ngr <= 4 * kFew) {
-            for (int j0 = 0; j0 < ngr * LG; j0 += kRow) {
-                const int j = j0 + t;
-                float x[N];
-                int i0 = 0;
+        const int ngr = H.found, i0 = bins ? kAbove : 0;
+        if (ngr <= kGroups) {
+            // Eight pieces a thread in one round trip, and one copy of what is done
+            // with them (several would be fetched from memory for a run or two).
+            constexpr int U = 8;
+            const int pieces = ngr * LG;
+#pragma unroll 1
+            for (int j0 = 0; j0 < pieces; j0 += kRow * U) {
+                uint4 v[U];
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = -INFINITY;
-                if (j < ngr * LG) {
-                    const int g = H.groups[j / LG] * LG + j % LG;
-                    piece<KIND>(q, P.vocab, g, x);
-                    i0 = g * N - q.off;
+                for (int u = 0; u < U; ++u) {
+                    const int j = j0 + u * kRow + t;
+                    v[u] = make_uint4(0, 0, 0, 0);
+                    if (j < pieces) v[u] = raw_piece<KIND>(q, P.vocab, H.groups[j / LG] * LG + j % LG);
                 }
+#pragma unroll 1
+                for (int u = 0; u < U && j0 + u * kRow < pieces; ++u) {
+                    const int j = j0 + u * kRow + t;
+                    const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
+                    float x[N];
+                    unpack<KIND>(v[0], x);
+                    unsigned may = 0, does = 0;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const bool some = x[e] != -INFINITY && in(x[e]);
-                    const int at = place_of(some, &H.n);
-                    if (some && at < kList) {
-                        H.key[at] = key_of(x[e]);
-                        H.idx[at] = i0 + e;
+                    for (int e = 0; e < N; ++e) {
+                        const bool ok = x[e] != -INFINITY && i + e >= 0 && i + e < P.vocab;
+                        const int k = ok ? kind_of(x[e]) : 0;
+                        may |= (unsigned)(k == 1) << e;
+                        does |= (unsigned)(k == 2) << e;
                     }
+                    auto put = [&](unsigned bits, int* n, int at, int most) {
+                        at += place_of(__popc(bits), n);
+                        for (; bits && at < most; bits &= bits - 1, ++at) {
+                            const int e = __ffs(bits) - 1;
+                            H.key[at] = key_of(value_in<KIND>(v[0], e));
+                            H.idx[at] = i + e;
+                        }
+                    };
+                    put(may, &H.n, i0, kList);
+                    if (bins) put(does, &H.above_n, 0, kAbove);
+#pragma unroll
+                    for (int w = 0; w + 1 < U; ++w) v[w] = v[w + 1];
                 }
             }
             __syncthreads();
-            const int n = H.n;
-            if (n <= kList) {
-                if (n <= kFew) cut_and_draw_few(P, H, n, r, A, W, z);
-                else cut_and_draw(P, H, Gathered{H, n}, r, A, W, m, z);
+            const int n = H.n, above = bins ? H.above_n : 0;
+            if (n <= kList - i0 && above <= kAbove) {
+                const Gathered src{H, above, i0, n};
+                if (above + n <= kFew) cut_and_draw_few(P, H, src, r, A, W, z);
+                else cut_and_draw(P, H, src, r, A, W, m, z);
                 return;
             }
-        }
-        __syncthreads();
-    }
-    if (bins && last < kBins - 1) {
-        // Thousands stay: all above top-p's bin, whose own tokens are gathered.
-        if (t == 0) { H.n = 0; H.stay = 0; }
-        const double left = H.left;
-        __syncthreads();
-        const float edge = top - (float)last;
-        int above = 0;
-        const int pieces = (P.vocab + q.off + N - 1) / N;
-        for (int g0 = 0; g0 < pieces; g0 += kRow) {
-            float x[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = -INFINITY;
-            if (g0 + t < pieces) piece<KIND>(q, P.vocab, g0 + t, x);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float b = bin_at(x[e], hstep);
-                above += b > edge;
-                const bool some = b == edge && x[e] != -INFINITY;
-                const int at = place_of(some, &H.n);
-                if (some && at < kList) {
-                    H.key[at] = key_of(x[e]);
-                    H.idx[at] = (g0 + t) * N - q.off + e;
+            if (bins && n <= kList - kAbove) {
+                // Thousands stay: all above top-p's bin, and of its own tokens, which
+                // are gathered, those to be found.
+                const int kept = above;
+                const double left = H.left;
+                Cut cut{0, 0x7fffffff};
+                const double y = ceil((A.top_p * z - left) * W.scale);
+                if (locate<true, false>(H, Gathered{H, 0, kAbove, n}, W, cut, (edge + 1.0f) / hstep, 1.0f / hstep, P.vocab,
+                                        [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
+                    cut = H.at;
+                __syncthreads();
+                // the chunks' sums: a wave a chunk, its bins above the cut's, then those
+                // of the bin's tokens that stay
+                const int per = P.k * kThreads * N;
+                for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
+                __syncthreads();
+                int more = 0;
+                Gathered{H, 0, kAbove, n}.each([&](unsigned key, int i) {
+                    if (!stays(cut, key, i)) return;
+                    ++more;
+                    atomicAdd(&H.chunk.more[(i + q.off) / per], W(key));
+                });
+                more = (int)wave_add((u64)more);
+                if (lane == 0) atomicAdd(&H.stay, more);
+                __syncthreads();
+                for (int c = wave; c < P.nch; c += kWaves) {
+                    const Part x = part[c];
+                    const int bins_in = x.m == -INFINITY ? 0 : last - (int)fminf(top - (float)x.n, (float)kHist);
+                    u64 f = 0;
+                    for (int b = lane; b < bins_in; b += 64)
+                        f += P.hist[((int64_t)r * P.nch + c) * kHist + slot_of(x.n, b)];
+                    f = wave_add(f);
+                    if (lane == 0)
+                        H.chunk.sum[c] = (x.m == -INFINITY ? 0.0 : (double)f * 0x1p-50 * weight(x.m, S, H.tab)) +
+                                         (double)H.chunk.more[c] / W.scale;
                 }
+                __syncthreads();
+                return draw_in_chunks<KIND>(P, H, r, q, S, kept + H.stay, [&](float x, int i) {
+                    const float b = bin_at(x, hstep);
+                    return b > edge || (b == edge && stays(cut, key_of(x), i));
+                });
             }
-        }
-        u64 kept;
-        block_scan((u64)above, H.wave, kept);
-        const int n = H.n;
-        if (n <= kList) {
-            Cut cut{0, 0x7fffffff};
-            const float range = (float)fmin((double)(P.q + 1) * 0.7 / A.inv, 1e30);
-            const double y = ceil((A.top_p * z - left) * W.scale);
-            if (locate<true, false>(H, Gathered{H, n}, W, cut, m, range, P.vocab,
-                                    [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
-                cut = H.at;
-            __syncthreads();
-            // the chunks' sums: a wave a chunk, its bins above the cut's, then those
-            // of the bin's tokens that stay
-            const int per = P.k * kThreads * N;
-            for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
-            __syncthreads();
-            int more = 0;
-            Gathered{H, n}.each([&](unsigned key, int i) {
-                if (!stays(cut, key, i)) return;
-                ++more;
-                atomicAdd(&H.chunk.more[(i + q.off) / per], W(key));
-            });
-            more = (int)wave_add((u64)more);
-            if (lane == 0) atomicAdd(&H.stay, more);
-            __syncthreads();
-            for (int c = wave; c < P.nch; c += kWaves) {
-                const Part x = part[c];
-                const int bins_in = x.m == -INFINITY ? 0 : last - (int)fminf(top - (float)x.n, (float)kHist);
-                u64 f = 0;
-                for (int b = lane; b < bins_in; b += 64) f += P.hist[((int64_t)r * P.nch + c) * kHist + b];
-                f = wave_add(f);
-                if (lane == 0)
-                    H.chunk.sum[c] = (x.m == -INFINITY ? 0.0 : (double)f * 0x1p-50 * weight(x.m, S, H.tab)) +
-                                     (double)H.chunk.more[c] / W.scale;
-            }
-            __syncthreads();
-            return draw_in_chunks<KIND>(P, H, r, q, S, (int)kept + H.stay, [&](float x, int i) {
-                const float b = bin_at(x, hstep);
-                return b > edge || (b == edge && stays(cut, key_of(x), i));
-            });
         }
         __syncthreads();
     }
