@@ -62,7 +62,7 @@ constexpr int kThreads = 256;  // of launch 1
 constexpr int kRow = 512;      // of launch 2
 constexpr int kWaves = kRow / 64;
 constexpr int kBins = 1024;
-constexpr int kFew = 192;      // tokens that compare themselves with each other
+constexpr int kFew = 128;      // tokens that compare themselves with each other
 constexpr int kList = 4096;    // tokens gathered from a row; under top-p alone
 constexpr int kAbove = 1024;   // the first of these are for those above its bin
 constexpr int kGroup = 64;     // logits of a group
@@ -273,6 +273,7 @@ __device__ __forceinline__ bool stays(const Cut& c, unsigned key, int i) {
     return key > c.key || (key == c.key && i <= c.idx);
 }
 constexpr int kGroups = 2048;  // groups that are read again, at most
+constexpr int kHoldBins = 10;  // chunks whose bins a thread holds
 
 struct RowShared {
     double tab[64];
@@ -304,6 +305,9 @@ struct RowShared {
     unsigned lo, hi;
     u64 above, total;
     double left, sum;
+    int down[2 * kHoldBins];  // the first chunks' bins below the row's
+    double weight[2 * kHoldBins];  // of their maxima
+    u64 first[2 * kHoldBins]; // the sums of their bins above top-p's
     float x;
     Cut at;
 };
@@ -392,6 +396,12 @@ __device__ __forceinline__ float value_in(const uint4& v, int e) {
     if (KIND == VGX_E_Q16) return (float)(short)u * (1.0f / 256);
     if (KIND == VGX_E_BF16) return clean(__uint_as_float(u << 16));
     return clean((float)__builtin_bit_cast(_Float16, (unsigned short)u));
+}
+// Which of a piece's n values, the first of index i, are inside the row.
+__device__ __forceinline__ unsigned ends_of(int i, int n, int vocab) {
+    unsigned r = 0;
+    for (int e = 0; e < n; ++e) r |= (unsigned)(i + e >= 0 && i + e < vocab) << e;
+    return r;
 }
 // f(value, index) of a piece's values inside the row, one after the other: a loop
 // that shifts them down, as many copies of a long f would not stay in the
@@ -781,10 +791,24 @@ __device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, con
     return m;
 }
 
+// The least float of a bin; false where its search is long (products that
+// underflow).
+__device__ __forceinline__ bool first_in(float bin, float step, float& x) {
+    auto next = [](float y, int d) {
+        const unsigned k = key_of(y) + d;
+        return value_of(k == 0x7fffffffu && d < 0 ? k - 1 : k);  // (-0 is 0)
+    };
+    x = bin / step;
+    if (!(fabsf(x) < FLT_MAX)) return false;
+    int n = 0;
+    while (n < 64 && bin_at(x, step) < bin) { x = next(x, 1); ++n; }
+    while (n < 64 && bin_at(next(x, -1), step) >= bin) { x = next(x, -1); ++n; }
+    return n < 64;
+}
+
 // Top-p's bin from the chunks' bins: H.bin (-1: none of them, or they are not
 // whole), the weights above it H.left, all weights H.sum.  held: the thread's slot
 // of its first chunks (every second one: half the threads take the others).
-constexpr int kHoldBins = 10;
 __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, const Part* part, const Part& own,
                                          const u64 (&held)[kHoldBins], int r, const Ask& A, const Scale& S, float top) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, slot = t & (kHist - 1), half = t / kHist;
@@ -801,6 +825,10 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
             if (some && x.n == 0x7fffffff) far = true;
             H.merge.f[t] = f;
             H.merge.down[t] = some && !far ? (int)fminf(top - (float)x.n, (float)kHist) : kHist;
+            if (c0 == 0 && t < 2 * kHoldBins) {
+                H.down[t] = H.merge.down[t];
+                H.weight[t] = f;
+            }
             z += x.z * f;
         }
         __syncthreads();
@@ -968,33 +996,47 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
             last = H.bin;
         }
     }
-    if (open && P.vocab <= kList) open = false;  // (then all of it is gathered)
-    const bool bins = A.bins() && last < kHist - 1;  // top-p's bin is known
+    bool bins = A.bins() && last < kHist - 1;  // top-p's bin is known
+    // What may stay is lo or more, what does (bins) hi or more.
+    float lo = -FLT_MAX, hi = INFINITY;
     const float edge = top - (float)last;
-    // 0: cannot stay; 1: may; 2 (bins): stays
-    auto kind_of = [&](float x) {
-        if (bins) {
-            const float b = bin_at(x, hstep);
-            return b > edge ? 2 : b == edge ? 1 : 0;
-        }
-        return x >= floor_m && (last == kBins - 1 || (int)fminf((m - x) * step, (float)(kBins - 1)) <= last) ? 1 : 0;
-    };
+    if (bins) {
+        bins = first_in(edge, hstep, lo) && first_in(edge + 1.0f, hstep, hi);
+        open = !bins;
+        if (open) hi = INFINITY;
+    } else if (floor_m > -INFINITY) {
+        lo = fmaxf(floor_m, -FLT_MAX);
+    } else if (last < kBins - 1) {  // (a rounding below the bin's border)
+        lo = fmaxf(m - (float)(last + 1) / step * 1.000001f - fabsf(m) * 1e-6f, -FLT_MAX);
+    }
+    if (open && P.vocab <= kList) {  // all of it is gathered
+        open = false;
+        lo = -FLT_MAX;
+    }
     if (!open) {
         __syncthreads();
         if (t == 0) { H.n = 0; H.above_n = 0; H.stay = 0; H.found = 0; }
         __syncthreads();
         each_group([&](int g, float x) {
-            const bool some = x != -INFINITY && kind_of(x);
+            const bool some = x >= lo;
             const int at = place_of(some, &H.found);
             if (some && at < kGroups) H.groups[at] = g;
+            const int sure = __popcll(__ballot(x >= hi));
+            if (sure && lane == 0) atomicAdd(&H.stay, sure);
         });
         __syncthreads();
+        // (groups with a token above top-p's bin: past half the list's room those
+        // tokens are only counted)
         const int ngr = H.found, i0 = bins ? kAbove : 0;
+        const bool many = H.stay > kAbove / 2;
+        __syncthreads();
+        if (t == 0) H.stay = 0;
         if (ngr <= kGroups) {
-            // Eight pieces a thread in one round trip, and one copy of what is done
-            // with them (several would be fetched from memory for a run or two).
-            constexpr int U = 8;
+            // Pieces in one round trip, and one copy of what is done with them
+            // (several would be fetched from memory for a run or two).
+            constexpr int U = 4;
             const int pieces = ngr * LG;
+            int sure = 0;
 #pragma unroll 1
             for (int j0 = 0; j0 < pieces; j0 += kRow * U) {
                 uint4 v[U];
@@ -1002,22 +1044,29 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                 for (int u = 0; u < U; ++u) {
                     const int j = j0 + u * kRow + t;
                     v[u] = make_uint4(0, 0, 0, 0);
-                    if (j < pieces) v[u] = raw_piece<KIND>(q, P.vocab, H.groups[j / LG] * LG + j % LG);
+                    const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
+                    if (i >= 0 && i + N <= P.vocab)
+                        v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i * kBytes<KIND>);
                 }
 #pragma unroll 1
                 for (int u = 0; u < U && j0 + u * kRow < pieces; ++u) {
                     const int j = j0 + u * kRow + t;
                     const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
+                    unsigned inside = (1u << N) - 1;
+                    if (i < 0 || i + N > P.vocab) {  // (a row's ends)
+                        inside = ends_of(i, N, P.vocab);
+                        if (inside) v[0] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
+                    }
                     float x[N];
                     unpack<KIND>(v[0], x);
                     unsigned may = 0, does = 0;
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
-                        const bool ok = x[e] != -INFINITY && i + e >= 0 && i + e < P.vocab;
-                        const int k = ok ? kind_of(x[e]) : 0;
-                        may |= (unsigned)(k == 1) << e;
-                        does |= (unsigned)(k == 2) << e;
+                        may |= (unsigned)(x[e] >= lo) << e;
+                        does |= (unsigned)(x[e] >= hi) << e;
                     }
+                    does &= inside;
+                    may = may & inside & ~does;
                     auto put = [&](unsigned bits, int* n, int at, int most) {
                         at += place_of(__popc(bits), n);
                         for (; bits && at < most; bits &= bits - 1, ++at) {
@@ -1027,14 +1076,21 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                         }
                     };
                     put(may, &H.n, i0, kList);
-                    if (bins) put(does, &H.above_n, 0, kAbove);
+                    if (bins) {
+                        if (many) sure += __popc(does);
+                        else put(does, &H.above_n, 0, kAbove);
+                    }
 #pragma unroll
                     for (int w = 0; w + 1 < U; ++w) v[w] = v[w + 1];
                 }
             }
+            if (many) {
+                sure = (int)wave_add((u64)sure);
+                if (lane == 0) atomicAdd(&H.above_n, sure);
+            }
             __syncthreads();
             const int n = H.n, above = bins ? H.above_n : 0;
-            if (n <= kList - i0 && above <= kAbove) {
+            if (n <= kList - i0 && above <= kAbove && !many) {
                 const Gathered src{H, above, i0, n};
                 if (above + n <= kFew) cut_and_draw_few(P, H, src, r, A, W, z);
                 else cut_and_draw(P, H, src, r, A, W, m, z);
@@ -1051,10 +1107,11 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                                         [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
                     cut = H.at;
                 __syncthreads();
-                // the chunks' sums: a wave a chunk, its bins above the cut's, then those
-                // of the bin's tokens that stay
+                // the chunks' sums: their bins above the cut's (the first chunks' are
+                // held), then those of the bin's tokens that stay
                 const int per = P.k * kThreads * N;
                 for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
+                if (t < 2 * kHoldBins) H.first[t] = 0;
                 __syncthreads();
                 int more = 0;
                 Gathered{H, 0, kAbove, n}.each([&](unsigned key, int i) {
@@ -1064,22 +1121,31 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                 });
                 more = (int)wave_add((u64)more);
                 if (lane == 0) atomicAdd(&H.stay, more);
+                const int mine = ((int)top - t) & (kHist - 1);
+#pragma unroll
+                for (int k = 0; k < kHoldBins; ++k) {
+                    const int c = t / kHist + 2 * k;
+                    if (c >= P.nch) continue;
+                    const int at = mine - H.down[c];
+                    const u64 f = wave_add(at >= 0 && at < kHist - 1 && mine < last ? bins_of[k] : 0);
+                    if (lane == 0 && f) atomicAdd(&H.first[c], f);
+                }
                 __syncthreads();
-                for (int c = wave; c < P.nch; c += kWaves) {
-                    const Part x = part[c];
-                    const int bins_in = x.m == -INFINITY ? 0 : last - (int)fminf(top - (float)x.n, (float)kHist);
+                if (t < min(P.nch, 2 * kHoldBins))
+                    H.chunk.sum[t] = (double)H.first[t] * 0x1p-50 * H.weight[t] + (double)H.chunk.more[t] / W.scale;
+                for (int c = 2 * kHoldBins + wave; c < P.nch; c += kWaves) {
+                    const float cm = part[c].m;
+                    const int n = part[c].n, bins_in = cm == -INFINITY ? 0 : last - (int)fminf(top - (float)n, (float)kHist);
                     u64 f = 0;
                     for (int b = lane; b < bins_in; b += 64)
-                        f += P.hist[((int64_t)r * P.nch + c) * kHist + slot_of(x.n, b)];
+                        f += P.hist[((int64_t)r * P.nch + c) * kHist + slot_of(n, b)];
                     f = wave_add(f);
                     if (lane == 0)
-                        H.chunk.sum[c] = (x.m == -INFINITY ? 0.0 : (double)f * 0x1p-50 * weight(x.m, S, H.tab)) +
-                                         (double)H.chunk.more[c] / W.scale;
+                        H.chunk.sum[c] = (double)f * 0x1p-50 * weight(cm, S, H.tab) + (double)H.chunk.more[c] / W.scale;
                 }
                 __syncthreads();
                 return draw_in_chunks<KIND>(P, H, r, q, S, kept + H.stay, [&](float x, int i) {
-                    const float b = bin_at(x, hstep);
-                    return b > edge || (b == edge && stays(cut, key_of(x), i));
+                    return x >= hi || (x >= lo && stays(cut, key_of(x), i));
                 });
             }
         }
