@@ -1157,6 +1157,8 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
 // rows and 8 at 16000 positions, 117 us (178 as tiles only, 136 in two launches);
 // 20 sequences of 1 .. 700 rows, window 1024, 16 / 8 heads of 64, 21 us, the
 // longest tile's chain.
+template <int HD, bool TREE>
+constexpr int both_nb = !TREE ? 1 : HD == 64 ? 3 : 2;  // blocks of 16 columns of the rows' way
 struct BothArgs {
     AttnArgs rows, tile;
     int rows_wgs, tile_wgs;   // workgroups of one split
@@ -1170,7 +1172,7 @@ __global__ void __launch_bounds__(256, EX ? 2 : 1) paged_both_kernel(const BothA
         tile_body<KIND, HD, EX, TREE>(B.tile, bx - split * B.tile_wgs, B.tile_wgs, split);
     } else {
         const int r = bx - B.tile_all, split = r / B.rows_wgs;
-        rows_body<KIND, HD, EX, 1, 4, TREE>(B.rows, r - split * B.rows_wgs, split);
+        rows_body<KIND, HD, EX, both_nb<HD, TREE>, 4, TREE>(B.rows, r - split * B.rows_wgs, split);
     }
 }
 
@@ -1326,6 +1328,12 @@ void fn_of(const PagedDev& A, int64_t cols, bool few, Launch& p) {
     return hd <= 128 ? fn_of<KIND, 128, false, TREE>(cols, few, p) : fn_of<KIND, 256, false, TREE>(cols, few, p);
 }
 
+// The head size that fn_of's kernel has room for.
+int fn_hd(const PagedDev& A) {
+    const bool whole = A.psize % 16 == 0 && A.krow < (1 << 26) && A.vrow < (1 << 26);
+    return whole && (A.hd == 64 || A.hd == 96) ? A.hd : A.hd <= 128 ? 128 : 256;
+}
+
 // The columns the rows kernel takes at most.
 int64_t max_cols(const PagedDev& A) { return A.hd <= 128 ? 48 : 16; }
 
@@ -1347,7 +1355,8 @@ Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t co
     p.cmax = p.rows ? p.tm : INT32_MAX;
     // (a sequence of more than cmin columns has at most columns / tm + 1 tiles)
     const int64_t all = (int64_t)A.ntok * A.grp;
-    const int64_t tiles = p.rows ? A.nseq : all / p.tm + std::min<int64_t>(A.nseq, std::max<int64_t>(all / (cmin + 1), 1));
+    int64_t tiles = p.rows ? A.nseq : all / p.tm + std::min<int64_t>(A.nseq, std::max<int64_t>(all / (cmin + 1), 1));
+    if (TREE && !p.rows) tiles = std::min<int64_t>(tiles, A.nseq * ((cols + p.tm - 1) / p.tm));
     p.wgs = tiles * A.kvh;
     // Splits.  A workgroup of the rows kernel costs about 8 us before and after
     // its keys (the tables' and first rows' round trips, the join of its waves),
@@ -1364,6 +1373,15 @@ Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t co
     int64_t len = std::max<int64_t>((span + want - 1) / want, 256);
     if (p.rows && A.nseq > 1)
         len = span <= kWhole ? span : std::min<int64_t>(std::max<int64_t>(len, 512), p.wgs >= num_cu ? 1024 : 768);
+    // Trees: the tile kernel's launch is small (a tile or two a sequence and KV
+    // head), so its sequences are split as well, to 1024 keys or a sixteenth of
+    // the longest (whose parts the join has to read): 24 trees of 5 to 61 rows at
+    // 300 to 8000, 16 / 8 heads of 64, 59 us (75 by the rule above, 74 at 512
+    // keys, 61 at 2048); 2 of 64 rows at 60001, 32 / 8 of 128, 207 (251; 290 at
+    // 1024).  The rows kernel beside it takes 1024 too (768: 3 us more).
+    if (TREE && A.nseq > 1 && !alone && p.rows) len = std::max<int64_t>(len, 1024);
+    if (TREE && A.nseq > 1 && !p.rows)
+        len = std::min<int64_t>(std::max<int64_t>(len, 512), std::max<int64_t>(1024, span / 16));
     len = (len + 127) / 128 * 128;
     if (p.threads == 512) len = std::max<int64_t>(span, 128);
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
@@ -1393,9 +1411,11 @@ Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     Plan p{};
     const int64_t cols = (int64_t)A.max_q * A.grp;
     const int64_t least = A.ntok - (int64_t)(A.nseq - 1) * A.max_q;  // rows of the shortest sequence, if all others are full
-    if (cols > max_cols(A) && A.hd <= 128 && A.grp <= 16 && A.nseq > 1 && least * A.grp <= 16) {
-        p.l[0] = launch_of<TREE>(A, kind, window, num_cu, 16, 0, false);
-        p.l[1] = launch_of<TREE>(A, kind, window, num_cu, cols, 16, false);
+    // (the columns of the rows' way: what fn_of's kernels have for these heads)
+    const int rows = 16 * (fn_hd(A) == 64 ? both_nb<64, TREE> : both_nb<128, TREE>);
+    if (cols > max_cols(A) && A.hd <= 128 && A.grp <= rows && A.nseq > 1 && least * A.grp <= rows) {
+        p.l[0] = launch_of<TREE>(A, kind, window, num_cu, rows, 0, false);
+        p.l[1] = launch_of<TREE>(A, kind, window, num_cu, cols, rows, false);
         p.n = 2;
         p.by_seq = 1;
     } else {
