@@ -140,7 +140,7 @@ def test_copy():
 
 
 @pytest.mark.parametrize("kw, what", [
-    (dict(nrows=-1), "nrows"), (dict(nrows=(1 << 20) + 1), "nrows"), (dict(vocab=0), "vocab"),
+    (dict(nrows=-1), "nrows"), (dict(nrows=65536), "nrows"), (dict(vocab=0), "vocab"),
     (dict(vocab=(1 << 21) + 1, stride=1 << 22), "vocab"), (dict(kind=vl.E_Q8), "f32, bf16"), (dict(kind=0), "f32, bf16"),
     (dict(logits=0), "NULL"), (dict(u=0), "NULL"), (dict(token=0), "NULL"), (dict(stride=99), "stride"),
     (dict(stride=1 << 41), "stride"), (dict(logits=BUF + 2), "aligned"),
@@ -150,11 +150,14 @@ def test_sample(kw, what):
 
 
 def test_sample_workspace():
-    need = L.vgx_sample_ws(3, 100, vl.E_F32)
-    if need:
-        bad(sample(ws=0), "workspace")
-        bad(sample(ws_bytes=need - 1), "workspace")
-        bad(sample(ws=BUF + 8), "workspace")
+    kw = dict(vocab=20000, stride=20000)
+    need = L.vgx_sample_ws(3, 20000, vl.E_F32)
+    assert need > 0
+    bad(sample(ws=0, **kw), "workspace")
+    bad(sample(ws_bytes=need - 1, **kw), "workspace")
+    bad(sample(ws=BUF + 8, **kw), "workspace")
+    assert sample(ws_bytes=need, **kw)[1].endswith("no context")
+    assert L.vgx_sample_ws(3, 100, vl.E_F32) == 0 and sample(ws=0, ws_bytes=0)[1].endswith("no context")
     assert L.vgx_sample_ws(3, 0, vl.E_F32) == 0 and L.vgx_sample_ws(-1, 10, vl.E_F32) == 0
     assert said(L.vgx_sample, None)[0] == vl.VGX_EINVAL
 

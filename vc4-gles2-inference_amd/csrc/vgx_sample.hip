@@ -308,6 +308,7 @@ struct RowShared {
     int down[2 * kHoldBins];  // the first chunks' bins below the row's
     double weight[2 * kHoldBins];  // of their maxima
     u64 first[2 * kHoldBins]; // the sums of their bins above top-p's
+    Part one;
     float x;
     Cut at;
 };
@@ -770,7 +771,7 @@ __device__ __forceinline__ void draw_in_chunks(const SampleArgs& P, RowShared& H
         if (P.prob) P.prob[r] = (float)(weight(H.x, S, H.tab) / H.sum);
     }
 }
-static_assert(4 * kThreads / kRow * 8 <= 64, "a thread's values of a chunk: a lane each");
+static_assert(4 * kThreads / kRow * 8 <= 64 && 8192 / kRow <= 64, "a thread's values of a chunk: a lane each");
 
 // The maximum of a row's chunks, and (greedy) its first index.
 __device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, const Part* part, bool first, int& a) {
@@ -877,36 +878,145 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
     __syncthreads();
 }
 
+// What launch 1 does, for a row that this launch holds whole: its groups' maxima
+// (a group is a piece: u * kRow + t of thread t), the one chunk's statistics (H.one) and
+// the thread's slot of its bins.
+template <int KIND, int U>
+__device__ __forceinline__ void read_row(const SampleArgs& P, RowShared& H, int r, const Row& q, float (&gm)[U], Part& own,
+                                         u64& slot) {
+    constexpr int N = kPer<KIND>;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i0 = (u * kRow + t) * N - q.off;
+        raw[u] = make_uint4(0, 0, 0, 0);
+        if (i0 >= 0 && i0 + N <= P.vocab) raw[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i0 * kBytes<KIND>);
+    }
+    const Ask A = ask_of(P, r);
+    fill_table(H.tab);
+    if (t < kHist) H.h.sum[t] = 0;
+    float x[U][N], m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i0 = (u * kRow + t) * N - q.off;
+        unpack<KIND>(raw[u], x[u]);
+        if (!(i0 >= 0 && i0 + N <= P.vocab)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[u][e] = i0 + e >= 0 && i0 + e < P.vocab ? one<KIND>(q.p, i0 + e) : -INFINITY;
+        }
+        gm[u] = x[u][0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) gm[u] = fmaxf(gm[u], x[u][e]);
+        m = fmaxf(m, gm[u]);
+    }
+    m = wave_max(m);
+    if (lane == 0) H.m[wave] = m;
+    if (t == 0) { H.found = 0x7fffffff; H.n = 0; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, H.m[w]);
+    own = Part{m, 0x7fffffff, 0, 0, 0.0};
+    slot = 0;
+    if (A.greedy) {
+        int a = 0x7fffffff;
+#pragma unroll
+        for (int u = U - 1; u >= 0; --u)
+#pragma unroll
+            for (int e = N - 1; e >= 0; --e)
+                if (x[u][e] == m) a = (u * kRow + t) * N - q.off + e;
+        if (a != 0x7fffffff) atomicMin(&H.found, a);
+    }
+    if (A.sum() && m != -INFINITY) {
+        const Scale S = scale_of(m, A.inv);
+        const float step = A.step(), top = bin_at(m, step);
+        const bool bins = A.bins();
+        double z = 0.0;
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double w = add_pow(fmax(((double)x[u][e] - S.m) * S.a, -63700.0), 0.0, H.tab);
+                if (bins) {
+                    const u64 f = fixed(w, 0x1p50);
+                    if (f) atomicAdd(&H.h.sum[(int)fminf(top - bin_at(x[u][e], step), (float)(kHist - 1))], f);
+                } else {
+                    z += w;
+                    n += x[u][e] != -INFINITY;
+                }
+            }
+        __syncthreads();
+        if (bins) {
+            own.n = fabsf(m * step) < kFar ? (int)top : 0x7fffffff;
+            if (t < kHist) slot = H.h.sum[(own.n - t) & (kHist - 1)];
+            const u64 f = wave_add(t < kHist ? slot : 0);
+            z = (double)f * 0x1p-50;
+        } else {
+            z = wave_sum(z);
+            n = (int)wave_add((u64)n);
+        }
+        if (lane == 0) {
+            H.wave[wave] = __builtin_bit_cast(u64, z);
+            if (!bins) atomicAdd(&H.n, n);
+        }
+    }
+    __syncthreads();
+    if (A.sum() && m != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) own.z += __builtin_bit_cast(double, H.wave[w]);
+        if (!A.bins()) own.n = H.n;
+    }
+    own.arg = H.found;
+    if (t == 0) H.one = own;
+    __syncthreads();
+}
+
+// WHOLE: a row of up to kSmall pieces, which one launch reads and decides.
 template <int KIND>
+constexpr int kSmall = 8192 / kPer<KIND>;
+template <int KIND, bool WHOLE>
 __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
-    constexpr int N = kPer<KIND>, LG = kGroup / N, kHold = 3;
+    constexpr int N = kPer<KIND>, LG = WHOLE ? 1 : kGroup / N, kHold = WHOLE ? kSmall<KIND> / kRow : 3;
     __shared__ RowShared H;
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Row q = row_at<KIND>(P.x, P.xs, r);
-    const Part* part = P.part + (int64_t)r * P.nch;
+    const Part* part = WHOLE ? &H.one : P.part + (int64_t)r * P.nch;
     const float* gmax = P.gmax + (int64_t)r * P.ng;
     // the thread's chunk, and the groups' maxima, the first ones held (not used where
     // the row has none)
-    const Part own = part[min(t, P.nch - 1)];
+    Part own;
     float held[kHold];
+    u64 bins_of[kHoldBins];
+    if constexpr (WHOLE) {
+        read_row<KIND, kHold>(P, H, r, q, held, own, bins_of[0]);
+    } else {
+        own = part[min(t, P.nch - 1)];
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) held[i] = gmax[min(t + i * kRow, P.ng - 1)];
+        for (int i = 0; i < kHold; ++i) held[i] = gmax[min(t + i * kRow, P.ng - 1)];
+    }
     auto each_group = [&](auto f) {
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int i = 0; i < kHold; ++i) {
-            const bool in = t + i * kRow < P.ng;
-            f(t + i * kRow, in ? held[i] : -INFINITY);
+            for (int i = 0; i < kHold; ++i) f(i * kRow + t, held[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kHold; ++i) {
+                const bool in = t + i * kRow < P.ng;
+                f(t + i * kRow, in ? held[i] : -INFINITY);
+            }
+            for (int g = t + kHold * kRow; g - t < P.ng; g += kRow) f(g, g < P.ng ? gmax[g] : -INFINITY);
         }
-        for (int g = t + kHold * kRow; g - t < P.ng; g += kRow) f(g, g < P.ng ? gmax[g] : -INFINITY);
     };
     const Ask A = ask_of(P, r);
-    u64 bins_of[kHoldBins];
-    if (A.bins()) {
-        const u64* hist = P.hist + (int64_t)r * P.nch * kHist + (t & (kHist - 1));
+    if constexpr (!WHOLE) {
+        if (A.bins()) {
+            const u64* hist = P.hist + (int64_t)r * P.nch * kHist + (t & (kHist - 1));
 #pragma unroll
-        for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + 2 * k, P.nch - 1) * kHist];
+            for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + 2 * k, P.nch - 1) * kHist];
+        }
+        fill_table(H.tab);
     }
-    fill_table(H.tab);
     int a;
     if (A.greedy || A.none()) {
         const float m = join_max(P, H, part, A.greedy, a);
@@ -1162,6 +1272,11 @@ struct Chunks {
 Chunks chunks_of(int nrows, int vocab, int kind) {
     const int per = kind == VGX_E_F32 ? 4 : 8;
     Chunks c;
+    if (vocab + per - 1 <= 8192) {  // one launch
+        c.k = 8192 / per / kThreads;
+        c.nch = c.ng = 0;
+        return c;
+    }
     c.k = 1;
     c.nch = (vocab + per - 1 + per * kThreads - 1) / (per * kThreads);
     if ((int64_t)nrows * c.nch > 1024) {
@@ -1174,9 +1289,13 @@ Chunks chunks_of(int nrows, int vocab, int kind) {
 
 template <int KIND>
 void launch(const SampleArgs& P, hipStream_t st) {
+    if (P.ng == 0) {
+        hipLaunchKernelGGL((sample_pick_kernel<KIND, true>), dim3(P.nrows), dim3(kRow), 0, st, P);
+        return;
+    }
     hipLaunchKernelGGL((P.k == 1 ? sample_stats_kernel<KIND, 1> : sample_stats_kernel<KIND, 4>), dim3(P.nch, P.nrows),
                        dim3(kThreads), 0, st, P);
-    hipLaunchKernelGGL(sample_pick_kernel<KIND>, dim3(P.nrows), dim3(kRow), 0, st, P);
+    hipLaunchKernelGGL((sample_pick_kernel<KIND, false>), dim3(P.nrows), dim3(kRow), 0, st, P);
 }
 
 bool kind_ok(int k) { return k == VGX_E_F32 || k == VGX_E_BF16 || k == VGX_E_F16 || k == VGX_E_Q16; }
@@ -1218,7 +1337,7 @@ int vgx_sample(vgx_ctx* ctx, const vgx_sampling* a) {
     int lg = 0;
     while ((1 << lg) < a->vocab) ++lg;
     P.q = std::min(50, 62 - lg);
-    P.nch = c.nch; P.k = c.k; P.ng = c.ng;
+    P.nch = std::max(c.nch, 1); P.k = c.k; P.ng = c.ng;
     P.hist = static_cast<u64*>(a->ws);
     P.part = reinterpret_cast<Part*>(P.hist + (size_t)a->nrows * c.nch * kHist);
     P.gmax = reinterpret_cast<float*>(P.part + (size_t)a->nrows * c.nch);
