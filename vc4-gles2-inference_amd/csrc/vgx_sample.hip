@@ -61,13 +61,15 @@ struct SampleArgs {
 constexpr int kThreads = 256;  // of launch 1
 constexpr int kRow = 512;      // of launch 2
 constexpr int kWaves = kRow / 64;
-constexpr int kBins = 1024;
+constexpr int kBinBits = 10, kBins = 1 << kBinBits;
+static_assert(kBins == 2 * kRow, "two bins a thread");
 constexpr int kFew = 128;      // tokens that compare themselves with each other
 constexpr int kList = 4096;    // tokens gathered from a row; under top-p alone
 constexpr int kAbove = 1024;   // the first of these are for those above its bin
 constexpr int kGroup = 64;     // logits of a group
 constexpr int kHist = kThreads; // bins of a chunk; the last holds all below
-constexpr int kMaxChunks = 1024;
+constexpr int kMaxChunks = 520;
+constexpr int kSides = kRow / kHist;  // of a launch 2's threads, chunks by turns
 constexpr int kMaxVocab = 1 << 21;
 
 // What a row asks for.
@@ -295,7 +297,7 @@ struct RowShared {
             u64 more[kMaxChunks];
         } chunk;
         struct {
-            double f[kRow], part[2][kHist], wave[4];
+            double f[kRow], part[kSides][kHist], wave[4];
             int down[kRow];
         } merge;
     };
@@ -305,9 +307,9 @@ struct RowShared {
     unsigned lo, hi;
     u64 above, total;
     double left, sum;
-    int down[2 * kHoldBins];  // the first chunks' bins below the row's
-    double weight[2 * kHoldBins];  // of their maxima
-    u64 first[2 * kHoldBins]; // the sums of their bins above top-p's
+    int down[kSides * kHoldBins];  // the first chunks' bins below the row's
+    double weight[kSides * kHoldBins];  // of their maxima
+    u64 first[kSides * kHoldBins]; // the sums of their bins above top-p's
     Part one;
     float x;
     Cut at;
@@ -500,7 +502,7 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
     u64 before = 0, want = 0;
 #pragma unroll 1
     for (bool first = true;; first = false) {
-        const int sh = mode == VALUE ? 0 : max(0, 32 - __clz((int)(hi - lo)) - 10);
+        const int sh = mode == VALUE ? 0 : max(0, 32 - __clz((int)(hi - lo)) - kBinBits);
         auto bin_of = [&](unsigned key, int i) -> int {
             if (!stays(in, key, i)) return -1;
             if (mode == VALUE) return kBins - 1 - (int)fminf(fmaxf((m - value_of(key)) * step, 0.0f), (float)(kBins - 1));
@@ -809,7 +811,7 @@ __device__ __forceinline__ bool first_in(float bin, float step, float& x) {
 
 // Top-p's bin from the chunks' bins: H.bin (-1: none of them, or they are not
 // whole), the weights above it H.left, all weights H.sum.  held: the thread's slot
-// of its first chunks (every second one: half the threads take the others).
+// of its first chunks (every kSides-th one).
 __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, const Part* part, const Part& own,
                                          const u64 (&held)[kHoldBins], int r, const Ask& A, const Scale& S, float top) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, slot = t & (kHist - 1), half = t / kHist;
@@ -826,7 +828,7 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
             if (some && x.n == 0x7fffffff) far = true;
             H.merge.f[t] = f;
             H.merge.down[t] = some && !far ? (int)fminf(top - (float)x.n, (float)kHist) : kHist;
-            if (c0 == 0 && t < 2 * kHoldBins) {
+            if (c0 == 0 && t < kSides * kHoldBins) {
                 H.down[t] = H.merge.down[t];
                 H.weight[t] = f;
             }
@@ -841,10 +843,10 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
         if (c0 == 0) {
 #pragma unroll
             for (int k = 0; k < kHoldBins; ++k)
-                if (half + 2 * k < n) add(half + 2 * k, held[k]);
+                if (half + kSides * k < n) add(half + kSides * k, held[k]);
         }
 #pragma unroll 4
-        for (int c = half + (c0 ? 0 : 2 * kHoldBins); c < n; c += 2) add(c, hist[(int64_t)(c0 + c) * kHist]);
+        for (int c = half + (c0 ? 0 : kSides * kHoldBins); c < n; c += kSides) add(c, hist[(int64_t)(c0 + c) * kHist]);
     }
     // (z: threads in order; a row of up to 512 chunks has one each)
     z = wave_sum(z);
@@ -860,7 +862,7 @@ __device__ __forceinline__ void find_bin(const SampleArgs& P, RowShared& H, cons
         z += __builtin_bit_cast(double, H.wave[w]);
         far = far || H.a[w];
     }
-    v = half ? 0.0 : (H.merge.part[0][slot] + H.merge.part[1][slot]) * 0x1p-50;
+    v = half ? 0.0 : (H.merge.part[0][slot] + (kSides > 1 ? H.merge.part[kSides - 1][slot] : 0.0)) * 0x1p-50;
     double run = wave_scan(v);
     if (!half && lane == 63) H.merge.wave[wave] = run;
     __syncthreads();
@@ -1013,7 +1015,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         if (A.bins()) {
             const u64* hist = P.hist + (int64_t)r * P.nch * kHist + (t & (kHist - 1));
 #pragma unroll
-            for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + 2 * k, P.nch - 1) * kHist];
+            for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + kSides * k, P.nch - 1) * kHist];
         }
         fill_table(H.tab);
     }
@@ -1159,30 +1161,39 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                         v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i * kBytes<KIND>);
                 }
 #pragma unroll 1
-                for (int u = 0; u < U && j0 + u * kRow < pieces; ++u) {
-                    const int j = j0 + u * kRow + t;
-                    const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
-                    unsigned inside = (1u << N) - 1;
-                    if (i < 0 || i + N > P.vocab) {  // (a row's ends)
-                        inside = ends_of(i, N, P.vocab);
-                        if (inside) v[0] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
-                    }
-                    float x[N];
-                    unpack<KIND>(v[0], x);
+                for (int u = 0; u < U && j0 + u * kRow < pieces; u += 2) {  // two a time
                     unsigned may = 0, does = 0;
+                    int at0[2];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        may |= (unsigned)(x[e] >= lo) << e;
-                        does |= (unsigned)(x[e] >= hi) << e;
+                    for (int w = 0; w < 2; ++w) {
+                        const int j = j0 + (u + w) * kRow + t;
+                        const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
+                        at0[w] = i;
+                        unsigned inside = (1u << N) - 1;
+                        if (i < 0 || i + N > P.vocab) {  // (a row's ends)
+                            inside = ends_of(i, N, P.vocab);
+                            if (inside) v[w] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
+                        }
+                        float x[N];
+                        unpack<KIND>(v[w], x);
+                        unsigned a = 0, b = 0;
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            a |= (unsigned)(x[e] >= lo) << e;
+                            b |= (unsigned)(x[e] >= hi) << e;
+                        }
+                        may |= (a & inside & ~b) << N * w;
+                        does |= (b & inside) << N * w;
                     }
-                    does &= inside;
-                    may = may & inside & ~does;
                     auto put = [&](unsigned bits, int* n, int at, int most) {
                         at += place_of(__popc(bits), n);
                         for (; bits && at < most; bits &= bits - 1, ++at) {
-                            const int e = __ffs(bits) - 1;
-                            H.key[at] = key_of(value_in<KIND>(v[0], e));
-                            H.idx[at] = i + e;
+                            const int k = __ffs(bits) - 1, e = k & (N - 1);
+                            const bool second = k >= N;
+                            const uint4 y = make_uint4(second ? v[1].x : v[0].x, second ? v[1].y : v[0].y,
+                                                       second ? v[1].z : v[0].z, second ? v[1].w : v[0].w);
+                            H.key[at] = key_of(value_in<KIND>(y, e));
+                            H.idx[at] = (second ? at0[1] : at0[0]) + e;
                         }
                     };
                     put(may, &H.n, i0, kList);
@@ -1191,7 +1202,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                         else put(does, &H.above_n, 0, kAbove);
                     }
 #pragma unroll
-                    for (int w = 0; w + 1 < U; ++w) v[w] = v[w + 1];
+                    for (int w = 0; w + 2 < U; ++w) v[w] = v[w + 2];
                 }
             }
             if (many) {
@@ -1221,7 +1232,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                 // held), then those of the bin's tokens that stay
                 const int per = P.k * kThreads * N;
                 for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
-                if (t < 2 * kHoldBins) H.first[t] = 0;
+                if (t < kSides * kHoldBins) H.first[t] = 0;
                 __syncthreads();
                 int more = 0;
                 Gathered{H, 0, kAbove, n}.each([&](unsigned key, int i) {
@@ -1234,16 +1245,16 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
                 const int mine = ((int)top - t) & (kHist - 1);
 #pragma unroll
                 for (int k = 0; k < kHoldBins; ++k) {
-                    const int c = t / kHist + 2 * k;
+                    const int c = t / kHist + kSides * k;
                     if (c >= P.nch) continue;
                     const int at = mine - H.down[c];
                     const u64 f = wave_add(at >= 0 && at < kHist - 1 && mine < last ? bins_of[k] : 0);
                     if (lane == 0 && f) atomicAdd(&H.first[c], f);
                 }
                 __syncthreads();
-                if (t < min(P.nch, 2 * kHoldBins))
+                if (t < min(P.nch, kSides * kHoldBins))
                     H.chunk.sum[t] = (double)H.first[t] * 0x1p-50 * H.weight[t] + (double)H.chunk.more[t] / W.scale;
-                for (int c = 2 * kHoldBins + wave; c < P.nch; c += kWaves) {
+                for (int c = kSides * kHoldBins + wave; c < P.nch; c += kWaves) {
                     const float cm = part[c].m;
                     const int n = part[c].n, bins_in = cm == -INFINITY ? 0 : last - (int)fminf(top - (float)n, (float)kHist);
                     u64 f = 0;
@@ -1265,7 +1276,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
 }
 
 // Pieces a thread and chunk (K) and chunks of a row; chunks of 256 pieces while
-// they are 1024 or fewer.
+// they are 1024 or fewer, 128 a row.
 struct Chunks {
     int k, nch, ng;
 };
@@ -1279,7 +1290,7 @@ Chunks chunks_of(int nrows, int vocab, int kind) {
     }
     c.k = 1;
     c.nch = (vocab + per - 1 + per * kThreads - 1) / (per * kThreads);
-    if ((int64_t)nrows * c.nch > 1024) {
+    if ((int64_t)nrows * c.nch > 1024 || c.nch > 128) {
         c.k = 4;
         c.nch = (vocab + per - 1 + per * kThreads * 4 - 1) / (per * kThreads * 4);
     }
