@@ -568,7 +568,8 @@ int vgx_paged_attn_tree(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* 
 /* vgx_tree_accept: the walk down each sequence's tree (parent as above, tokens:
  * device int[ntok], each row's token) by the token that each row's logits gave
  * (chosen: device int[ntok]): from row 0 on to the first child whose token is
- * the chosen one, until there is none.  path (device int[ntok]): at
+ * the chosen one, until there is none (a negative token, as vgx_sample gives a
+ * row without any, is no child's).  path (device int[ntok]): at
  * qstart[s] + k the number of the k-th row of the way among the sequence's
  * rows (the first is row 0), -1 behind its end; accepted[s]: rows of the way
  * but the first; next[s]: the last one's chosen token.  A sequence without

@@ -257,6 +257,18 @@ def test_accept(gpu, nq):
     batch.check()
 
 
+def test_a_row_without_a_token_ends_the_way(gpu):
+    """A masked row's -1 is not the -1 of a padded child."""
+    b = Batch(31, [4, 3], [4, 3], 1, 16, 16, "bf16")
+    _, batch = make(gpu, b, 1)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    parent = torch.tensor([-1, 0, 1, 2, -1, 0, 0], **i32)
+    tokens = torch.tensor([5, 6, -1, -1, 5, -1, 7], **i32)
+    chosen = torch.tensor([6, -1, -1, 3, -1, 9, 9], **i32)
+    path, acc, nxt = (x.tolist() for x in batch.accept(parent, tokens, chosen))
+    assert path == [0, 1, -1, -1, 0, -1, -1] and acc == [1, 0] and nxt == [-1, -1]
+
+
 def layer_pools(b, n, strided=False):
     """The K and V of n layers: the batch's, and others of random values."""
     out = []

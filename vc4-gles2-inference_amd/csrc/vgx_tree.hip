@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(64) tree_accept_kernel(const PagedDev A, const
         int child = -1;
         for (int b = (cur + 1) & ~63; b < q.n && child < 0; b += 64) {
             const int i = b + lane;
-            const unsigned long long fit = __ballot(i > cur && i < q.n && up[i] == cur && tok[i] == want);
+            const unsigned long long fit =
+                __ballot(i > cur && i < q.n && up[i] == cur && tok[i] == want && want >= 0);  // (-1: no token)
             if (fit) child = b + __ffsll(fit) - 1;
         }
         if (child < 0) break;
