@@ -252,3 +252,29 @@ def test_far_from_zero(gpu, shift, temp):
     check(gpu, x, u, temp=[temp] * 4, top_k=[100] * 4)
     check(gpu, x, u, temp=[temp] * 4, min_p=[0.1] * 4)
     check(gpu, x, u, temp=[temp] * 4)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab", [4099, 5000, 8000, 30011, 64402, 200003])
+def test_large_top_k(gpu, kind, vocab):
+    """Top-k by thousands: past the groups, past what is gathered."""
+    k = [v for v in (300, 700, 1000, 1500, 2500, 3300, 4000, 4096, 4097, 9000, 60000) if v < vocab]
+    x, u = rows_of(17, len(k), vocab, kind, spread=2.0, top=9.0, pad=1)
+    check(gpu, x, u, top_k=k, temp=[1.3] * len(k))
+    check(gpu, x, u, top_k=k, top_p=[0.9] * len(k), min_p=[1e-5] * len(k))
+    x[:, : vocab // 2] = -32768 if kind == torch.int16 else -math.inf
+    check(gpu, x, u, top_k=k, temp=[2.0] * len(k))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("vocab, per", [(6400, 4), (6400, 8), (64402, 64)])
+def test_top_k_of_logits_in_order(gpu, kind, vocab, per):
+    """The first ones lie one a group, so fewer reach what groups' maxima do than
+    logits without an order would; or side by side, so that far more do."""
+    i = torch.arange(vocab)
+    even = 10.0 - (i % per) * (16.0 / per) - (i // per) * (3.0 / vocab)
+    row = torch.stack([even, 10.0 - i * (16.0 / vocab)])
+    x, u = cast(row.repeat(4, 1), kind), rows_of(18, 8, 8, kind)[1]
+    for k in (vocab // per * 3 // 4, vocab // per - 9):
+        check(gpu, x, u, top_k=[k] * 8, temp=[1.5] * 8)
+        check(gpu, x, u, top_k=[k] * 8, temp=[1.5] * 8, top_p=[0.8] * 8)

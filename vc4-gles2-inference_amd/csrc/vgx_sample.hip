@@ -606,17 +606,18 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
     }
 }
 
-// The cuts and the draw over a source that holds all that may stay.  z: the sum
-// of all weights, negative where the source holds them all.
+// Weights below 2^-q, which are 0, are this far below the maximum.
+__device__ __forceinline__ float range_of(const SampleArgs& P, const Ask& A) {
+    return (float)fmin((double)(P.q + 1) * 0.7 / A.inv, 1e30);
+}
+// Top-k's and top-p's place in a source that holds all that may stay (but for
+// min_p, W.least: 0).  z: the sum of all weights, negative where the source holds
+// them all.
 template <class Source>
-__device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, const Source& src, int r, const Ask& A, Weigh W, float m,
-                             double z) {
-    const int t = threadIdx.x;
-    const double least = W.least;
-    W.least = 0.0;
+__device__ __forceinline__ Cut find_cut(const SampleArgs& P, RowShared& H, const Source& src, const Ask& A, const Weigh& W,
+                                        float m, double z) {
     Cut cut{0, 0x7fffffff};
-    // weights below 2^-q are 0
-    const float range = (float)fmin((double)(P.q + 1) * 0.7 / A.inv, 1e30);
+    const float range = range_of(P, A);
     if (A.k && locate<false, false>(H, src, W, cut, m, range, P.vocab, [&](u64) { return (u64)A.top_k; })) cut = H.at;
     if (A.p) {
         const bool some = locate<true, false>(H, src, W, cut, m, range, P.vocab, [&](u64 total) {
@@ -626,6 +627,17 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
         if (some) cut = H.at;
     }
     __syncthreads();
+    return cut;
+}
+
+// The cuts and the draw over such a source.
+template <class Source>
+__device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, const Source& src, int r, const Ask& A, Weigh W, float m,
+                             double z) {
+    const int t = threadIdx.x;
+    const double least = W.least;
+    W.least = 0.0;
+    const Cut cut = find_cut(P, H, src, A, W, m, z);
     W.least = least;
     const double u = P.u[r];
     // how many stay
@@ -637,7 +649,7 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
     if ((t & 63) == 0 && n) atomicAdd(&H.stay, (int)n);
     u64 sum = 0;
     // (a draw of 1 or more, or no number, takes the last token)
-    locate<true, true>(H, src, W, cut, m, range, P.vocab, [&](u64 total) {
+    locate<true, true>(H, src, W, cut, m, range_of(P, A), P.vocab, [&](u64 total) {
         sum = total;
         return u >= 0.0 && u < 1.0 ? min((u64)(u * (double)total), total - 1) + 1 : u < 0.0 ? 1ull : total;
     });
@@ -797,6 +809,63 @@ __device__ __forceinline__ void draw_in_chunks(const SampleArgs& P, RowShared& H
     }
 }
 static_assert(4 * kThreads / kRow * 8 <= 64 && 8192 / kRow <= 64, "a thread's values of a chunk: a lane each");
+
+// The cuts and the draw where what may stay was not gathered: the cut from passes
+// over the whole row, then the chunks' sums of what stays.
+template <int KIND>
+__device__ __forceinline__ void cut_and_draw_whole(const SampleArgs& P, RowShared& H, int r, const Row& q, const Ask& A,
+                                                   Weigh W, float m) {
+    constexpr int N = kPer<KIND>;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const double least = W.least;
+    W.least = 0.0;
+    const Cut cut = find_cut(P, H, WholeRow<KIND>{P, q}, A, W, m, -1.0);
+    auto stay = [&](float x, int i) { return stays(cut, key_of(x), i) && (least == 0.0 || weight(x, W.S, W.tab) >= least); };
+    // (a row of one chunk: a part of it a wave)
+    const int parts = P.nch == 1 ? kWaves : 1, units = P.nch * parts, per = P.k * kThreads / parts;
+    if (t == 0) H.stay = 0;
+    __syncthreads();
+    int n = 0;
+#pragma unroll 1
+    for (int c = wave; c < units; c += kWaves) {
+        double s = 0.0;
+#pragma unroll 1
+        for (int j0 = lane; j0 < per; j0 += 4 * 64) {
+            uint4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                v[u] = make_uint4(0, 0, 0, 0);
+                if (j0 + u * 64 < per) v[u] = raw_piece<KIND>(q, P.vocab, c * per + j0 + u * 64);
+            }
+#pragma unroll 1
+            for (int u = 0; u < 4 && j0 + u * 64 < per; ++u) {
+                const int i0 = (c * per + j0 + u * 64) * N - q.off;
+                const unsigned inside = i0 >= 0 && i0 + N <= P.vocab ? (1u << N) - 1 : ends_of(i0, N, P.vocab);
+                float x[N];
+                unpack<KIND>(v[0], x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const bool in = inside >> e & 1 && x[e] != -INFINITY && stays(cut, key_of(x[e]), i0 + e);
+                    const double w = in ? weight(x[e], W.S, W.tab) : 0.0;
+                    const bool some = in && w >= least;
+                    s += some ? w : 0.0;
+                    n += some;
+                }
+#pragma unroll
+                for (int w = 0; w + 1 < 4; ++w) v[w] = v[w + 1];
+            }
+        }
+        s = wave_sum(s);
+        if (lane == 0) H.chunk.sum[c] = s;
+    }
+    n = (int)wave_add((u64)n);
+    if (lane == 0) atomicAdd(&H.stay, n);
+    __syncthreads();
+    if (parts > 1 && t == 0)
+        for (int w = 1; w < kWaves; ++w) H.chunk.sum[0] += H.chunk.sum[w];
+    __syncthreads();
+    draw_in_chunks<KIND>(P, H, r, q, W.S, H.stay, stay);
+}
 
 // The maximum of a row's chunks, and (greedy) its first index.
 __device__ __forceinline__ float join_max(const SampleArgs& P, RowShared& H, const Part* part, bool first, int& a) {
@@ -1103,6 +1172,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
     float floor_m = -INFINITY, step = 0.0f;
     int last = kBins - 1;
     bool open = true;  // nothing is known of the row
+    int must = 0;      // tokens that have to reach it
     if (A.bins()) {
         find_bin(P, H, part, own, bins_of, r, A, S, top);
         z = H.sum;
@@ -1129,12 +1199,21 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         __syncthreads();
         u64 groups;
         const unsigned c0 = H.h.cnt[2 * t], c1 = H.h.cnt[2 * t + 1];
-        const u64 want = (u64)A.top_k, run = block_scan(c0 + c1, H.wave, groups);
+        const u64 run = block_scan(c0 + c1, H.wave, groups);
+        // Where k nears the number of groups that would be nearly all logits.  Of
+        // logits that lie in no order a share f is found in 1 - (1 - f)^(a group's
+        // size) of the groups; asked for is a quarter more than k, and whether k
+        // reach it is counted.
+        constexpr int size = WHOLE ? N : kGroup;
+        const float f = 1.25f * (float)A.top_k / ((float)groups * size);
+        const float likely = f < 1.0f ? (float)groups * (1.0f - expf(size * log1pf(-f))) : (float)groups;
+        const u64 want = min((u64)A.top_k, (u64)likely + 1);
         if (run >= want && run - c0 - c1 < want) H.bin = run - c1 >= want ? 2 * t : 2 * t + 1;
         __syncthreads();
-        if (want <= groups) {
+        if (want <= groups && A.top_k <= kList) {
             open = false;
             last = H.bin;
+            if (want < (u64)A.top_k) must = A.top_k;
         }
     }
     bool bins = A.bins() && last < kHist - 1;  // top-p's bin is known
@@ -1168,140 +1247,140 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         __syncthreads();
         // (groups with a token above top-p's bin: past half the list's room those
         // tokens are only counted)
-        const int ngr = H.found, i0 = bins ? kAbove : 0;
+        const bool listed = H.found <= kGroups;  // else all are read
+        const int ngr = listed ? H.found : P.ng, i0 = bins ? kAbove : 0;
+        auto group_of = [&](int j) { return listed ? H.groups[j / LG] * LG + j % LG : j; };
         const bool many = H.stay > kAbove / 2;
         __syncthreads();
         if (t == 0) H.stay = 0;
-        if (ngr <= kGroups) {
-            // Pieces in one round trip, and one copy of what is done with them
-            // (several would be fetched from memory for a run or two).
-            constexpr int U = 4;
-            const int pieces = ngr * LG;
-            int sure = 0;
+        // Pieces in one round trip, and one copy of what is done with them
+        // (several would be fetched from memory for a run or two).
+        constexpr int U = 4;
+        const int pieces = ngr * LG;
+        int sure = 0;
 #pragma unroll 1
-            for (int j0 = 0; j0 < pieces; j0 += kRow * U) {
-                uint4 v[U];
+        for (int j0 = 0; j0 < pieces; j0 += kRow * U) {
+            uint4 v[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int j = j0 + u * kRow + t;
-                    v[u] = make_uint4(0, 0, 0, 0);
-                    const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
-                    if (i >= 0 && i + N <= P.vocab)
-                        v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i * kBytes<KIND>);
-                }
-#pragma unroll 1
-                for (int u = 0; u < U && j0 + u * kRow < pieces; u += 2) {  // two a time
-                    unsigned may = 0, does = 0;
-                    int at0[2];
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const int j = j0 + (u + w) * kRow + t;
-                        const int i = j < pieces ? (H.groups[j / LG] * LG + j % LG) * N - q.off : P.vocab;
-                        at0[w] = i;
-                        unsigned inside = (1u << N) - 1;
-                        if (i < 0 || i + N > P.vocab) {  // (a row's ends)
-                            inside = ends_of(i, N, P.vocab);
-                            if (inside) v[w] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
-                        }
-                        float x[N];
-                        unpack<KIND>(v[w], x);
-                        unsigned a = 0, b = 0;
-#pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            a |= (unsigned)(x[e] >= lo) << e;
-                            b |= (unsigned)(x[e] >= hi) << e;
-                        }
-                        may |= (a & inside & ~b) << N * w;
-                        does |= (b & inside) << N * w;
-                    }
-                    auto put = [&](unsigned bits, int* n, int at, int most) {
-                        at += place_of(__popc(bits), n);
-                        for (; bits && at < most; bits &= bits - 1, ++at) {
-                            const int k = __ffs(bits) - 1, e = k & (N - 1);
-                            const bool second = k >= N;
-                            const uint4 y = make_uint4(second ? v[1].x : v[0].x, second ? v[1].y : v[0].y,
-                                                       second ? v[1].z : v[0].z, second ? v[1].w : v[0].w);
-                            H.key[at] = key_of(value_in<KIND>(y, e));
-                            H.idx[at] = (second ? at0[1] : at0[0]) + e;
-                        }
-                    };
-                    put(may, &H.n, i0, kList);
-                    if (bins) {
-                        if (many) sure += __popc(does);
-                        else put(does, &H.above_n, 0, kAbove);
-                    }
-#pragma unroll
-                    for (int w = 0; w + 2 < U; ++w) v[w] = v[w + 2];
-                }
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * kRow + t;
+                v[u] = make_uint4(0, 0, 0, 0);
+                const int i = j < pieces ? group_of(j) * N - q.off : P.vocab;
+                if (i >= 0 && i + N <= P.vocab)
+                    v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i * kBytes<KIND>);
             }
-            if (many) {
-                sure = (int)wave_add((u64)sure);
-                if (lane == 0) atomicAdd(&H.above_n, sure);
+#pragma unroll 1
+            for (int u = 0; u < U && j0 + u * kRow < pieces; u += 2) {  // two a time
+                unsigned may = 0, does = 0;
+                int at0[2];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int j = j0 + (u + w) * kRow + t;
+                    const int i = j < pieces ? group_of(j) * N - q.off : P.vocab;
+                    at0[w] = i;
+                    unsigned inside = (1u << N) - 1;
+                    if (i < 0 || i + N > P.vocab) {  // (a row's ends)
+                        inside = ends_of(i, N, P.vocab);
+                        if (inside) v[w] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
+                    }
+                    float x[N];
+                    unpack<KIND>(v[w], x);
+                    unsigned a = 0, b = 0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        a |= (unsigned)(x[e] >= lo) << e;
+                        b |= (unsigned)(x[e] >= hi) << e;
+                    }
+                    may |= (a & inside & ~b) << N * w;
+                    does |= (b & inside) << N * w;
+                }
+                auto put = [&](unsigned bits, int* n, int at, int most) {
+                    at += place_of(__popc(bits), n);
+                    for (; bits && at < most; bits &= bits - 1, ++at) {
+                        const int k = __ffs(bits) - 1, e = k & (N - 1);
+                        const bool second = k >= N;
+                        const uint4 y = make_uint4(second ? v[1].x : v[0].x, second ? v[1].y : v[0].y,
+                                                   second ? v[1].z : v[0].z, second ? v[1].w : v[0].w);
+                        H.key[at] = key_of(value_in<KIND>(y, e));
+                        H.idx[at] = (second ? at0[1] : at0[0]) + e;
+                    }
+                };
+                put(may, &H.n, i0, kList);
+                if (bins) {
+                    if (many) sure += __popc(does);
+                    else put(does, &H.above_n, 0, kAbove);
+                }
+#pragma unroll
+                for (int w = 0; w + 2 < U; ++w) v[w] = v[w + 2];
+            }
+        }
+        if (many) {
+            sure = (int)wave_add((u64)sure);
+            if (lane == 0) atomicAdd(&H.above_n, sure);
+        }
+        __syncthreads();
+        const int n = H.n, above = bins ? H.above_n : 0;
+        if (n <= kList - i0 && above <= kAbove && !many && n >= must) {
+            const Gathered src{H, above, i0, n};
+            if (above + n <= kFew) cut_and_draw_few(P, H, src, r, A, W, z);
+            else cut_and_draw(P, H, src, r, A, W, m, z);
+            return;
+        }
+        if (bins && n <= kList - kAbove) {
+            // Thousands stay: all above top-p's bin, and of its own tokens, which
+            // are gathered, those to be found.
+            const int kept = above;
+            const double left = H.left;
+            Cut cut{0, 0x7fffffff};
+            const double y = ceil((A.top_p * z - left) * W.scale);
+            if (locate<true, false>(H, Gathered{H, 0, kAbove, n}, W, cut, (edge + 1.0f) / hstep, 1.0f / hstep, P.vocab,
+                                    [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
+                cut = H.at;
+            __syncthreads();
+            // the chunks' sums: their bins above the cut's (the first chunks' are
+            // held), then those of the bin's tokens that stay
+            const int per = P.k * kThreads * N;
+            for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
+            if (t < kSides * kHoldBins) H.first[t] = 0;
+            __syncthreads();
+            int more = 0;
+            Gathered{H, 0, kAbove, n}.each([&](unsigned key, int i) {
+                if (!stays(cut, key, i)) return;
+                ++more;
+                atomicAdd(&H.chunk.more[(i + q.off) / per], W(key));
+            });
+            more = (int)wave_add((u64)more);
+            if (lane == 0) atomicAdd(&H.stay, more);
+            const int mine = ((int)top - t) & (kHist - 1);
+#pragma unroll
+            for (int k = 0; k < kHoldBins; ++k) {
+                const int c = t / kHist + kSides * k;
+                if (c >= P.nch) continue;
+                const int at = mine - H.down[c];
+                const u64 f = wave_add(at >= 0 && at < kHist - 1 && mine < last ? bins_of[k] : 0);
+                if (lane == 0 && f) atomicAdd(&H.first[c], f);
             }
             __syncthreads();
-            const int n = H.n, above = bins ? H.above_n : 0;
-            if (n <= kList - i0 && above <= kAbove && !many) {
-                const Gathered src{H, above, i0, n};
-                if (above + n <= kFew) cut_and_draw_few(P, H, src, r, A, W, z);
-                else cut_and_draw(P, H, src, r, A, W, m, z);
-                return;
+            if (t < min(P.nch, kSides * kHoldBins))
+                H.chunk.sum[t] = (double)H.first[t] * 0x1p-50 * H.weight[t] + (double)H.chunk.more[t] / W.scale;
+            for (int c = kSides * kHoldBins + wave; c < P.nch; c += kWaves) {
+                const float cm = part[c].m;
+                const int n = part[c].n, bins_in = cm == -INFINITY ? 0 : last - (int)fminf(top - (float)n, (float)kHist);
+                u64 f = 0;
+                for (int b = lane; b < bins_in; b += 64)
+                    f += P.hist[((int64_t)r * P.nch + c) * kHist + slot_of(n, b)];
+                f = wave_add(f);
+                if (lane == 0)
+                    H.chunk.sum[c] = (double)f * 0x1p-50 * weight(cm, S, H.tab) + (double)H.chunk.more[c] / W.scale;
             }
-            if (bins && n <= kList - kAbove) {
-                // Thousands stay: all above top-p's bin, and of its own tokens, which
-                // are gathered, those to be found.
-                const int kept = above;
-                const double left = H.left;
-                Cut cut{0, 0x7fffffff};
-                const double y = ceil((A.top_p * z - left) * W.scale);
-                if (locate<true, false>(H, Gathered{H, 0, kAbove, n}, W, cut, (edge + 1.0f) / hstep, 1.0f / hstep, P.vocab,
-                                        [&](u64) { return y < 1.0 ? 1ull : (u64)y; }))
-                    cut = H.at;
-                __syncthreads();
-                // the chunks' sums: their bins above the cut's (the first chunks' are
-                // held), then those of the bin's tokens that stay
-                const int per = P.k * kThreads * N;
-                for (int c = t; c < P.nch; c += kRow) H.chunk.more[c] = 0;
-                if (t < kSides * kHoldBins) H.first[t] = 0;
-                __syncthreads();
-                int more = 0;
-                Gathered{H, 0, kAbove, n}.each([&](unsigned key, int i) {
-                    if (!stays(cut, key, i)) return;
-                    ++more;
-                    atomicAdd(&H.chunk.more[(i + q.off) / per], W(key));
-                });
-                more = (int)wave_add((u64)more);
-                if (lane == 0) atomicAdd(&H.stay, more);
-                const int mine = ((int)top - t) & (kHist - 1);
-#pragma unroll
-                for (int k = 0; k < kHoldBins; ++k) {
-                    const int c = t / kHist + kSides * k;
-                    if (c >= P.nch) continue;
-                    const int at = mine - H.down[c];
-                    const u64 f = wave_add(at >= 0 && at < kHist - 1 && mine < last ? bins_of[k] : 0);
-                    if (lane == 0 && f) atomicAdd(&H.first[c], f);
-                }
-                __syncthreads();
-                if (t < min(P.nch, kSides * kHoldBins))
-                    H.chunk.sum[t] = (double)H.first[t] * 0x1p-50 * H.weight[t] + (double)H.chunk.more[t] / W.scale;
-                for (int c = kSides * kHoldBins + wave; c < P.nch; c += kWaves) {
-                    const float cm = part[c].m;
-                    const int n = part[c].n, bins_in = cm == -INFINITY ? 0 : last - (int)fminf(top - (float)n, (float)kHist);
-                    u64 f = 0;
-                    for (int b = lane; b < bins_in; b += 64)
-                        f += P.hist[((int64_t)r * P.nch + c) * kHist + slot_of(n, b)];
-                    f = wave_add(f);
-                    if (lane == 0)
-                        H.chunk.sum[c] = (double)f * 0x1p-50 * weight(cm, S, H.tab) + (double)H.chunk.more[c] / W.scale;
-                }
-                __syncthreads();
-                return draw_in_chunks<KIND>(P, H, r, q, S, kept + H.stay, [&](float x, int i) {
-                    return x >= hi || (x >= lo && stays(cut, key_of(x), i));
-                });
-            }
+            __syncthreads();
+            return draw_in_chunks<KIND>(P, H, r, q, S, kept + H.stay, [&](float x, int i) {
+                return x >= hi || (x >= lo && stays(cut, key_of(x), i));
+            });
         }
         __syncthreads();
     }
-    cut_and_draw(P, H, WholeRow<KIND>{P, q}, r, A, W, m, -1.0);
+    cut_and_draw_whole<KIND>(P, H, r, q, A, W, m);
 }
 
 // Pieces a thread and chunk (K) and chunks of a row; chunks of 256 pieces while
