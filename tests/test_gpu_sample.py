@@ -278,3 +278,14 @@ def test_top_k_of_logits_in_order(gpu, kind, vocab, per):
     for k in (vocab // per * 3 // 4, vocab // per - 9):
         check(gpu, x, u, top_k=[k] * 8, temp=[1.5] * 8)
         check(gpu, x, u, top_k=[k] * 8, temp=[1.5] * 8, top_p=[0.8] * 8)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows, vocab", [(3, 6000), (9, 30011), (700, 9001)])
+def test_cuts_left_out_or_open(gpu, kind, rows, vocab):
+    """No array of cuts and one that keeps all are the same."""
+    x, u = rows_of(19, rows, vocab, kind)
+    for cuts in (dict(), dict(top_k=[50] * rows), dict(min_p=[0.03] * rows), dict(temp=[0.0] * rows)):
+        given = {**dict(temp=[1.0] * rows, top_k=[0] * rows, top_p=[1.0] * rows, min_p=[0.0] * rows), **cuts}
+        for a, b in zip(run(gpu, x, u, **cuts), run(gpu, x, u, **given)):
+            assert torch.equal(a, b)

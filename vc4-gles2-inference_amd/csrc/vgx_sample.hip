@@ -1075,8 +1075,12 @@ __device__ __forceinline__ void read_row(const SampleArgs& P, RowShared& H, int 
 // logits 15.6 -> 11 us a call, as the second launch's 4 go.
 template <int KIND>
 constexpr int kSmall = 8192 / kPer<KIND>;
-template <int KIND, bool WHOLE>
-__global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
+// BINS: a row may ask for top-p.  Calls without need neither the bins nor what
+// follows from them, and in 80 registers three rows fit a CU instead of two (f32's
+// would not without memory): 640 rows of 64402 by top-k 50 36 -> 32 us a call, 400 51
+// -> 43, without a cut 51 -> 47.
+template <int KIND, bool WHOLE, bool BINS>
+__global__ void __launch_bounds__(kRow, BINS || KIND == VGX_E_F32 ? 1 : 6) sample_pick_kernel(const SampleArgs P) {
     constexpr int N = kPer<KIND>, LG = WHOLE ? 1 : kGroup / N, kHold = WHOLE ? kSmall<KIND> / kRow : 3;
     __shared__ RowShared H;
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -1109,8 +1113,9 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
         }
     };
     const Ask A = ask_of(P, r);
+    const bool by_bins = BINS && A.bins();
     if constexpr (!WHOLE) {
-        if (A.bins()) {
+        if (by_bins) {
             const u64* hist = P.hist + (int64_t)r * P.nch * kHist + (t & (kHist - 1));
 #pragma unroll
             for (int k = 0; k < kHoldBins; ++k) bins_of[k] = hist[(int64_t)min(t / kHist + kSides * k, P.nch - 1) * kHist];
@@ -1173,7 +1178,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
     int last = kBins - 1;
     bool open = true;  // nothing is known of the row
     int must = 0;      // tokens that have to reach it
-    if (A.bins()) {
+    if (by_bins) {
         find_bin(P, H, part, own, bins_of, r, A, S, top);
         z = H.sum;
         if (H.bin >= 0) {
@@ -1216,7 +1221,7 @@ __global__ void __launch_bounds__(kRow) sample_pick_kernel(const SampleArgs P) {
             if (want < (u64)A.top_k) must = A.top_k;
         }
     }
-    bool bins = A.bins() && last < kHist - 1;  // top-p's bin is known
+    bool bins = by_bins && last < kHist - 1;  // top-p's bin is known
     // What may stay is lo or more, what does (bins) hi or more.
     float lo = -FLT_MAX, hi = INFINITY;
     const float edge = top - (float)last;
@@ -1409,12 +1414,13 @@ Chunks chunks_of(int nrows, int vocab, int kind) {
 template <int KIND>
 void launch(const SampleArgs& P, hipStream_t st) {
     if (P.ng == 0) {
-        hipLaunchKernelGGL((sample_pick_kernel<KIND, true>), dim3(P.nrows), dim3(kRow), 0, st, P);
+        hipLaunchKernelGGL((sample_pick_kernel<KIND, true, true>), dim3(P.nrows), dim3(kRow), 0, st, P);
         return;
     }
     hipLaunchKernelGGL((P.k == 1 ? sample_stats_kernel<KIND, 1> : sample_stats_kernel<KIND, 4>), dim3(P.nch, P.nrows),
                        dim3(kThreads), 0, st, P);
-    hipLaunchKernelGGL((sample_pick_kernel<KIND, false>), dim3(P.nrows), dim3(kRow), 0, st, P);
+    hipLaunchKernelGGL((P.top_p ? sample_pick_kernel<KIND, false, true> : sample_pick_kernel<KIND, false, false>), dim3(P.nrows),
+                       dim3(kRow), 0, st, P);
 }
 
 bool kind_ok(int k) { return k == VGX_E_F32 || k == VGX_E_BF16 || k == VGX_E_F16 || k == VGX_E_Q16; }
