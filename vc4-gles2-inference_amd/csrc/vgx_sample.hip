@@ -456,6 +456,7 @@ __device__ __forceinline__ void each_of(uint4 v, int i0, int vocab, F f) {
 // The tokens of a row (f(key, index) of each that is not masked) ...
 template <int KIND>
 struct WholeRow {
+    static constexpr bool kWhole = true;
     const SampleArgs& P;
     Row q;
     template <class F>
@@ -485,6 +486,7 @@ struct WholeRow {
 // ... or those gathered from it: the list's places i0 .. i0 + n - 1, and the
 // first n0 ones.
 struct Gathered {
+    static constexpr bool kWhole = false;
     const RowShared& H;
     int n0, i0, n;
     __device__ __forceinline__ int place(int i) const { return i < n0 ? i : i - n0 + i0; }
@@ -513,7 +515,9 @@ struct Weigh {
 // that of their indices, reach `want` (of their total, once that is known): of
 // tokens, or of weights (WEIGHTED).  False: they do not.  Bins over the values
 // first (floats' keys spread over them badly), then over the keys of the bin that
-// holds the place, then over the indices of one key, until few are left.
+// holds the place, then over the indices of one key, until few are left.  Of a
+// whole row a bin's tokens are gathered as soon as there is room for them (640 rows
+// of 64402 by top-k 5000 262 -> 186 us).
 template <bool WEIGHTED, bool BY_INDEX, class Source, class Want>
 __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const Weigh& W, const Cut& in, float m, float range, int vocab,
                        Want want_of) {
@@ -580,6 +584,21 @@ __device__ __forceinline__ bool locate(RowShared& H, const Source& src, const We
                 H.at = BY_INDEX ? Cut{(unsigned)mine, (int)(mine >> 32)} : Cut{~(unsigned)(mine >> 32), (int)(unsigned)mine};
             __syncthreads();
             return true;
+        }
+        if constexpr (Source::kWhole) {
+            if (mode == VALUE && c <= kList) {  // the bin's tokens alone from here on
+                src.each([&](unsigned key, int i) {
+                    if (bin_of(key, i) != bin) return;
+                    const int at = atomicAdd(&H.n, 1);
+                    if (at >= kList) return;  // (never)
+                    H.key[at] = key;
+                    H.idx[at] = i;
+                });
+                __syncthreads();
+                const u64 left = want - before;
+                return locate<WEIGHTED, BY_INDEX>(H, Gathered{H, 0, 0, c}, W, in, m - (float)(kBins - 1 - bin) / step, 1.0f / step,
+                                                  vocab, [&](u64) { return left; });
+            }
         }
         if (mode == VALUE) {  // the keys of the bin
             unsigned a = ~0u, b = 0;
