@@ -35,22 +35,24 @@ __device__ __forceinline__ float one(const uint8_t* p, int i) {
     return clean((float)__builtin_bit_cast(_Float16, u));
 }
 
-template <int KIND>
+// CLEAN: masks and infinities as they count.
+template <int KIND, bool CLEAN = true>
 __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kPer<KIND>]) {
+    auto tidy = [](float y) { return CLEAN ? clean(y) : y; };
     const unsigned u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (KIND == VGX_E_F32) {
-            x[i] = clean(__uint_as_float(u[i]));
+            x[i] = tidy(__uint_as_float(u[i]));
         } else if constexpr (KIND == VGX_E_Q16) {
             x[2 * i] = (float)(short)(u[i] & 0xffff) * (1.0f / 256);
             x[2 * i + 1] = (float)((int)u[i] >> 16) * (1.0f / 256);
         } else if constexpr (KIND == VGX_E_BF16) {
-            x[2 * i] = clean(__uint_as_float(u[i] << 16));
-            x[2 * i + 1] = clean(__uint_as_float(u[i] & 0xffff0000u));
+            x[2 * i] = tidy(__uint_as_float(u[i] << 16));
+            x[2 * i + 1] = tidy(__uint_as_float(u[i] & 0xffff0000u));
         } else {
-            x[2 * i] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
-            x[2 * i + 1] = clean((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
+            x[2 * i] = tidy((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffff)));
+            x[2 * i + 1] = tidy((float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16)));
         }
     }
 }

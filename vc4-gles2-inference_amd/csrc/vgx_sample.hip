@@ -1285,39 +1285,40 @@ __global__ void __launch_bounds__(kRow, BINS || KIND == VGX_E_F32 ? 1 : 6) sampl
 #pragma unroll 1
         for (int j0 = 0; j0 < pieces; j0 += kRow * U) {
             uint4 v[U];
+            int at0[U];  // the index of a piece's first value
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int j = j0 + u * kRow + t;
                 v[u] = make_uint4(0, 0, 0, 0);
-                const int i = j < pieces ? group_of(j) * N - q.off : P.vocab;
-                if (i >= 0 && i + N <= P.vocab)
-                    v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)i * kBytes<KIND>);
+                at0[u] = j < pieces ? group_of(j) * N - q.off : P.vocab;
+                if (at0[u] >= 0 && at0[u] + N <= P.vocab)
+                    v[u] = *reinterpret_cast<const uint4*>(q.p + (int64_t)at0[u] * kBytes<KIND>);
             }
 #pragma unroll 1
             for (int u = 0; u < U && j0 + u * kRow < pieces; u += 2) {  // two a time
-                unsigned may = 0, does = 0;
-                int at0[2];
+                // (as they lie in memory: NaN reaches nothing, infinity all)
+                float x[2][N];
+                const bool ends = at0[0] < 0 || at0[0] + N > P.vocab || at0[1] < 0 || at0[1] + N > P.vocab;
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const int j = j0 + (u + w) * kRow + t;
-                    const int i = j < pieces ? group_of(j) * N - q.off : P.vocab;
-                    at0[w] = i;
-                    unsigned inside = (1u << N) - 1;
-                    if (i < 0 || i + N > P.vocab) {  // (a row's ends)
-                        inside = ends_of(i, N, P.vocab);
-                        if (inside) v[w] = raw_piece<KIND>(q, P.vocab, (i + q.off) / N);
-                    }
-                    float x[N];
-                    unpack<KIND>(v[w], x);
-                    unsigned a = 0, b = 0;
+                for (int w = 0; w < 2; ++w) unpack<KIND, false>(v[w], x[w]);
+                if (__any(ends)) {  // (a row's)
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        a |= (unsigned)(x[e] >= lo) << e;
-                        b |= (unsigned)(x[e] >= hi) << e;
+                    for (int w = 0; w < 2; ++w) {
+                        const unsigned inside = ends_of(at0[w], N, P.vocab);
+                        if (inside) v[w] = raw_piece<KIND>(q, P.vocab, (at0[w] + q.off) / N);
+                        unpack<KIND, false>(v[w], x[w]);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) x[w][e] = inside >> e & 1 ? x[w][e] : -INFINITY;
                     }
-                    may |= (a & inside & ~b) << N * w;
-                    does |= (b & inside) << N * w;
                 }
+                // a bit a value: an addition with its carry each
+                auto reach = [&](float y) {
+                    unsigned r = 0, past;
+#pragma unroll
+                    for (int e = 2 * N - 1; e >= 0; --e) r = __builtin_addc(r, r, (unsigned)(x[e / N][e % N] >= y), &past);
+                    return r;
+                };
+                const unsigned does = bins ? reach(hi) : 0, may = reach(lo) & ~does;
                 auto put = [&](unsigned bits, int* n, int at, int most) {
                     at += place_of(__popc(bits), n);
                     for (; bits && at < most; bits &= bits - 1, ++at) {
@@ -1335,7 +1336,10 @@ __global__ void __launch_bounds__(kRow, BINS || KIND == VGX_E_F32 ? 1 : 6) sampl
                     else put(does, &H.above_n, 0, kAbove);
                 }
 #pragma unroll
-                for (int w = 0; w + 2 < U; ++w) v[w] = v[w + 2];
+                for (int w = 0; w + 2 < U; ++w) {
+                    v[w] = v[w + 2];
+                    at0[w] = at0[w + 2];
+                }
             }
         }
         if (many) {
