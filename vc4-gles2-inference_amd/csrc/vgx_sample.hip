@@ -313,6 +313,8 @@ struct RowShared {
         struct {
             u64 order[kRow], w[kRow], before[kRow];
             unsigned rank[kRow];
+            u64 sum[kWaves];
+            int count[kWaves];
         } few;
         int groups[kGroups];
         struct {
@@ -654,11 +656,10 @@ template <class Source>
 __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, const Source& src, int r, const Ask& A, Weigh W, float m,
                              double z) {
     const int t = threadIdx.x;
-    const double least = W.least;
+    const double least = W.least, u = P.u[r];
     W.least = 0.0;
     const Cut cut = find_cut(P, H, src, A, W, m, z);
     W.least = least;
-    const double u = P.u[r];
     // how many stay
     unsigned n = 0;
     if (t == 0) H.stay = 0;
@@ -685,6 +686,7 @@ __device__ __forceinline__ void cut_and_draw(const SampleArgs& P, RowShared& H, 
 __device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared& H, const Gathered& src, int r,
                                                  const Ask& A, const Weigh& W, double z) {
     const int t = threadIdx.x, n = src.n0 + src.n;
+    const double u = P.u[r];  // (here it comes in beside the first comparisons)
     const bool in = t < n;
     const unsigned key = in ? H.key[src.place(t)] : 0;
     const int idx = in ? H.idx[src.place(t)] : 0;
@@ -696,30 +698,34 @@ __device__ __forceinline__ void cut_and_draw_few(const SampleArgs& P, RowShared&
     compare_all(H, n);
     const u64 before = H.few.before[t];
     bool stay = in && (!A.k || (int)H.few.rank[t] < A.top_k);
-    u64 total;
+    const int lane = t & 63, wave = t >> 6;  // (all tokens are the first two waves')
     if (A.p) {
         double all = z * W.scale;
         if (A.k) {
-            block_scan(stay ? w : 0, H.wave, total);
-            all = (double)total;
+            const u64 s = wave_add(stay ? w : 0);
+            if (lane == 0) H.wave[wave] = s;
+            __syncthreads();
+            all = (double)(H.wave[0] + H.wave[1]);
         }
         const double y = ceil(A.top_p * all);
         stay = stay && before < (y < 1.0 ? 1ull : (u64)y);
     }
     stay = stay && real >= W.least;
     if (!stay) w = 0;
-    block_scan(w, H.wave, total);
-    const u64 sum = total;
-    block_scan(stay, H.wave, total);
+    const u64 s = wave_add(w);
+    const int some = __popcll(__ballot(stay));
+    if (lane == 0) {
+        H.few.sum[wave] = s;
+        H.few.count[wave] = some;
+    }
     H.few.order[t] = stay ? (u64)(unsigned)idx : ~0ull;
     H.few.w[t] = w;
     compare_all(H, n);
-    const u64 c = H.few.before[t];
-    const double u = P.u[r];
+    const u64 c = H.few.before[t], sum = H.few.sum[0] + H.few.sum[1];
     const u64 want = u >= 0.0 && u < 1.0 ? min((u64)(u * (double)sum), sum - 1) : u < 0.0 ? 0 : sum - 1;
     if (stay && c <= want && want < c + w) {
         P.token[r] = idx;
-        if (P.kept) P.kept[r] = (int)total;
+        if (P.kept) P.kept[r] = H.few.count[0] + H.few.count[1];
         if (P.prob) P.prob[r] = (float)(real / ((double)sum / W.scale));
     }
 }
@@ -1227,11 +1233,14 @@ __global__ void __launch_bounds__(kRow, BINS || KIND == VGX_E_F32 ? 1 : 6) sampl
         // Where k nears the number of groups that would be nearly all logits.  Of
         // logits that lie in no order a share f is found in 1 - (1 - f)^(a group's
         // size) of the groups; asked for is a quarter more than k, and whether k
-        // reach it is counted.
-        constexpr int size = WHOLE ? N : kGroup;
-        const float f = 1.25f * (float)A.top_k / ((float)groups * size);
-        const float likely = f < 1.0f ? (float)groups * (1.0f - expf(size * log1pf(-f))) : (float)groups;
-        const u64 want = min((u64)A.top_k, (u64)likely + 1);
+        // reach it is counted.  (Up to a third of the groups that is above k.)
+        u64 want = (u64)A.top_k;
+        if (want * 3 > groups) {
+            constexpr int size = WHOLE ? N : kGroup;
+            const float f = 1.25f * (float)A.top_k / ((float)groups * size);
+            const float likely = f < 1.0f ? (float)groups * (1.0f - expf(size * log1pf(-f))) : (float)groups;
+            want = min(want, (u64)likely + 1);
+        }
         if (run >= want && run - c0 - c1 < want) H.bin = run - c1 >= want ? 2 * t : 2 * t + 1;
         __syncthreads();
         if (want <= groups && A.top_k <= kList) {

@@ -308,8 +308,8 @@ class RaggedBatch:
         g = self.gpu
         for t, name in ((parent, "parent"), (tokens, "tokens"), (chosen, "chosen")):
             g.need_values(t, _I32, self.ntok, name)
-        path = torch.empty(self.ntok, dtype=_I32, device=g.device)
-        accepted, nxt = (torch.empty(self.nseq, dtype=_I32, device=g.device) for _ in range(2))
+        path, accepted = torch.empty_like(parent), torch.empty(self.nseq, dtype=_I32, device=g.device)
+        nxt = torch.empty_like(accepted)
         g.on_current(_l.load().vgx_tree_accept, self.ref, parent.data_ptr(), tokens.data_ptr(), chosen.data_ptr(),
                      path.data_ptr(), accepted.data_ptr(), nxt.data_ptr())
         return path, accepted, nxt
@@ -778,8 +778,8 @@ class GPU:
                 self.need_values(t, dtype, n, name)
         L, dev = _l.load(), self.device
         need = int(L.vgx_sample_ws(n, vocab, kind))
-        token, kept = (torch.empty(n, dtype=_I32, device=dev) for _ in range(2))
-        prob = torch.empty(n, dtype=_F32, device=dev)
+        token = torch.empty(n, dtype=_I32, device=dev)
+        kept, prob = torch.empty_like(token), torch.empty_like(u)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         a = _l.Sampling(n, vocab, kind, logits.data_ptr(), stride, u.data_ptr(), _at(temp), _at(top_k), _at(top_p),
                         _at(min_p), token.data_ptr(), kept.data_ptr(), prob.data_ptr(), _at(ws), need)
