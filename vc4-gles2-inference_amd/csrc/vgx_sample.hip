@@ -1092,9 +1092,9 @@ __device__ __forceinline__ void read_row(const SampleArgs& P, RowShared& H, int 
 }
 
 // A workgroup a row: a chain of LDS passes and barriers, with few bytes behind them.
-// One row of 6400 (WHOLE) 9.7 us, 640 rows by top-k 25 (5 to 17 a row, two rows a CU
-// at once), 160 by top-p 36, where thousands stay: the bin's tokens gathered 18, its
-// search 4, the chunks' sums 4, the draw 6.  512 threads: with 256
+// One row of 6400 (WHOLE) 9.5 us, 640 rows by top-k 24 (7 to 15 a row), 160 by top-p
+// 36, where thousands stay: the bin's tokens gathered 15 to 18, its search 4, the
+// chunks' sums 4, the draw 6.  512 threads: with 256
 // 640 rows by top-k 400 took 45 us instead of 50 a call, 48 flat rows 86 instead of 51.
 // WHOLE: a row of up to kSmall pieces, which one launch reads and decides: 6400
 // logits 15.6 -> 11 us a call, as the second launch's 4 go.
