@@ -549,7 +549,8 @@ int vgx_tree_masks(vgx_ctx* ctx, const vgx_ragged* batch, const int* parent, int
 /* vgx_paged_append with the rows in their sequence's slots as they come, but
  * turned by the angles of position kvlen - rows + depth (device int[ntok]).  A
  * depth that is negative or above the row's number sets VGX_FAULT_LENGTH, and
- * the row is written nowhere. */
+ * the row is written nowhere.  So does, under a rotation, a depth whose position
+ * is negative (more rows than kvlen) where the row has a slot. */
 int vgx_paged_append_tree(vgx_ctx* ctx, const vgx_paged* cache, const vgx_ragged* batch, const vgx_paged_rows* rows,
                           const int* depth);
 

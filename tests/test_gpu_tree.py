@@ -598,3 +598,50 @@ def test_part_of_a_batch(gpu):
     rest = list(range(6)) + list(range(21, 26))
     assert (q[rest] == 7).all() and (out[rest] == 3).all()
     assert not (q[6:21] == 7).all(-1).any() and not (out[6:21] == 3).all(-1).any()
+
+
+def check_append_past_the_start(gpu, kind, parents, kv, rotated):
+    """Sequences of more rows than positions: a row before position 0 has no
+    slot and is skipped; one with a slot is written, or, where it has no angle
+    (its depth's position is before 0), reported and written nowhere."""
+    from vgx import lib as vl
+    nq, heads, hd = [len(p) for p in parents], 4, 64
+    b = Batch(59, nq, kv, 2, hd, 16, kind)
+    angles = [t.cuda() for t in tables(60, hd)] if rotated else []
+    x = (1.5 * b.randn(b.ntok, (heads + 4) * hd)).to(torch.bfloat16).cuda()
+    cache, batch = make(gpu, b, heads)
+    q = torch.full((b.ntok, heads, hd), 7.0, dtype=ref.CTYPE[kind], device="cuda")
+    cache.append(batch, x, *angles, out=q, tree=batch.tree(flat(parents)))
+    want_k, want_v, fault = b.k.clone().cuda(), b.v.clone().cuda(), False
+    for s, n in enumerate(nq):
+        depth = tr.lines(parents[s])[0]
+        for r in range(n):
+            t, pos, at = int(b.qs[s]) + r, kv[s] - n + r, kv[s] - n + depth[r]
+            lost = rotated and pos >= 0 and at < 0
+            fault = fault or lost
+            if pos < 0 or lost:
+                assert (q[t] == 7).all(), (s, r)
+                continue
+            # the same row alone, as a sequence that ends at its angles' position
+            one = Batch(60, [1], [max(at, 0) + 1], 2, hd, 16, kind)
+            c1, b1 = make(gpu, one, heads)
+            assert torch.equal(q[t], c1.append(b1, x[t:t + 1], *angles)[0]), (s, r)
+            src = (int(one.table[0, max(at, 0) // 16]), slice(None), max(at, 0) % 16)
+            dst = (int(b.table[s, pos // 16]), slice(None), pos % 16)
+            want_k[dst], want_v[dst] = c1.k[src], c1.v[src]
+    assert torch.equal(cache.k, want_k) and torch.equal(cache.v, want_v)
+    if fault:
+        with pytest.raises(vl.VgxError, match="length"):
+            batch.check()
+    else:
+        batch.check()
+    return fault
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q8"])
+@pytest.mark.parametrize("rotated", [False, True])
+def test_append_of_more_rows_than_positions(gpu, kind, rotated):
+    wide = [[-1] + [0] * 4, [-1, 0, 0, 1, 3, 4, 5, 6, 7, 8, 9, 2], [-1, 0, 1]]
+    assert check_append_past_the_start(gpu, kind, wide, [3, 7, 0], rotated) == rotated
+    chains = [list(range(-1, n - 1)) for n in (5, 12, 3)]  # a row's depth is its number
+    assert not check_append_past_the_start(gpu, kind, chains, [3, 7, 0], rotated)

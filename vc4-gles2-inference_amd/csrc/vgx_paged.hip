@@ -218,11 +218,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs P) {
         ok = ok && d >= 0 && d <= i;
         at = pos - i + d;
     }
-    if (!ok || (P.rot && at >= P.npos)) {
+    // (a tree's row that has a slot but no angle is a fault: its descendants would
+    // see what lay in the slot)
+    if (!ok || (P.rot && (at >= P.npos || (at < 0 && pos >= 0)))) {
         if (threadIdx.x == 0) set_fault(A, VGX_FAULT_LENGTH);
         return;
     }
-    if (i < 0 || i >= sq.n || pos < 0 || at < 0) return;
+    if (i < 0 || i >= sq.n || pos < 0) return;
     const int pi = page_of(A, pos), slot = pos - pi * A.psize;
     const int pg = A.table[(int64_t)s * A.tstride + pi];
     float c[8], n[8];
