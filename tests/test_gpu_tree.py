@@ -645,3 +645,23 @@ def test_append_of_more_rows_than_positions(gpu, kind, rotated):
     assert check_append_past_the_start(gpu, kind, wide, [3, 7, 0], rotated) == rotated
     chains = [list(range(-1, n - 1)) for n in (5, 12, 3)]  # a row's depth is its number
     assert not check_append_past_the_start(gpu, kind, chains, [3, 7, 0], rotated)
+
+
+def test_a_batch_over_caches_of_other_strides(gpu):
+    """What a batch keeps of one cache's calls does not serve another's whose
+    rows lie further apart: the same results as by a batch of its own."""
+    nq, kv, heads, hd = [61, 20, 2], [3000, 2500, 3500], 2, 64
+    b = Batch(61, nq, kv, 1, hd, 16, "f16")
+    parents = trees_of(nq, 62)
+    row = 1 << 25  # 64 MiB between a page's positions
+    pool = torch.zeros(16 * row, dtype=torch.float16, device="cuda")
+    far = [pool.as_strided((b.pages, 1, 16, hd), (hd, hd, row, 1), i * b.pages * hd) for i in range(2)]
+    far[0].copy_(b.k)
+    far[1].copy_(b.v)
+    spread = gpu.paged_cache(heads, 1, hd, "f16", *far)
+    near, own = make(gpu, b, heads, max_q=61, max_kv=3500)
+    q = b.randn(b.ntok, heads, hd).to(torch.float16).cuda()
+    want = near.attend(own, q, tree=own.tree(flat(parents)))[0]
+    both = spread.batch(*b.device(), b.ntok, max_q=61, max_kv=3500)
+    check(gpu, b, heads, parents, q=q.cpu(), cache=spread, batch=both)
+    assert torch.equal(near.attend(both, q, tree=both.tree(flat(parents)))[0], want)

@@ -293,7 +293,7 @@ class RaggedBatch:
                            table.data_ptr(), table.shape[1], table.stride(0) if nseq > 1 else table.shape[1],
                            self.fault.data_ptr())
         self.ref = ctypes.byref(self.d)
-        self.ws = {}  # workspace bytes by (cache, window)
+        self.ws = {}  # workspace bytes by what of a cache and call decides them (PagedCache.attend)
 
     def tree(self, parent, window=0):
         """The rows as drafted trees: parent[r] is the number of row r's parent
@@ -469,7 +469,8 @@ class PagedCache:
             self._same_batch(batch, tree)
             if tree.window != window:
                 raise ValueError("the tree's window is %d, not %d" % (tree.window, window))
-        key = (self.d.kind, self.heads, self.kv_heads, self.head_dim, self.d.page_size, window, tree is None)
+        d = self.d
+        key = (d.kind, self.heads, self.kv_heads, self.head_dim, d.page_size, d.k_row, d.v_row, window, tree is None)
         need = batch.ws.get(key)
         L = _l.load()
         known = need is not None
