@@ -665,3 +665,35 @@ def test_a_batch_over_caches_of_other_strides(gpu):
     both = spread.batch(*b.device(), b.ntok, max_q=61, max_kv=3500)
     check(gpu, b, heads, parents, q=q.cpu(), cache=spread, batch=both)
     assert torch.equal(near.attend(both, q, tree=both.tree(flat(parents)))[0], want)
+
+
+def test_workspace_of_many_trees(gpu):
+    """Where the tiles alone fill the chip their splits end: 16 rounds of
+    resident workgroups (two a CU, three for heads of 64), 128 columns each, of
+    hd + 2 floats, whatever the bounds."""
+    import ctypes
+
+    from test_paged_refusals import batch, cache
+    from vgx import lib as vl
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    for heads, kvh, hd in ((32, 8, 128), (16, 8, 64), (16, 2, 64), (8, 4, 96), (4, 1, 256)):
+        c = cache(heads=heads, kv_heads=kvh, head_dim=hd, num_pages=1 << 20, k_row=hd, v_row=hd, k_head=16 * hd,
+                  v_head=16 * hd, k_page=16 * hd * kvh, v_page=16 * hd * kvh)
+        for nseq in (2, 24, 128, 256, 1000):
+            for bound in (300, 8192, 32768, 1 << 20):
+                for window in (0, 4096):
+                    b = batch(nseq=nseq, ntok=64 * nseq, max_q=64, max_kv=bound, table_cols=1 << 16, table_stride=1 << 16)
+                    ws = vl.load().vgx_paged_attn_tree_ws(gpu.ctx, ctypes.byref(c), ctypes.byref(b), window)
+                    most = 16 * cus * (3 if hd <= 64 else 2) * 128 * (hd + 2) * 4 + b.ntok * heads * 8
+                    assert ws <= most, (heads, kvh, hd, nseq, bound, window, ws)
+
+
+def test_many_trees_that_fill_the_chip(gpu):
+    """1600 workgroups of tiles, their splits ended: short sequences and two
+    that take several."""
+    nq = [17] * 200
+    kv = [17 + i * 37 % 200 for i in range(200)]
+    kv[3], kv[150] = 3001, 1409
+    b = Batch(63, nq, kv, 4, 64, 16, "bf16")
+    b.table = torch.nn.functional.pad(b.table, (0, 563 - b.table.shape[1]), value=-1)  # (room for the bound)
+    check(gpu, b, 32, trees_of(nq, 64), max_q=17, max_kv=9000)

@@ -1265,6 +1265,8 @@ typedef void (*BothFn)(const BothArgs);
 typedef void (*JoinFn)(const AttnArgs, int, const JoinArgs);
 // Positions up to which one workgroup takes a sequence whole.
 constexpr int64_t kWhole = 1024;
+// Rounds of resident workgroups that a tree's tiles are split into, at most.
+constexpr int kTreeRounds = 16;
 
 struct Launch {
     AttnFn fn;
@@ -1377,15 +1379,23 @@ Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t co
     int64_t len = std::max<int64_t>((span + want - 1) / want, 256);
     if (p.rows && A.nseq > 1)
         len = span <= kWhole ? span : std::min<int64_t>(std::max<int64_t>(len, 512), p.wgs >= num_cu ? 1024 : 768);
-    // Trees: the tile kernel's launch is small (a tile or two a sequence and KV
-    // head), so its sequences are split as well, to 1024 keys or a sixteenth of
-    // the longest (whose parts the join has to read): 24 trees of 5 to 61 rows at
-    // 300 to 8000, 16 / 8 heads of 64, 59 us (75 by the rule above, 74 at 512
-    // keys, 61 at 2048); 2 of 64 rows at 60001, 32 / 8 of 128, 207 (251; 290 at
-    // 1024).  The rows kernel beside it takes 1024 too (768: 3 us more).
+    // Trees: a tile launch is a tile or two a sequence and KV head, so its longest
+    // sequence would run on after all others, and sequences are split to 1024 keys
+    // or a sixteenth of the longest (whose parts the join has to read): 24 trees of 5
+    // to 61 rows at 300 to 8000, 16 / 8 heads of 64, 59 us (75 by the rule above, 74
+    // at 512 keys, 61 at 2048); 2 of 64 rows at 60001, 32 / 8 of 128, 207 (251; 290 at
+    // 1024).  That ends at 16 rounds of resident workgroups by the bounds, as the
+    // partial results of more cost memory and time: of 64 rows, 32 / 8 heads of 128,
+    // 128 at 8192 1664 us with 0.55 GB (without the end 1878 and 1.09; at 8 rounds
+    // 1565, at none 1474), 128 of 500 under a bound of 32768 164 (296; 160; 156), one
+    // at 32768 among 127 of 500 427 (425 and 2.2 GB; 651; 980).  The rows kernel
+    // beside it takes 1024 keys too (768: 3 us more).
     if (TREE && A.nseq > 1 && !alone && p.rows) len = std::max<int64_t>(len, 1024);
-    if (TREE && A.nseq > 1 && !p.rows)
-        len = std::min<int64_t>(std::max<int64_t>(len, 512), std::max<int64_t>(1024, span / 16));
+    if (TREE && A.nseq > 1 && !p.rows) {
+        const int64_t most = std::max<int64_t>((int64_t)kTreeRounds * num_cu * fill / p.wgs, 1);
+        len = std::min<int64_t>(std::max<int64_t>(len, 512),
+                                std::max<int64_t>({1024, span / 16, (span + most - 1) / most}));
+    }
     len = (len + 127) / 128 * 128;
     if (p.threads == 512) len = std::max<int64_t>(span, 128);
     p.split_len = (int)std::min<int64_t>(len, INT32_MAX);
