@@ -27,11 +27,13 @@
 //
 // Over a tree (TREE) a row sees the positions before the new rows, and of those
 // the ones that its mask names: where a tile of keys holds new rows, a column's
-// visible keys are 32 or 64 bits of that mask, shifted to the tile.  As the tiles
-// before those are untouched, the bounds are the plain forms': 24 trees of 5 to 61 rows
-// over 300 to 8000 positions (16/8 heads of 64, f16) 57 us with the join, 48 under a
-// window of 4096 (16/2 of 64, q8) 42, 2 of 64 rows over 60001 (32/8 of 128, bf16) 184
-// (491 MB, 126 GFLOP), one of 8 rows over 700 8.6, a launch and its round trips.
+// visible keys are 32 or 64 bits of that mask, shifted to the tile; the tiles
+// before those are untouched.  A call: one tree of 8 rows over 700 positions 8.6 us,
+// a launch and its round trips; 24 of 5 to 61 rows over 300 to 8000 (16/8 heads of
+// 64, f16) 57 with the join, 48 under a window of 4096 (16/2 of 64, q8) 42, both
+// waiting for the next tile's loads 43% of the wave cycles (vector work 23 and 25%);
+// 2 of 64 rows over 60001 (32/8 of 128, bf16) 189, of which the tiles are 171: 126
+// GFLOP at 740 TFLOP/s, in one round of workgroups, two of which stage the same keys.
 #pragma once
 
 #include <algorithm>
@@ -1156,7 +1158,8 @@ __global__ void __launch_bounds__(256, HD <= 128 && EX ? 2 : 1) paged_tile_kerne
 }
 
 // Prompts and single tokens in one batch: the sequences of at most 16 columns a
-// KV head as the rows kernel takes them, the others as tiles, in one launch (the
+// KV head (over trees 16 both_nb) as the rows kernel takes them, the others as
+// tiles, in one launch (the
 // tiles first), so that the ones' bytes come in while the others multiply: 512
 // rows and 8 at 16000 positions, 117 us (178 as tiles only, 136 in two launches);
 // 20 sequences of 1 .. 700 rows, window 1024, 16 / 8 heads of 64, 21 us, the
@@ -1419,7 +1422,7 @@ Launch launch_of(const PagedDev& A, int kind, int window, int num_cu, int64_t co
 }
 
 // One kind of sequences, or both where some may have many columns and others up
-// to 16: l[0] then takes these, whose long caches it splits, l[1] the others.
+// to 16 both_nb: l[0] then takes these, whose long caches it splits, l[1] the others.
 template <bool TREE>
 Plan plan_of(const PagedDev& A, int kind, int window, int num_cu) {
     Plan p{};

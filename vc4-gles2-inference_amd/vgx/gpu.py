@@ -303,8 +303,8 @@ class RaggedBatch:
     def accept(self, parent, tokens, chosen):
         """The walk down each sequence's tree by the token that each row's
         logits gave: (path: the rows of the way, at qstart[s] + k the k-th,
-        -1 behind its end; accepted: rows of the way but the first; next: the
-        last one's token)."""
+        -1 behind its end, undefined for rows of no sequence; accepted: rows of
+        the way but the first; next: the last one's token)."""
         g = self.gpu
         for t, name in ((parent, "parent"), (tokens, "tokens"), (chosen, "chosen")):
             g.need_values(t, _I32, self.ntok, name)
